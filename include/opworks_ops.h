@@ -150,6 +150,75 @@ OPW_API int opw_gemm_f16x2(const uint16_t *W, const uint16_t *x_hi, const uint16
 OPW_API int opw_gemm_f16x2_pair(const uint16_t *W, const uint16_t *x_hi, const uint16_t *x_lo, float *out, int N,
                                 int K, int M, void *stream);
 
+/* ---- 8-bit paged KV cache (include/ops/kv_quant.cuh). Extensions of this
+ * library (no reference counterpart).
+ *
+ * Pages of 16 tokens and block tables as in the fp32 pools; the pool holds one
+ * record of 32 * head_dim + 128 bytes per (block, kv head): K codes
+ * [16][head_dim], V codes [16][head_dim], K scales f32[16], V scales f32[16].
+ * format: 1 = int8, 2 = e4m3; a row is code * scale with scale = max|x| / 127
+ * (448), rounded to nearest even; a row with an infinity or a NaN has scale
+ * NaN and codes 0. type of plain rows: 0 = fp32, 1 = bf16. head_dim 64 or 128.
+ * Rows are ragged: sequence b owns rows [row_start[b], row_start[b + 1])
+ * (device int32, batch + 1 of them, row_start[batch] == rows), at positions
+ * first_pos[b] + 0, 1, ...; K and V of row r, head h lie at r * row_stride + h
+ * * head_dim elements. Plain rows and the pool are 16-byte aligned, row_stride
+ * too. Rows of positions outside the block table's row are left out. */
+OPW_API int opw_kv_quant_record_bytes(int head_dim); /* -1: not a supported head_dim */
+OPW_API int opw_kv_quant_write(const void *k, const void *v, int type, int64_t row_stride, uint8_t *pool, int format,
+                               const int32_t *block_table, int table_stride, const int32_t *first_pos,
+                               const int32_t *row_start, int batch, int rows, int num_kv_heads, int head_dim,
+                               void *stream);
+OPW_API int opw_kv_quant_read(const uint8_t *pool, int format, const int32_t *block_table, int table_stride,
+                              const int32_t *first_pos, const int32_t *row_start, int batch, int rows,
+                              int num_kv_heads, int head_dim, void *k, void *v, int type, int64_t row_stride,
+                              void *stream);
+
+/* ---- Several new tokens per sequence over a paged cache
+ * (include/ops/tree_attention.cuh, include/ops/tree_commit.cuh). Extensions of
+ * this library.
+ *
+ * The new (drafted) tokens of sequence b are nodes 0 .. n - 1 = rows
+ * [row_start[b], row_start[b + 1]) of q and out; their K/V rows are already in
+ * the cache at positions ctx_lens[b] + node. Node i attends to the context and
+ * to the nodes j with bit j % 32 of mask[row][j / 32] set; mask NULL: to the
+ * nodes j <= i (one row per sequence is a plain decode step). A node that sees
+ * nothing gets zeros; a masked key has no influence whatever it holds.
+ * max_rows: the most rows of one sequence (at most 32 * mask_words with a
+ * mask); max_ctx: an upper bound of ctx_lens, which plans the launch only.
+ * type: q and out fp32 (0) or bf16 (1); scores are scale * q . k; any number
+ * of query heads per kv head; q_stride and out_stride in elements. */
+OPW_API int opw_tree_attention(const void *q, int type, int64_t q_stride, const float *kpool, const float *vpool,
+                               const int32_t *block_table, int table_stride, const int32_t *ctx_lens,
+                               const int32_t *row_start, const uint32_t *mask, int mask_words, int batch, int rows,
+                               int max_rows, int max_ctx, int num_q_heads, int num_kv_heads, int head_dim, float scale,
+                               void *out, int64_t out_stride, void *stream);
+OPW_API int opw_tree_attention_q8(const void *q, int type, int64_t q_stride, const uint8_t *pool, int format,
+                                  const int32_t *block_table, int table_stride, const int32_t *ctx_lens,
+                                  const int32_t *row_start, const uint32_t *mask, int mask_words, int batch, int rows,
+                                  int max_rows, int max_ctx, int num_q_heads, int num_kv_heads, int head_dim,
+                                  float scale, void *out, int64_t out_stride, void *stream);
+/* Verifies drafted trees and keeps the accepted paths. draft[row]: the node's
+ * token; target[row]: the token that the model chose after the node;
+ * parent[row]: the node it follows (below it; -1 for node 0, the root, which is
+ * always accepted). From a node the walk goes on to its child whose draft is
+ * the node's target (the first of several). Writes path[row] (the accepted
+ * nodes of each sequence in order, then -1), count[b], next[b] (the target of
+ * the last accepted node; -1 for an empty tree) and new_lens[b] = ctx_lens[b] +
+ * count[b] (not in place), and moves cache row ctx + path[i] to ctx + i in all
+ * `layers` pools, layer_stride elements apart (floats; bytes in the _q8 form).
+ * At most 2048 nodes per sequence. */
+OPW_API int opw_tree_commit(const int32_t *draft, const int32_t *target, const int32_t *parent,
+                            const int32_t *row_start, const int32_t *ctx_lens, int batch, int max_rows, float *kpool,
+                            float *vpool, int64_t layer_stride, int layers, const int32_t *block_table,
+                            int table_stride, int num_kv_heads, int head_dim, int32_t *path, int32_t *count,
+                            int32_t *next, int32_t *new_lens, void *stream);
+OPW_API int opw_tree_commit_q8(const int32_t *draft, const int32_t *target, const int32_t *parent,
+                               const int32_t *row_start, const int32_t *ctx_lens, int batch, int max_rows,
+                               uint8_t *pool, int64_t layer_stride, int layers, const int32_t *block_table,
+                               int table_stride, int num_kv_heads, int head_dim, int32_t *path, int32_t *count,
+                               int32_t *next, int32_t *new_lens, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -44,10 +44,11 @@ def _stale(target, sources):
 def _targets():
     hdrs = _headers()
     out = []
+    ops_srcs = sorted(glob.glob(os.path.join(CSRC, "ops_*.cu")))
     out.append((os.path.join(LIBDIR, "libopworks_ops.so"),
-                [NVCC] + NVCC_FLAGS + ["-I", INC, os.path.join(CSRC, "ops_c_api.cu"), "-o",
-                                       os.path.join(LIBDIR, "libopworks_ops.so")],
-                hdrs + [os.path.join(CSRC, "ops_c_api.cu")]))
+                [NVCC] + NVCC_FLAGS + ["--threads", "0", "-I", INC] + ops_srcs + ["-o",
+                                                                                 os.path.join(LIBDIR, "libopworks_ops.so")],
+                hdrs + ops_srcs + glob.glob(os.path.join(CSRC, "*.h"))))
     llama_srcs = sorted(glob.glob(os.path.join(CSRC, "llama*.cu")))
     if llama_srcs:
         out.append((os.path.join(LIBDIR, "libopworks_llama.so"),

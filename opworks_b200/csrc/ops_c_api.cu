@@ -9,6 +9,7 @@
 #include <string>
 
 #include "opworks_ops.h"
+#include "ops_guard.h"
 #include "ops/add.cuh"
 #include "ops/argmax.cuh"
 #include "ops/attention_decode.cuh"
@@ -25,21 +26,14 @@
 #include "ops/split_heads.cuh"
 #include "ops/swiglu.cuh"
 
+std::string &opworks_ops::last_error() {
+    static thread_local std::string message;
+    return message;
+}
+
 namespace {
 
-thread_local std::string g_error;
-
-template <typename F> int guarded(F &&f) {
-    try {
-        f();
-        return 0;
-    } catch (const std::exception &e) {
-        g_error = e.what();
-    } catch (...) {
-        g_error = "unknown C++ exception";
-    }
-    return -1;
-}
+using opworks_ops::guarded;
 
 cudaStream_t as_stream(void *s) { return static_cast<cudaStream_t>(s); }
 
@@ -112,7 +106,7 @@ template <typename Op> void reduce_static_with(const float *in, float *out, int 
 
 extern "C" {
 
-const char *opw_ops_last_error(void) { return g_error.c_str(); }
+const char *opw_ops_last_error(void) { return opworks_ops::last_error().c_str(); }
 
 int opw_ops_sync(void *stream) {
     OPWORKS_CUDA_CHECK(cudaStreamSynchronize(as_stream(stream)));
@@ -121,7 +115,7 @@ int opw_ops_sync(void *stream) {
     OPWORKS_CUDA_CHECK(cudaMemcpy(&value, word, sizeof(int), cudaMemcpyDeviceToHost));
     if (value != 0) {
         OPWORKS_CUDA_CHECK(cudaMemset(word, 0, sizeof(int)));
-        g_error = "a device-side wait timed out (error code " + std::to_string(value) + ")";
+        opworks_ops::last_error() = "a device-side wait timed out (error code " + std::to_string(value) + ")";
         return -1;
     }
     return 0;

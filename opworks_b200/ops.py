@@ -50,6 +50,13 @@ SIGNATURES = {
     "opw_gemm_f16x2": [P, P, P, P, I, I, I, I, P],
     "opw_gemm_f16x2_pair": [P, P, P, P, I, I, I, P],
     "opw_paged_attention_prefill": [P, P, P, P, I, I, I, I, I, I, I, P, I, P],
+    "opw_kv_quant_record_bytes": [I],
+    "opw_kv_quant_write": [P, P, I, I64, P, I, P, I, P, P, I, I, I, I, P],
+    "opw_kv_quant_read": [P, I, P, I, P, P, I, I, I, I, P, P, I, I64, P],
+    "opw_tree_attention": [P, I, I64, P, P, P, I, P, P, P, I, I, I, I, I, I, I, I, F, P, I64, P],
+    "opw_tree_attention_q8": [P, I, I64, P, I, P, I, P, P, P, I, I, I, I, I, I, I, I, F, P, I64, P],
+    "opw_tree_commit": [P, P, P, P, P, I, I, P, P, I64, I, P, I, I, I, P, P, P, P, P],
+    "opw_tree_commit_q8": [P, P, P, P, P, I, I, P, I64, I, P, I, I, I, P, P, P, P, P],
 }
 
 
