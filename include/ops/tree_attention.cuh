@@ -14,127 +14,11 @@
 // A node that sees nothing gets zeros. Scores, softmax statistics and sums are
 // fp32. A masked key has no influence, whatever its row holds.
 
-#include <cstdint>
-#include <cuda_bf16.h>
-
-#include "../core/cuda_utils.cuh"
-#include "attention_kernels.cuh"
-#include "kv_quant.cuh"
+#include "tree_attention_common.cuh"
+#include "tree_attention_rows.cuh"
 
 namespace opworks {
-
-// A batch of trees over a cache (device pointers).
-struct TreeBatch {
-    const int *block_table; // [batch][table_stride]
-    int table_stride;
-    const int *ctx_lens;    // [batch]
-    const int *row_start;   // [batch + 1]
-    const uint32_t *mask;   // [rows][mask_words], or null: a chain
-    int mask_words;
-    int batch, rows, max_rows; // max_rows: the most rows of one sequence
-    int max_ctx;               // an upper bound of ctx_lens; plans the launch only
-};
-
 namespace detail {
-
-struct TreeArgs {
-    TreeBatch t;
-    const void *k; // fp32 K pool, or the 8-bit pool
-    const void *v; // fp32 V pool
-    int qh, kvh;
-    float scale_log2; // scale * log2(e): scores in log2 units
-    int64_t q_stride, out_stride;
-};
-
-// Keys and rows of a sequence, held inside the table and the row count.
-struct TreeSpan {
-    int row0, n, ctx, keys;
-    __device__ TreeSpan(const TreeBatch &t, int b) {
-        row0 = max(0, t.row_start[b]);
-        n = max(0, min(min(t.row_start[b + 1], t.rows) - row0, t.max_rows));
-        ctx = max(0, t.ctx_lens[b]);
-        const int64_t all = min(static_cast<int64_t>(ctx) + n, static_cast<int64_t>(t.table_stride) * kKvPage);
-        keys = static_cast<int>(all);
-    }
-};
-
-__device__ __forceinline__ bool tree_sees(const TreeBatch &t, int row, int i, int j) {
-    if (t.mask == nullptr)
-        return j <= i;
-    return (t.mask[static_cast<int64_t>(row) * t.mask_words + (j >> 5)] >> (j & 31)) & 1u;
-}
-
-constexpr int kTreeThreads = 128;
-
-// One CTA per (row, query head); its warps take the keys in turn and are
-// merged at the end.
-template <typename T, int D, KvFormat kFmt>
-static __global__ void __launch_bounds__(kTreeThreads)
-    tree_attention_kernel(const T *__restrict__ q, T *__restrict__ out, TreeArgs a) {
-    constexpr int kE = D / 32, kWarps = kTreeThreads / 32;
-    __shared__ float om[kWarps][D], mm[kWarps], ll[kWarps];
-    const int i = blockIdx.x, hq = blockIdx.y, b = blockIdx.z, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const TreeSpan s(a.t, b);
-    if (i >= s.n)
-        return;
-    const int row = s.row0 + i, h = hq / (a.qh / a.kvh);
-    float qr[kE], o[kE] = {}, m = kNegInf, l = 0.f;
-    for (int e = 0; e < kE; ++e)
-        qr[e] = static_cast<float>(q[row * a.q_stride + hq * D + lane * kE + e]) * a.scale_log2;
-    for (int t = warp; t < s.keys; t += kWarps) {
-        if (t >= s.ctx && !tree_sees(a.t, row, i, t - s.ctx))
-            continue;
-        const int64_t rec = static_cast<int64_t>(a.t.block_table[static_cast<int64_t>(b) * a.t.table_stride + t / kKvPage]) * a.kvh + h;
-        const int slot = t % kKvPage;
-        float kk[kE], vv[kE];
-        if constexpr (kFmt == KvFormat::kF32) {
-            const int64_t at = (rec * kKvPage + slot) * D + lane * kE;
-            for (int e = 0; e < kE; ++e) {
-                kk[e] = static_cast<const float *>(a.k)[at + e];
-                vv[e] = static_cast<const float *>(a.v)[at + e];
-            }
-        } else {
-            using R = KvRecord<D>;
-            const uint8_t *p = static_cast<const uint8_t *>(a.k) + rec * R::kBytes;
-            const float ks = *reinterpret_cast<const float *>(p + R::kKScale + 4 * slot);
-            const float vs = *reinterpret_cast<const float *>(p + R::kVScale + 4 * slot);
-            for (int e = 0; e < kE; ++e) {
-                float x[4];
-                kv_decode4<kFmt>(p[slot * D + lane * kE + e], ks, x);
-                kk[e] = x[0];
-                kv_decode4<kFmt>(p[R::kCodes + slot * D + lane * kE + e], vs, x);
-                vv[e] = x[0];
-            }
-        }
-        float x = 0.f;
-        for (int e = 0; e < kE; ++e)
-            x = fmaf(qr[e], kk[e], x);
-        for (int off = 16; off; off >>= 1)
-            x += __shfl_xor_sync(kFullWarpMask, x, off);
-        const float m1 = fmaxf(m, x);
-        const float c = m == kNegInf ? 0.f : exp2f(m - m1), p = exp2f(x - m1);
-        m = m1;
-        l = l * c + p;
-        for (int e = 0; e < kE; ++e)
-            o[e] = o[e] * c + p * vv[e];
-    }
-    for (int e = 0; e < kE; ++e)
-        om[warp][lane * kE + e] = o[e];
-    if (lane == 0)
-        mm[warp] = m, ll[warp] = l;
-    __syncthreads();
-    for (int d = threadIdx.x; d < D; d += kTreeThreads) {
-        float top = kNegInf, L = 0.f, O = 0.f;
-        for (int w = 0; w < kWarps; ++w)
-            top = fmaxf(top, mm[w]);
-        for (int w = 0; w < kWarps; ++w) {
-            const float f = mm[w] == kNegInf ? 0.f : exp2f(mm[w] - top);
-            L += f * ll[w];
-            O += f * om[w][d];
-        }
-        out[row * a.out_stride + hq * D + d] = static_cast<T>(L > 0.f || L != L ? O / L : 0.f);
-    }
-}
 
 inline void validate_tree(const TreeBatch &t, const void *q, const void *out, int64_t q_stride, int64_t out_stride,
                           int elem, int q_heads, int kv_heads, int head_dim, const void *k, const void *v) {
@@ -158,8 +42,11 @@ inline void validate_tree(const TreeBatch &t, const void *q, const void *out, in
 
 template <typename T, int D, KvFormat kFmt>
 inline void tree_attention_launch(const T *q, T *out, const TreeArgs &a, cudaStream_t stream) {
-    launch_ex(tree_attention_kernel<T, D, kFmt>, dim3(a.t.max_rows, a.qh, a.t.batch), dim3(kTreeThreads), 0, stream, q,
-              out, a);
+    using One = TreeRowsGeo<T, D, kFmt, 1>;
+    if (static_cast<int64_t>(a.t.max_rows) * (a.qh / a.kvh) <= One::kRows)
+        tree_rows_launch<T, D, kFmt, 1>(q, out, a, stream);
+    else
+        tree_rows_launch<T, D, kFmt, 2>(q, out, a, stream);
 }
 
 template <typename T>
