@@ -12,7 +12,8 @@
 // given (a chain of tokens; n = 1 is a plain decode step):
 //   o = sum_j softmax_j(scale q . k_j) v_j
 // A node that sees nothing gets zeros. Scores, softmax statistics and sums are
-// fp32. A masked key has no influence, whatever its row holds.
+// fp32. A masked key has no influence, whatever its row holds; an infinity or a
+// NaN in a K or V row that a node does see makes the node's whole output NaN.
 
 #include "tree_attention_common.cuh"
 #include "tree_attention_rows.cuh"
@@ -42,11 +43,14 @@ inline void validate_tree(const TreeBatch &t, const void *q, const void *out, in
 
 template <typename T, int D, KvFormat kFmt>
 inline void tree_attention_launch(const T *q, T *out, const TreeArgs &a, cudaStream_t stream) {
-    using One = TreeRowsGeo<T, D, kFmt, 1>;
-    if (static_cast<int64_t>(a.t.max_rows) * (a.qh / a.kvh) <= One::kRows)
+    constexpr int kTile = TreeRowsGeo<T, D, kFmt, 1>::kRows;
+    const int64_t tiles = (static_cast<int64_t>(a.t.max_rows) * (a.qh / a.kvh) + kTile - 1) / kTile;
+    if (tiles == 1)
         tree_rows_launch<T, D, kFmt, 1>(q, out, a, stream);
-    else
+    else if (D == 128 || tiles == 2)
         tree_rows_launch<T, D, kFmt, 2>(q, out, a, stream);
+    else
+        tree_rows_launch<T, D, kFmt, D == 64 ? 3 : 2>(q, out, a, stream);
 }
 
 template <typename T>

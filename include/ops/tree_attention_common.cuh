@@ -40,7 +40,8 @@ struct TreeArgs {
     int64_t q_stride, out_stride;
 };
 
-// Lets `kernel` have `bytes` of dynamic shared memory on the current device
+// Lets `kernel` have `bytes` of dynamic shared memory and clusters of up to 16
+// CTAs on the current device
 // (set once per kernel and device; setting it twice does no harm).
 template <typename... P> inline void allow_shared_bytes(void (*kernel)(P...), int bytes) {
     static std::mutex mu;
@@ -52,6 +53,7 @@ template <typename... P> inline void allow_shared_bytes(void (*kernel)(P...), in
     const std::lock_guard<std::mutex> lock(mu);
     if (std::find(set.begin(), set.end(), key) == set.end()) {
         OPWORKS_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+        OPWORKS_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
         set.push_back(key);
     }
     seen.push_back(key);
@@ -70,7 +72,7 @@ struct TreeSpan {
 };
 
 // Bit i: node `node` (row `row` of the mask) sees the key j0 + i, i < 16, where
-// keys below 0 are context and there are none from `limit` on. j0 > -16.
+// keys below 0 are context and there are none from `limit` on. j0 > -32.
 __device__ __forceinline__ uint32_t tree_sees16(const TreeBatch &t, int row, int node, int j0, int limit) {
     uint32_t bits;
     if (t.mask == nullptr) {
@@ -88,12 +90,6 @@ __device__ __forceinline__ uint32_t tree_sees16(const TreeBatch &t, int row, int
     }
     const int left = limit - j0;
     return left >= 16 ? bits & 0xffffu : left <= 0 ? 0u : bits & ((1u << left) - 1u);
-}
-
-__device__ __forceinline__ uint32_t tf32_rna(float x) {
-    uint32_t r;
-    asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(r) : "f"(x));
-    return r;
 }
 
 __device__ __forceinline__ void cluster_sync_all() {

@@ -12,26 +12,32 @@
 // form a thread-block cluster and are joined through distributed shared memory
 // in rank order: one launch, no workspace, the same bits every time.
 //
-// Warps are independent until the end: warp w takes pages w, w + kWarps, ... of
-// the split through its own ring of bulk copies (an 8-bit page of a head is one
-// copy), with its own softmax state.
+// Warps are independent until the end: warp w takes chunks w, w + kWarps, ...
+// of the split (a chunk is two 8-bit pages or one fp32 page) through its own
+// ring of bulk copies (an 8-bit page of a head is one copy), with its own
+// softmax state.
 //
 // Products on mma.sync: with few rows a tcgen05 tile of 128 would be mostly
 // empty, and fragments go from shared memory to registers directly, so 8-bit
 // codes are widened to fp16 (exactly) on the way and no widened tile is
 // written anywhere. Layout: S = Q K^T has the rows of Q along M = 16, so the
-// accumulator of S is the A operand of O = P V. fp32 rows are two terms hi + lo
-// (22 bits): a tile holds 8 rows, hi in its upper half and lo in its lower, so
-// one product gives both and a lane adds its own two accumulators. bf16 rows
-// fit in one term: 16 rows to a tile. K and V: 8-bit codes are exact in fp16,
-// their scales are applied to S and folded into P; fp32 pools are two tf32
-// terms. Contraction indices and output columns are permuted so that a lane's
-// fragments are contiguous bytes of a row (see the index comments below).
+// accumulator of S is the A operand of O = P V. fp32 rows are two fp16 terms hi
+// + lo (22 bits): a tile holds 8 rows, hi in its upper half and lo in its
+// lower, so one product gives both and a lane adds its own two accumulators.
+// bf16 rows fit in one term: 16 rows to a tile. K and V: 8-bit codes are exact
+// in fp16, their scales are applied to S and folded into P; fp32 pools are two
+// fp16 terms too, after a power of two that the warp shares (of the 8 keys for
+// K, running for V) has brought them into range. tf32 terms took as many
+// conversions and twice the tensor time. Contraction indices and output columns
+// are permuted so that a lane's fragments are contiguous bytes of a row (see
+// the index comments below).
 //
 // Softmax: one pass, running maximum in log2 units. The maximum is a reference
-// only: it is raised when a score passes it by kLazy, so most pages rescale
+// only: it is raised when a score passes it by kLazy, so most chunks rescale
 // nothing. P is held as 2^kLift times its value, so that fp16 keeps 22 bits of
-// two terms down to 2^-28 of the largest weight.
+// two terms down to 2^-28 of the largest weight. The V scales of 8-bit pools
+// are folded into P, relative to a running power of two that counts as part of
+// the reference (l and O carry it both).
 
 #include <cuda_fp16.h>
 
@@ -41,6 +47,9 @@ namespace opworks::detail {
 
 constexpr float kLazy = 4.f;  // log2 units a score may pass the reference maximum by
 constexpr float kLift = 10.f; // P is scaled by 2^kLift: at most 2^14
+// V scales below this are not told apart from it (fp16 loses their low bits);
+// lower, and l in their units would leave fp32's range
+constexpr float kMinVLog = -80.f, kMinVTop = 0x1p-80f;
 
 template <typename T, int D, KvFormat kFmt, int kMT> struct TreeRowsGeo {
     static constexpr bool kTwo = std::is_same_v<T, float>; // two terms of Q and P
@@ -49,15 +58,19 @@ template <typename T, int D, KvFormat kFmt, int kMT> struct TreeRowsGeo {
     static constexpr int kRows = kMT * kTileRows;
     static constexpr bool kWide = kFmt == KvFormat::kF32;
     static constexpr int kPageBytes = kWide ? 2 * kKvPage * D * 4 : KvRecord<D>::kBytes;
-    static constexpr int kWarps = kWide ? 4 : 8;
+    static constexpr int kChunk = kWide ? 1 : 2; // pages
+    static constexpr int kChunkBytes = kChunk * kPageBytes;
+    static constexpr int kWarps = kWide ? (D == 128 ? 6 : 4) : kMT == 1 ? 8 : 4;
     static constexpr int kThreads = 32 * kWarps;
-    static constexpr int kStages = kWide ? 3 : 4;
-    static constexpr int kRing = kWarps * kStages * kPageBytes;
+    static constexpr int kStages = kWide && D == 128 ? 2 : 3; // chunks
+    static constexpr int kRing = kWarps * kStages * kChunkBytes;
     static constexpr int kPitch = D + 4; // floats per row of a warp's partial result
     static constexpr int kMerge = kWarps * kRows * kPitch * 4;
-    static constexpr int kBuf = (kRing > kMerge ? kRing : kMerge);
+    static constexpr int kBuf = kRing > kMerge ? kRing : kMerge;
     static constexpr int kBytes = kBuf + 8 * kWarps * kStages + 4 * (2 * kWarps + 2) * kRows;
-    static constexpr int kQRegs = kWide ? D / 8 : D / 16; // k steps
+    static constexpr int kSteps = D / 16; // k steps of Q K^T
+    // resident CTAs: what shared memory and about (48 D / 64 kMT + 70) registers a thread leave
+    static constexpr int kCtas = kWide ? (D == 64 ? 2 : 1) : kMT == 1 ? (D == 64 ? 2 : 1) : kMT == 2 && D == 64 ? 2 : 1;
 };
 
 // d += a (16 x 16 fp16) b (16 x 8 fp16)
@@ -67,20 +80,6 @@ __device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], u
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-// d += a (16 x 8 tf32) b (8 x 8 tf32)
-__device__ __forceinline__ void mma_tf32(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
-                 "{%0, %1, %2, %3};"
-                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-
-// x as two tf32 terms: rounded to the nearest (by magnitude), and the rest,
-// whose last bit the tensor cores drop: 2^-24 of x. Truncation instead left
-// 2^-21, all of it towards zero, which showed in the results.
-__device__ __forceinline__ uint32_t tf32_hi(float x) { return (__float_as_uint(x) + 0x1000u) & 0xffffe000u; }
-__device__ __forceinline__ uint32_t tf32_lo(float x) { return __float_as_uint(x - __uint_as_float(tf32_hi(x))); }
-
 // fp16 pair (a, b) as one register, a in the low half
 __device__ __forceinline__ uint32_t half2_rn(float a, float b) {
     const __half2 h = __floats2half2_rn(a, b);
@@ -109,7 +108,44 @@ template <KvFormat kFmt> __device__ __forceinline__ void codes_to_half(uint32_t 
     }
 }
 
+// int8 codes as K operands: fp16 subnormals (c + 128) 2^-24, exact too. The
+// offset is taken off by the accumulators' start, -128 sum q: two instructions
+// a pair fewer than codes_to_half. (Not for V: its sums of many keys cancel,
+// so the offset would cost the result's last bits.)
+template <KvFormat kFmt> __device__ __forceinline__ void k_codes_to_half(uint32_t w, uint32_t &lo, uint32_t &hi) {
+    if constexpr (kFmt == KvFormat::kInt8) {
+        const uint32_t u = w ^ 0x80808080u;
+        lo = __byte_perm(u, 0u, 0x4140);
+        hi = __byte_perm(u, 0u, 0x4342);
+    } else {
+        codes_to_half<kFmt>(w, lo, hi);
+    }
+}
+
+// x f and y f as two fp16 terms each (the first cut off after 11 bits); `top`
+// keeps the largest magnitude of the first terms, NaN and infinity included.
+__device__ __forceinline__ void split_half2(float x, float y, float f, uint32_t &hi, uint32_t &lo, __half2 &top) {
+    const float2 u = __fmul2_rn(make_float2(x, y), make_float2(f, f));
+    const float2 h = make_float2(__uint_as_float(__float_as_uint(u.x) & 0xffffe000u),
+                                 __uint_as_float(__float_as_uint(u.y) & 0xffffe000u));
+    const float2 r = __fadd2_rn(u, make_float2(-h.x, -h.y));
+    hi = half2_rn(h.x, h.y);
+    lo = half2_rn(r.x, r.y);
+    top = __hmax2_nan(top, __habs2(*reinterpret_cast<const __half2 *>(&hi)));
+}
+// Whether a magnitude in `top` is over 2^14, infinite or NaN.
+__device__ __forceinline__ bool over_half2(__half2 top) {
+    return !(__low2float(top) <= 16384.f && __high2float(top) <= 16384.f);
+}
+
 __device__ __forceinline__ float finite_or_zero(float x) { return fabsf(x) <= 3.4028235e38f ? x : 0.f; }
+
+// The power of two next above magnitude `top` (bits of it) as an exponent
+// field, held where its inverse and its products with 2^10 are normal too.
+__device__ __forceinline__ uint32_t exponent_above(uint32_t top_bits) {
+    return min(max((top_bits >> 23) + 1u, 16u), 240u);
+}
+__device__ __forceinline__ float pow2_field(uint32_t ex) { return __uint_as_float(ex << 23); }
 
 // e4m3 NaN codes (never written by ops::kv_quant_write) replaced by zero: a
 // masked row may hold them, and zero times NaN is NaN.
@@ -118,10 +154,11 @@ __device__ __forceinline__ uint32_t clear_e4m3_nan(uint32_t w) {
 }
 
 template <typename T, int D, KvFormat kFmt, int kMT>
-static __global__ void __launch_bounds__(TreeRowsGeo<T, D, kFmt, kMT>::kThreads)
+static __global__ void __launch_bounds__(TreeRowsGeo<T, D, kFmt, kMT>::kThreads, TreeRowsGeo<T, D, kFmt, kMT>::kCtas)
     tree_rows_kernel(const T *__restrict__ q, T *__restrict__ out, TreeArgs a, int groups, int splits, int *err) {
     using G = TreeRowsGeo<T, D, kFmt, kMT>;
     using R = KvRecord<D>;
+    constexpr int kC = G::kChunk;
     extern __shared__ __align__(128) uint8_t smem[];
     uint64_t *bars = reinterpret_cast<uint64_t *>(smem + G::kBuf);
     float *stat = reinterpret_cast<float *>(bars + G::kWarps * G::kStages); // m [warps][rows], l [warps][rows]
@@ -142,30 +179,38 @@ static __global__ void __launch_bounds__(TreeRowsGeo<T, D, kFmt, kMT>::kThreads)
     pdl_trigger();
     pdl_wait();
 
+    // The chunks of a sequence go round the cluster's warps, so that a warp knows
+    // its pages before it knows the sequence's length: chunk i of a warp is
+    // first + i * step. Lane c of a chunk's first kC lanes copies its page c, and
+    // a lane holds the block id of one page of the next 32 / kC chunks.
+    const int first = rank * G::kWarps + warp, step = splits * G::kWarps;
+    const int *table = a.t.block_table + static_cast<int64_t>(b) * a.t.table_stride;
+    int ids = 0;
+    const auto refill = [&](int base) {
+        const int64_t page = (first + static_cast<int64_t>(base + lane / kC) * step) * kC + lane % kC;
+        ids = page < a.t.table_stride ? table[page] : -1;
+    };
+    refill(0);
+
     const TreeSpan span(a.t, b);
     const int row_base = group * G::kRows, rows = span.n * rep; // query rows of this (sequence, head)
     int keys = span.keys;
     if (a.t.mask == nullptr) // a chain: nothing after the group's last node is seen
         keys = min(keys, span.ctx + (min(row_base + G::kRows, rows) + rep - 1) / rep);
     const int pages = row_base < rows ? (keys + kKvPage - 1) / kKvPage : 0;
-    const int per = (pages + splits - 1) / splits;
-    const int p0 = min(pages, rank * per), p1 = min(pages, p0 + per);
-    const int mine = p1 - p0 > warp ? (p1 - p0 - warp + G::kWarps - 1) / G::kWarps : 0; // pages of this warp
-    uint8_t *ring = smem + warp * G::kStages * G::kPageBytes;
+    const int chunks = (pages + kC - 1) / kC;
+    const int mine = chunks > first ? (chunks - first + step - 1) / step : 0; // chunks of this warp
+    uint8_t *ring = smem + warp * G::kStages * G::kChunkBytes;
 
-    const int *table = a.t.block_table + static_cast<int64_t>(b) * a.t.table_stride;
-    int ids = 0; // block ids of 32 pages of this warp, one per lane
-    const auto refill = [&](int base) {
-        const int i = base + lane;
-        ids = i < mine ? table[p0 + warp + i * G::kWarps] : 0;
-    };
-    const auto issue = [&](int i) { // page i of this warp into its stage
-        const int blk = __shfl_sync(kFullWarpMask, ids, i & 31);
-        if (lane == 0) {
-            const int s = i % G::kStages;
-            uint8_t *dst = ring + s * G::kPageBytes;
+    const auto issue = [&](int i, int s) { // chunk i of this warp into stage s
+        const int blk = __shfl_sync(kFullWarpMask, ids, (i * kC + lane % kC) & 31);
+        const int n = min(kC, pages - (first + i * step) * kC);
+        if (lane == 0)
+            sm100::mbar_arrive_expect_tx(&bar[s], static_cast<uint32_t>(n * G::kPageBytes));
+        __syncwarp();
+        if (lane < n) {
+            uint8_t *dst = ring + s * G::kChunkBytes + lane * G::kPageBytes;
             const int64_t rec = static_cast<int64_t>(blk) * a.kvh + h;
-            sm100::mbar_arrive_expect_tx(&bar[s], G::kPageBytes);
             if constexpr (G::kWide) {
                 constexpr int kHalf = kKvPage * D * 4;
                 sm100::bulk_load(dst, static_cast<const uint8_t *>(a.k) + rec * kHalf, kHalf, &bar[s]);
@@ -175,15 +220,14 @@ static __global__ void __launch_bounds__(TreeRowsGeo<T, D, kFmt, kMT>::kThreads)
             }
         }
     };
-    refill(0);
     for (int i = 0; i < min(mine, G::kStages); ++i)
-        issue(i);
+        issue(i, i);
 
-    // Q fragments. fp16: k step s = 4c + i of 16 dims, lane t holds dims 64c +
-    // 16t + 4i + {0, 1} (k = 2t, 2t + 1) and + {2, 3} (k = 2t + 8, 2t + 9).
-    // tf32: k step 2c + e of 8 dims, dims 16c + 4t + 2e (k = t), + 1 (k = t + 4).
-    uint32_t qf[kMT][G::kQRegs][4];
-    float row_scale[kMT][G::kRPL];
+    // Q fragments: k step s = 4c + i of 16 dims; lane t holds dims 64c + 16t +
+    // 4i + {0, 1} (k = 2t, 2t + 1) and + {2, 3} (k = 2t + 8, 2t + 9). A negative
+    // scale turns their sign, so that row_scale is not below zero.
+    uint32_t qf[kMT][G::kSteps][4];
+    float row_scale[kMT][G::kRPL], start[kMT][2];
 #pragma unroll
     for (int mt = 0; mt < kMT; ++mt) {
         float x[G::kRPL][D / 4];
@@ -192,126 +236,193 @@ static __global__ void __launch_bounds__(TreeRowsGeo<T, D, kFmt, kMT>::kThreads)
             const int r = row_base + mt * G::kTileRows + rr * 8 + g;
             const bool live = r < rows;
             const T *src = q + static_cast<int64_t>(span.row0 + (live ? r / rep : 0)) * a.q_stride +
-                           static_cast<int64_t>(h * rep + (live ? r % rep : 0)) * D;
-            if constexpr (G::kWide && !G::kTwo) { // 4 bf16 values at a time
+                           static_cast<int64_t>(h * rep + (live ? r % rep : 0)) * D + 16 * t;
+            constexpr int kN = KvVec<T>::kN;
 #pragma unroll
-                for (int c = 0; c < D / 16; ++c) {
-                    const uint2 w = live ? *reinterpret_cast<const uint2 *>(src + 16 * c + 4 * t) : make_uint2(0, 0);
-                    x[rr][4 * c] = __uint_as_float(w.x << 16), x[rr][4 * c + 1] = __uint_as_float(w.x & 0xffff0000u);
-                    x[rr][4 * c + 2] = __uint_as_float(w.y << 16), x[rr][4 * c + 3] = __uint_as_float(w.y & 0xffff0000u);
-                }
-            } else {
-                constexpr int kN = KvVec<T>::kN, kRun = G::kWide ? 4 : 16; // kRun: contiguous dims of a lane
+            for (int v = 0; v < D / 4 / kN; ++v) {
+                float y[kN] = {};
+                if (live)
+                    KvVec<T>::unpack(*reinterpret_cast<const uint4 *>(src + v * kN / 16 * 64 + v * kN % 16), y);
 #pragma unroll
-                for (int v = 0; v < D / 4 / kN; ++v) {
-                    float y[kN] = {};
-                    if (live)
-                        KvVec<T>::unpack(*reinterpret_cast<const uint4 *>(src + v * kN / kRun * 4 * kRun + kRun * t + v * kN % kRun), y);
-#pragma unroll
-                    for (int e = 0; e < kN; ++e)
-                        x[rr][v * kN + e] = y[e];
-                }
+                for (int e = 0; e < kN; ++e)
+                    x[rr][v * kN + e] = y[e];
             }
+            // a power of two brings the row's largest magnitude to 2^9 .. 2^10,
+            // so that fp16 holds the row to 2^-22 of it in two terms (and a
+            // bf16 row exactly in one)
+            uint32_t top = 0;
+#pragma unroll
+            for (int e = 0; e < D / 4; ++e)
+                top = max(top, __float_as_uint(x[rr][e]) & 0x7fffffffu);
+            top = max(top, __shfl_xor_sync(kFullWarpMask, top, 1));
+            top = max(top, __shfl_xor_sync(kFullWarpMask, top, 2));
+            const uint32_t ex = exponent_above(top);
+            const float f = copysignf(pow2_field(254u - ex + 10u), a.scale_log2);
+            row_scale[mt][rr] = fabsf(a.scale_log2) * pow2_field(ex - 10u) * (kFmt == KvFormat::kInt8 ? 16777216.f : 1.f);
+#pragma unroll
+            for (int e = 0; e < D / 4; ++e)
+                x[rr][e] *= f;
         }
+        float sum[2] = {0.f, 0.f}; // of rows g and g + 8 of the tile
 #pragma unroll
-        for (int rr = 0; rr < G::kRPL; ++rr) {
-            row_scale[mt][rr] = a.scale_log2;
-            if constexpr (!G::kWide) {
-                // a power of two brings the row's largest magnitude to 2^10 ..
-                // 2^11, so that fp16 holds the row to 2^-22 of it in two terms
-                // (and a bf16 row exactly in one)
-                float top = 0.f;
+        for (int s = 0; s < G::kSteps; ++s)
 #pragma unroll
-                for (int e = 0; e < D / 4; ++e)
-                    top = fmaxf(top, fabsf(x[rr][e]));
-                top = fmaxf(top, __shfl_xor_sync(kFullWarpMask, top, 1));
-                top = fmaxf(top, __shfl_xor_sync(kFullWarpMask, top, 2));
-                const int ex = top > 0.f ? static_cast<int>(__float_as_uint(top) >> 23) - 127 : 0; // floor(log2)
-                const int up = max(-100, min(100, 10 - ex));
-                const float f = __uint_as_float(static_cast<uint32_t>(127 + up) << 23);
-                row_scale[mt][rr] *= __uint_as_float(static_cast<uint32_t>(127 - up) << 23);
-#pragma unroll
-                for (int e = 0; e < D / 4; ++e)
-                    x[rr][e] *= f;
+            for (int e = 0; e < 2; ++e) {
+                const float u = x[0][4 * s + 2 * e], v = x[0][4 * s + 2 * e + 1];
+                const uint32_t hi = half2_rn(u, v);
+                const float2 f = half2_floats(hi);
+                const uint32_t lo = G::kTwo ? half2_rn(u - f.x, v - f.y)
+                                            : half2_rn(x[G::kRPL - 1][4 * s + 2 * e], x[G::kRPL - 1][4 * s + 2 * e + 1]);
+                qf[mt][s][2 * e] = hi;
+                qf[mt][s][2 * e + 1] = lo;
+                sum[0] += f.x + f.y;
+                sum[1] += half2_floats(lo).x + half2_floats(lo).y;
             }
-        }
-        if constexpr (G::kWide) {
 #pragma unroll
-            for (int s = 0; s < G::kQRegs; ++s)
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    const float hi = x[0][2 * s + e];
-                    qf[mt][s][2 * e] = G::kTwo ? tf32_hi(hi) : __float_as_uint(hi);
-                    qf[mt][s][2 * e + 1] = G::kTwo ? tf32_lo(hi) : __float_as_uint(x[G::kRPL - 1][2 * s + e]);
-                }
-        } else {
-#pragma unroll
-            for (int s = 0; s < G::kQRegs; ++s)
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    const float u = x[0][4 * s + 2 * e], v = x[0][4 * s + 2 * e + 1];
-                    const uint32_t hi = half2_rn(u, v);
-                    qf[mt][s][2 * e] = hi;
-                    if constexpr (G::kTwo) {
-                        const float2 f = half2_floats(hi);
-                        qf[mt][s][2 * e + 1] = half2_rn(u - f.x, v - f.y);
-                    } else {
-                        qf[mt][s][2 * e + 1] = half2_rn(x[1][4 * s + 2 * e], x[1][4 * s + 2 * e + 1]);
-                    }
-                }
+        for (int i = 0; i < 2; ++i) {
+            start[mt][i] = 0.f;
+            if constexpr (kFmt == KvFormat::kInt8) {
+                sum[i] += __shfl_xor_sync(kFullWarpMask, sum[i], 1);
+                sum[i] += __shfl_xor_sync(kFullWarpMask, sum[i], 2);
+                start[mt][i] = sum[i] * (-128.f / 16777216.f);
+            }
         }
     }
 
     float o[kMT][D / 8][4] = {};
+    // m: the reference that weights are relative to, 2^(x - m)
     float m[kMT][G::kRPL], l[kMT][G::kRPL];
-    float vtop = 0.f, vinv = 0.f; // power of two above every V scale so far, and 1 / it
+    // 8-bit: a power of two above every V scale so far and its log2, part of m.
+    // fp32: the powers of two that K and V are multiplied by (0: not chosen yet)
+    float vtop = kMinVTop, vlog = kMinVLog, kmul = 0.f, vmul = 0.f;
 #pragma unroll
     for (int mt = 0; mt < kMT; ++mt)
 #pragma unroll
         for (int rr = 0; rr < G::kRPL; ++rr)
             m[mt][rr] = -1e30f, l[mt][rr] = 0.f;
-
-    bool ok = true;
-    int done = 0;
-    for (; done < mine; ++done) {
-        const int s = done % G::kStages;
-        if (!sm100::mbar_wait_warp(&bar[s], static_cast<uint32_t>(done / G::kStages) & 1u)) {
-            ok = false;
-            break;
+    const auto rescale = [&](int mt, const float (&fix)[G::kRPL]) {
+#pragma unroll
+        for (int n = 0; n < D / 8; ++n) {
+            o[mt][n][0] *= fix[0];
+            o[mt][n][1] *= fix[0];
+            o[mt][n][2] *= fix[G::kRPL - 1];
+            o[mt][n][3] *= fix[G::kRPL - 1];
         }
-        const uint8_t *page = ring + s * G::kPageBytes;
-        const int key0 = (p0 + warp + done * G::kWarps) * kKvPage;
-        const bool edge = key0 + kKvPage > span.ctx; // holds nodes, or places after the last key
+    };
+    const auto poison = [&] { // a row that every node sees holds an infinity or a NaN
+#pragma unroll
+        for (int mt = 0; mt < kMT; ++mt)
+#pragma unroll
+            for (int rr = 0; rr < G::kRPL; ++rr)
+                l[mt][rr] = __uint_as_float(0x7fc00000u);
+    };
 
-        // S. Score column g of n tile j is key 8j + 4 (g & 1) + g / 2, so that
-        // lane t's columns 2t + col are keys 8j + 4 col + t.
-        float sc[kMT][2][4] = {};
+    // One chunk. Edge chunks hold nodes, or places after the last key.
+    // Score column g of n tile j of a page is key 8j + 4 (g & 1) + g / 2, so that
+    // lane t's columns 2t + col are keys 8j + 4 col + t: value i = 2j + col of a
+    // lane is key 4i + t.
+    const auto take = [&](const uint8_t *chunk, int key0, auto edge_tag) {
+        constexpr bool kEdge = decltype(edge_tag)::value;
+        float sc[kMT][2 * kC][4];
+        float kfac[4 * kC], vfac[4 * kC]; // factors of a lane's scores and weights
+        uint32_t bad = 0;                 // bit i: fp32 row i of the lane holds an infinity or a NaN
+        float x[kMT][G::kRPL][4 * kC];
+        const auto zero_scores = [&] {
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            const int krow = 8 * j + 4 * (g & 1) + (g >> 1);
-            if constexpr (G::kWide) {
-                const float4 *src = reinterpret_cast<const float4 *>(page + krow * D * 4) + t;
+            for (int mt = 0; mt < kMT; ++mt)
 #pragma unroll
-                for (int c = 0; c < D / 16; ++c) {
-                    const float4 w = src[4 * c];
-                    const float y[4] = {w.x, w.y, w.z, w.w};
+                for (int j = 0; j < 2 * kC; ++j) {
+                    sc[mt][j][0] = sc[mt][j][1] = start[mt][0];
+                    sc[mt][j][2] = sc[mt][j][3] = start[mt][1];
+                }
+        };
+        // fp32: a value of a key that is there and finite, else zero
+        const auto sane = [&](float v, int key) { return key0 + key < keys ? finite_or_zero(v) : 0.f; };
+        // fp32: largest magnitude (bits) among the K or V rows of the chunk
+        const auto top_of = [&](const uint8_t *part) {
+            uint32_t top = 0;
+#pragma unroll 8
+            for (int i = lane; i < kKvPage * D / 4; i += 32) {
+                const float4 w = reinterpret_cast<const float4 *>(part)[i];
+                const float y[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-                    for (int e = 0; e < 2; ++e)
+                for (int e = 0; e < 4; ++e)
+                    top = max(top, __float_as_uint(kEdge ? sane(y[e], i / (D / 4)) : y[e]) & 0x7fffffffu);
+            }
+            return __reduce_max_sync(kFullWarpMask, top);
+        };
+
+        if constexpr (G::kWide) {
+            if (kEdge) {
+                // rows that are not finite: lanes 4 key .. of a ballot hold a key's eighths
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int part = 0; part < 2; ++part) {
+                        const float4 *src = reinterpret_cast<const float4 *>(chunk + (part * kKvPage + 4 * i + t) * D * 4) + g;
+                        bool odd = false;
+#pragma unroll
+                        for (int c = 0; c < D / 32; ++c) {
+                            const float4 w = src[8 * c];
+                            odd |= !(fabsf(w.x) <= 3.4028235e38f && fabsf(w.y) <= 3.4028235e38f &&
+                                     fabsf(w.z) <= 3.4028235e38f && fabsf(w.w) <= 3.4028235e38f);
+                        }
+                        bad |= ((__ballot_sync(kFullWarpMask, odd) >> t) & 0x11111111u) != 0u ? 1u << i : 0u;
+                    }
+            }
+            bool over = kmul == 0.f;
+            zero_scores();
+#pragma unroll 1
+            for (int attempt = 0; attempt < 3; ++attempt) { // again after a new kmul
+                if (__any_sync(kFullWarpMask, over)) {
+                    const uint32_t top = top_of(chunk);
+                    if (top >= 0x7f800000u) {
+                        poison();
+                        break;
+                    }
+                    kmul = pow2_field(254u - exponent_above(top) + 8u); // to 2^7 .. 2^8
+                } else if (attempt > 0) {
+                    break;
+                }
+                zero_scores();
+                __half2 seen_top = __float2half2_rn(0.f);
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    const int krow = 8 * j + 4 * (g & 1) + (g >> 1);
+                    const uint8_t *src = chunk + krow * D * 4 + 64 * t;
+#pragma unroll
+                    for (int st = 0; st < G::kSteps; ++st) {
+                        const float4 w = *reinterpret_cast<const float4 *>(src + st / 4 * 256 + st % 4 * 16);
+                        float y[4] = {w.x, w.y, w.z, w.w};
+                        if (kEdge)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e)
+                                y[e] = sane(y[e], krow);
+                        uint32_t h0, h1, l0, l1;
+                        split_half2(y[0], y[1], kmul, h0, l0, seen_top);
+                        split_half2(y[2], y[3], kmul, h1, l1, seen_top);
 #pragma unroll
                         for (int mt = 0; mt < kMT; ++mt) {
-                            mma_tf32(sc[mt][j], qf[mt][2 * c + e], tf32_hi(y[2 * e]), tf32_hi(y[2 * e + 1]));
-                            mma_tf32(sc[mt][j], qf[mt][2 * c + e], tf32_lo(y[2 * e]), tf32_lo(y[2 * e + 1]));
+                            mma_f16(sc[mt][j], qf[mt][st], h0, h1);
+                            mma_f16(sc[mt][j], qf[mt][st], l0, l1);
                         }
+                    }
                 }
-            } else {
+                over = over_half2(seen_top);
+            }
+        } else {
+            zero_scores();
+#pragma unroll
+            for (int j = 0; j < 2 * kC; ++j) {
+                const uint8_t *src = chunk + j / 2 * G::kPageBytes + (8 * (j % 2) + 4 * (g & 1) + (g >> 1)) * D + 16 * t;
 #pragma unroll
                 for (int c = 0; c < D / 64; ++c) {
-                    const uint4 w4 = *reinterpret_cast<const uint4 *>(page + krow * D + 64 * c + 16 * t);
+                    const uint4 w4 = *reinterpret_cast<const uint4 *>(src + 64 * c);
                     const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         uint32_t b0, b1;
-                        codes_to_half<kFmt>(w[i], b0, b1);
+                        k_codes_to_half<kFmt>(w[i], b0, b1);
 #pragma unroll
                         for (int mt = 0; mt < kMT; ++mt)
                             mma_f16(sc[mt][j], qf[mt][4 * c + i], b0, b1);
@@ -319,60 +430,80 @@ static __global__ void __launch_bounds__(TreeRowsGeo<T, D, kFmt, kMT>::kThreads)
                 }
             }
         }
-        // scores in log2 units, masked ones -inf; V factors
-        float kscale[4], vfac[4];
+        // factors of the scores, and the largest V scale of the lane
+        float vscale = 0.f;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            kscale[i] = G::kWide ? 1.f : *reinterpret_cast<const float *>(page + R::kKScale + 16 * i + 4 * t);
-            vfac[i] = G::kWide ? 1.f : *reinterpret_cast<const float *>(page + R::kVScale + 16 * i + 4 * t);
+        for (int i = 0; i < 4 * kC; ++i) {
+            if constexpr (G::kWide) {
+                kfac[i] = pow2_field(254u - (__float_as_uint(kmul) >> 23));
+                vfac[i] = 1.f;
+            } else {
+                const uint8_t *page = chunk + i / 4 * G::kPageBytes + 16 * (i % 4) + 4 * t;
+                kfac[i] = *reinterpret_cast<const float *>(page + R::kKScale);
+                vfac[i] = *reinterpret_cast<const float *>(page + R::kVScale);
+                float usable = vfac[i];
+                if (kEdge) { // masked rows may have any scale; places after the last key have none
+                    if (key0 + 4 * i + t >= keys)
+                        vfac[i] = 0.f;
+                    usable = finite_or_zero(vfac[i]);
+                }
+                vscale = fmaxf(vscale, usable);
+            }
         }
-        float x[kMT][G::kRPL][4];
-        bool raise = false;
+        // scores less their row's scale, masked ones -inf
+        bool raise = vscale > vtop;
+        const float slack = G::kWide ? kLazy + kLift : kLazy + kLift - vlog;
 #pragma unroll
         for (int mt = 0; mt < kMT; ++mt)
 #pragma unroll
             for (int rr = 0; rr < G::kRPL; ++rr) {
-                uint32_t seen = 0xffffu;
-                if (edge) {
+#pragma unroll
+                for (int i = 0; i < 4 * kC; ++i) {
+                    const float *c = sc[mt][i >> 1];
+                    x[mt][rr][i] = (G::kTwo ? c[i & 1] + c[2 + (i & 1)] : c[2 * rr + (i & 1)]) * kfac[i];
+                }
+                if (kEdge) {
                     const int r = row_base + mt * G::kTileRows + rr * 8 + g;
-                    seen = r < rows ? tree_sees16(a.t, span.row0 + r / rep, r / rep, key0 - span.ctx, keys - span.ctx) : 0u;
+                    uint32_t seen = 0;
+                    if (r < rows)
+#pragma unroll
+                        for (int pg = 0; pg < kC; ++pg)
+                            seen |= tree_sees16(a.t, span.row0 + r / rep, r / rep, key0 + pg * kKvPage - span.ctx, keys - span.ctx) << (16 * pg);
+#pragma unroll
+                    for (int i = 0; i < 4 * kC; ++i) {
+                        if (G::kWide && (bad >> i & 1u))
+                            x[mt][rr][i] = __uint_as_float(0x7fc00000u);
+                        if (!(seen >> (4 * i + t) & 1u))
+                            x[mt][rr][i] = kNegInf;
+                    }
                 }
                 float top = kNegInf;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float *c = sc[mt][i >> 1];
-                    float v = G::kTwo ? c[i & 1] + c[2 + (i & 1)] : c[2 * rr + (i & 1)];
-                    v *= row_scale[mt][rr] * kscale[i];
-                    if (edge && !((seen >> (4 * i + t)) & 1u))
-                        v = kNegInf;
-                    x[mt][rr][i] = v;
-                    top = fmaxf(top, v);
-                }
-                raise |= top > m[mt][rr] + kLazy;
+                for (int i = 0; i < 4 * kC; ++i)
+                    top = fmaxf(top, x[mt][rr][i]);
+                raise |= top * row_scale[mt][rr] > m[mt][rr] + slack;
             }
-        if constexpr (!G::kWide) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                if (edge && (key0 + 4 * i + t >= keys))
-                    vfac[i] = 0.f;
-                raise |= vfac[i] > vtop && vfac[i] < 3e38f;
-            }
-        }
         if (__any_sync(kFullWarpMask, raise)) {
-            float vfix = 1.f;
-            if constexpr (!G::kWide) {
-                float top = 0.f;
+            const uint32_t top = __reduce_max_sync(kFullWarpMask, __float_as_uint(vscale)); // not below zero
+            if (!G::kWide && __uint_as_float(top) > vtop) {
+                if (top >= 0x7f800000u) {
+                    poison();
+                } else {
+                    const uint32_t ex = exponent_above(top);
+                    const float log = static_cast<float>(static_cast<int>(ex) - 127), up = log - vlog;
+                    vtop = pow2_field(ex);
+                    vlog = log;
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    top = vfac[i] < 3e38f ? fmaxf(top, vfac[i]) : top;
-                top = fmaxf(top, __shfl_xor_sync(kFullWarpMask, top, 1));
-                top = fmaxf(top, __shfl_xor_sync(kFullWarpMask, top, 2));
-                if (top > vtop) { // the same in every lane of the warp
-                    // next power of two, held where its inverse is a normal number too
-                    const uint32_t ex = min(max((__float_as_uint(top) >> 23) + 1u, 4u), 250u);
-                    vfix = vtop * __uint_as_float((254u - ex) << 23);
-                    vtop = __uint_as_float(ex << 23);
-                    vinv = __uint_as_float((254u - ex) << 23);
+                    for (int mt = 0; mt < kMT; ++mt) {
+                        float fix[G::kRPL];
+#pragma unroll
+                        for (int rr = 0; rr < G::kRPL; ++rr) {
+                            fix[rr] = exp2_approx(-up);
+                            m[mt][rr] += up;
+                            l[mt][rr] *= fix[rr];
+                        }
+                        rescale(mt, fix);
+                    }
                 }
             }
 #pragma unroll
@@ -380,154 +511,172 @@ static __global__ void __launch_bounds__(TreeRowsGeo<T, D, kFmt, kMT>::kThreads)
                 float fix[G::kRPL];
 #pragma unroll
                 for (int rr = 0; rr < G::kRPL; ++rr) {
-                    float top = fmaxf(fmaxf(x[mt][rr][0], x[mt][rr][1]), fmaxf(x[mt][rr][2], x[mt][rr][3]));
-                    top = fmaxf(top, __shfl_xor_sync(kFullWarpMask, top, 1));
-                    top = fmaxf(top, __shfl_xor_sync(kFullWarpMask, top, 2));
-                    const float up = fmaxf(m[mt][rr], top);
+                    float up = kNegInf;
+#pragma unroll
+                    for (int i = 0; i < 4 * kC; ++i)
+                        up = fmaxf(up, x[mt][rr][i]);
+                    up = fmaxf(up, __shfl_xor_sync(kFullWarpMask, up, 1));
+                    up = fmaxf(up, __shfl_xor_sync(kFullWarpMask, up, 2));
+                    up = fmaxf(m[mt][rr], up * row_scale[mt][rr] + (G::kWide ? -kLift : vlog - kLift));
                     fix[rr] = exp2_approx(m[mt][rr] - up);
                     m[mt][rr] = up;
                     l[mt][rr] *= fix[rr];
-                    fix[rr] *= vfix;
                 }
-#pragma unroll
-                for (int n = 0; n < D / 8; ++n) {
-                    o[mt][n][0] *= fix[0];
-                    o[mt][n][1] *= fix[0];
-                    o[mt][n][2] *= fix[G::kRPL - 1];
-                    o[mt][n][3] *= fix[G::kRPL - 1];
-                }
-            }
-        }
-        // A V row with an infinity or a NaN must not reach the rows that do not
-        // see it (zero times either is NaN). Only nodes are seen by some rows
-        // and not by others, so on edge pages such values count as zero below
-        // and the rows that do see them turn NaN here.
-        uint32_t bad = 0;
-        if (G::kWide && edge) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                bool odd = false;
-                const float4 *v = reinterpret_cast<const float4 *>(page + kKvPage * D * 4 + (4 * i + t) * D * 4) + g;
-#pragma unroll
-                for (int c = 0; c < D / 32; ++c)
-                    odd |= !(finite_or_zero(v[8 * c].x) == v[8 * c].x && finite_or_zero(v[8 * c].y) == v[8 * c].y &&
-                             finite_or_zero(v[8 * c].z) == v[8 * c].z && finite_or_zero(v[8 * c].w) == v[8 * c].w);
-                bad |= ((__ballot_sync(kFullWarpMask, odd) >> t) & 0x11111111u) != 0u ? 1u << i : 0u;
+                rescale(mt, fix);
             }
         }
         // P as A fragments; l sums the weights before they are rounded
-        uint32_t pf[kMT][G::kWide ? 2 : 1][4];
+        uint32_t pf[kMT][kC][4];
 #pragma unroll
         for (int mt = 0; mt < kMT; ++mt) {
-            float p[G::kRPL][4];
+            float p[G::kRPL][4 * kC];
 #pragma unroll
             for (int rr = 0; rr < G::kRPL; ++rr)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    p[rr][i] = exp2_approx(x[mt][rr][i] - m[mt][rr] + kLift);
-                    l[mt][rr] += p[rr][i];
-                    if (G::kWide && edge && (bad >> i & 1u) && x[mt][rr][i] != kNegInf)
-                        l[mt][rr] = __uint_as_float(0x7fc00000u);
-                    if constexpr (!G::kWide) {
-                        const float w = p[rr][i] * (vfac[i] * vinv);
-                        p[rr][i] = x[mt][rr][i] == kNegInf ? 0.f : w;
-                    }
+                for (int i = 0; i < 4 * kC; ++i) {
+                    float w = exp2_approx(fmaf(x[mt][rr][i], row_scale[mt][rr], -m[mt][rr]));
+                    const bool masked = kEdge && x[mt][rr][i] == kNegInf; // no weight, whatever the row's scales
+                    if (masked)
+                        w = 0.f;
+                    l[mt][rr] += w;
+                    p[rr][i] = G::kWide || masked ? w : w * vfac[i];
                 }
-            if constexpr (G::kWide) {
 #pragma unroll
-                for (int j = 0; j < 2; ++j)
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        const float v = p[0][2 * j + e];
-                        if constexpr (G::kTwo) {
-                            pf[mt][j][2 * e] = tf32_hi(v);
-                            pf[mt][j][2 * e + 1] = tf32_lo(v);
-                        } else {
-                            pf[mt][j][2 * e] = tf32_rna(v);
-                            pf[mt][j][2 * e + 1] = tf32_rna(p[G::kRPL - 1][2 * j + e]);
-                        }
-                    }
-            } else {
-#pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    const uint32_t hi = half2_rn(p[0][2 * j], p[0][2 * j + 1]);
-                    pf[mt][0][2 * j] = hi;
-                    if constexpr (G::kTwo) {
-                        const float2 f = half2_floats(hi);
-                        pf[mt][0][2 * j + 1] = half2_rn(p[0][2 * j] - f.x, p[0][2 * j + 1] - f.y);
-                    } else {
-                        pf[mt][0][2 * j + 1] = half2_rn(p[G::kRPL - 1][2 * j], p[G::kRPL - 1][2 * j + 1]);
-                    }
+            for (int i = 0; i < 2 * kC; ++i) {
+                const uint32_t hi = half2_rn(p[0][2 * i], p[0][2 * i + 1]);
+                pf[mt][i >> 1][2 * (i & 1)] = hi;
+                if constexpr (G::kTwo) {
+                    const float2 f = half2_floats(hi);
+                    pf[mt][i >> 1][2 * (i & 1) + 1] = half2_rn(p[0][2 * i] - f.x, p[0][2 * i + 1] - f.y);
+                } else {
+                    pf[mt][i >> 1][2 * (i & 1) + 1] = half2_rn(p[G::kRPL - 1][2 * i], p[G::kRPL - 1][2 * i + 1]);
                 }
             }
         }
         // O += P V. 8-bit: column g of n tile n is dim (D / 8) g + n. fp32:
         // column g of n tile 4c + e is dim 32c + 4g + e.
         if constexpr (G::kWide) {
-            const uint8_t *v = page + kKvPage * D * 4;
 #pragma unroll
-            for (int j = 0; j < 2; ++j)
-#pragma unroll
-                for (int c = 0; c < D / 32; ++c) {
-                    float4 u = *reinterpret_cast<const float4 *>(v + (8 * j + t) * D * 4 + 128 * c + 16 * g);
-                    float4 w = *reinterpret_cast<const float4 *>(v + (8 * j + 4 + t) * D * 4 + 128 * c + 16 * g);
-                    float ue[4] = {u.x, u.y, u.z, u.w}, we[4] = {w.x, w.y, w.z, w.w};
-                    if (edge)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            ue[e] = finite_or_zero(ue[e]);
-                            we[e] = finite_or_zero(we[e]);
+            for (int c = 0; c < D / 32; ++c) {
+                uint32_t hi[4][2], lo[4][2]; // of dims 32c + 4g + e, keys (t, 4 + t) and (8 + t, 12 + t)
+                bool over = c == 0 && vmul == 0.f;
+#pragma unroll 1
+                for (int attempt = 0; attempt < 3; ++attempt) {
+                    if (__any_sync(kFullWarpMask, over)) {
+                        const uint32_t top = top_of(chunk + kKvPage * D * 4);
+                        if (top >= 0x7f800000u) {
+                            poison();
+                            break;
                         }
+                        const float next = pow2_field(254u - exponent_above(top) + 8u); // to 2^7 .. 2^8
+                        const float up = vmul == 0.f ? 0.f : next * pow2_field(254u - (__float_as_uint(vmul) >> 23));
+#pragma unroll
+                        for (int mt = 0; mt < kMT; ++mt) {
+                            float fix[G::kRPL];
+#pragma unroll
+                            for (int rr = 0; rr < G::kRPL; ++rr)
+                                fix[rr] = up;
+                            rescale(mt, fix);
+                        }
+                        vmul = next;
+                    } else if (attempt > 0) {
+                        break;
+                    }
+                    float y[4][4]; // value i's key, dim e
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const float4 w = *reinterpret_cast<const float4 *>(chunk + (kKvPage + 4 * i + t) * D * 4 + 128 * c + 16 * g);
+                        y[i][0] = w.x, y[i][1] = w.y, y[i][2] = w.z, y[i][3] = w.w;
+                        if (kEdge)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e)
+                                y[i][e] = sane(y[i][e], 4 * i + t);
+                    }
+                    __half2 seen_top = __float2half2_rn(0.f);
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
 #pragma unroll
-                        for (int mt = 0; mt < kMT; ++mt) {
+                        for (int j = 0; j < 2; ++j) {
                             if constexpr (G::kTwo) {
-                                mma_tf32(o[mt][4 * c + e], pf[mt][j], tf32_hi(ue[e]), tf32_hi(we[e]));
-                                mma_tf32(o[mt][4 * c + e], pf[mt][j], tf32_lo(ue[e]), tf32_lo(we[e]));
+                                split_half2(y[2 * j][e], y[2 * j + 1][e], vmul, hi[e][j], lo[e][j], seen_top);
                             } else {
-                                mma_tf32(o[mt][4 * c + e], pf[mt][j], tf32_rna(ue[e]), tf32_rna(we[e]));
+                                hi[e][j] = half2_rn(y[2 * j][e] * vmul, y[2 * j + 1][e] * vmul);
+                                seen_top = __hmax2_nan(seen_top, __habs2(*reinterpret_cast<const __half2 *>(&hi[e][j])));
                             }
                         }
+                    over = over_half2(seen_top);
                 }
-        } else {
-            constexpr int kWords = D / 32;
-            uint32_t w[4][kWords];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const uint8_t *src = page + R::kCodes + (4 * i + t) * D + (D / 8) * g;
-                if constexpr (kWords == 2) {
-                    const uint2 u = *reinterpret_cast<const uint2 *>(src);
-                    w[i][0] = u.x, w[i][1] = u.y;
-                } else {
-                    const uint4 u = *reinterpret_cast<const uint4 *>(src);
-                    w[i][0] = u.x, w[i][1] = u.y, w[i][kWords - 2] = u.z, w[i][kWords - 1] = u.w;
-                }
-                if (kFmt == KvFormat::kE4M3 && edge)
-#pragma unroll
-                    for (int c = 0; c < kWords; ++c)
-                        w[i][c] = clear_e4m3_nan(w[i][c]);
-            }
-#pragma unroll
-            for (int c = 0; c < kWords; ++c) {
-                uint32_t b0[4], b1[4]; // keys (t, 4 + t) and (8 + t, 12 + t) of dims 4c .. 4c + 3
-                codes_to_half<kFmt>(__byte_perm(w[0][c], w[1][c], 0x5140), b0[0], b0[1]);
-                codes_to_half<kFmt>(__byte_perm(w[0][c], w[1][c], 0x7362), b0[2], b0[3]);
-                codes_to_half<kFmt>(__byte_perm(w[2][c], w[3][c], 0x5140), b1[0], b1[1]);
-                codes_to_half<kFmt>(__byte_perm(w[2][c], w[3][c], 0x7362), b1[2], b1[3]);
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
 #pragma unroll
-                    for (int mt = 0; mt < kMT; ++mt)
-                        mma_f16(o[mt][4 * c + e], pf[mt][0], b0[e], b1[e]);
+                    for (int mt = 0; mt < kMT; ++mt) {
+                        mma_f16(o[mt][4 * c + e], pf[mt][0], hi[e][0], hi[e][1]);
+                        if constexpr (G::kTwo)
+                            mma_f16(o[mt][4 * c + e], pf[mt][0], lo[e][0], lo[e][1]);
+                    }
+            }
+        } else {
+#pragma unroll
+            for (int pg = 0; pg < kC; ++pg) {
+                constexpr int kWords = D / 32;
+                uint32_t w[4][kWords];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const uint8_t *src = chunk + pg * G::kPageBytes + R::kCodes + (4 * i + t) * D + (D / 8) * g;
+                    if constexpr (kWords == 2) {
+                        const uint2 u = *reinterpret_cast<const uint2 *>(src);
+                        w[i][0] = u.x, w[i][1] = u.y;
+                    } else {
+                        const uint4 u = *reinterpret_cast<const uint4 *>(src);
+                        w[i][0] = u.x, w[i][1] = u.y, w[i][kWords - 2] = u.z, w[i][kWords - 1] = u.w;
+                    }
+                    if (kFmt == KvFormat::kE4M3 && kEdge)
+#pragma unroll
+                        for (int c = 0; c < kWords; ++c)
+                            w[i][c] = clear_e4m3_nan(w[i][c]);
+                }
+#pragma unroll
+                for (int c = 0; c < kWords; ++c) {
+                    uint32_t b0[4], b1[4]; // keys (t, 4 + t) and (8 + t, 12 + t) of dims 4c .. 4c + 3
+                    codes_to_half<kFmt>(__byte_perm(w[0][c], w[1][c], 0x5140), b0[0], b0[1]);
+                    codes_to_half<kFmt>(__byte_perm(w[0][c], w[1][c], 0x7362), b0[2], b0[3]);
+                    codes_to_half<kFmt>(__byte_perm(w[2][c], w[3][c], 0x5140), b1[0], b1[1]);
+                    codes_to_half<kFmt>(__byte_perm(w[2][c], w[3][c], 0x7362), b1[2], b1[3]);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+#pragma unroll
+                        for (int mt = 0; mt < kMT; ++mt)
+                            mma_f16(o[mt][4 * c + e], pf[mt][pg], b0[e], b1[e]);
+                }
             }
         }
+    };
+
+    bool ok = true;
+    int done = 0, stage = 0;
+    uint32_t parity = 0;
+    for (; done < mine; ++done) {
+        if (!sm100::mbar_wait_warp(&bar[stage], parity)) {
+            ok = false;
+            break;
+        }
+        const uint8_t *chunk = ring + stage * G::kChunkBytes;
+        const int key0 = (first + done * step) * kC * kKvPage;
+        if (key0 + kC * kKvPage > span.ctx)
+            take(chunk, key0, std::true_type{});
+        else
+            take(chunk, key0, std::false_type{});
         __syncwarp(); // every lane has read the stage
         const int next = done + G::kStages;
-        if ((next & 31) == 0 && next < mine)
-            refill(next);
-        if (next < mine)
-            issue(next);
+        if (next < mine) {
+            if (next % (32 / kC) == 0)
+                refill(next);
+            issue(next, stage);
+        }
+        if (++stage == G::kStages) {
+            stage = 0;
+            parity ^= 1u;
+        }
     }
     // a wait that ran out: the copies still in flight must land before the ring is used again
     if (!ok)
@@ -538,6 +687,7 @@ static __global__ void __launch_bounds__(TreeRowsGeo<T, D, kFmt, kMT>::kThreads)
 
     // the warps' results over the ring, joined in warp order
     float *part = reinterpret_cast<float *>(smem);
+    const float vunit = G::kWide && vmul != 0.f ? pow2_field(254u - (__float_as_uint(vmul) >> 23)) : 1.f;
 #pragma unroll
     for (int mt = 0; mt < kMT; ++mt)
 #pragma unroll
@@ -547,14 +697,13 @@ static __global__ void __launch_bounds__(TreeRowsGeo<T, D, kFmt, kMT>::kThreads)
             sum += __shfl_xor_sync(kFullWarpMask, sum, 1);
             sum += __shfl_xor_sync(kFullWarpMask, sum, 2);
             float *dst = part + (warp * G::kRows + r) * G::kPitch;
-            const float unit_v = G::kWide ? 1.f : vtop;
 #pragma unroll
             for (int n = 0; n < D / 8; ++n)
 #pragma unroll
                 for (int col = 0; col < 2; ++col) {
                     const float v = G::kTwo ? o[mt][n][col] + o[mt][n][2 + col] : o[mt][n][2 * rr + col];
                     const int d = G::kWide ? 32 * (n / 4) + 4 * (2 * t + col) + n % 4 : (D / 8) * (2 * t + col) + n;
-                    dst[d] = v * unit_v;
+                    dst[d] = v * vunit;
                 }
             if (t == 0) {
                 stat[warp * G::kRows + r] = m[mt][rr];
@@ -622,10 +771,15 @@ inline void tree_rows_launch(const T *q, T *out, const TreeArgs &a, cudaStream_t
     const int64_t groups = (rows + G::kRows - 1) / G::kRows;
     const int64_t units = groups * a.kvh;
     const int64_t pages = (static_cast<int64_t>(a.t.max_ctx) + a.t.max_rows + kKvPage - 1) / kKvPage;
-    // splits until two CTAs per SM are filled, while each warp still has two pages
+    // Splits while all CTAs still run at once and a warp keeps a chunk: a CTA
+    // has about 5 us of latencies to pay for (lengths, table, first copies,
+    // joining), so a second wave costs more than it evens out (32 sequences of
+    // 2180 tokens, 8 kv heads: 19.3 us with 1 split, 25.6 with 2, 33.7 with 4).
+    // 16 CTAs to a cluster only where each warp has much to do.
+    const int64_t slots = static_cast<int64_t>(G::kCtas) * device_facts().sm_count;
+    const int64_t per_warp = pages / (G::kWarps * G::kChunk);
     int splits = 1;
-    while (splits < 8 && units * a.t.batch * splits * 2 <= 2 * device_facts().sm_count &&
-           pages >= static_cast<int64_t>(splits) * 2 * G::kWarps * 2)
+    while (splits < 16 && units * a.t.batch * splits * 2 <= slots && per_warp >= (splits < 8 ? splits : 64))
         splits *= 2;
     require(units * splits <= 0x7fffffff, "tree attention: too many rows for one call");
     launch_ex_cluster(kernel, dim3(static_cast<unsigned>(units * splits), a.t.batch), dim3(splits), dim3(G::kThreads),
