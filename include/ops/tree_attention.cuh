@@ -17,6 +17,7 @@
 
 #include "tree_attention_common.cuh"
 #include "tree_attention_rows.cuh"
+#include "tree_attention_tiles.cuh"
 
 namespace opworks {
 namespace detail {
@@ -44,13 +45,38 @@ inline void validate_tree(const TreeBatch &t, const void *q, const void *out, in
 template <typename T, int D, KvFormat kFmt>
 inline void tree_attention_launch(const T *q, T *out, const TreeArgs &a, cudaStream_t stream) {
     constexpr int kTile = TreeRowsGeo<T, D, kFmt, 1>::kRows;
-    const int64_t tiles = (static_cast<int64_t>(a.t.max_rows) * (a.qh / a.kvh) + kTile - 1) / kTile;
-    if (tiles == 1)
+    const int64_t rows = static_cast<int64_t>(a.t.max_rows) * (a.qh / a.kvh), tiles = (rows + kTile - 1) / kTile;
+    // The rows kernel's time grows with the rows, that of 128-row tiles does not:
+    // 8 sequences of 4096 tokens, 8 kv heads, us with rows / with tiles
+    //   fp32 rows, 8-bit, D 64    32 rows 44 / 51   64: 55 / 53   128: 90 / 58
+    //   fp32 rows, 8-bit, D 128   64 rows 82 / 98   128: 136 / 106 (e4m3 121 / 115)
+    //   fp32 rows, fp32, D 64     16 rows 39 / 69   32: 81 / 70   128: 197 / 76
+    //   bf16 rows, 8-bit, D 64    32 rows 22 / 37   64: 56 / 39   128: 67 / 45
+    //   bf16 rows, 8-bit, D 128   32 rows 53 / 45   64: 76 / 49   128: 117 / 57
+    // (ragged trees of up to 26 nodes x 4 heads, fp32, e4m3: 54 / 58). fp32 rows of
+    // 128 dims over 8-bit pools stay with rows: their operands as two terms each
+    // leave shared memory for one stage of tiles, and more rounding in the sums.
+    constexpr bool kBf16 = std::is_same_v<T, __nv_bfloat16>, kWide = kFmt == KvFormat::kF32;
+    constexpr bool kHasTiles = kBf16 || kWide || D == 64;
+    constexpr int kFrom = kBf16 ? 32 : kWide ? 24 : 104;
+    if constexpr (kHasTiles) {
+        if (rows > kFrom) {
+            // two row tiles to a CTA where shared memory holds both
+            constexpr int kPair = D == 64 || (!kWide && kBf16) ? 2 : 1;
+            if (rows <= 128 || kPair == 1)
+                tree_tiles_launch<T, D, kFmt, 1>(q, out, a, stream);
+            else
+                tree_tiles_launch<T, D, kFmt, kPair>(q, out, a, stream);
+            return;
+        }
+    }
+    if (tiles == 1) {
         tree_rows_launch<T, D, kFmt, 1>(q, out, a, stream);
-    else if (D == 128 || tiles == 2)
+    } else if (D == 128 || tiles == 2) {
         tree_rows_launch<T, D, kFmt, 2>(q, out, a, stream);
-    else
+    } else { // more tiles to a CTA: K and V are widened once for all of them
         tree_rows_launch<T, D, kFmt, D == 64 ? 3 : 2>(q, out, a, stream);
+    }
 }
 
 template <typename T>

@@ -7,6 +7,7 @@
 #include <algorithm>
 #include <cstdint>
 #include <cuda_bf16.h>
+#include <cuda_fp16.h>
 #include <mutex>
 #include <utility>
 #include <vector>
@@ -71,13 +72,39 @@ struct TreeSpan {
     }
 };
 
-// Bit i: node `node` (row `row` of the mask) sees the key j0 + i, i < 16, where
-// keys below 0 are context and there are none from `limit` on. j0 > -32.
-__device__ __forceinline__ uint32_t tree_sees16(const TreeBatch &t, int row, int node, int j0, int limit) {
-    uint32_t bits;
+// The sequence with the `order`-th most work (the longest context, equal ones by
+// index), so that CTAs that wait for a place come longest first: what is left
+// over at the end is short. Every thread of the block calls it; `room` is shared
+// memory for batch + 1 ints, batch <= the block's threads.
+__device__ __forceinline__ int sequence_by_work(const TreeBatch &t, int order, int *room) {
+    const int tid = threadIdx.x;
+    if (tid < t.batch) {
+        const int n = t.row_start[tid + 1] - t.row_start[tid];
+        room[1 + tid] = n > 0 ? t.ctx_lens[tid] : -1;
+    }
+    __syncthreads();
+    if (tid < t.batch) {
+        const int mine = room[1 + tid];
+        int before = 0;
+        for (int i = 0; i < t.batch; ++i)
+            before += room[1 + i] > mine || (room[1 + i] == mine && i < tid) ? 1 : 0;
+        if (before == order)
+            room[0] = tid;
+    }
+    __syncthreads();
+    const int b = room[0];
+    __syncthreads();
+    return b;
+}
+
+// Bit i: node `node` (row `row` of the mask) sees the key j0 + i, i < 32, where
+// keys below 0 are context and there are none from `limit` (>= 0) on.
+__device__ __forceinline__ uint32_t tree_sees32(const TreeBatch &t, int row, int node, int j0, int limit) {
+    uint32_t bits = ~0u;
+    if (j0 <= -32)
+        return bits;
     if (t.mask == nullptr) {
         limit = min(limit, node + 1);
-        bits = 0xffffu;
     } else {
         const uint32_t *w = t.mask + static_cast<int64_t>(row) * t.mask_words;
         if (j0 < 0) {
@@ -89,7 +116,56 @@ __device__ __forceinline__ uint32_t tree_sees16(const TreeBatch &t, int row, int
         }
     }
     const int left = limit - j0;
-    return left >= 16 ? bits & 0xffffu : left <= 0 ? 0u : bits & ((1u << left) - 1u);
+    return left >= 32 ? bits : left <= 0 ? 0u : bits & ((1u << left) - 1u);
+}
+
+constexpr float kLazy = 4.f;  // log2 units a score may pass the reference maximum by
+constexpr float kLift = 10.f; // P is scaled by 2^kLift: at most 2^14
+// V scales below this are not told apart from it (fp16 loses their low bits);
+// lower, and l in their units would leave fp32's range
+constexpr float kMinVLog = -80.f, kMinVTop = 0x1p-80f;
+
+// fp16 pair (a, b) as one register, a in the low half
+__device__ __forceinline__ uint32_t half2_rn(float a, float b) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+__device__ __forceinline__ float2 half2_floats(uint32_t h) {
+    return __half22float2(*reinterpret_cast<const __half2 *>(&h));
+}
+
+// Two pairs of fp16 from the four codes of a word: (0, 1) and (2, 3). Exact.
+template <KvFormat kFmt> __device__ __forceinline__ void codes_to_half(uint32_t w, uint32_t &lo, uint32_t &hi) {
+    if constexpr (kFmt == KvFormat::kInt8) {
+        // byte + 128 in the low bits of fp16 1024 .. 1279, minus 1152
+        const uint32_t u = w ^ 0x80808080u;
+        const uint32_t bias = 0x64806480u; // fp16 1152, twice
+        const uint32_t a = __byte_perm(u, 0x64646464u, 0x4140), b = __byte_perm(u, 0x64646464u, 0x4342);
+        const __half2 x = __hsub2(*reinterpret_cast<const __half2 *>(&a), *reinterpret_cast<const __half2 *>(&bias));
+        const __half2 y = __hsub2(*reinterpret_cast<const __half2 *>(&b), *reinterpret_cast<const __half2 *>(&bias));
+        lo = *reinterpret_cast<const uint32_t *>(&x);
+        hi = *reinterpret_cast<const uint32_t *>(&y);
+    } else {
+        asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\t"
+            "cvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}"
+            : "=r"(lo), "=r"(hi)
+            : "r"(w));
+    }
+}
+
+__device__ __forceinline__ float finite_or_zero(float x) { return fabsf(x) <= 3.4028235e38f ? x : 0.f; }
+
+// The power of two next above magnitude `top` (bits of it) as an exponent
+// field, held where its inverse and its products with 2^10 are normal too.
+__device__ __forceinline__ uint32_t exponent_above(uint32_t top_bits) {
+    return min(max((top_bits >> 23) + 1u, 16u), 240u);
+}
+__device__ __forceinline__ float pow2_field(uint32_t ex) { return __uint_as_float(ex << 23); }
+
+// e4m3 NaN codes (never written by ops::kv_quant_write) replaced by zero: a
+// masked row may hold them, and zero times NaN is NaN.
+__device__ __forceinline__ uint32_t clear_e4m3_nan(uint32_t w) {
+    return w & ~__vcmpeq4(w & 0x7f7f7f7fu, 0x7f7f7f7fu);
 }
 
 __device__ __forceinline__ void cluster_sync_all() {

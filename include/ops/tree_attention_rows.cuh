@@ -39,17 +39,9 @@
 // are folded into P, relative to a running power of two that counts as part of
 // the reference (l and O carry it both).
 
-#include <cuda_fp16.h>
-
 #include "tree_attention_common.cuh"
 
 namespace opworks::detail {
-
-constexpr float kLazy = 4.f;  // log2 units a score may pass the reference maximum by
-constexpr float kLift = 10.f; // P is scaled by 2^kLift: at most 2^14
-// V scales below this are not told apart from it (fp16 loses their low bits);
-// lower, and l in their units would leave fp32's range
-constexpr float kMinVLog = -80.f, kMinVTop = 0x1p-80f;
 
 template <typename T, int D, KvFormat kFmt, int kMT> struct TreeRowsGeo {
     static constexpr bool kTwo = std::is_same_v<T, float>; // two terms of Q and P
@@ -80,34 +72,6 @@ __device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], u
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-// fp16 pair (a, b) as one register, a in the low half
-__device__ __forceinline__ uint32_t half2_rn(float a, float b) {
-    const __half2 h = __floats2half2_rn(a, b);
-    return *reinterpret_cast<const uint32_t *>(&h);
-}
-__device__ __forceinline__ float2 half2_floats(uint32_t h) {
-    return __half22float2(*reinterpret_cast<const __half2 *>(&h));
-}
-
-// Two pairs of fp16 from the four codes of a word: (0, 1) and (2, 3). Exact.
-template <KvFormat kFmt> __device__ __forceinline__ void codes_to_half(uint32_t w, uint32_t &lo, uint32_t &hi) {
-    if constexpr (kFmt == KvFormat::kInt8) {
-        // byte + 128 in the low bits of fp16 1024 .. 1279, minus 1152
-        const uint32_t u = w ^ 0x80808080u;
-        const uint32_t bias = 0x64806480u; // fp16 1152, twice
-        const uint32_t a = __byte_perm(u, 0x64646464u, 0x4140), b = __byte_perm(u, 0x64646464u, 0x4342);
-        const __half2 x = __hsub2(*reinterpret_cast<const __half2 *>(&a), *reinterpret_cast<const __half2 *>(&bias));
-        const __half2 y = __hsub2(*reinterpret_cast<const __half2 *>(&b), *reinterpret_cast<const __half2 *>(&bias));
-        lo = *reinterpret_cast<const uint32_t *>(&x);
-        hi = *reinterpret_cast<const uint32_t *>(&y);
-    } else {
-        asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\t"
-            "cvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}"
-            : "=r"(lo), "=r"(hi)
-            : "r"(w));
-    }
-}
-
 // int8 codes as K operands: fp16 subnormals (c + 128) 2^-24, exact too. The
 // offset is taken off by the accumulators' start, -128 sum q: two instructions
 // a pair fewer than codes_to_half. (Not for V: its sums of many keys cancel,
@@ -122,35 +86,19 @@ template <KvFormat kFmt> __device__ __forceinline__ void k_codes_to_half(uint32_
     }
 }
 
-// x f and y f as two fp16 terms each (the first cut off after 11 bits); `top`
-// keeps the largest magnitude of the first terms, NaN and infinity included.
+// x f and y f as two fp16 terms each, both rounded to nearest: 2^-24 is lost (a
+// first term cut off instead: 2^-22, which showed in the results). `top` keeps
+// the largest magnitude of the first terms, NaN and infinity included.
 __device__ __forceinline__ void split_half2(float x, float y, float f, uint32_t &hi, uint32_t &lo, __half2 &top) {
     const float2 u = __fmul2_rn(make_float2(x, y), make_float2(f, f));
-    const float2 h = make_float2(__uint_as_float(__float_as_uint(u.x) & 0xffffe000u),
-                                 __uint_as_float(__float_as_uint(u.y) & 0xffffe000u));
-    const float2 r = __fadd2_rn(u, make_float2(-h.x, -h.y));
-    hi = half2_rn(h.x, h.y);
+    hi = half2_rn(u.x, u.y);
+    const float2 h = half2_floats(hi), r = __fadd2_rn(u, make_float2(-h.x, -h.y));
     lo = half2_rn(r.x, r.y);
     top = __hmax2_nan(top, __habs2(*reinterpret_cast<const __half2 *>(&hi)));
 }
 // Whether a magnitude in `top` is over 2^14, infinite or NaN.
 __device__ __forceinline__ bool over_half2(__half2 top) {
     return !(__low2float(top) <= 16384.f && __high2float(top) <= 16384.f);
-}
-
-__device__ __forceinline__ float finite_or_zero(float x) { return fabsf(x) <= 3.4028235e38f ? x : 0.f; }
-
-// The power of two next above magnitude `top` (bits of it) as an exponent
-// field, held where its inverse and its products with 2^10 are normal too.
-__device__ __forceinline__ uint32_t exponent_above(uint32_t top_bits) {
-    return min(max((top_bits >> 23) + 1u, 16u), 240u);
-}
-__device__ __forceinline__ float pow2_field(uint32_t ex) { return __uint_as_float(ex << 23); }
-
-// e4m3 NaN codes (never written by ops::kv_quant_write) replaced by zero: a
-// masked row may hold them, and zero times NaN is NaN.
-__device__ __forceinline__ uint32_t clear_e4m3_nan(uint32_t w) {
-    return w & ~__vcmpeq4(w & 0x7f7f7f7fu, 0x7f7f7f7fu);
 }
 
 template <typename T, int D, KvFormat kFmt, int kMT>
@@ -385,6 +333,7 @@ static __global__ void __launch_bounds__(TreeRowsGeo<T, D, kFmt, kMT>::kThreads,
                     break;
                 }
                 zero_scores();
+                float small[kMT][2][4] = {}; // the small products: an accumulator is cut off at every step, to its size
                 __half2 seen_top = __float2half2_rn(0.f);
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
@@ -404,10 +353,15 @@ static __global__ void __launch_bounds__(TreeRowsGeo<T, D, kFmt, kMT>::kThreads,
 #pragma unroll
                         for (int mt = 0; mt < kMT; ++mt) {
                             mma_f16(sc[mt][j], qf[mt][st], h0, h1);
-                            mma_f16(sc[mt][j], qf[mt][st], l0, l1);
+                            mma_f16(small[mt][j], qf[mt][st], l0, l1);
                         }
                     }
                 }
+#pragma unroll
+                for (int mt = 0; mt < kMT; ++mt)
+#pragma unroll
+                    for (int n = 0; n < 8; ++n)
+                        sc[mt][n / 4][n % 4] += small[mt][n / 4][n % 4];
                 over = over_half2(seen_top);
             }
         } else {
@@ -466,9 +420,7 @@ static __global__ void __launch_bounds__(TreeRowsGeo<T, D, kFmt, kMT>::kThreads,
                     const int r = row_base + mt * G::kTileRows + rr * 8 + g;
                     uint32_t seen = 0;
                     if (r < rows)
-#pragma unroll
-                        for (int pg = 0; pg < kC; ++pg)
-                            seen |= tree_sees16(a.t, span.row0 + r / rep, r / rep, key0 + pg * kKvPage - span.ctx, keys - span.ctx) << (16 * pg);
+                        seen = tree_sees32(a.t, span.row0 + r / rep, r / rep, key0 - span.ctx, keys - span.ctx);
 #pragma unroll
                     for (int i = 0; i < 4 * kC; ++i) {
                         if (G::kWide && (bad >> i & 1u))

@@ -1,0 +1,913 @@
+#pragma once
+
+// Tree attention, kernel for many query rows per KV head (ops/tree_attention.cuh
+// has the definition of the operator): tcgen05 tiles of 128 rows x 128 keys.
+//
+// Bound: the tensor cores and, nearly level with them, the exponential unit.
+//
+// Two streams per CTA keep both busy: while the softmax of one stream's tile
+// runs, the products of the other's do. With more than 128 query rows (row =
+// node * rep + head in group) the streams are two row tiles over the same keys;
+// with at most 128 they are the even and the odd key tiles of one row tile,
+// joined at the end. Each stream has S (128 columns) and O (D columns) in tensor
+// memory and a warpgroup that owns a row per thread.
+//
+//   warps 0-7    softmax of stream 0, 1: S from tensor memory, weights P back
+//                over it as fp16 (the A operand of P V), O rescaled in place
+//                when the reference maximum is raised (rare, see kLazy)
+//   warps 8-14   widen pages from global memory, through registers, to fp16
+//                tiles in shared memory (128-byte swizzle; K as it lies is
+//                K-major, V as it lies is MN-major), one item of keys per warp,
+//                its next item already on its way
+//   warp 15      tensor memory, and one thread that issues all products
+//
+// Precision as in the rows kernel: fp32 queries and weights are two fp16 terms
+// (a product each, into the same accumulator), bf16 rows one. K and V rows are
+// widened with their scale (one term; two for fp32 rows, and for 8-bit rows too
+// where the queries are fp32: hi hi + hi lo + lo hi), but for a power of two
+// that the keys of an item share. The softmax applies that to 8, 16 or 32
+// scores at once, as an addition to the exponent. Factors of each key instead
+// would be a shared-memory broadcast per score: a wavefront each, 2,048 a tile,
+// which held the kernel (482 us against 358 without them, 32 x 64 nodes over
+// 8192 keys, D = 128).
+//
+// Splits of the keys form a cluster and are joined through distributed shared
+// memory in rank order.
+
+#include "detail/sm100.cuh"
+#include "tree_attention_common.cuh"
+
+namespace opworks::detail {
+
+constexpr int kTileKeys = 128;
+constexpr int kTileThreads = 512; // 8 softmax warps, 7 widening, 1 tensor: 4 on each scheduler, 128 registers a thread
+constexpr int kWidenWarps = 7;
+// Weights are 2^(x - m): the first tile's largest gets 2^kTileLift, and m is
+// raised when one would pass 2^kTileTop, so scores are looked at once, with no
+// pass for a maximum. V units enter the exponent down to 2^-kTileShift of the
+// largest; beyond that they multiply, or l would lose its weights.
+constexpr float kTileLift = 8.f, kTileTop = 14.f, kTileShift = 24.f;
+
+template <typename T, int D, KvFormat kFmt, int kM> struct TreeTilesGeo {
+    static constexpr bool kWide = kFmt == KvFormat::kF32;
+    static constexpr int kQT = std::is_same_v<T, float> ? 2 : 1; // terms of Q and P
+    static constexpr int kKT = kWide || kQT == 2 ? 2 : 1;        // terms of K and V
+    static constexpr int kSlabs = D / 64;                        // 64 dims: 128 bytes of fp16
+    static constexpr int kSlab = kTileKeys * 128;                // bytes
+    static constexpr int kQBytes = kQT * kSlabs * kM * kSlab;
+    static constexpr int kOperand = kKT * kSlabs * kSlab; // K or V of a tile
+    static constexpr int kStages = kKT == 2 && D == 128 ? 1 : 2;
+    // O's small products in an accumulator of their own, where tensor memory has
+    // the room: an accumulator is cut off at every step, to its size
+    static constexpr bool kSplitO = kQT == 2 && D == 64;
+    static constexpr int kKvBytes = 2 * kStages * kOperand;
+    static constexpr int kRowBytes = D * (kWide ? 4 : 1);
+    // an item: 4 KB of K or of V, but at most 32 keys: a tile has at least as many
+    // items as there are widening warps, so that no warp passes over a whole tile
+    static constexpr int kItemKeys = 4096 / kRowBytes < 32 ? 4096 / kRowBytes : 32;
+    static constexpr int kItems = kTileKeys / kItemKeys; // of K, and again of V
+    static constexpr int kLoads = kItemKeys * kRowBytes / 512; // of 16 bytes a lane
+    static constexpr int kItemPages = (kItemKeys + kKvPage - 1) / kKvPage;
+    static constexpr int kRows = kM * 128;
+    static constexpr int kPitch = D + 4;
+    static constexpr int kJoin = 256 * kPitch * 4; // partial results of both streams
+    static constexpr int kTiles = kQBytes + kKvBytes;
+    static constexpr int kBuf = kTiles > kJoin ? kTiles : kJoin;
+    // shared powers of two of K (4 tiles) and V (their log2), and the rows that are not finite;
+    // row factors; m and l of 2 x 128 rows; joined m and l; barriers
+    static constexpr int kFactors = 2 * (4 + kStages) * 16 * 4;
+    static constexpr int kBytes = kBuf + kFactors + 4 * 256 + 8 * 256 + 8 * 256 + 256;
+};
+
+// K-major tile rows of 128 bytes: the byte of 16-byte chunk c of row r.
+__device__ __forceinline__ int swizzled(int r, int c) { return r * 128 + ((c ^ (r & 7)) << 4); }
+
+// MN-major 16-bit operand in the 128-byte swizzle: atoms of 8 keys x 64 dims
+// (8 rows of 128 bytes), `lbo` bytes from one 64 dims to the next, 1024 from 8
+// keys to the next.
+__device__ __forceinline__ uint64_t sdesc_mn128_16b(uint32_t smem_addr, uint32_t lbo) {
+    uint64_t d = 0;
+    d |= static_cast<uint64_t>((smem_addr & 0x3FFFFu) >> 4);
+    d |= static_cast<uint64_t>((lbo >> 4) & 0x3FFFu) << 16;
+    d |= static_cast<uint64_t>(1024u >> 4) << 32;
+    d |= static_cast<uint64_t>(1u) << 46;
+    d |= static_cast<uint64_t>(2u) << 61;
+    return d;
+}
+
+// D[tmem] (+)= A[tmem] B[smem]^T, 16-bit operands.
+__device__ __forceinline__ void umma_16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc,
+                                           uint32_t accumulate) {
+    asm volatile("{\n\t.reg .pred p;\n\t"
+                 "setp.ne.b32 p, %4, 0;\n\t"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
+                 "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
+                 : "memory");
+}
+
+__device__ __forceinline__ void tile_tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+                 "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr),
+                 "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
+                 "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+                 : "memory");
+}
+__device__ __forceinline__ void tile_tmem_st8(uint32_t taddr, const uint32_t (&r)[8]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr), "r"(r[0]),
+                 "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+                 : "memory");
+}
+__device__ __forceinline__ void tile_tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+template <typename T, int D, KvFormat kFmt, int kM>
+static __global__ void __launch_bounds__(kTileThreads, 1)
+    tree_tiles_kernel(const T *__restrict__ q, T *__restrict__ out, TreeArgs a, int groups, int splits, bool sorted, int *err) {
+    using G = TreeTilesGeo<T, D, kFmt, kM>;
+    using R = KvRecord<D>;
+    extern __shared__ __align__(1024) uint8_t tile_smem[];
+    uint8_t *smem = tile_smem;
+    if ((sm100::smem_u32(smem) & 1023u) != 0) { // never taken: no static shared memory. The whole grid returns.
+        if (threadIdx.x == 0)
+            atomicExch(err, 5);
+        return;
+    }
+    uint8_t *qs = smem, *ks = qs + G::kQBytes, *vs = ks + G::kStages * G::kOperand;
+    // K's are read until the weights are done, longer than the K tile: tile i's lie in place i % 4
+    float *k_unit = reinterpret_cast<float *>(smem + G::kBuf);         // [4][16]: of each item
+    float *v_log = k_unit + 4 * 16;                                     // [stages][16]: log2 of V's
+    uint32_t *k_odd = reinterpret_cast<uint32_t *>(v_log + G::kStages * 16); // [4][16]: bit per key of the item
+    uint32_t *v_odd = k_odd + 4 * 16;                                   // [stages][16]
+    float *row_fac = reinterpret_cast<float *>(v_odd + G::kStages * 16); // [256]
+    float *stat = row_fac + 256;                                    // m [256], l [256]
+    float *joined = stat + 512;                                     // m [256], l [256] of the CTA
+    uint64_t *bars = reinterpret_cast<uint64_t *>(joined + 512);
+    uint64_t *k_full = bars, *v_full = k_full + 4, *v_empty = v_full + 4; // [4]: tile i's at i % 4
+    // [stream][4]: step e's at e % 4. S is there; so the K tile is free (for two row
+    // tiles: with the second stream's), and all products before it are done
+    uint64_t *s_ready = v_empty + 4, *p_ready = s_ready + 8; // p_ready: [stream]
+    uint64_t *drain = p_ready + 2, *q_full = drain + 1;
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(q_full + 1);
+
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int rank = blockIdx.x % splits, unit = blockIdx.x / splits;
+    const int group = unit % groups, h = unit / groups;
+    const int rep = a.qh / a.kvh;
+    if (tid == 0) {
+        for (int i = 0; i < 4; ++i) {
+            sm100::mbar_init(&k_full[i], G::kItems);
+            sm100::mbar_init(&v_full[i], G::kItems);
+            sm100::mbar_init(&v_empty[i], 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            for (int n = 0; n < 4; ++n)
+                sm100::mbar_init(&s_ready[4 * i + n], 2); // the products, and the thread that issued them
+            sm100::mbar_init(&p_ready[i], 4); // warps: 128 threads arriving on one barrier take 600 cycles
+        }
+        sm100::mbar_init(drain, 1);
+        sm100::mbar_init(q_full, 8);
+        sm100::fence_mbarrier_init();
+    }
+    if (warp == 15) {
+        sm100::tmem_alloc(tmem_slot, 512);
+        sm100::tmem_relinquish();
+    }
+    pdl_trigger();
+    sm100::tc_fence_before();
+    __syncthreads();
+    sm100::tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+    pdl_wait();
+    const int b = sorted ? sequence_by_work(a.t, blockIdx.y, reinterpret_cast<int *>(stat)) : blockIdx.y;
+
+    const TreeSpan span(a.t, b);
+    const int row_base = group * G::kRows, rows = span.n * rep;
+    int keys = span.keys;
+    if (a.t.mask == nullptr) // a chain: nothing after the group's last node is seen
+        keys = min(keys, span.ctx + (min(row_base + G::kRows, rows) + rep - 1) / rep);
+    const int all_tiles = row_base < rows ? (keys + kTileKeys - 1) / kTileKeys : 0;
+    // tiles go round the cluster: this CTA's tile i is rank + i * splits
+    const int tiles = all_tiles > rank ? (all_tiles - rank + splits - 1) / splits : 0;
+    const auto key_of = [&](int i) { return (rank + i * splits) * kTileKeys; };
+    // Tile i's barriers are those at i % 4, in phase i / 4, whatever the number of
+    // stages: no waiter is as much as four tiles behind, so a parity is enough.
+    const auto phase_of = [](int i) { return static_cast<uint32_t>(i >> 2) & 1u; };
+    bool ok = true;
+
+    if (warp >= 8 && warp < 15) {
+        // ---- widening warps. The items of all tiles in one row: K of tile 0, V
+        // of tile 0, K of tile 1, ..; warp w takes items w, w + 7, ... So whatever
+        // an item waits for depends on items before it only. Two are in flight.
+        const int *table = a.t.block_table + static_cast<int64_t>(b) * a.t.table_stride;
+        const int pages = (keys + kKvPage - 1) / kKvPage, items = tiles * 2 * G::kItems;
+        struct Item {
+            uint4 r[G::kLoads];
+            float scale; // 8-bit: of key `lane`
+        };
+        // load j of a lane. fp32: rows one after another. 8-bit: 8 rows by 64 bytes,
+        // so that the eight lanes of a store phase are two rows, one even and one
+        // odd, and the swizzle keeps them on different banks.
+        constexpr int kRowLanes = G::kWide ? G::kRowBytes / 16 : 4, kRowsPerLoad = 32 / kRowLanes;
+        constexpr int kHalves = G::kWide ? 1 : G::kSlabs; // loads side by side in a row
+        const int lrow = lane / kRowLanes, lbyte = (lane % kRowLanes) * 16;
+        const auto item_key = [&](int item) { return key_of(item / (2 * G::kItems)) + item % G::kItems * G::kItemKeys; };
+        // A lane holds the block id of one page of the warp's next 32 or 16 items.
+        // Past the pages it is 0: what is read there is valid memory and takes no
+        // part (its keys come after the last one). A load that depended on the
+        // page being there would be followed by a select, and that waits for it.
+        constexpr int kIdItems = 32 / G::kItemPages;
+        int ids = 0;
+        const auto look_up = [&](int item) {
+            const int mine = item + lane / G::kItemPages * kWidenWarps;
+            const int page = item_key(mine) / kKvPage + lane % G::kItemPages;
+            ids = mine < items && page < pages ? table[page] : 0;
+        };
+        const auto fetch = [&](int item, Item &it) {
+            const bool v = item / G::kItems % 2;
+            const int key0 = item_key(item);
+            const int step = (item - (warp - 8)) / kWidenWarps % kIdItems; // which of the items looked up
+            if (step == 0)
+                look_up(item);
+            const int id = __shfl_sync(kFullWarpMask, ids, step * G::kItemPages + (lane & (G::kItemPages - 1)));
+            constexpr int kLoads = G::kLoads / G::kItemPages; // of a page
+#pragma unroll
+            for (int pg = 0; pg < G::kItemPages; ++pg) {
+                const int64_t rec = __shfl_sync(kFullWarpMask, id, pg);
+                const uint8_t *src;
+                if constexpr (G::kWide)
+                    src = static_cast<const uint8_t *>(v ? a.v : a.k) + ((rec * a.kvh + h) * kKvPage + key0 % kKvPage) * G::kRowBytes;
+                else
+                    src = static_cast<const uint8_t *>(a.k) + (rec * a.kvh + h) * R::kBytes + (v ? R::kCodes : 0);
+                src += lrow * G::kRowBytes + lbyte;
+#pragma unroll
+                for (int j = 0; j < kLoads; ++j)
+                    it.r[pg * kLoads + j] = __ldg(reinterpret_cast<const uint4 *>(src + j / kHalves * kRowsPerLoad * G::kRowBytes + j % kHalves * 64));
+            }
+            if constexpr (!G::kWide) { // an item is 32 keys
+                const int64_t rec = __shfl_sync(kFullWarpMask, id, lane / kKvPage);
+                it.scale = __ldg(reinterpret_cast<const float *>(static_cast<const uint8_t *>(a.k) + (rec * a.kvh + h) * R::kBytes +
+                                                                 (v ? R::kVScale : R::kKScale)) + lane % kKvPage);
+            }
+        };
+        // terms of two values into 4 bytes of the tile(s)
+        const auto terms = [&](float x, float y, uint32_t &hi, uint32_t &lo) {
+            if constexpr (G::kKT == 2) {
+                hi = half2_rn(x, y);
+                const float2 h = half2_floats(hi), r = __fadd2_rn(make_float2(x, y), make_float2(-h.x, -h.y));
+                lo = half2_rn(r.x, r.y);
+            } else {
+                hi = half2_rn(x, y);
+            }
+        };
+        // Widens an item into its tile. Values come to 2^10 at most, times a power
+        // of two that the item's keys share.
+        const auto widen = [&](int item, const Item &it) -> bool {
+            const int i = item / (2 * G::kItems), part = item % G::kItems, stage = i % G::kStages;
+            const bool v = item / G::kItems % 2;
+            const int row0 = part * G::kItemKeys, key0 = item_key(item), left = keys - key0;
+            const bool edge = key0 + G::kItemKeys > span.ctx;
+            const int before = i - G::kStages; // the tile that has the stage until its products are done
+            if (before >= 0) {
+                const int e = kM == 2 ? before : before >> 1; // its step, in the last stream that reads its K
+                uint64_t *bar = v ? &v_empty[before & 3] : &s_ready[(kM == 2 ? 4 : (before & 1) * 4) + (e & 3)];
+                if (!sm100::mbar_wait_warp(bar, phase_of(v ? before : e)))
+                    return false;
+            }
+            uint8_t *tile = (v ? vs : ks) + stage * G::kOperand;
+            // Rows that hold an infinity or a NaN: where all nodes see them (no
+            // edge) the unit says so; else they are zeros here and marked.
+            uint32_t odd = 0;
+            float unit;
+            if constexpr (G::kWide) {
+                uint32_t bits = 0;
+                float y[G::kLoads][4];
+#pragma unroll
+                for (int j = 0; j < G::kLoads; ++j) {
+                    y[j][0] = __uint_as_float(it.r[j].x), y[j][1] = __uint_as_float(it.r[j].y);
+                    y[j][2] = __uint_as_float(it.r[j].z), y[j][3] = __uint_as_float(it.r[j].w);
+                    if (edge) {
+                        bool bad = false;
+                        const bool there = j * kRowsPerLoad + lrow < left;
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const float z = there ? finite_or_zero(y[j][e]) : 0.f;
+                            bad |= there && !(z == y[j][e]);
+                            y[j][e] = z;
+                        }
+                        const uint32_t some = __ballot_sync(kFullWarpMask, bad);
+#pragma unroll
+                        for (int n = 0; n < kRowsPerLoad; ++n)
+                            if (some >> (n * kRowLanes) & (kRowLanes == 32 ? 0xffffffffu : (1u << (kRowLanes & 31)) - 1u))
+                                odd |= 1u << (j * kRowsPerLoad + n);
+                    }
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        bits = max(bits, __float_as_uint(y[j][e]) & 0x7fffffffu);
+                }
+                bits = __reduce_max_sync(kFullWarpMask, bits);
+                const uint32_t ex = exponent_above(bits);
+                const float f = pow2_field(254u - ex + 10u);
+#pragma unroll
+                for (int j = 0; j < G::kLoads; ++j) {
+                    uint32_t h0, h1, l0, l1;
+                    terms(y[j][0] * f, y[j][1] * f, h0, l0);
+                    terms(y[j][2] * f, y[j][3] * f, h1, l1);
+                    const int row = row0 + j * kRowsPerLoad + lrow, dim = lbyte / 4; // 4 dims: 8 bytes of fp16
+                    uint8_t *dst = tile + dim / 64 * G::kSlab + swizzled(row, dim % 64 / 8) + dim % 8 * 2;
+                    *reinterpret_cast<uint2 *>(dst) = make_uint2(h0, h1);
+                    *reinterpret_cast<uint2 *>(dst + G::kSlabs * G::kSlab) = make_uint2(l0, l1);
+                }
+                unit = bits < 0x7f800000u ? pow2_field(ex - 10u) : __uint_as_float(0x7fc00000u);
+            } else {
+                float scale = lane < left ? it.scale : 0.f;
+                const bool bad = !(fabsf(scale) <= 3.4028235e38f);
+                odd = __ballot_sync(kFullWarpMask, bad);
+                const uint32_t ex = exponent_above(__reduce_max_sync(kFullWarpMask, bad ? 0u : __float_as_uint(scale)));
+                scale = bad ? 0.f : scale * pow2_field(254u - ex + 1u); // at most 2
+#pragma unroll
+                for (int j = 0; j < G::kLoads; ++j) {
+                    const uint32_t w[4] = {it.r[j].x, it.r[j].y, it.r[j].z, it.r[j].w};
+                    const int r = j / kHalves * kRowsPerLoad + lrow, c = lbyte / 8;
+                    const float f = __shfl_sync(kFullWarpMask, scale, r);
+                    const float2 f2 = make_float2(f, f);
+                    uint32_t hi[8], lo[8];
+#pragma unroll
+                    for (int n = 0; n < 4; ++n) {
+                        float2 x, y;
+                        if constexpr (kFmt == KvFormat::kInt8) {
+                            // byte + 128 in the low bits of fp32 2^23 .. 2^23 + 255
+                            const uint32_t u = w[n] ^ 0x80808080u;
+                            const float2 bias = make_float2(-8388736.f, -8388736.f);
+                            x = __fadd2_rn(make_float2(__uint_as_float(__byte_perm(u, 0x4b000000u, 0x7440)), __uint_as_float(__byte_perm(u, 0x4b000000u, 0x7441))), bias);
+                            y = __fadd2_rn(make_float2(__uint_as_float(__byte_perm(u, 0x4b000000u, 0x7442)), __uint_as_float(__byte_perm(u, 0x4b000000u, 0x7443))), bias);
+                        } else {
+                            uint32_t h0, h1;
+                            codes_to_half<kFmt>(edge ? clear_e4m3_nan(w[n]) : w[n], h0, h1);
+                            x = half2_floats(h0), y = half2_floats(h1);
+                        }
+                        x = __fmul2_rn(x, f2), y = __fmul2_rn(y, f2);
+                        terms(x.x, x.y, hi[2 * n], lo[2 * n]);
+                        terms(y.x, y.y, hi[2 * n + 1], lo[2 * n + 1]);
+                    }
+                    uint8_t *slab = tile + j % kHalves * G::kSlab, *d0 = slab + swizzled(row0 + r, c), *d1 = slab + swizzled(row0 + r, c + 1);
+                    *reinterpret_cast<uint4 *>(d0) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                    *reinterpret_cast<uint4 *>(d1) = make_uint4(hi[4], hi[5], hi[6], hi[7]);
+                    if constexpr (G::kKT == 2) {
+                        *reinterpret_cast<uint4 *>(d0 + G::kSlabs * G::kSlab) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+                        *reinterpret_cast<uint4 *>(d1 + G::kSlabs * G::kSlab) = make_uint4(lo[4], lo[5], lo[6], lo[7]);
+                    }
+                }
+                unit = odd && !edge ? __uint_as_float(0x7fc00000u) : pow2_field(ex - 1u);
+            }
+            if (lane == 0) {
+                const int at = (v ? stage : i & 3) * 16 + part;
+                if (v) // NaN stays NaN
+                    v_log[at] = unit == unit ? static_cast<float>(static_cast<int>(__float_as_uint(unit) >> 23) - 127) : unit;
+                else
+                    k_unit[at] = unit;
+                (v ? v_odd : k_odd)[at] = odd;
+            }
+            sm100::fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0)
+                sm100::mbar_arrive(&(v ? v_full : k_full)[i & 3]);
+            return true;
+        };
+        Item even, odd;
+        int item = warp - 8;
+        fetch(item, even);
+        fetch(item + kWidenWarps, odd);
+        for (; item < items; item += 2 * kWidenWarps) {
+            if (!widen(item, even)) {
+                ok = false;
+                break;
+            }
+            fetch(item + 2 * kWidenWarps, even);
+            if (item + kWidenWarps < items && !widen(item + kWidenWarps, odd)) {
+                ok = false;
+                break;
+            }
+            fetch(item + 3 * kWidenWarps, odd);
+        }
+    } else if (warp == 15) {
+        // ---- all products. The warp runs together, so that what addresses them is
+        // uniform, and one lane issues: a product every 64 cycles leaves no room
+        // for moving each operand out of a thread's registers.
+        if (tiles > 0) {
+            const bool leader = lane == 0;
+            const uint32_t tm = __shfl_sync(kFullWarpMask, tmem, 0);
+            using Zero = std::integral_constant<int, 0>;
+            using One = std::integral_constant<int, 1>;
+            constexpr uint32_t idesc_s = sm100::idesc_make(sm100::kFmtF16, 128, kTileKeys);
+            constexpr uint32_t idesc_o = sm100::idesc_make(sm100::kFmtF16, 128, D) | (1u << 16); // B MN-major
+            // descriptors move by additions to their address field (16-byte units)
+            const uint64_t qd = sm100::sdesc_k128(sm100::smem_u32(qs)), kd = sm100::sdesc_k128(sm100::smem_u32(ks));
+            const uint64_t vd = sdesc_mn128_16b(sm100::smem_u32(vs), G::kSlab);
+            const auto scores = [&](int stream, int i) {
+                const uint64_t q0 = qd + static_cast<uint32_t>((kM == 2 ? stream : 0) * (G::kSlab >> 4));
+                const uint64_t k0 = kd + static_cast<uint32_t>((i % G::kStages) * (G::kOperand >> 4));
+                const uint32_t d = tm + static_cast<uint32_t>(stream * kTileKeys);
+                const auto product = [&](auto qt, auto kt, uint32_t acc) {
+#pragma unroll
+                    for (int s = 0; s < G::kSlabs; ++s)
+#pragma unroll
+                        for (int st = 0; st < 4; ++st) // 16 dims: 32 bytes
+                            sm100::umma_bf16(d, q0 + static_cast<uint32_t>(((decltype(qt)::value * G::kSlabs + s) * kM * G::kSlab + 32 * st) >> 4),
+                                             k0 + static_cast<uint32_t>(((decltype(kt)::value * G::kSlabs + s) * G::kSlab + 32 * st) >> 4),
+                                             idesc_s, s + st > 0 ? 1u : acc);
+                };
+                // small products first: the accumulator is cut off at every step, to its size at the time
+                if (leader) {
+                    if constexpr (G::kKT == 2)
+                        product(Zero{}, One{}, 0);
+                    if constexpr (G::kQT == 2)
+                        product(One{}, Zero{}, G::kKT == 2);
+                    product(Zero{}, Zero{}, G::kKT == 2 || G::kQT == 2);
+                }
+                __syncwarp();
+            };
+            const auto weigh = [&](int stream, int i, uint32_t acc) {
+                const uint64_t v0 = vd + static_cast<uint32_t>((i % G::kStages) * (G::kOperand >> 4));
+                const uint32_t d = tm + 256u + static_cast<uint32_t>(stream * D), p0 = tm + static_cast<uint32_t>(stream * kTileKeys);
+                const auto product = [&](auto pt, auto vt, uint32_t d, uint32_t first) {
+#pragma unroll
+                    for (int st = 0; st < kTileKeys / 16; ++st) // chunk of 32 keys: 16 columns of each term
+                        umma_16_ts(d, p0 + static_cast<uint32_t>(st / 2 * 32 + decltype(pt)::value * 16 + st % 2 * 8),
+                                   v0 + static_cast<uint32_t>((decltype(vt)::value * G::kSlabs * G::kSlab + st * 2048) >> 4),
+                                   idesc_o, st > 0 ? 1u : first);
+                };
+                if (leader) {
+                    product(Zero{}, Zero{}, d, acc);
+                    if constexpr (G::kQT == 2) {
+                        const uint32_t small = G::kSplitO ? tm + 384u + static_cast<uint32_t>(stream * D) : d;
+                        product(Zero{}, One{}, small, G::kSplitO ? acc : 1u);
+                        product(One{}, Zero{}, small, 1);
+                    }
+                }
+                __syncwarp();
+            };
+            const auto commit = [&](uint64_t *bar) {
+                if (leader)
+                    sm100::umma_commit(bar);
+                __syncwarp();
+            };
+            const auto k_ready = [&](int i) {
+                ok = sm100::mbar_wait_warp(&k_full[i & 3], phase_of(i));
+                sm100::tc_fence_after();
+                return ok;
+            };
+            // the thread's own arrival passes on what it has seen: the K units
+            const auto s_issued = [&](int stream, int e) {
+                uint64_t *bar = &s_ready[4 * stream + (e & 3)];
+                commit(bar);
+                if (leader)
+                    sm100::mbar_arrive(bar);
+            };
+            // step e of a stream: tile e (two row tiles) or 2 e + stream (even and odd key tiles)
+            const auto tile_of = [&](int stream, int e) { return kM == 2 ? e : 2 * e + stream; };
+            ok = sm100::mbar_wait_warp(q_full, 0);
+            for (int s = 0; ok && s < 2; ++s)
+                if (tile_of(s, 0) < tiles && (kM == 2 && s == 1 ? true : k_ready(tile_of(s, 0)))) {
+                    scores(s, tile_of(s, 0));
+                    s_issued(s, 0);
+                }
+            for (int e = 0; ok && tile_of(0, e) < tiles; ++e)
+                for (int s = 0; ok && s < 2; ++s) {
+                    const int i = tile_of(s, e), next = tile_of(s, e + 1);
+                    if (i >= tiles)
+                        break;
+                    if (!sm100::mbar_wait_warp(&p_ready[s], static_cast<uint32_t>(e) & 1u) ||
+                        !sm100::mbar_wait_warp(&v_full[i & 3], phase_of(i))) {
+                        ok = false;
+                        break;
+                    }
+                    sm100::tc_fence_after();
+                    weigh(s, i, e > 0);
+                    if (kM == 1 || s == 1)
+                        commit(&v_empty[i & 3]);
+                    if (next < tiles && (kM == 2 && s == 1 ? true : k_ready(next))) {
+                        scores(s, next);
+                        s_issued(s, e + 1);
+                    }
+                }
+            // every product is done before tensor memory and the tiles are used for anything else
+            commit(drain);
+            if (!sm100::mbar_wait_warp(drain, 0))
+                ok = false;
+        }
+    } else {
+        // ---- softmax warps. First Q: a warp per row, scaled to 2^9 .. 2^10 and split into terms
+        constexpr int kE = D / 32; // values per lane
+        constexpr int kBatch = 8; // rows whose loads are in flight together
+#pragma unroll 1
+        for (int r0 = warp; r0 < G::kRows; r0 += 8 * kBatch) {
+            float x[kBatch][kE];
+#pragma unroll
+            for (int n = 0; n < kBatch; ++n) {
+                const int row = row_base + r0 + 8 * n;
+                const T *src = q + static_cast<int64_t>(span.row0 + row / rep) * a.q_stride + static_cast<int64_t>(h * rep + row % rep) * D + kE * lane;
+#pragma unroll
+                for (int e = 0; e < kE; ++e)
+                    x[n][e] = row < rows ? static_cast<float>(src[e]) : 0.f;
+            }
+#pragma unroll
+            for (int n = 0; n < kBatch; ++n) {
+                const int r = r0 + 8 * n;
+                uint32_t top = 0;
+#pragma unroll
+                for (int e = 0; e < kE; ++e)
+                    top = max(top, __float_as_uint(x[n][e]) & 0x7fffffffu);
+                const uint32_t ex = exponent_above(__reduce_max_sync(kFullWarpMask, top));
+                const float f = copysignf(pow2_field(254u - ex + 10u), a.scale_log2);
+                const int dim = kE * lane;
+                uint8_t *dst = qs + (dim / 64 * kM + r / 128) * G::kSlab + swizzled(r % 128, dim % 64 / 8) + dim % 8 * 2;
+#pragma unroll
+                for (int e = 0; e < kE; e += 2) {
+                    const float u = x[n][e] * f, v = x[n][e + 1] * f;
+                    const uint32_t hi = half2_rn(u, v);
+                    *reinterpret_cast<uint32_t *>(dst + 2 * e) = hi;
+                    if constexpr (G::kQT == 2) {
+                        const float2 w = half2_floats(hi);
+                        *reinterpret_cast<uint32_t *>(dst + G::kSlabs * kM * G::kSlab + 2 * e) = half2_rn(u - w.x, v - w.y);
+                    }
+                }
+                if (lane == 0)
+                    row_fac[r] = fabsf(a.scale_log2) * pow2_field(ex - 10u);
+            }
+        }
+        sm100::fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0)
+            sm100::mbar_arrive(q_full);
+        if (!sm100::mbar_wait_warp(q_full, 0)) // row_fac of other warps' rows
+            ok = false;
+
+        const int stream = warp / 4, r = (warp % 4) * 32 + lane; // row of the tile
+        const int row = row_base + (kM == 2 ? stream * 128 : 0) + r;
+        const int node = row / rep;
+        const bool live = row < rows;
+        const float rs = row_fac[kM == 2 ? stream * 128 + r : r];
+        const uint32_t quarter = static_cast<uint32_t>((warp % 4) * 32) << 16;
+        const uint32_t st = tmem + quarter + static_cast<uint32_t>(stream * kTileKeys);
+        const uint32_t ot = tmem + quarter + 256u + static_cast<uint32_t>(stream * D);
+        float m = -1e30f, l = 0.f;
+        float vlog = kMinVLog; // log2 of a power of two, at least every V unit so far: O is in units of it
+        constexpr int kGroup = G::kItemKeys, kGroups = 32 / kGroup; // keys that share their units; such groups in a chunk
+        int e = 0; // steps done
+        for (; ok; ++e) {
+            const int i = kM == 2 ? e : 2 * e + stream;
+            if (i >= tiles)
+                break;
+            const int stage = i % G::kStages, key0 = key_of(i);
+            if (!sm100::mbar_wait_warp(&s_ready[4 * stream + (e & 3)], phase_of(e))) {
+                ok = false;
+                break;
+            }
+            sm100::tc_fence_after();
+            const float *ku = k_unit + (i & 3) * 16, *vl = v_log + stage * 16;
+            const bool edge = key0 + kTileKeys > span.ctx; // holds nodes, or places after the last key
+            const auto seen_of = [&](int c) {
+                return live ? tree_sees32(a.t, span.row0 + node, node, key0 + 32 * c - span.ctx, keys - span.ctx) : 0u;
+            };
+            // 32 scores of the row, from tensor memory: asked for, and there
+            const auto ask = [&](int c, uint32_t (&x)[2][16]) {
+                sm100::tmem_ld_32x16(st + static_cast<uint32_t>(32 * c), x[0]);
+                sm100::tmem_ld_32x16(st + static_cast<uint32_t>(32 * c + 16), x[1]);
+            };
+            const auto await = [&](uint32_t (&x)[2][16]) {
+                sm100::tmem_wait_ld();
+                sm100::tmem_reg_fence(x[0]);
+                sm100::tmem_reg_fence(x[1]);
+            };
+            // a chunk's keys that the row sees, and those that are not finite
+            const auto odd_of = [&](int c) {
+                uint32_t bits = 0;
+#pragma unroll
+                for (int n = 0; n < kGroups; ++n)
+                    bits |= (k_odd[(i & 3) * 16 + kGroups * c + n] | v_odd[stage * 16 + kGroups * c + n]) << (n * kGroup & 31);
+                return bits;
+            };
+            // two scores of a chunk in log2 units less `m`; masked ones -inf (edge tiles)
+            const auto scored = [&](const uint32_t (&x)[2][16], int n, float2 f, float2 m2, uint32_t seen, uint32_t odd, auto edge_tag) {
+                float2 y = __ffma2_rn(make_float2(__uint_as_float(x[n / 16][n % 16]), __uint_as_float(x[n / 16][n % 16 + 1])), f, m2);
+                if constexpr (decltype(edge_tag)::value) {
+                    const float bad = __uint_as_float(0x7fc00000u);
+                    y.x = !(seen >> n & 1u) ? kNegInf : odd >> n & 1u ? bad : y.x;
+                    y.y = !(seen >> (n + 1) & 1u) ? kNegInf : odd >> (n + 1) & 1u ? bad : y.y;
+                }
+                return y;
+            };
+            uint32_t xa[2][16], xb[2][16];
+            ask(0, xa);
+            if (!sm100::mbar_wait_warp(&v_full[i & 3], phase_of(i))) {
+                await(xa);
+                ok = false;
+                break;
+            }
+            float vnew = kMinVLog;
+#pragma unroll
+            for (int c = 0; c < G::kItems; ++c)
+                vnew = fmaxf(vnew, vl[c]);
+            // O, where there is one, times fix; the weights of this tile's first `c` chunks too
+            const auto rescale = [&](float fix, int c) {
+                if (e > 0) {
+                    // (this tile's S is there, so the products before it are done)
+#pragma unroll 1
+                    for (int n = 0; n < (G::kSplitO ? 2 * D : D); n += 16) {
+                        const int d = n < D ? n : n - D + 128; // the small products' columns lie 128 on
+                        uint32_t o[16];
+                        sm100::tmem_ld_32x16(ot + static_cast<uint32_t>(d), o);
+                        sm100::tmem_wait_ld();
+                        sm100::tmem_reg_fence(o);
+#pragma unroll
+                        for (int k = 0; k < 16; ++k)
+                            o[k] = __float_as_uint(__uint_as_float(o[k]) * fix);
+                        tile_tmem_st16(ot + static_cast<uint32_t>(d), o);
+                    }
+                }
+                tile_tmem_wait_st(); // chunks' weights are stored before they are read
+                const __half2 half_fix = __float2half2_rn(fix);
+#pragma unroll 1
+                for (int d = 0; d < 32 * c; d += 16) {
+                    uint32_t o[16];
+                    sm100::tmem_ld_32x16(st + static_cast<uint32_t>(d), o);
+                    sm100::tmem_wait_ld();
+                    sm100::tmem_reg_fence(o);
+#pragma unroll
+                    for (int k = 0; k < 16; ++k) {
+                        const __half2 p = __hmul2(*reinterpret_cast<const __half2 *>(&o[k]), half_fix);
+                        o[k] = *reinterpret_cast<const uint32_t *>(&p);
+                    }
+                    tile_tmem_st16(st + static_cast<uint32_t>(d), o);
+                }
+                tile_tmem_wait_st();
+            };
+            if (vnew > vlog) { // the same in every thread of the stream
+                await(xa);
+                rescale(exp2_approx(vlog - vnew), 0);
+                vlog = vnew;
+            }
+            const auto tile = [&](auto edge_tag) {
+                constexpr bool kEdge = decltype(edge_tag)::value;
+                if (e == 0) { // the first reference: the largest score of the first tile
+                    float top = kNegInf;
+#pragma unroll 1
+                    for (int c = 0; c < 4; ++c) {
+                        ask(c, xb);
+                        await(xb);
+                        const uint32_t seen = kEdge ? seen_of(c) : 0u;
+#pragma unroll
+                        for (int n = 0; n < 32; n += 2) {
+                            const float f = rs * ku[kGroups * c + n / kGroup];
+                            const float2 y = scored(xb, n, make_float2(f, f), make_float2(0.f, 0.f), seen, 0u, edge_tag);
+                            top = fmaxf(top, fmaxf(y.x, y.y));
+                        }
+                    }
+                    m = fmaxf(m, top - kTileLift);
+                }
+                // one chunk of 32 keys, whose scores are in x, the next one's on their way to `next`
+                const auto chunk = [&](int c, uint32_t (&x)[2][16], uint32_t (&next)[2][16]) {
+                    // weights come out as 2^(score - m + shift): the V unit (over vtop) is in the exponent
+                    float f[kGroups], shift[kGroups], less_v[kGroups];
+                    bool small = false;
+#pragma unroll
+                    for (int n = 0; n < kGroups; ++n) {
+                        const float log = vl[kGroups * c + n] - vlog;
+                        f[n] = rs * ku[kGroups * c + n];
+                        less_v[n] = log < -kTileShift ? log + kTileShift : 0.f;
+                        shift[n] = log - less_v[n]; // NaN: every weight is
+                        small |= less_v[n] != 0.f;
+                    }
+                    await(x);
+                    if (c < 3)
+                        ask(c + 1, next);
+                    const uint32_t seen = kEdge ? seen_of(c) : 0u, odd = kEdge ? odd_of(c) : 0u;
+                    // Scores and weights at once, for weights up to 2^kTileTop fit in
+                    // fp16 but for a rare chunk: one with a larger one raises the
+                    // reference and is done again (its scores are still there).
+#pragma unroll 1
+                    for (;;) {
+                        float top[4] = {kNegInf, kNegInf, kNegInf, kNegInf};
+#pragma unroll
+                        for (int n = 0; n < 32; n += 2) {
+                            const int k = n / kGroup;
+                            const float base = shift[k] - m;
+                            const float2 y = scored(x, n, make_float2(f[k], f[k]), make_float2(base, base), seen, odd, edge_tag);
+                            top[n / 2 % 4] = fmaxf(top[n / 2 % 4], fmaxf(y.x, y.y));
+                            x[n / 16][n % 16] = __float_as_uint(y.x);
+                            x[n / 16][n % 16 + 1] = __float_as_uint(y.y);
+                        }
+#pragma unroll
+                        for (int n = 0; n < 32; ++n)
+                            x[n / 16][n % 16] = __float_as_uint(exp2_approx(__uint_as_float(x[n / 16][n % 16])));
+                        const float most = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+                        if (!__any_sync(kFullWarpMask, most > kTileTop))
+                            break;
+                        const float less = fmaxf(0.f, ceilf(most - kTileLift)), fix = exp2_approx(-less);
+                        if (c < 3)
+                            await(next);
+                        rescale(fix, c);
+                        l *= fix;
+                        m += less;
+                        ask(c, x);
+                        await(x);
+                    }
+                    float take[kGroups]; // from weights as they come out to l
+#pragma unroll
+                    for (int n = 0; n < kGroups; ++n)
+                        take[n] = exp2_approx(-shift[n]);
+                    if (small) { // V rows that small against others: l first, then the rest of their unit
+#pragma unroll
+                        for (int n = 0; n < 32; ++n) {
+                            const float p = __uint_as_float(x[n / 16][n % 16]);
+                            l = fmaf(p, take[n / kGroup], l);
+                            x[n / 16][n % 16] = __float_as_uint(p * exp2_approx(fmaxf(less_v[n / kGroup], -120.f)));
+                        }
+#pragma unroll
+                        for (int n = 0; n < kGroups; ++n)
+                            take[n] = 0.f;
+                    }
+                    float2 sum[kGroups];
+#pragma unroll
+                    for (int n = 0; n < kGroups; ++n)
+                        sum[n] = make_float2(0.f, 0.f);
+#pragma unroll
+                    for (int part = 0; part < 2; ++part) { // 16 keys, a step of the product
+                        uint32_t hi[8], lo[8];
+#pragma unroll
+                        for (int n = 0; n < 8; ++n) {
+                            const int k = (16 * part + 2 * n) / kGroup;
+                            const float2 p = make_float2(__uint_as_float(x[part][2 * n]), __uint_as_float(x[part][2 * n + 1]));
+                            sum[k] = __fadd2_rn(sum[k], p);
+                            hi[n] = half2_rn(p.x, p.y);
+                            if constexpr (G::kQT == 2) {
+                                const float2 w = half2_floats(hi[n]);
+                                const float2 r = __fadd2_rn(p, make_float2(-w.x, -w.y));
+                                lo[n] = half2_rn(r.x, r.y);
+                            }
+                        }
+                        tile_tmem_st8(st + static_cast<uint32_t>(32 * c + 8 * part), hi);
+                        if constexpr (G::kQT == 2)
+                            tile_tmem_st8(st + static_cast<uint32_t>(32 * c + 16 + 8 * part), lo);
+                    }
+#pragma unroll
+                    for (int n = 0; n < kGroups; ++n)
+                        l = fmaf(sum[n].x + sum[n].y, take[n], l);
+                };
+#pragma unroll 1
+                for (int c = 0; c < 4; c += 2) {
+                    chunk(c, xa, xb);
+                    chunk(c + 1, xb, xa);
+                }
+            };
+            if (edge)
+                tile(std::true_type{});
+            else
+                tile(std::false_type{});
+            tile_tmem_wait_st();
+            sm100::tc_fence_before();
+            __syncwarp();
+            if (lane == 0)
+                sm100::mbar_arrive(&p_ready[stream]);
+        }
+        // the stream's O, m and l
+        const bool any = ok && e > 0;
+        if (any && !sm100::mbar_wait_warp(drain, 0)) // all products: O is there, and the tiles are free
+            ok = false;
+        sm100::tc_fence_after();
+        const float vtop = pow2_field(static_cast<uint32_t>(127 + static_cast<int>(vlog)));
+        const bool direct = kM == 2 && splits == 1;
+        // where nothing is joined a row goes out as it is; else to shared memory, once all products are done
+        if (!direct)
+            asm volatile("bar.sync 1, 256;" ::: "memory"); // both streams have waited for that
+        const float inv = l == 0.f ? 0.f : vtop / l;
+        T *dst = out + static_cast<int64_t>(span.row0 + node) * a.out_stride + static_cast<int64_t>(h * rep + row % rep) * D;
+        float *part = reinterpret_cast<float *>(smem) + (stream * 128 + r) * G::kPitch;
+#pragma unroll 1
+        for (int c = 0; c < D; c += 16) {
+            uint32_t o[16];
+            __syncwarp();
+            if (any) { // the same in a warp
+                sm100::tmem_ld_32x16(ot + static_cast<uint32_t>(c), o);
+                sm100::tmem_wait_ld();
+                sm100::tmem_reg_fence(o);
+                if constexpr (G::kSplitO) {
+                    uint32_t small[16];
+                    sm100::tmem_ld_32x16(ot + static_cast<uint32_t>(c + 128), small);
+                    sm100::tmem_wait_ld();
+                    sm100::tmem_reg_fence(small);
+#pragma unroll
+                    for (int k = 0; k < 16; ++k)
+                        o[k] = __float_as_uint(__uint_as_float(o[k]) + __uint_as_float(small[k]));
+                }
+            } else {
+#pragma unroll
+                for (int k = 0; k < 16; ++k)
+                    o[k] = 0;
+            }
+            if (direct) {
+                if (live)
+#pragma unroll
+                    for (int k = 0; k < 16; k += KvVec<T>::kN) {
+                        float y[KvVec<T>::kN];
+#pragma unroll
+                        for (int n = 0; n < KvVec<T>::kN; ++n)
+                            y[n] = l == 0.f ? 0.f : __uint_as_float(o[k + n]) * inv;
+                        *reinterpret_cast<uint4 *>(dst + c + k) = KvVec<T>::pack(y);
+                    }
+            } else {
+#pragma unroll
+                for (int k = 0; k < 16; k += 4)
+                    *reinterpret_cast<float4 *>(part + c + k) =
+                        make_float4(__uint_as_float(o[k]) * vtop, __uint_as_float(o[k + 1]) * vtop,
+                                    __uint_as_float(o[k + 2]) * vtop, __uint_as_float(o[k + 3]) * vtop);
+            }
+        }
+        stat[stream * 128 + r] = m;
+        stat[256 + stream * 128 + r] = l;
+    }
+    if (!ok)
+        atomicExch(err, 7);
+    sm100::tc_fence_before();
+    __syncthreads();
+    if (warp == 15) {
+        sm100::tc_fence_after();
+        sm100::tmem_dealloc(tmem, 512);
+    }
+    if (kM == 2 && splits == 1)
+        return;
+    // join: the two streams of a row tile, then the cluster's CTAs
+    float *part = reinterpret_cast<float *>(smem);
+    const int rows_here = min(G::kRows, rows - row_base); // may be negative
+    const auto put = [&](int r, int d, float O, float L) {
+        const int row = row_base + r;
+        out[static_cast<int64_t>(span.row0 + row / rep) * a.out_stride + static_cast<int64_t>(h * rep + row % rep) * D + d] =
+            static_cast<T>(L == 0.f ? 0.f : O / L);
+    };
+    if (kM == 1) {
+        for (int i = tid; i < 128 * D; i += kTileThreads) {
+            const int r = i / D, d = i % D;
+            if (r >= rows_here)
+                break;
+            const float m0 = stat[r], m1 = stat[128 + r], top = fmaxf(m0, m1);
+            const float f0 = exp2_approx(m0 - top), f1 = exp2_approx(m1 - top);
+            const float O = f0 * part[r * G::kPitch + d] + f1 * part[(128 + r) * G::kPitch + d];
+            const float L = f0 * stat[256 + r] + f1 * stat[384 + r];
+            if (splits == 1) {
+                put(r, d, O, L);
+            } else {
+                part[r * G::kPitch + d] = O; // read by this thread alone
+                if (d == 0) {
+                    joined[r] = top;
+                    joined[256 + r] = L;
+                }
+            }
+        }
+    } else {
+        for (int r = tid; r < 256; r += kTileThreads) {
+            joined[r] = stat[r];
+            joined[256 + r] = stat[256 + r];
+        }
+    }
+    if (splits == 1)
+        return;
+    __syncthreads();
+    cluster_sync_all();
+    for (int i = rank * kTileThreads + tid; i < G::kRows * D; i += splits * kTileThreads) {
+        const int r = i / D, d = i % D;
+        if (r >= rows_here)
+            break;
+        float top = -1e30f, L = 0.f, O = 0.f;
+        for (int c = 0; c < splits; ++c)
+            top = fmaxf(top, peer_load(&joined[r], c));
+        for (int c = 0; c < splits; ++c) {
+            const float f = exp2_approx(peer_load(&joined[r], c) - top);
+            L += f * peer_load(&joined[256 + r], c);
+            O += f * peer_load(&part[r * G::kPitch + d], c);
+        }
+        put(r, d, O, L);
+    }
+    __syncthreads();
+    cluster_sync_all(); // peers read this CTA's shared memory until here
+}
+
+template <typename T, int D, KvFormat kFmt, int kM>
+inline void tree_tiles_launch(const T *q, T *out, const TreeArgs &a, cudaStream_t stream) {
+    using G = TreeTilesGeo<T, D, kFmt, kM>;
+    static_assert(G::kItems <= 16 && 2 * G::kItems >= kWidenWarps && G::kBytes <= 232448, "shared memory");
+    const auto kernel = tree_tiles_kernel<T, D, kFmt, kM>;
+    allow_shared_bytes(kernel, G::kBytes);
+    const int64_t rows = static_cast<int64_t>(a.t.max_rows) * (a.qh / a.kvh);
+    const int64_t groups = (rows + G::kRows - 1) / G::kRows, units = groups * a.kvh;
+    const int64_t tiles = (static_cast<int64_t>(a.t.max_ctx) + a.t.max_rows + kTileKeys - 1) / kTileKeys;
+    // splits while all CTAs still run at once and each has four tiles
+    int splits = 1;
+    while (splits < 8 && units * a.t.batch * splits * 2 <= device_facts().sm_count && tiles >= 8 * splits)
+        splits *= 2;
+    require(units * splits <= 0x7fffffff, "tree attention: too many rows for one call");
+    // more CTAs than places: sequences in the order of their length
+    const bool sorted = a.t.batch > 1 && a.t.batch <= kTileThreads - 1 && units * splits * a.t.batch > device_facts().sm_count;
+    launch_ex_cluster(kernel, dim3(static_cast<unsigned>(units * splits), a.t.batch), dim3(splits), dim3(kTileThreads),
+                      G::kBytes, stream, q, out, a, static_cast<int>(groups), splits, sorted, sm100::device_error_word());
+}
+
+} // namespace opworks::detail

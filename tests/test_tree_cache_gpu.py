@@ -203,6 +203,15 @@ def test_chains_without_a_mask(ops, fmt, kind, dim, kvh, rep, ctx, rows):
 
 
 @pytest.mark.parametrize("fmt", [0, 1, 2])
+@pytest.mark.parametrize("kind", [0, 1])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("kvh,rep,ctx,rows", [(1, 4, [5003], [11]), (2, 8, [2600, 4100], [24, 3]), (1, 2, [7000], [2])])
+def test_long_contexts(ops, fmt, kind, dim, kvh, rep, ctx, rows):
+    """Every ring and barrier phase of the kernels many times over, on few CTAs and on several that are joined."""
+    attention_case(ops, fmt, kind, dim, kvh, rep, ctx, rows, seed=5)
+
+
+@pytest.mark.parametrize("fmt", [0, 1, 2])
 @pytest.mark.parametrize("dim", [64, 128])
 @pytest.mark.parametrize("n", [3, 40])
 def test_rows_that_see_nothing_are_zero(ops, fmt, dim, n):
