@@ -36,10 +36,16 @@ def load(name):
     return _libs[name]
 
 
-def ops_lib():
-    from . import ops
+_ops = None
 
-    return ops.bind(load("libopworks_ops.so"))
+
+def ops_lib():
+    global _ops
+    if _ops is None:
+        from . import ops
+
+        _ops = ops.bind(load("libopworks_ops.so"))
+    return _ops
 
 
 def llama_lib():

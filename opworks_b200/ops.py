@@ -81,14 +81,21 @@ class OpsLib:
     def __getattr__(self, name):
         fn = getattr(self.lib, "opw_" + name)
 
+        # A call of 20 arguments costs as much here as its launch: numbers go
+        # through as they are, and the caller is kept (the next access finds it).
         def call(*args):
-            return self.check(fn(*[_arg(a) for a in args]))
+            rc = fn(*[a if a.__class__ in _PLAIN else _arg(a) for a in args])
+            return self.check(rc) if rc else rc
 
+        setattr(self, name, call)
         return call
 
     def raw(self, name):
         fn = getattr(self.lib, "opw_" + name)
         return lambda *args: fn(*[_arg(a) for a in args])
+
+
+_PLAIN = frozenset((int, float, type(None)))
 
 
 def _arg(a):
