@@ -1,0 +1,141 @@
+"""Drafted-token decoding over a paged cache: the torch-side wrapper of
+``kv_quant_*``, ``tree_attention*`` and ``tree_commit*`` (include/opworks_ops.h).
+
+``PagedCache`` owns the pools of all layers and the block table of a batch, in
+fp32 or in 8 bits; a step writes the new tokens' K and V, attends, and commits::
+
+    cache = PagedCache(layers=2, batch=4, max_tokens=512, kv_heads=2, head_dim=64, format="int8")
+    rows = Rows([len(p) for p in prompts])                 # ragged: a chain per sequence
+    for layer in ...:
+        cache.write(layer, k, v, rows)                      # at cache.lens + 0, 1, ...
+        cache.attend(layer, q, rows, out, scale)            # q, out [rows, q_heads, head_dim]
+    cache.advance(rows)                                     # a prompt: all of it stays
+    ...
+    rows = Rows([n] * 4, parents)                           # a drafted tree per sequence
+    path, count, next = cache.commit(draft, target, rows)   # only the accepted path stays
+
+Everything runs on torch's current stream; nothing here waits for the device.
+"""
+
+from __future__ import annotations
+
+import numpy as np
+import torch
+
+from . import ops_lib
+
+FORMATS = {"f32": 0, "int8": 1, "e4m3": 2}
+TYPES = {torch.float32: 0, torch.bfloat16: 1}
+
+
+def tree_mask(parents, words):
+    """Rows of bits, one per node: its ancestors and itself. parents: of one tree, -1 for the root."""
+    sees = np.zeros((len(parents), words * 32), np.uint32)
+    for i, p in enumerate(parents):
+        if p >= i or p < -1:
+            raise ValueError("a node comes after its parent")
+        if p >= 0:
+            sees[i] = sees[p]
+        sees[i, i] = 1
+    return (sees.reshape(len(parents), words, 32) << np.arange(32, dtype=np.uint32)).sum(-1, dtype=np.uint32).view(np.int32)
+
+
+class Rows:
+    """The new tokens of a step: ``counts[b]`` rows of each sequence, one after another. With ``parents`` (a list per
+    sequence) they are trees, else chains."""
+
+    def __init__(self, counts, parents=None, device="cuda"):
+        start = np.concatenate([[0], np.cumsum(counts)]).astype(np.int32)
+        self.counts, self.total, self.most = list(counts), int(start[-1]), max(counts, default=0)
+        self.start = torch.from_numpy(start).to(device)
+        self.mask, self.words, self.parents = None, 0, None
+        if parents is not None:
+            if [len(p) for p in parents] != self.counts:
+                raise ValueError("parents: one list per sequence, as long as its rows")
+            self.words = max(1, -(-self.most // 32))
+            self.mask = torch.from_numpy(np.concatenate([tree_mask(p, self.words) for p in parents])).to(device)
+            self.parents = torch.from_numpy(np.concatenate(parents).astype(np.int32)).to(device)
+
+
+class PagedCache:
+    PAGE = 16
+
+    def __init__(self, layers, batch, max_tokens, kv_heads, head_dim, format="int8", device="cuda"):
+        self.ops, self.format = ops_lib(), FORMATS[format]
+        self.layers, self.batch, self.kv_heads, self.head_dim = layers, batch, kv_heads, head_dim
+        self.stride = -(-max_tokens // self.PAGE)
+        blocks = batch * self.stride
+        if self.format:
+            record = self.ops.raw("kv_quant_record_bytes")(head_dim)
+            if record < 0:
+                raise ValueError(self.ops.last_error())
+            self.pool = torch.zeros(layers, blocks, kv_heads, record, dtype=torch.uint8, device=device)
+        else:
+            self.k = torch.zeros(layers, blocks, kv_heads, self.PAGE, head_dim, device=device)
+            self.v = torch.zeros_like(self.k)
+        # each sequence's pages spread over the pool, as an allocator would leave them
+        self.table = torch.arange(blocks, dtype=torch.int32, device=device).view(self.stride, batch).t().contiguous()
+        self.lens = torch.zeros(batch, dtype=torch.int32, device=device)
+        self.max_len = 0  # an upper bound of lens that the host knows
+
+    @staticmethod
+    def _stream():
+        return torch.cuda.current_stream().cuda_stream
+
+    def _room(self, rows):
+        if self.max_len + rows.most > self.stride * self.PAGE:
+            raise ValueError("the cache has no room for these rows")
+
+    def write(self, layer, k, v, rows):
+        """K and V rows [total, kv_heads * head_dim] (any row stride) at positions lens + 0, 1, ... of their sequences."""
+        self._room(rows)
+        if self.format:
+            self.ops.kv_quant_write(k, v, TYPES[k.dtype], k.stride(0), self.pool[layer], self.format, self.table, self.stride,
+                                    self.lens, rows.start, self.batch, rows.total, self.kv_heads, self.head_dim, self._stream())
+            return
+        owner = torch.repeat_interleave(torch.arange(self.batch, device=k.device), rows.start.diff(), output_size=rows.total)
+        pos = self.lens.long()[owner] + torch.arange(rows.total, device=k.device) - rows.start.long()[owner]
+        block, slot = self.table.long()[owner, pos // self.PAGE], pos % self.PAGE
+        shape = (rows.total, self.kv_heads, self.head_dim)
+        self.k[layer][block, :, slot] = k.float().view(shape)
+        self.v[layer][block, :, slot] = v.float().view(shape)
+
+    def read(self, layer, rows, dtype=torch.float32):
+        """The rows at positions lens + 0, 1, ... of an 8-bit cache, as [total, kv_heads, head_dim] K and V."""
+        if not self.format:
+            raise ValueError("read: of an 8-bit cache; the fp32 pools are plain tensors")
+        k = torch.empty(rows.total, self.kv_heads, self.head_dim, dtype=dtype, device=self.lens.device)
+        v = torch.empty_like(k)
+        self.ops.kv_quant_read(self.pool[layer], self.format, self.table, self.stride, self.lens, rows.start, self.batch,
+                               rows.total, self.kv_heads, self.head_dim, k, v, TYPES[dtype], self.kv_heads * self.head_dim,
+                               self._stream())
+        return k, v
+
+    def attend(self, layer, q, rows, out, scale):
+        """q, out [total, q_heads, head_dim], fp32 or bf16, rows contiguous; the rows' K and V are written already."""
+        heads = q.shape[1]
+        rest = (self.table, self.stride, self.lens, rows.start, rows.mask, rows.words, self.batch, rows.total, rows.most,
+                self.max_len, heads, self.kv_heads, self.head_dim, scale, out, out.stride(0), self._stream())
+        if self.format:
+            self.ops.tree_attention_q8(q, TYPES[q.dtype], q.stride(0), self.pool[layer], self.format, *rest)
+        else:
+            self.ops.tree_attention(q, TYPES[q.dtype], q.stride(0), self.k[layer], self.v[layer], *rest)
+
+    def advance(self, rows):
+        """Keeps all rows (a prompt, or a chain that needs no verification)."""
+        self.lens = self.lens + rows.start.diff()
+        self.max_len += rows.most
+
+    def commit(self, draft, target, rows):
+        """Keeps each tree's accepted path (all layers). Returns (path, count, next), int32 on the device."""
+        new = lambda n: torch.empty(n, dtype=torch.int32, device=self.lens.device)  # noqa: E731
+        path, count, nxt, lens = new(rows.total), new(self.batch), new(self.batch), new(self.batch)
+        head = (draft, target, rows.parents, rows.start, self.lens, self.batch, rows.most)
+        tail = (self.layers, self.table, self.stride, self.kv_heads, self.head_dim, path, count, nxt, lens, self._stream())
+        if self.format:
+            self.ops.tree_commit_q8(*head, self.pool, self.pool.stride(0), *tail)
+        else:
+            self.ops.tree_commit(*head, self.k, self.v, self.k.stride(0), *tail)
+        self.lens = lens
+        self.max_len += rows.most
+        return path, count, nxt
