@@ -103,7 +103,7 @@ __device__ __forceinline__ bool over_half2(__half2 top) {
 
 template <typename T, int D, KvFormat kFmt, int kMT>
 static __global__ void __launch_bounds__(TreeRowsGeo<T, D, kFmt, kMT>::kThreads, TreeRowsGeo<T, D, kFmt, kMT>::kCtas)
-    tree_rows_kernel(const T *__restrict__ q, T *__restrict__ out, TreeArgs a, int groups, int splits, int *err) {
+    tree_rows_kernel(const T *__restrict__ q, T *__restrict__ out, TreeArgs a, int groups, int splits, int first_wave, int *err) {
     using G = TreeRowsGeo<T, D, kFmt, kMT>;
     using R = KvRecord<D>;
     constexpr int kC = G::kChunk;
@@ -114,7 +114,7 @@ static __global__ void __launch_bounds__(TreeRowsGeo<T, D, kFmt, kMT>::kThreads,
 
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
     const int rank = blockIdx.x % splits, unit = blockIdx.x / splits;
-    const int group = unit % groups, h = unit / groups, b = blockIdx.y;
+    const int group = unit % groups, h = unit / groups;
     const int rep = a.qh / a.kvh;
 
     uint64_t *bar = bars + warp * G::kStages;
@@ -126,6 +126,12 @@ static __global__ void __launch_bounds__(TreeRowsGeo<T, D, kFmt, kMT>::kThreads,
     __syncwarp();
     pdl_trigger();
     pdl_wait();
+    // Sequences longest first as far as every CTA gets an SM to itself, then
+    // shortest first: the SMs that hold two CTAs hold a long and a short one (32
+    // sequences of 1090 to 2180 tokens: 19.5 -> 18.9 us).
+    int b = blockIdx.y;
+    if (first_wave > 0)
+        b = sequence_by_work(a.t, b < first_wave ? b : a.t.batch - 1 - (b - first_wave), reinterpret_cast<int *>(smem));
 
     // The chunks of a sequence go round the cluster's warps, so that a warp knows
     // its pages before it knows the sequence's length: chunk i of a warp is
@@ -734,8 +740,11 @@ inline void tree_rows_launch(const T *q, T *out, const TreeArgs &a, cudaStream_t
     while (splits < 16 && units * a.t.batch * splits * 2 <= slots && per_warp >= (splits < 8 ? splits : 64))
         splits *= 2;
     require(units * splits <= 0x7fffffff, "tree attention: too many rows for one call");
+    const int64_t per_sequence = units * splits, sms = device_facts().sm_count;
+    const bool sort = a.t.batch > 1 && a.t.batch < G::kThreads && per_sequence * a.t.batch > sms;
+    const int first_wave = sort ? static_cast<int>((sms + per_sequence - 1) / per_sequence) : 0;
     launch_ex_cluster(kernel, dim3(static_cast<unsigned>(units * splits), a.t.batch), dim3(splits), dim3(G::kThreads),
-                      G::kBytes, stream, q, out, a, static_cast<int>(groups), splits, sm100::device_error_word());
+                      G::kBytes, stream, q, out, a, static_cast<int>(groups), splits, first_wave, sm100::device_error_word());
 }
 
 } // namespace opworks::detail
