@@ -174,9 +174,13 @@ template <KvFormat kFmt> __device__ __forceinline__ void kv_decode4(uint32_t w, 
 }
 
 constexpr int kKvThreads = 256;
-constexpr int kKvPasses = 4; // 16-byte loads a lane has in flight (8: the same for long calls, 3.6 us against 3.0 for a decode step)
+// 16-byte pieces that a lane has in flight. Writing: 8 take as long for prompts
+// and 3.6 us for 3.0 in a decode step; reading: 4 take 60.4 us for 55.1 (16
+// prefixes of 4096 tokens, 128 dims, bf16), as the second half of a row then
+// comes long after the first.
+constexpr int kKvWritePasses = 4, kKvReadPasses = 8;
 
-// A warp takes one row and kKvPasses x (32 / lanes per item) of its 2 x kvh
+// A warp takes one row and kKvWritePasses x (32 / lanes per item) of its 2 x kvh
 // items (K and V of each head). An item's D values lie on D / kN lanes, which
 // find the maximum together.
 template <typename T, int D, KvFormat kFmt>
@@ -190,11 +194,11 @@ static __global__ void __launch_bounds__(kKvThreads)
     const int row = static_cast<int>(blockIdx.x) * (kKvThreads / 32) + static_cast<int>(threadIdx.x >> 5);
     if (row >= a.rows)
         return;
-    const int item0 = static_cast<int>(blockIdx.y) * kKvPasses * kItems + lane / kLanes;
+    const int item0 = static_cast<int>(blockIdx.y) * kKvWritePasses * kItems + lane / kLanes;
     const int d0 = (lane % kLanes) * V::kN;
-    uint4 raw[kKvPasses];
+    uint4 raw[kKvWritePasses];
 #pragma unroll
-    for (int p = 0; p < kKvPasses; ++p) {
+    for (int p = 0; p < kKvWritePasses; ++p) {
         const int item = item0 + p * kItems;
         raw[p] = make_uint4(0, 0, 0, 0);
         if (item < 2 * a.kvh)
@@ -206,7 +210,7 @@ static __global__ void __launch_bounds__(kKvThreads)
         return;
     uint8_t *recs = pool + block * a.kvh * R::kBytes;
 #pragma unroll
-    for (int p = 0; p < kKvPasses; ++p) {
+    for (int p = 0; p < kKvWritePasses; ++p) {
         const int item = item0 + p * kItems;
         float x[V::kN];
         V::unpack(raw[p], x);
@@ -254,16 +258,16 @@ static __global__ void __launch_bounds__(kKvThreads)
     const int row = static_cast<int>(blockIdx.x) * (kKvThreads / 32) + static_cast<int>(threadIdx.x >> 5);
     if (row >= a.rows)
         return;
-    const int item0 = static_cast<int>(blockIdx.y) * kKvPasses * kItems + lane / kLanes;
+    const int item0 = static_cast<int>(blockIdx.y) * kKvReadPasses * kItems + lane / kLanes;
     const int d0 = (lane % kLanes) * V::kN;
     int64_t block;
     int slot;
     if (!kv_row_place(a, row, lane, block, slot))
         return;
-    uint2 codes[kKvPasses];
-    float scale[kKvPasses];
+    uint2 codes[kKvReadPasses];
+    float scale[kKvReadPasses];
 #pragma unroll
-    for (int p = 0; p < kKvPasses; ++p) {
+    for (int p = 0; p < kKvReadPasses; ++p) {
         const int item = item0 + p * kItems;
         codes[p] = make_uint2(0, 0);
         scale[p] = 0.f;
@@ -278,7 +282,7 @@ static __global__ void __launch_bounds__(kKvThreads)
         }
     }
 #pragma unroll
-    for (int p = 0; p < kKvPasses; ++p) {
+    for (int p = 0; p < kKvReadPasses; ++p) {
         const int item = item0 + p * kItems;
         if (item >= 2 * a.kvh)
             continue;
@@ -308,9 +312,9 @@ inline void validate_kv_io(const void *k, const void *v, int64_t stride, const v
             "kv cache rows: rows and pool must be 16-byte aligned");
 }
 
-// A warp per row and kKvPasses x (32 / lanes per item) of its items.
-template <typename T, int D> inline dim3 kv_row_grid(int rows, int kvh) {
-    constexpr int kPer = kKvPasses * 32 / (D / KvVec<T>::kN), kWarps = kKvThreads / 32;
+// A warp per row and kPasses x (32 / lanes per item) of its items.
+template <typename T, int D, int kPasses> inline dim3 kv_row_grid(int rows, int kvh) {
+    constexpr int kPer = kPasses * 32 / (D / KvVec<T>::kN), kWarps = kKvThreads / 32;
     return dim3(static_cast<unsigned>(rows / kWarps + (rows % kWarps != 0)), static_cast<unsigned>((2 * kvh + kPer - 1) / kPer));
 }
 
@@ -330,7 +334,7 @@ template <typename T> struct KvWriteCall {
     KvRowsArgs a;
     cudaStream_t stream;
     template <int D, KvFormat kFmt> void operator()() const {
-        launch_ex(kv_quant_write_kernel<T, D, kFmt>, kv_row_grid<T, D>(a.rows, a.kvh), dim3(kKvThreads), 0, stream, k, v,
+        launch_ex(kv_quant_write_kernel<T, D, kFmt>, kv_row_grid<T, D, kKvWritePasses>(a.rows, a.kvh), dim3(kKvThreads), 0, stream, k, v,
                   stride, pool, a);
     }
 };
@@ -342,7 +346,7 @@ template <typename T> struct KvReadCall {
     KvRowsArgs a;
     cudaStream_t stream;
     template <int D, KvFormat kFmt> void operator()() const {
-        launch_ex(kv_quant_read_kernel<T, D, kFmt>, kv_row_grid<T, D>(a.rows, a.kvh), dim3(kKvThreads), 0, stream, pool,
+        launch_ex(kv_quant_read_kernel<T, D, kFmt>, kv_row_grid<T, D, kKvReadPasses>(a.rows, a.kvh), dim3(kKvThreads), 0, stream, pool,
                   k, v, stride, a);
     }
 };
