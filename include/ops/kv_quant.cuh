@@ -18,6 +18,12 @@
 // so the attention fetches a page of a head (K, V and both scales) with one
 // bulk copy: 2,176 bytes at D = 64 against 8,192 in the fp32 pools.
 //
+// Both directions are bound by HBM; a row takes the memory it must and nothing is
+// staged. Measured (kernel time, one B200; copy rate 6.45 TB/s): writing 32,768
+// rows of 8 heads x 64 fp32 as int8 28.1 us, 5.0 TB/s (instructions: 57 % of the
+// issue slots); reading 51,000 rows of 8 x 128 as bf16 55.4 us, 6.1 TB/s; the 32
+// rows of a decode step 2.8 us, launch included.
+//
 // Rows are ragged: row r belongs to the sequence b with row_start[b] <= r <
 // row_start[b + 1] and to position first_pos[b] + r - row_start[b].
 
