@@ -4,12 +4,10 @@
 // sequence, the tree mask, cluster helpers (ops/tree_attention.cuh has the
 // operator).
 
-#include <algorithm>
 #include <cstdint>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <mutex>
-#include <utility>
 #include <vector>
 
 #include "../core/cuda_utils.cuh"
@@ -41,23 +39,49 @@ struct TreeArgs {
     int64_t q_stride, out_stride;
 };
 
-// Lets `kernel` have `bytes` of dynamic shared memory and clusters of up to 16
-// CTAs on the current device
-// (set once per kernel and device; setting it twice does no harm).
-template <typename... P> inline void allow_shared_bytes(void (*kernel)(P...), int bytes) {
+// Lets `kernel` have `bytes` of dynamic shared memory and clusters above 8 CTAs on
+// the current device, and returns the largest cluster that it may be launched
+// with: 16, or the portable 8 where no part of the device has room for 16 such
+// CTAs. Asked once per kernel and device.
+template <typename... P> inline int allow_shared_bytes(void (*kernel)(P...), int threads, int bytes) {
+    struct Known {
+        const void *kernel;
+        int device, cluster;
+    };
     static std::mutex mu;
-    static std::vector<std::pair<const void *, int>> set;
-    static thread_local std::vector<std::pair<const void *, int>> seen; // no lock once a thread knows
-    const std::pair<const void *, int> key{reinterpret_cast<const void *>(kernel), device_facts().device};
-    if (std::find(seen.begin(), seen.end(), key) != seen.end())
-        return;
+    static std::vector<Known> all;
+    static thread_local std::vector<Known> mine; // no lock once a thread knows
+    const void *id = reinterpret_cast<const void *>(kernel);
+    const int device = device_facts().device;
+    for (const Known &k : mine)
+        if (k.kernel == id && k.device == device)
+            return k.cluster;
     const std::lock_guard<std::mutex> lock(mu);
-    if (std::find(set.begin(), set.end(), key) == set.end()) {
-        OPWORKS_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
-        OPWORKS_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
-        set.push_back(key);
+    for (const Known &k : all)
+        if (k.kernel == id && k.device == device) {
+            mine.push_back(k);
+            return k.cluster;
+        }
+    OPWORKS_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+    OPWORKS_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+    cudaLaunchConfig_t cfg{};
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = 16, attr.val.clusterDim.y = 1, attr.val.clusterDim.z = 1;
+    cfg.gridDim = dim3(16);
+    cfg.blockDim = dim3(static_cast<unsigned>(threads));
+    cfg.dynamicSmemBytes = static_cast<size_t>(bytes);
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    int clusters = 0;
+    if (cudaOccupancyMaxActiveClusters(&clusters, kernel, &cfg) != cudaSuccess) {
+        cudaGetLastError(); // no more than an answer to the question
+        clusters = 0;
     }
-    seen.push_back(key);
+    const Known k{id, device, clusters > 0 ? 16 : 8};
+    all.push_back(k);
+    mine.push_back(k);
+    return k.cluster;
 }
 
 // Keys and rows of a sequence, held inside the table and the row count.

@@ -731,7 +731,7 @@ template <typename T, int D, KvFormat kFmt, int kMT>
 inline void tree_rows_launch(const T *q, T *out, const TreeArgs &a, cudaStream_t stream) {
     using G = TreeRowsGeo<T, D, kFmt, kMT>;
     const auto kernel = tree_rows_kernel<T, D, kFmt, kMT>;
-    allow_shared_bytes(kernel, G::kBytes);
+    const int most = allow_shared_bytes(kernel, G::kThreads, G::kBytes);
     const int64_t rows = static_cast<int64_t>(a.t.max_rows) * (a.qh / a.kvh);
     const int64_t groups = (rows + G::kRows - 1) / G::kRows;
     const int64_t units = groups * a.kvh;
@@ -744,7 +744,7 @@ inline void tree_rows_launch(const T *q, T *out, const TreeArgs &a, cudaStream_t
     const int64_t slots = static_cast<int64_t>(G::kCtas) * device_facts().sm_count;
     const int64_t per_warp = pages / (G::kWarps * G::kChunk);
     int splits = 1;
-    while (splits < 16 && units * a.t.batch * splits * 2 <= slots && per_warp >= (splits < 8 ? splits : 64))
+    while (splits < most && units * a.t.batch * splits * 2 <= slots && per_warp >= (splits < 8 ? splits : 64))
         splits *= 2;
     require(units * splits <= 0x7fffffff, "tree attention: too many rows for one call");
     const int64_t per_sequence = units * splits, sms = device_facts().sm_count;

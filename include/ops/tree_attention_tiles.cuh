@@ -899,7 +899,7 @@ inline void tree_tiles_launch(const T *q, T *out, const TreeArgs &a, cudaStream_
     using G = TreeTilesGeo<T, D, kFmt, kM>;
     static_assert(G::kItems <= 16 && 2 * G::kItems >= kWidenWarps && G::kBytes <= 232448, "shared memory");
     const auto kernel = tree_tiles_kernel<T, D, kFmt, kM>;
-    allow_shared_bytes(kernel, G::kBytes);
+    allow_shared_bytes(kernel, kTileThreads, G::kBytes);
     const int64_t rows = static_cast<int64_t>(a.t.max_rows) * (a.qh / a.kvh);
     const int64_t groups = (rows + G::kRows - 1) / G::kRows, units = groups * a.kvh;
     const int64_t tiles = (static_cast<int64_t>(a.t.max_ctx) + a.t.max_rows + kTileKeys - 1) / kTileKeys;

@@ -270,6 +270,85 @@ def test_one_token_agrees_with_the_decode_attention(ops):
     assert (a - b).abs().max() <= 1e-5 * a.abs().max()
 
 
+@pytest.mark.parametrize("fmt", [0, 1, 2])
+def test_blocks_whose_offsets_pass_32_bits(ops, fmt):
+    """Pages at the far end of pools of over 2^31 elements (fp32) or 2^32 bytes (8 bits): written, read, attended, kept."""
+    dim, rep, ctx, rows = 64, 4, 20, 40
+    small = plain.Cache([ctx + rows], 1, dim, fmt, 6, junk=False)
+    pages = -(-(ctx + rows) // 16)
+    size = 16 * dim if fmt == 0 else 2176
+    blocks = 2**31 // size + 100 if fmt == 0 else 2**32 // size + 100
+    far = blocks - 1 - np.arange(small.stride)
+    table = dev(far[None].astype(np.int32))
+    ids = torch.from_numpy(small.table[0, :pages].astype(np.int64))
+    to = torch.from_numpy(far[:pages].copy()).cuda()
+    pools = [torch.empty(blocks, 1, 16, dim, device="cuda") for _ in range(2)] if fmt == 0 else [torch.empty(blocks, 1, size, dtype=torch.uint8, device="cuda")]
+    for big, one in zip(pools, (small.k, small.v) if fmt == 0 else (small.pool,)):
+        big[to] = one[ids].cuda()
+    parent, sees = plain.tree(np.random.default_rng(1), rows)
+    q = torch.randn(rows, rep * dim, generator=torch.Generator().manual_seed(3))
+    start, lens = dev(starts([rows])), dev(np.array([ctx], np.int32))
+    scale = 1 / math.sqrt(dim)
+    want, mass, top = plain.attention(small, q.view(rows, rep, dim), [ctx], [0, rows], [sees], scale)
+    for n in (rows, 5):  # 160 query rows, and 20
+        out = torch.empty(rows, rep * dim, device="cuda")
+        rest = (table, small.stride, lens, start if n == rows else dev(starts([n])), dev(plain.pack_mask(sees, 2)), 2, 1, n, n, ctx,
+                rep, 1, dim, scale, out, rep * dim, 0)
+        call = ops.tree_attention if fmt == 0 else ops.tree_attention_q8
+        call(dev(q), 0, rep * dim, *pools, *(() if fmt == 0 else (fmt,)), *rest)
+        err = (out[:n].cpu().double().view(n, rep, dim) - want[:n]).abs()
+        assert (err <= (2.0**-17 * mass * top + 20 * 2.0**-23 * top)[:n, :, None]).all()
+    path, count, nxt, new = (torch.empty(rows, dtype=torch.int32, device="cuda") for _ in range(4))
+    draft = np.arange(rows, dtype=np.int32)
+    target = np.full(rows, -7, np.int32)
+    for i in range(rows - 1, 0, -1):
+        target[parent[i]] = i  # the first child of each is right
+    head = (dev(draft), dev(target), dev(parent), start, lens, 1, rows)
+    tail = (1, table, small.stride, 1, dim, path, count, nxt, new, 0)
+    kept = plain.commit(draft, target, parent)
+    if fmt == 0:
+        ops.tree_commit(*head, *pools, 0, *tail)
+    else:
+        ops.tree_commit_q8(*head, *pools, 0, *tail)
+    assert path[: len(kept)].tolist() == kept and count[0].item() == len(kept) and len(kept) > 2
+    for big, one in zip(pools, (small.k, small.v) if fmt == 0 else (small.pool,)):
+        if fmt:
+            one, big = plain.views(one, dim, fmt)[0].view(torch.uint8), plain.views(big, dim, fmt)[0].view(torch.uint8)
+        for i, node in enumerate(kept):
+            src, dst = ctx + node, ctx + i
+            assert torch.equal(big[int(far[dst // 16]), 0, dst % 16].cpu(), one[int(small.table[0, src // 16]), 0, src % 16])
+    if fmt:
+        rows_in = torch.randn(rows, dim, device="cuda")
+        args = (table, small.stride, lens, start, 1, rows, 1, dim)
+        ops.kv_quant_write(rows_in, rows_in, 0, dim, pools[0], fmt, *args, 0)
+        back = torch.empty(2, rows, dim, device="cuda")
+        ops.kv_quant_read(pools[0], fmt, *args, back[0], back[1], 0, dim, 0)
+        c, s = plain.quantise(rows_in.cpu(), fmt)
+        assert torch.equal(back[0].cpu(), c.float() * s[:, None]) and torch.equal(back[0], back[1])
+
+
+@pytest.mark.parametrize("fmt", [0, 1])
+@pytest.mark.parametrize("rows", [2, 50])
+def test_a_visible_row_that_is_not_finite_shows(ops, fmt, rows):
+    """A NaN in the context makes every row NaN; in a node, the rows that see it and no others."""
+    dim, rep, ctx = 64, 2, 40
+    for bad in (7, ctx + 1):
+        cache = plain.Cache([ctx + rows], 1, dim, fmt, 3)
+        cache.spoil(0, bad)
+        q = torch.randn(rows, rep * dim, device="cuda")
+        out = torch.empty_like(q)
+        mask = plain.pack_mask(np.tril(np.ones((rows, rows), bool)), 2)
+        rest = (dev(cache.table), cache.stride, dev(np.array([ctx], np.int32)), dev(starts([rows])), dev(mask), 2, 1, rows, rows, ctx,
+                rep, 1, dim, 0.125, out, rep * dim, 0)
+        if fmt == 0:
+            ops.tree_attention(q, 0, rep * dim, dev(cache.k), dev(cache.v), *rest)
+        else:
+            ops.tree_attention_q8(q, 0, rep * dim, dev(cache.pool), fmt, *rest)
+        got = torch.isnan(out).cpu()
+        first = 0 if bad < ctx else bad - ctx
+        assert got[first:].all() and not got[:first].any()
+
+
 # ------------------------------------------------------------------ commit
 
 
