@@ -4,6 +4,7 @@
 // sequence, the tree mask, cluster helpers (ops/tree_attention.cuh has the
 // operator).
 
+#include <algorithm>
 #include <cstdint>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>

@@ -736,16 +736,16 @@ inline void tree_rows_launch(const T *q, T *out, const TreeArgs &a, cudaStream_t
     const int64_t groups = (rows + G::kRows - 1) / G::kRows;
     const int64_t units = groups * a.kvh;
     const int64_t pages = (static_cast<int64_t>(a.t.max_ctx) + a.t.max_rows + kKvPage - 1) / kKvPage;
-    // Splits while all CTAs still run at once and a warp keeps a chunk: a CTA
+    // As many splits as all CTAs still run at once and warps have a chunk: a CTA
     // has about 5 us of latencies to pay for (lengths, table, first copies,
     // joining), so a second wave costs more than it evens out (32 sequences of
     // 2180 tokens, 8 kv heads: 19.3 us with 1 split, 25.6 with 2, 33.7 with 4).
     // 16 CTAs to a cluster only where each warp has much to do.
     const int64_t slots = static_cast<int64_t>(G::kCtas) * device_facts().sm_count;
-    const int64_t per_warp = pages / (G::kWarps * G::kChunk);
-    int splits = 1;
-    while (splits < most && units * a.t.batch * splits * 2 <= slots && per_warp >= (splits < 8 ? splits : 64))
-        splits *= 2;
+    const int64_t per_warp = pages / (G::kWarps * G::kChunk), all = units * a.t.batch;
+    const int64_t room = slots / all;
+    const int64_t cap = room >= 16 && per_warp >= 64 ? most : std::min<int64_t>(8, 2 * per_warp);
+    const int splits = static_cast<int>(std::max<int64_t>(1, std::min(cap, room)));
     require(units * splits <= 0x7fffffff, "tree attention: too many rows for one call");
     const int64_t per_sequence = units * splits, sms = device_facts().sm_count;
     const bool sort = a.t.batch > 1 && a.t.batch < G::kThreads && per_sequence * a.t.batch > sms;

@@ -282,7 +282,7 @@ static __global__ void __launch_bounds__(kTileThreads, 1)
             uint32_t odd = 0;
             float unit;
             if constexpr (G::kWide) {
-                uint32_t bits = 0;
+                float most = 0.f; // largest magnitude, NaN if a value is
                 float y[G::kLoads][4];
 #pragma unroll
                 for (int j = 0; j < G::kLoads; ++j) {
@@ -303,18 +303,17 @@ static __global__ void __launch_bounds__(kTileThreads, 1)
                             if (some >> (n * kRowLanes) & (kRowLanes == 32 ? 0xffffffffu : (1u << (kRowLanes & 31)) - 1u))
                                 odd |= 1u << (j * kRowsPerLoad + n);
                     }
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        bits = max(bits, __float_as_uint(y[j][e]) & 0x7fffffffu);
+                    most = max_abs_nan(max_abs_nan(most, y[j][0], y[j][1]), y[j][2], y[j][3]);
                 }
-                bits = __reduce_max_sync(kFullWarpMask, bits);
+                const uint32_t bits = __reduce_max_sync(kFullWarpMask, __float_as_uint(most));
                 const uint32_t ex = exponent_above(bits);
                 const float f = pow2_field(254u - ex + 10u);
 #pragma unroll
                 for (int j = 0; j < G::kLoads; ++j) {
                     uint32_t h0, h1, l0, l1;
-                    terms(y[j][0] * f, y[j][1] * f, h0, l0);
-                    terms(y[j][2] * f, y[j][3] * f, h1, l1);
+                    const float2 a = __fmul2_rn(make_float2(y[j][0], y[j][1]), make_float2(f, f)), b = __fmul2_rn(make_float2(y[j][2], y[j][3]), make_float2(f, f));
+                    terms(a.x, a.y, h0, l0);
+                    terms(b.x, b.y, h1, l1);
                     const int row = row0 + j * kRowsPerLoad + lrow, dim = lbyte / 4; // 4 dims: 8 bytes of fp16
                     uint8_t *dst = tile + dim / 64 * G::kSlab + swizzled(row, dim % 64 / 8) + dim % 8 * 2;
                     *reinterpret_cast<uint2 *>(dst) = make_uint2(h0, h1);
@@ -903,10 +902,9 @@ inline void tree_tiles_launch(const T *q, T *out, const TreeArgs &a, cudaStream_
     const int64_t rows = static_cast<int64_t>(a.t.max_rows) * (a.qh / a.kvh);
     const int64_t groups = (rows + G::kRows - 1) / G::kRows, units = groups * a.kvh;
     const int64_t tiles = (static_cast<int64_t>(a.t.max_ctx) + a.t.max_rows + kTileKeys - 1) / kTileKeys;
-    // splits while all CTAs still run at once and each has four tiles
-    int splits = 1;
-    while (splits < 8 && units * a.t.batch * splits * 2 <= device_facts().sm_count && tiles >= 8 * splits)
-        splits *= 2;
+    // as many splits as all CTAs still run at once and each has four tiles
+    const int64_t all = units * a.t.batch;
+    const int splits = static_cast<int>(std::max<int64_t>(1, std::min(std::min<int64_t>(8, tiles / 4), device_facts().sm_count / all)));
     require(units * splits <= 0x7fffffff, "tree attention: too many rows for one call");
     // more CTAs than places: sequences in the order of their length
     const bool sorted = a.t.batch > 1 && a.t.batch <= kTileThreads - 1 && units * splits * a.t.batch > device_facts().sm_count;
