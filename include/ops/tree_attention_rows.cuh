@@ -41,7 +41,7 @@
 
 // Measured (kernel time): a decode step of 32 sequences of 1090 to 2180 tokens, 32
 // query and 8 kv heads of 64, int8: 18.8 us, 3.1 TB/s; 4 chains of 5 rows over up
-// to 8192 tokens, fp32 pools: 48.6 us, 2.2 TB/s; one row over 511 tokens: 7.4 us.
+// to 8192 tokens, fp32 pools: 48.6 us, 2.2 TB/s; one row over 511 tokens: 7.7 us.
 // What bounds it is instruction latency: 200 instructions per 8-bit page and tile
 // (880 per fp32 page and three tiles), 7 cycles each at the 16 (8) warps per SM
 // that registers leave room for.
