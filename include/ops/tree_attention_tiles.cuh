@@ -13,7 +13,8 @@
 // runs, the products of the other's do. With more than 128 query rows (row =
 // node * rep + head in group) the streams are two row tiles over the same keys;
 // with at most 128 they are the even and the odd key tiles of one row tile,
-// joined at the end. Each stream has S (128 columns) and O (D columns) in tensor
+// joined at the end. (fp32 rows of 128 dims: one stream, all key tiles; see
+// kSplitO.) Each stream has S (128 columns) and O (D columns) in tensor
 // memory and a warpgroup that owns a row per thread.
 //
 //   warps 0-7    softmax of stream 0, 1: S from tensor memory, weights P back
@@ -26,7 +27,10 @@
 //   warp 15      tensor memory, and one thread that issues all products
 //
 // Precision as in the rows kernel: fp32 queries and weights are two fp16 terms
-// (a product each, into the same accumulator), bf16 rows one. K and V rows are
+// (a product each), bf16 rows one. The tensor cores cut an accumulator off at
+// every step, so the error of fp32 rows grows with the keys of a CTA: relative to
+// 64 bits 1.1e-6 over 2000 keys, 6.6e-6 over 7000 in one CTA (D = 128, fp32 pools;
+// fp32 sums in torch: 1.2e-6, 1.5e-6). K and V rows are
 // widened with their scale (one term; two for fp32 rows, and for 8-bit rows too
 // where the queries are fp32: hi hi + hi lo + lo hi), but for a power of two
 // that the keys of an item share. The softmax applies that to 8, 16 or 32
@@ -61,9 +65,11 @@ template <typename T, int D, KvFormat kFmt, int kM> struct TreeTilesGeo {
     static constexpr int kQBytes = kQT * kSlabs * kM * kSlab;
     static constexpr int kOperand = kKT * kSlabs * kSlab; // K or V of a tile
     static constexpr int kStages = kKT == 2 && D == 128 ? 1 : 2;
-    // O's small products in an accumulator of their own, where tensor memory has
-    // the room: an accumulator is cut off at every step, to its size
-    static constexpr bool kSplitO = kQT == 2 && D == 64;
+    // O's small products have an accumulator of their own: one is cut off at every
+    // step, to its size. At D = 128 tensor memory has room for that with one
+    // stream (widening is what takes the time there, so that little is lost).
+    static constexpr bool kSplitO = kQT == 2;
+    static constexpr int kStreams = kSplitO && D == 128 ? 1 : 2;
     static constexpr int kKvBytes = 2 * kStages * kOperand;
     static constexpr int kRowBytes = D * (kWide ? 4 : 1);
     // an item: 4 KB of K or of V, but at most 32 keys: a tile has at least as many
@@ -82,6 +88,12 @@ template <typename T, int D, KvFormat kFmt, int kM> struct TreeTilesGeo {
     static constexpr int kFactors = 2 * (4 + kStages) * 16 * 4;
     static constexpr int kBytes = kBuf + kFactors + 4 * 256 + 8 * 256 + 8 * 256 + 256;
 };
+
+// Step e of a stream: tile e (two row tiles, or one stream), or tile 2 e + stream
+// (even and odd key tiles); from `tiles` on there is none.
+template <int kStreams, int kM> __device__ __forceinline__ int tile_at(int stream, int e, int tiles) {
+    return kStreams == 1 ? (stream == 0 ? e : tiles) : kM == 2 ? e : 2 * e + stream;
+}
 
 // K-major tile rows of 128 bytes: the byte of 16-byte chunk c of row r.
 __device__ __forceinline__ int swizzled(int r, int c) { return r * 128 + ((c ^ (r & 7)) << 4); }
@@ -271,8 +283,9 @@ static __global__ void __launch_bounds__(kTileThreads, 1)
             const bool edge = key0 + G::kItemKeys > span.ctx;
             const int before = i - G::kStages; // the tile that has the stage until its products are done
             if (before >= 0) {
-                const int e = kM == 2 ? before : before >> 1; // its step, in the last stream that reads its K
-                uint64_t *bar = v ? &v_empty[before & 3] : &s_ready[(kM == 2 ? 4 : (before & 1) * 4) + (e & 3)];
+                constexpr bool kAlternate = kM == 1 && G::kStreams == 2;
+                const int e = kAlternate ? before >> 1 : before; // its step, in the last stream that reads its K
+                uint64_t *bar = v ? &v_empty[before & 3] : &s_ready[(kM == 2 ? 4 : kAlternate ? (before & 1) * 4 : 0) + (e & 3)];
                 if (!sm100::mbar_wait_warp(bar, phase_of(v ? before : e)))
                     return false;
             }
@@ -465,8 +478,7 @@ static __global__ void __launch_bounds__(kTileThreads, 1)
                 if (leader)
                     sm100::mbar_arrive(bar);
             };
-            // step e of a stream: tile e (two row tiles) or 2 e + stream (even and odd key tiles)
-            const auto tile_of = [&](int stream, int e) { return kM == 2 ? e : 2 * e + stream; };
+            const auto tile_of = [&](int stream, int e) { return tile_at<G::kStreams, kM>(stream, e, tiles); };
             ok = sm100::mbar_wait_warp(q_full, 0);
             for (int s = 0; ok && s < 2; ++s)
                 if (tile_of(s, 0) < tiles && (kM == 2 && s == 1 ? true : k_ready(tile_of(s, 0)))) {
@@ -557,7 +569,7 @@ static __global__ void __launch_bounds__(kTileThreads, 1)
         constexpr int kGroup = G::kItemKeys, kGroups = 32 / kGroup; // keys that share their units; such groups in a chunk
         int e = 0; // steps done
         for (; ok; ++e) {
-            const int i = kM == 2 ? e : 2 * e + stream;
+            const int i = tile_at<G::kStreams, kM>(stream, e, tiles);
             if (i >= tiles)
                 break;
             const int stage = i % G::kStages, key0 = key_of(i);
