@@ -698,9 +698,11 @@ static __global__ void __launch_bounds__(kTileThreads, 1)
                     const uint32_t seen = kEdge ? seen_of(c) : 0u, odd = kEdge ? odd_of(c) : 0u;
                     // Scores and weights at once, for weights up to 2^kTileTop fit in
                     // fp16 but for a rare chunk: one with a larger one raises the
-                    // reference and is done again (its scores are still there).
+                    // reference and is done again (its scores are still there), once:
+                    // scores of 2^28 and more are rounded by more than kTileTop, so that
+                    // what is still too large then is cut off.
 #pragma unroll 1
-                    for (;;) {
+                    for (bool again = false;; again = true) {
                         float top[4] = {kNegInf, kNegInf, kNegInf, kNegInf};
 #pragma unroll
                         for (int n = 0; n < 32; n += 2) {
@@ -717,6 +719,15 @@ static __global__ void __launch_bounds__(kTileThreads, 1)
                         const float most = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
                         if (!__any_sync(kFullWarpMask, most > kTileTop))
                             break;
+                        if (again) {
+                            const float cap = exp2_approx(kTileTop);
+#pragma unroll
+                            for (int n = 0; n < 32; ++n) { // (a NaN stays)
+                                const float p = __uint_as_float(x[n / 16][n % 16]);
+                                x[n / 16][n % 16] = __float_as_uint(p > cap ? cap : p);
+                            }
+                            break;
+                        }
                         const float less = fmaxf(0.f, ceilf(most - kTileLift)), fix = exp2_approx(-less);
                         if (c < 3)
                             await(next);

@@ -1,0 +1,140 @@
+"""GPU tests of tree attention at the ends of its range: large scores, rows of unlike size, masks that leave whole tiles
+empty, long prompts.
+
+Tolerance, as in tests/test_tree_cache_gpu.py: 2^-17 mass max|v| + (keys / 16 + 16) 2^-23 max|v|, both maxima over the
+keys that the row sees (a key that it does not see has no influence), and for bf16 rows 2^-8 |o| + 2^-10 max|v| more."""
+
+import math
+
+import numpy as np
+import pytest
+
+import tree_cache_plain as plain
+
+pytestmark = pytest.mark.gpu
+torch = pytest.importorskip("torch")
+
+TYPES = {0: torch.float32, 1: torch.bfloat16}
+
+
+@pytest.fixture(scope="module")
+def ops():
+    import opworks_b200
+
+    return opworks_b200.ops_lib()
+
+
+def dev(a):
+    return (a if isinstance(a, torch.Tensor) else torch.from_numpy(np.ascontiguousarray(a))).cuda()
+
+
+def starts(rows):
+    return np.concatenate([[0], np.cumsum(rows)]).astype(np.int32)
+
+
+def attend(ops, cache, q, ctx, rows, sees, scale, max_ctx=None):
+    """q [total, q_heads, dim] over the cache -> out in 64 bits. sees: a list of [n, n] truth values, or None for chains."""
+    total, qh, dim = q.shape
+    words = max(1, -(-max(rows) // 32))
+    mask = None if sees is None else dev(np.concatenate([plain.pack_mask(s, words) for s in sees]))
+    out = torch.full((total, qh, dim), 777.0, dtype=q.dtype, device="cuda")
+    kind = 0 if q.dtype == torch.float32 else 1
+    # (held until the call has run: an operator takes plain addresses)
+    table, lens, start, dq = dev(cache.table), dev(np.array(ctx, np.int32)), dev(starts(rows)), dev(q)
+    pools = (dev(cache.k), dev(cache.v)) if cache.fmt == 0 else (dev(cache.pool),)
+    rest = (table, cache.stride, lens, start, mask, words, len(rows), total, max(rows), max(ctx) if max_ctx is None else max_ctx,
+            qh, cache.kvh, dim, scale, out, qh * dim, 0)
+    if cache.fmt == 0:
+        ops.tree_attention(dq, kind, qh * dim, *pools, *rest)
+    else:
+        ops.tree_attention_q8(dq, kind, qh * dim, *pools, cache.fmt, *rest)
+    ops.ops_sync(0)
+    return out.cpu().double()
+
+
+def expected(cache, q, ctx, rows, sees, scale):
+    """Output in 64 bits, and per row and head the largest scale sum |q k| and the largest |v| that it sees."""
+    total, qh, dim = q.shape
+    rep, start = qh // cache.kvh, starts(rows)
+    out, mass, top = torch.zeros(total, qh, dim, dtype=torch.float64), torch.zeros(total, qh, dtype=torch.float64), torch.zeros(total, qh, dtype=torch.float64)
+    for b, n in enumerate(rows):
+        if n == 0:
+            continue
+        k, v = cache.rows(b, 0, ctx[b] + n)
+        nodes = np.tril(np.ones((n, n), bool)) if sees is None else sees[b]
+        seen = torch.cat([torch.ones(n, ctx[b], dtype=torch.bool), torch.from_numpy(nodes)], 1)
+        some = seen.any(0)
+        k, v = (torch.where(some[:, None, None], x, torch.zeros((), dtype=torch.float64)) for x in (k, v))
+        for h in range(qh):
+            x = q[start[b] : start[b + 1], h].double()
+            kk, vv = k[:, h // rep], v[:, h // rep]
+            s = (scale * (x @ kk.T)).masked_fill(~seen, -math.inf)
+            w = torch.softmax(s, 1).nan_to_num(0.0)  # a row of -inf: zeros
+            sl = slice(start[b], start[b + 1])
+            out[sl, h] = w @ vv
+            mass[sl, h] = (abs(scale) * (x.abs() @ kk.abs().T)).masked_fill(~seen, 0.0).amax(1)
+            top[sl, h] = vv.abs().amax(1)[None].expand(n, -1).masked_fill(~seen, 0.0).amax(1)
+    return out, mass, top
+
+
+def tolerance(want, mass, top, keys, kind):
+    tol = (2.0**-17 * mass * top + (keys / 16 + 16) * 2.0**-23 * top)[..., None].expand_as(want)
+    return tol + 2.0**-8 * want.abs() + 2.0**-10 * top[..., None] if kind == 1 else tol
+
+
+def check(got, want, mass, top, keys, kind):
+    tol = tolerance(want, mass, top, keys, kind)
+    assert torch.isfinite(got).all()
+    err = (got - want).abs()
+    assert (err <= tol).all(), f"error {err.max():.3g}, over by {(err - tol).max():.3g}, at {(err - tol).flatten().argmax().item()}"
+
+
+def queries(total, qh, dim, kind, seed):
+    return torch.randn(total, qh, dim, generator=torch.Generator().manual_seed(seed)).to(TYPES[kind])
+
+
+def set_rows(cache, b, pos, k=None, v=None):
+    """Writes rows [n, kvh, dim] of K and V at positions `pos` of sequence b."""
+    pos = np.asarray(pos)
+    blk, slot = torch.from_numpy(cache.table[b, pos // 16].astype(np.int64)), torch.from_numpy(pos % 16)
+    for which, x in ((0, k), (1, v)):
+        if x is None:
+            continue
+        if cache.fmt == 0:
+            (cache.k, cache.v)[which][blk, :, slot] = x.float()
+        else:
+            parts = plain.views(cache.pool, cache.dim, cache.fmt)
+            c, s = plain.quantise(x, cache.fmt)
+            parts[which].view(torch.uint8)[blk, :, slot] = c.view(torch.uint8)
+            parts[2 + which][blk, :, slot] = s
+
+
+def scale_rows(cache, b, pos, factor):
+    """Multiplies the K and V rows at the positions by `factor` (8-bit: their scales)."""
+    pos = np.asarray(pos)
+    blk, slot = torch.from_numpy(cache.table[b, pos // 16].astype(np.int64)), torch.from_numpy(pos % 16)
+    if cache.fmt == 0:
+        for x in (cache.k, cache.v):
+            x[blk, :, slot] = x[blk, :, slot] * factor
+    else:
+        for x in plain.views(cache.pool, cache.dim, cache.fmt)[2:]:
+            x[blk, :, slot] = x[blk, :, slot] * factor
+
+
+# ------------------------------------------------------------------ large scores
+
+
+@pytest.mark.parametrize("size", [1e4, 1e5, 1e6])
+@pytest.mark.parametrize("fmt,kind,dim,ctx", [
+    (0, 0, 64, 500), (0, 0, 128, 500), (0, 0, 64, 3000), (0, 1, 64, 500), (0, 1, 128, 500), (1, 0, 64, 500), (1, 0, 64, 3000),
+    (1, 1, 64, 500), (1, 1, 128, 500), (2, 0, 64, 500), (2, 1, 64, 500), (2, 1, 128, 3000)])
+def test_scores_that_leave_no_bits_for_their_difference_end(ops, fmt, kind, size, dim, ctx):
+    """Scores of 2^28 to 2^40 with 50 nodes: the call returns, and what it gives is a finite mean of V rows."""
+    rows = [50]
+    cache = plain.Cache([ctx + 50], 1, dim, fmt, 5)
+    q = (queries(50, 4, dim, 0, 6) * size).to(TYPES[kind])
+    k, _ = cache.rows(0)
+    set_rows(cache, 0, np.arange(ctx + 50), k=k * size)
+    got = attend(ops, cache, q, [ctx], rows, None, 1 / math.sqrt(dim))
+    assert torch.isfinite(got).all()
+    assert got.abs().max() <= cache.rows(0)[1].abs().max() * 1.01
