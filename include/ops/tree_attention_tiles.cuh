@@ -5,9 +5,9 @@
 //
 // The floor is the tensor cores' time, nearly level with the exponential unit's.
 // What bounds it now is the chain of a tile: scores, softmax, weights, sum, each
-// waiting for the one before (6,000 cycles for 256 rows x 128 keys, of which the
+// waiting for the one before (6,800 cycles for 256 rows x 128 keys, of which the
 // products are 2,048). Measured: 32 sequences of 4096 to 8192 tokens with up to 64
-// nodes of 32 heads (8 kv heads, D = 128, int8, bf16 rows): 328 us, 0.52 PFLOP/s.
+// nodes of 32 heads (8 kv heads, D = 128, int8, bf16 rows): 372 us, 0.46 PFLOP/s.
 //
 // Two streams per CTA keep both busy: while the softmax of one stream's tile
 // runs, the products of the other's do. With more than 128 query rows (row =
@@ -30,14 +30,14 @@
 // (a product each), bf16 rows one. The tensor cores cut an accumulator off at
 // every step, so the error of fp32 rows grows with the keys of a CTA: relative to
 // 64 bits 1.1e-6 over 2000 keys, 6.6e-6 over 7000 in one CTA (D = 128, fp32 pools;
-// fp32 sums in torch: 1.2e-6, 1.5e-6). K and V rows are
-// widened with their scale (one term; two for fp32 rows, and for 8-bit rows too
-// where the queries are fp32: hi hi + hi lo + lo hi), but for a power of two
-// that the keys of an item share. The softmax applies that to 8, 16 or 32
-// scores at once, as an addition to the exponent. Factors of each key instead
-// would be a shared-memory broadcast per score: a wavefront each, 2,048 a tile
-// (an earlier form with them took 482 us for the case above, 358 with them left
-// out).
+// fp32 sums in torch: 1.2e-6, 1.5e-6). K's 8-bit codes are one exact term, and the
+// softmax multiplies a score by its key's scale, four to a shared-memory broadcast
+// (372 us for the case above, 327 with codes and scale rounded to one term, which
+// left weights of scores near -60 off by 1e-2 and more).
+// V's codes are widened with their scale, and fp32 rows as they are (one term for
+// bf16 queries over 8-bit pools, 11 bits of V being more than the output has;
+// else two: hi hi + hi lo + lo hi), but for a power of two that the keys of an
+// item share, which the softmax adds to the exponent.
 //
 // Splits of the keys form a cluster and are joined through distributed shared
 // memory in rank order.
@@ -59,18 +59,19 @@ constexpr float kTileLift = 8.f, kTileTop = 14.f, kTileShift = 24.f;
 template <typename T, int D, KvFormat kFmt, int kM> struct TreeTilesGeo {
     static constexpr bool kWide = kFmt == KvFormat::kF32;
     static constexpr int kQT = std::is_same_v<T, float> ? 2 : 1; // terms of Q and P
-    static constexpr int kKT = kWide || kQT == 2 ? 2 : 1;        // terms of K and V
+    static constexpr int kKT = kWide ? 2 : 1;                    // terms of K: 8-bit codes are exact
+    static constexpr int kVT = kWide || kQT == 2 ? 2 : 1;        // terms of V
     static constexpr int kSlabs = D / 64;                        // 64 dims: 128 bytes of fp16
     static constexpr int kSlab = kTileKeys * 128;                // bytes
     static constexpr int kQBytes = kQT * kSlabs * kM * kSlab;
-    static constexpr int kOperand = kKT * kSlabs * kSlab; // K or V of a tile
-    static constexpr int kStages = kKT == 2 && D == 128 ? 1 : 2;
+    static constexpr int kKBytes = kKT * kSlabs * kSlab, kVBytes = kVT * kSlabs * kSlab; // of a tile
+    static constexpr int kStages = kVT == 2 && D == 128 ? 1 : 2;
     // O's small products have an accumulator of their own: one is cut off at every
     // step, to its size. At D = 128 tensor memory has room for that with one
     // stream (widening is what takes the time there, so that little is lost).
     static constexpr bool kSplitO = kQT == 2;
     static constexpr int kStreams = kSplitO && D == 128 ? 1 : 2;
-    static constexpr int kKvBytes = 2 * kStages * kOperand;
+    static constexpr int kKvBytes = kStages * (kKBytes + kVBytes);
     static constexpr int kRowBytes = D * (kWide ? 4 : 1);
     // an item: 4 KB of K or of V, but at most 32 keys: a tile has at least as many
     // items as there are widening warps, so that no warp passes over a whole tile
@@ -83,9 +84,9 @@ template <typename T, int D, KvFormat kFmt, int kM> struct TreeTilesGeo {
     static constexpr int kJoin = 256 * kPitch * 4; // partial results of both streams
     static constexpr int kTiles = kQBytes + kKvBytes;
     static constexpr int kBuf = kTiles > kJoin ? kTiles : kJoin;
-    // shared powers of two of K (4 tiles) and V (their log2), and the rows that are not finite;
-    // row factors; m and l of 2 x 128 rows; joined m and l; barriers
-    static constexpr int kFactors = 2 * (4 + kStages) * 16 * 4;
+    // factors of K's keys (4 tiles), shared powers of two of V (their log2), and the rows that
+    // are not finite; row factors; m and l of 2 x 128 rows; joined m and l; barriers
+    static constexpr int kFactors = 4 * (4 * kTileKeys + kStages * 16 + (4 + kStages) * 16);
     static constexpr int kBytes = kBuf + kFactors + 4 * 256 + 8 * 256 + 8 * 256 + 256;
 };
 
@@ -147,10 +148,10 @@ static __global__ void __launch_bounds__(kTileThreads, 1)
             atomicExch(err, 5);
         return;
     }
-    uint8_t *qs = smem, *ks = qs + G::kQBytes, *vs = ks + G::kStages * G::kOperand;
+    uint8_t *qs = smem, *ks = qs + G::kQBytes, *vs = ks + G::kStages * G::kKBytes;
     // K's are read until the weights are done, longer than the K tile: tile i's lie in place i % 4
-    float *k_unit = reinterpret_cast<float *>(smem + G::kBuf);         // [4][16]: of each item
-    float *v_log = k_unit + 4 * 16;                                     // [stages][16]: log2 of V's
+    float *k_unit = reinterpret_cast<float *>(smem + G::kBuf);         // [4][128]: of each key
+    float *v_log = k_unit + 4 * kTileKeys;                              // [stages][16]: log2 of V's, of each item
     uint32_t *k_odd = reinterpret_cast<uint32_t *>(v_log + G::kStages * 16); // [4][16]: bit per key of the item
     uint32_t *v_odd = k_odd + 4 * 16;                                   // [stages][16]
     float *row_fac = reinterpret_cast<float *>(v_odd + G::kStages * 16); // [256]
@@ -266,7 +267,7 @@ static __global__ void __launch_bounds__(kTileThreads, 1)
         };
         // terms of two values into 4 bytes of the tile(s)
         const auto terms = [&](float x, float y, uint32_t &hi, uint32_t &lo) {
-            if constexpr (G::kKT == 2) {
+            if constexpr (G::kVT == 2) {
                 hi = half2_rn(x, y);
                 const float2 h = half2_floats(hi), r = __fadd2_rn(make_float2(x, y), make_float2(-h.x, -h.y));
                 lo = half2_rn(r.x, r.y);
@@ -289,7 +290,7 @@ static __global__ void __launch_bounds__(kTileThreads, 1)
                 if (!sm100::mbar_wait_warp(bar, phase_of(v ? before : e)))
                     return false;
             }
-            uint8_t *tile = (v ? vs : ks) + stage * G::kOperand;
+            uint8_t *tile = v ? vs + stage * G::kVBytes : ks + stage * G::kKBytes;
             // Rows that hold an infinity or a NaN: where all nodes see them (no
             // edge) the unit says so; else they are zeros here and marked.
             uint32_t odd = 0;
@@ -337,49 +338,65 @@ static __global__ void __launch_bounds__(kTileThreads, 1)
                 float scale = lane < left ? it.scale : 0.f;
                 const bool bad = !(fabsf(scale) <= 3.4028235e38f);
                 odd = __ballot_sync(kFullWarpMask, bad);
-                const uint32_t ex = exponent_above(__reduce_max_sync(kFullWarpMask, bad ? 0u : __float_as_uint(scale)));
-                scale = bad ? 0.f : scale * pow2_field(254u - ex + 1u); // at most 2
+                if (!v) { // the codes as they are; the softmax has a key's scale as the factor of its scores
+                    unit = bad ? edge ? 0.f : __uint_as_float(0x7fc00000u) : scale;
 #pragma unroll
-                for (int j = 0; j < G::kLoads; ++j) {
-                    const uint32_t w[4] = {it.r[j].x, it.r[j].y, it.r[j].z, it.r[j].w};
-                    const int r = j / kHalves * kRowsPerLoad + lrow, c = lbyte / 8;
-                    const float f = __shfl_sync(kFullWarpMask, scale, r);
-                    const float2 f2 = make_float2(f, f);
-                    uint32_t hi[8], lo[8];
+                    for (int j = 0; j < G::kLoads; ++j) {
+                        const uint32_t w[4] = {it.r[j].x, it.r[j].y, it.r[j].z, it.r[j].w};
+                        const int r = row0 + j / kHalves * kRowsPerLoad + lrow, c = lbyte / 8;
+                        uint32_t h[8];
 #pragma unroll
-                    for (int n = 0; n < 4; ++n) {
-                        float2 x, y;
-                        if constexpr (kFmt == KvFormat::kInt8) {
-                            // byte + 128 in the low bits of fp32 2^23 .. 2^23 + 255
-                            const uint32_t u = w[n] ^ 0x80808080u;
-                            const float2 bias = make_float2(-8388736.f, -8388736.f);
-                            x = __fadd2_rn(make_float2(__uint_as_float(__byte_perm(u, 0x4b000000u, 0x7440)), __uint_as_float(__byte_perm(u, 0x4b000000u, 0x7441))), bias);
-                            y = __fadd2_rn(make_float2(__uint_as_float(__byte_perm(u, 0x4b000000u, 0x7442)), __uint_as_float(__byte_perm(u, 0x4b000000u, 0x7443))), bias);
-                        } else {
-                            uint32_t h0, h1;
-                            codes_to_half<kFmt>(edge ? clear_e4m3_nan(w[n]) : w[n], h0, h1);
-                            x = half2_floats(h0), y = half2_floats(h1);
+                        for (int n = 0; n < 4; ++n)
+                            codes_to_half<kFmt>(kFmt == KvFormat::kE4M3 && edge ? clear_e4m3_nan(w[n]) : w[n], h[2 * n], h[2 * n + 1]);
+                        uint8_t *slab = tile + j % kHalves * G::kSlab;
+                        *reinterpret_cast<uint4 *>(slab + swizzled(r, c)) = make_uint4(h[0], h[1], h[2], h[3]);
+                        *reinterpret_cast<uint4 *>(slab + swizzled(r, c + 1)) = make_uint4(h[4], h[5], h[6], h[7]);
+                    }
+                } else {
+                    const uint32_t ex = exponent_above(__reduce_max_sync(kFullWarpMask, bad ? 0u : __float_as_uint(scale)));
+                    scale = bad ? 0.f : scale * pow2_field(254u - ex + 1u); // at most 2
+#pragma unroll
+                    for (int j = 0; j < G::kLoads; ++j) {
+                        const uint32_t w[4] = {it.r[j].x, it.r[j].y, it.r[j].z, it.r[j].w};
+                        const int r = j / kHalves * kRowsPerLoad + lrow, c = lbyte / 8;
+                        const float f = __shfl_sync(kFullWarpMask, scale, r);
+                        const float2 f2 = make_float2(f, f);
+                        uint32_t hi[8], lo[8];
+#pragma unroll
+                        for (int n = 0; n < 4; ++n) {
+                            float2 x, y;
+                            if constexpr (kFmt == KvFormat::kInt8) {
+                                // byte + 128 in the low bits of fp32 2^23 .. 2^23 + 255
+                                const uint32_t u = w[n] ^ 0x80808080u;
+                                const float2 bias = make_float2(-8388736.f, -8388736.f);
+                                x = __fadd2_rn(make_float2(__uint_as_float(__byte_perm(u, 0x4b000000u, 0x7440)), __uint_as_float(__byte_perm(u, 0x4b000000u, 0x7441))), bias);
+                                y = __fadd2_rn(make_float2(__uint_as_float(__byte_perm(u, 0x4b000000u, 0x7442)), __uint_as_float(__byte_perm(u, 0x4b000000u, 0x7443))), bias);
+                            } else {
+                                uint32_t h0, h1;
+                                codes_to_half<kFmt>(edge ? clear_e4m3_nan(w[n]) : w[n], h0, h1);
+                                x = half2_floats(h0), y = half2_floats(h1);
+                            }
+                            x = __fmul2_rn(x, f2), y = __fmul2_rn(y, f2);
+                            terms(x.x, x.y, hi[2 * n], lo[2 * n]);
+                            terms(y.x, y.y, hi[2 * n + 1], lo[2 * n + 1]);
                         }
-                        x = __fmul2_rn(x, f2), y = __fmul2_rn(y, f2);
-                        terms(x.x, x.y, hi[2 * n], lo[2 * n]);
-                        terms(y.x, y.y, hi[2 * n + 1], lo[2 * n + 1]);
+                        uint8_t *slab = tile + j % kHalves * G::kSlab, *d0 = slab + swizzled(row0 + r, c), *d1 = slab + swizzled(row0 + r, c + 1);
+                        *reinterpret_cast<uint4 *>(d0) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                        *reinterpret_cast<uint4 *>(d1) = make_uint4(hi[4], hi[5], hi[6], hi[7]);
+                        if constexpr (G::kVT == 2) {
+                            *reinterpret_cast<uint4 *>(d0 + G::kSlabs * G::kSlab) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+                            *reinterpret_cast<uint4 *>(d1 + G::kSlabs * G::kSlab) = make_uint4(lo[4], lo[5], lo[6], lo[7]);
+                        }
                     }
-                    uint8_t *slab = tile + j % kHalves * G::kSlab, *d0 = slab + swizzled(row0 + r, c), *d1 = slab + swizzled(row0 + r, c + 1);
-                    *reinterpret_cast<uint4 *>(d0) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-                    *reinterpret_cast<uint4 *>(d1) = make_uint4(hi[4], hi[5], hi[6], hi[7]);
-                    if constexpr (G::kKT == 2) {
-                        *reinterpret_cast<uint4 *>(d0 + G::kSlabs * G::kSlab) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-                        *reinterpret_cast<uint4 *>(d1 + G::kSlabs * G::kSlab) = make_uint4(lo[4], lo[5], lo[6], lo[7]);
-                    }
+                    unit = odd && !edge ? __uint_as_float(0x7fc00000u) : pow2_field(ex - 1u);
                 }
-                unit = odd && !edge ? __uint_as_float(0x7fc00000u) : pow2_field(ex - 1u);
             }
+            if (!v && lane < G::kItemKeys)
+                k_unit[(i & 3) * kTileKeys + row0 + lane] = unit;
             if (lane == 0) {
                 const int at = (v ? stage : i & 3) * 16 + part;
                 if (v) // NaN stays NaN
                     v_log[at] = unit == unit ? static_cast<float>(static_cast<int>(__float_as_uint(unit) >> 23) - 127) : unit;
-                else
-                    k_unit[at] = unit;
                 (v ? v_odd : k_odd)[at] = odd;
             }
             sm100::fence_proxy_async_smem();
@@ -420,7 +437,7 @@ static __global__ void __launch_bounds__(kTileThreads, 1)
             const uint64_t vd = sdesc_mn128_16b(sm100::smem_u32(vs), G::kSlab);
             const auto scores = [&](int stream, int i) {
                 const uint64_t q0 = qd + static_cast<uint32_t>((kM == 2 ? stream : 0) * (G::kSlab >> 4));
-                const uint64_t k0 = kd + static_cast<uint32_t>((i % G::kStages) * (G::kOperand >> 4));
+                const uint64_t k0 = kd + static_cast<uint32_t>((i % G::kStages) * (G::kKBytes >> 4));
                 const uint32_t d = tm + static_cast<uint32_t>(stream * kTileKeys);
                 const auto product = [&](auto qt, auto kt, uint32_t acc) {
 #pragma unroll
@@ -442,7 +459,7 @@ static __global__ void __launch_bounds__(kTileThreads, 1)
                 __syncwarp();
             };
             const auto weigh = [&](int stream, int i, uint32_t acc) {
-                const uint64_t v0 = vd + static_cast<uint32_t>((i % G::kStages) * (G::kOperand >> 4));
+                const uint64_t v0 = vd + static_cast<uint32_t>((i % G::kStages) * (G::kVBytes >> 4));
                 const uint32_t d = tm + 256u + static_cast<uint32_t>(stream * D), p0 = tm + static_cast<uint32_t>(stream * kTileKeys);
                 const auto product = [&](auto pt, auto vt, uint32_t d, uint32_t first) {
 #pragma unroll
@@ -578,7 +595,7 @@ static __global__ void __launch_bounds__(kTileThreads, 1)
                 break;
             }
             sm100::tc_fence_after();
-            const float *ku = k_unit + (i & 3) * 16, *vl = v_log + stage * 16;
+            const float *ku = k_unit + (i & 3) * kTileKeys, *vl = v_log + stage * 16;
             const bool edge = key0 + kTileKeys > span.ctx; // holds nodes, or places after the last key
             const auto seen_of = [&](int c) {
                 return live ? tree_sees32(a.t, span.row0 + node, node, key0 + 32 * c - span.ctx, keys - span.ctx) : 0u;
@@ -600,6 +617,17 @@ static __global__ void __launch_bounds__(kTileThreads, 1)
                 for (int n = 0; n < kGroups; ++n)
                     bits |= (k_odd[(i & 3) * 16 + kGroups * c + n] | v_odd[stage * 16 + kGroups * c + n]) << (n * kGroup & 31);
                 return bits;
+            };
+            // what two scores of chunk c are multiplied by: 8-bit keys have a factor each, four to
+            // a broadcast; the keys of a group of fp32 rows share theirs
+            const auto factors = [&](int c, int n) {
+                if constexpr (G::kWide) {
+                    const float f = rs * ku[32 * c + n / kGroup * kGroup];
+                    return make_float2(f, f);
+                } else {
+                    const float4 f = *reinterpret_cast<const float4 *>(ku + 32 * c + n / 4 * 4);
+                    return __fmul2_rn(n % 4 == 0 ? make_float2(f.x, f.y) : make_float2(f.z, f.w), make_float2(rs, rs));
+                }
             };
             // two scores of a chunk in log2 units less `m`; masked ones -inf (edge tiles)
             const auto scored = [&](const uint32_t (&x)[2][16], int n, float2 f, float2 m2, uint32_t seen, uint32_t odd, auto edge_tag) {
@@ -672,8 +700,7 @@ static __global__ void __launch_bounds__(kTileThreads, 1)
                         const uint32_t seen = kEdge ? seen_of(c) : 0u;
 #pragma unroll
                         for (int n = 0; n < 32; n += 2) {
-                            const float f = rs * ku[kGroups * c + n / kGroup];
-                            const float2 y = scored(xb, n, make_float2(f, f), make_float2(0.f, 0.f), seen, 0u, edge_tag);
+                            const float2 y = scored(xb, n, factors(c, n), make_float2(0.f, 0.f), seen, 0u, edge_tag);
                             top = fmaxf(top, fmaxf(y.x, y.y));
                         }
                     }
@@ -682,12 +709,11 @@ static __global__ void __launch_bounds__(kTileThreads, 1)
                 // one chunk of 32 keys, whose scores are in x, the next one's on their way to `next`
                 const auto chunk = [&](int c, uint32_t (&x)[2][16], uint32_t (&next)[2][16]) {
                     // weights come out as 2^(score - m + shift): the V unit (over vtop) is in the exponent
-                    float f[kGroups], shift[kGroups], less_v[kGroups];
+                    float shift[kGroups], less_v[kGroups];
                     bool small = false;
 #pragma unroll
                     for (int n = 0; n < kGroups; ++n) {
                         const float log = vl[kGroups * c + n] - vlog;
-                        f[n] = rs * ku[kGroups * c + n];
                         less_v[n] = log < -kTileShift ? log + kTileShift : 0.f;
                         shift[n] = log - less_v[n]; // NaN: every weight is
                         small |= less_v[n] != 0.f;
@@ -708,7 +734,7 @@ static __global__ void __launch_bounds__(kTileThreads, 1)
                         for (int n = 0; n < 32; n += 2) {
                             const int k = n / kGroup;
                             const float base = shift[k] - m;
-                            const float2 y = scored(x, n, make_float2(f[k], f[k]), make_float2(base, base), seen, odd, edge_tag);
+                            const float2 y = scored(x, n, factors(c, n), make_float2(base, base), seen, odd, edge_tag);
                             top[n / 2 % 4] = fmaxf(top[n / 2 % 4], fmaxf(y.x, y.y));
                             x[n / 16][n % 16] = __float_as_uint(y.x);
                             x[n / 16][n % 16 + 1] = __float_as_uint(y.y);

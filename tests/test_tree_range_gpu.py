@@ -138,3 +138,25 @@ def test_scores_that_leave_no_bits_for_their_difference_end(ops, fmt, kind, size
     got = attend(ops, cache, q, [ctx], rows, None, 1 / math.sqrt(dim))
     assert torch.isfinite(got).all()
     assert got.abs().max() <= cache.rows(0)[1].abs().max() * 1.01
+
+
+# ------------------------------------------------------------------ bits of the scores
+
+
+def opposed(rng_seed, n, heads, dim, size):
+    """n rows about -size along the direction that `along` queries have, with noise."""
+    return torch.randn(n, heads, dim, generator=torch.Generator().manual_seed(rng_seed)) - size
+
+
+@pytest.mark.parametrize("fmt", [0, 1, 2])
+@pytest.mark.parametrize("kind", [0, 1])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("ctx,rows", [(300, 3), (300, 60), (2000, 140)])
+@pytest.mark.parametrize("size", [60, 200])
+def test_scores_keep_their_bits(ops, fmt, kind, dim, ctx, rows, size):
+    """Scores of -60 and -200 in log2 units that differ by about one: a K row rounded to 11 bits would show."""
+    cache = plain.Cache([ctx + rows], 1, dim, fmt, 7)
+    set_rows(cache, 0, np.arange(ctx + rows), k=opposed(1, ctx + rows, 1, dim, size / (math.log2(math.e) * math.sqrt(dim))))
+    q = (0.2 * queries(rows, 4, dim, 0, 8) + 1.0).to(TYPES[kind])
+    got = attend(ops, cache, q, [ctx], [rows], None, 1 / math.sqrt(dim))
+    check(got, *expected(cache, q, [ctx], [rows], None, 1 / math.sqrt(dim)), ctx + rows, kind)
