@@ -50,11 +50,12 @@ namespace opworks::detail {
 constexpr int kTileKeys = 128;
 constexpr int kTileThreads = 512; // 8 softmax warps, 7 widening, 1 tensor: 4 on each scheduler, 128 registers a thread
 constexpr int kWidenWarps = 7;
-// Weights are 2^(x - m): the first tile's largest gets 2^kTileLift, and m is
+// Weights are 2^(x - m): the first visible tile's largest gets 2^kTileLift, and m is
 // raised when one would pass 2^kTileTop, so scores are looked at once, with no
 // pass for a maximum. V units enter the exponent down to 2^-kTileShift of the
 // largest; beyond that they multiply, or l would lose its weights.
 constexpr float kTileLift = 8.f, kTileTop = 14.f, kTileShift = 24.f;
+constexpr float kTileNone = -1e30f; // m of a row that has seen nothing yet
 
 template <typename T, int D, KvFormat kFmt, int kM> struct TreeTilesGeo {
     static constexpr bool kWide = kFmt == KvFormat::kF32;
@@ -581,7 +582,7 @@ static __global__ void __launch_bounds__(kTileThreads, 1)
         const uint32_t quarter = static_cast<uint32_t>((warp % 4) * 32) << 16;
         const uint32_t st = tmem + quarter + static_cast<uint32_t>(stream * kTileKeys);
         const uint32_t ot = tmem + quarter + 256u + static_cast<uint32_t>(stream * D);
-        float m = -1e30f, l = 0.f;
+        float m = kTileNone, l = 0.f;
         float vlog = kMinVLog; // log2 of a power of two, at least every V unit so far: O is in units of it
         constexpr int kGroup = G::kItemKeys, kGroups = 32 / kGroup; // keys that share their units; such groups in a chunk
         int e = 0; // steps done
@@ -691,7 +692,10 @@ static __global__ void __launch_bounds__(kTileThreads, 1)
             }
             const auto tile = [&](auto edge_tag) {
                 constexpr bool kEdge = decltype(edge_tag)::value;
-                if (e == 0) { // the first reference: the largest score of the first tile
+                // The first reference: the largest score of the first tile of which the row sees
+                // anything. It has to come from the scores: against m's first value every
+                // score is the same number.
+                if (__any_sync(kFullWarpMask, live && m == kTileNone)) {
                     float top = kNegInf;
 #pragma unroll 1
                     for (int c = 0; c < 4; ++c) {
@@ -704,7 +708,8 @@ static __global__ void __launch_bounds__(kTileThreads, 1)
                             top = fmaxf(top, fmaxf(y.x, y.y));
                         }
                     }
-                    m = fmaxf(m, top - kTileLift);
+                    if (m == kTileNone)
+                        m = fmaxf(m, top - kTileLift);
                 }
                 // one chunk of 32 keys, whose scores are in x, the next one's on their way to `next`
                 const auto chunk = [&](int c, uint32_t (&x)[2][16], uint32_t (&next)[2][16]) {

@@ -160,3 +160,35 @@ def test_scores_keep_their_bits(ops, fmt, kind, dim, ctx, rows, size):
     q = (0.2 * queries(rows, 4, dim, 0, 8) + 1.0).to(TYPES[kind])
     got = attend(ops, cache, q, [ctx], [rows], None, 1 / math.sqrt(dim))
     check(got, *expected(cache, q, [ctx], [rows], None, 1 / math.sqrt(dim)), ctx + rows, kind)
+
+
+# ------------------------------------------------------------------ masks that leave whole tiles empty
+
+
+def node_mask(shape, n):
+    i, j = np.arange(n)[:, None], np.arange(n)[None]
+    if shape == "self":  # every node is a root of its own
+        return i == j
+    if shape == "window":  # the last 20 nodes
+        return (j <= i) & (j > i - 20)
+    return (j <= i) & (i // 90 == j // 90)  # packed pieces of 90 tokens
+
+
+@pytest.mark.parametrize("fmt", [0, 1, 2])
+@pytest.mark.parametrize("kind", [0, 1])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("shape,ctx,rows", [("self", [0], [200]), ("window", [0, 100], [300, 170]), ("pieces", [0, 3], [600, 150]),
+                                            ("self", [30], [1100]), ("pieces", [0], [1300])])
+@pytest.mark.parametrize("below", [15, 60])
+def test_rows_whose_first_tile_is_masked(ops, fmt, kind, dim, shape, ctx, rows, below):
+    """Nodes that see none of the first 128 (or, in a split, any earlier) keys, with scores of about -15 and -60 in log2
+    units: one CTA's tiles, and several CTAs' (1100 nodes and more)."""
+    sees = [node_mask(shape, n) for n in rows]
+    cache = plain.Cache([c + n for c, n in zip(ctx, rows)], 1, dim, fmt, 7)
+    size = below / (math.log2(math.e) * math.sqrt(dim))
+    for b, (c, n) in enumerate(zip(ctx, rows)):
+        set_rows(cache, b, np.arange(c + n), k=opposed(b, c + n, 1, dim, size))
+    q = (0.2 * queries(sum(rows), 2, dim, 0, 8) + 1.0).to(TYPES[kind])
+    got = attend(ops, cache, q, ctx, rows, sees, 1 / math.sqrt(dim))
+    want = expected(cache, q, ctx, rows, sees, 1 / math.sqrt(dim))
+    check(got, *want, max(c + n for c, n in zip(ctx, rows)), kind)
