@@ -162,6 +162,21 @@ def test_scores_keep_their_bits(ops, fmt, kind, dim, ctx, rows, size):
     check(got, *expected(cache, q, [ctx], [rows], None, 1 / math.sqrt(dim)), ctx + rows, kind)
 
 
+@pytest.mark.parametrize("fmt", [0, 1, 2])
+@pytest.mark.parametrize("kind", [0, 1])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("size", [60, 200, 800])
+def test_scores_keep_their_bits_over_few_keys(ops, fmt, kind, dim, size):
+    """The same with 20 keys to a node, among which errors do not average out; 100 nodes are one tile of keys."""
+    rows = 100
+    cache = plain.Cache([rows], 1, dim, fmt, 9)
+    set_rows(cache, 0, np.arange(rows), k=opposed(2, rows, 1, dim, size / (math.log2(math.e) * math.sqrt(dim))))
+    q = (0.2 * queries(rows, 4, dim, 0, 8) + 1.0).to(TYPES[kind])
+    sees = [node_mask("window", rows)]
+    got = attend(ops, cache, q, [0], [rows], sees, 1 / math.sqrt(dim))
+    check(got, *expected(cache, q, [0], [rows], sees, 1 / math.sqrt(dim)), rows, kind)
+
+
 # ------------------------------------------------------------------ masks that leave whole tiles empty
 
 
