@@ -5,9 +5,9 @@
 //
 // The floor is the tensor cores' time, nearly level with the exponential unit's.
 // What bounds it now is the chain of a tile: scores, softmax, weights, sum, each
-// waiting for the one before (6,800 cycles for 256 rows x 128 keys, of which the
+// waiting for the one before (6,450 cycles for 256 rows x 128 keys, of which the
 // products are 2,048). Measured: 32 sequences of 4096 to 8192 tokens with up to 64
-// nodes of 32 heads (8 kv heads, D = 128, int8, bf16 rows): 372 us, 0.46 PFLOP/s.
+// nodes of 32 heads (8 kv heads, D = 128, int8, bf16 rows): 353 us, 0.49 PFLOP/s.
 //
 // Two streams per CTA keep both busy: while the softmax of one stream's tile
 // runs, the products of the other's do. With more than 128 query rows (row =
@@ -32,12 +32,12 @@
 // 64 bits 1.1e-6 over 2000 keys, 6.6e-6 over 7000 in one CTA (D = 128, fp32 pools;
 // fp32 sums in torch: 1.2e-6, 1.5e-6). K's 8-bit codes are one exact term, and the
 // softmax multiplies a score by its key's scale, four to a shared-memory broadcast
-// (372 us for the case above, 327 with codes and scale rounded to one term, which
+// (353 us for the case above, 25 less with codes and scale rounded to one term, which
 // left weights of scores near -60 off by 1e-2 and more).
 // V's codes are widened with their scale, and fp32 rows as they are (one term for
 // bf16 queries over 8-bit pools, 11 bits of V being more than the output has;
 // else two: hi hi + hi lo + lo hi), but for a power of two that the keys of an
-// item share, which the softmax adds to the exponent.
+// item share, which the softmax adds to the exponent (see kUnlike).
 //
 // Splits of the keys form a cluster and are joined through distributed shared
 // memory in rank order.
@@ -50,11 +50,16 @@ namespace opworks::detail {
 constexpr int kTileKeys = 128;
 constexpr int kTileThreads = 512; // 8 softmax warps, 7 widening, 1 tensor: 4 on each scheduler, 128 registers a thread
 constexpr int kWidenWarps = 7;
-// Weights are 2^(x - m): the first visible tile's largest gets 2^kTileLift, and m is
+// Weights are 2^(x - m), with the log2 of the key's V unit in x, so that they are
+// what O takes up: the first visible tile's largest gets 2^kTileLift, and m is
 // raised when one would pass 2^kTileTop, so scores are looked at once, with no
-// pass for a maximum. V units enter the exponent down to 2^-kTileShift of the
-// largest; beyond that they multiply, or l would lose its weights.
-constexpr float kTileLift = 8.f, kTileTop = 14.f, kTileShift = 24.f;
+// pass for a maximum. l sums them over their V units.
+constexpr float kTileLift = 8.f, kTileTop = 14.f;
+// The keys of an item share a unit unless some of its nodes' rows are 2^kUnlike
+// smaller than its largest: then each has its own, for a row that a node does not
+// see takes no bits from those that it sees. V units are 2^-60 at least (exponent
+// field kMinVField - 1): lower, and l would leave fp32's range beside large rows.
+constexpr uint32_t kUnlike = 12, kMinVField = 68;
 constexpr float kTileNone = -1e30f; // m of a row that has seen nothing yet
 
 template <typename T, int D, KvFormat kFmt, int kM> struct TreeTilesGeo {
@@ -85,9 +90,10 @@ template <typename T, int D, KvFormat kFmt, int kM> struct TreeTilesGeo {
     static constexpr int kJoin = 256 * kPitch * 4; // partial results of both streams
     static constexpr int kTiles = kQBytes + kKvBytes;
     static constexpr int kBuf = kTiles > kJoin ? kTiles : kJoin;
-    // factors of K's keys (4 tiles), shared powers of two of V (their log2), and the rows that
-    // are not finite; row factors; m and l of 2 x 128 rows; joined m and l; barriers
-    static constexpr int kFactors = 4 * (4 * kTileKeys + kStages * 16 + (4 + kStages) * 16);
+    // factors of K's keys (4 tiles), V's units as log2 and turned round (stages), the rows that
+    // are not finite, and the items whose keys have a unit each; row factors; m and l of 2 x 128
+    // rows; joined m and l; barriers
+    static constexpr int kFactors = 4 * ((4 + 2 * kStages) * kTileKeys + (4 + kStages) * 16) + (4 + kStages) * 16;
     static constexpr int kBytes = kBuf + kFactors + 4 * 256 + 8 * 256 + 8 * 256 + 256;
 };
 
@@ -152,10 +158,12 @@ static __global__ void __launch_bounds__(kTileThreads, 1)
     uint8_t *qs = smem, *ks = qs + G::kQBytes, *vs = ks + G::kStages * G::kKBytes;
     // K's are read until the weights are done, longer than the K tile: tile i's lie in place i % 4
     float *k_unit = reinterpret_cast<float *>(smem + G::kBuf);         // [4][128]: of each key
-    float *v_log = k_unit + 4 * kTileKeys;                              // [stages][16]: log2 of V's, of each item
-    uint32_t *k_odd = reinterpret_cast<uint32_t *>(v_log + G::kStages * 16); // [4][16]: bit per key of the item
+    float *v_log = k_unit + 4 * kTileKeys;                              // [stages][128]: log2 of V's unit
+    float *v_inv = v_log + G::kStages * kTileKeys;                      // [stages][128]: 2^-v_log
+    uint32_t *k_odd = reinterpret_cast<uint32_t *>(v_inv + G::kStages * kTileKeys); // [4][16]: bit per key of the item
     uint32_t *v_odd = k_odd + 4 * 16;                                   // [stages][16]
-    float *row_fac = reinterpret_cast<float *>(v_odd + G::kStages * 16); // [256]
+    uint8_t *k_each = reinterpret_cast<uint8_t *>(v_odd + G::kStages * 16), *v_each = k_each + 4 * 16; // [4][16], [stages][16]
+    float *row_fac = reinterpret_cast<float *>(v_each + G::kStages * 16); // [256]
     float *stat = row_fac + 256;                                    // m [256], l [256]
     float *joined = stat + 512;                                     // m [256], l [256] of the CTA
     uint64_t *bars = reinterpret_cast<uint64_t *>(joined + 512);
@@ -295,7 +303,17 @@ static __global__ void __launch_bounds__(kTileThreads, 1)
             // Rows that hold an infinity or a NaN: where all nodes see them (no
             // edge) the unit says so; else they are zeros here and marked.
             uint32_t odd = 0;
+            bool each = false; // the item's keys have a unit each, not one for all
             float unit;
+            const auto put_unit = [&](int row, float unit) { // of the tile's key `row`; NaN stays NaN
+                if (v) {
+                    const int field = static_cast<int>(__float_as_uint(unit) >> 23);
+                    v_log[stage * kTileKeys + row] = unit == unit ? static_cast<float>(field - 127) : unit;
+                    v_inv[stage * kTileKeys + row] = pow2_field(254 - field);
+                } else {
+                    k_unit[(i & 3) * kTileKeys + row] = unit;
+                }
+            };
             if constexpr (G::kWide) {
                 float most = 0.f; // largest magnitude, NaN if a value is
                 float y[G::kLoads][4];
@@ -321,8 +339,41 @@ static __global__ void __launch_bounds__(kTileThreads, 1)
                     most = max_abs_nan(max_abs_nan(most, y[j][0], y[j][1]), y[j][2], y[j][3]);
                 }
                 const uint32_t bits = __reduce_max_sync(kFullWarpMask, __float_as_uint(most));
-                const uint32_t ex = exponent_above(bits);
+                const uint32_t ex = max(exponent_above(bits), v ? kMinVField + 9u : 0u);
                 const float f = pow2_field(254u - ex + 10u);
+                unit = bits < 0x7f800000u ? pow2_field(ex - 10u) : __uint_as_float(0x7fc00000u);
+                if (edge) { // a row that some nodes do not see takes no bits from the others
+                    const float low = pow2_field(max(ex, kUnlike + 1u) - kUnlike);
+                    const auto top = [&](int j) { return max_abs_nan(max_abs_nan(y[j][0], y[j][1], y[j][2]), y[j][3], y[j][3]); };
+                    float least = low;
+#pragma unroll
+                    for (int j = 0; j < G::kLoads; ++j)
+                        least = fminf(least, top(j));
+                    if (__any_sync(kFullWarpMask, least < low)) // (four values of a row that are all small)
+#pragma unroll 1
+                        for (int n = 0; n < G::kItemKeys; ++n) {
+                            float t = 0.f;
+#pragma unroll
+                            for (int j = 0; j < G::kLoads; ++j)
+                                t = j * kRowsPerLoad + lrow == n ? top(j) : t;
+                            const uint32_t all = __reduce_max_sync(kFullWarpMask, __float_as_uint(t));
+                            each |= all > 0u && all < __float_as_uint(low);
+                        }
+                    if (each) // rows to the item's size, for their units to make up for
+#pragma unroll
+                        for (int j = 0; j < G::kLoads; ++j) {
+                            float t = top(j);
+#pragma unroll
+                            for (int off = 1; off < kRowLanes; off <<= 1)
+                                t = fmaxf(t, __shfl_xor_sync(kFullWarpMask, t, off));
+                            const uint32_t own = max(exponent_above(__float_as_uint(t)), v ? kMinVField + 9u : 0u);
+#pragma unroll
+                            for (int e = 0; e < 4; ++e)
+                                y[j][e] = y[j][e] * pow2_field(254u - own + 10u) * pow2_field(ex - 10u);
+                            if (lbyte == 0)
+                                put_unit(row0 + j * kRowsPerLoad + lrow, pow2_field(own - 10u));
+                        }
+                }
 #pragma unroll
                 for (int j = 0; j < G::kLoads; ++j) {
                     uint32_t h0, h1, l0, l1;
@@ -334,7 +385,6 @@ static __global__ void __launch_bounds__(kTileThreads, 1)
                     *reinterpret_cast<uint2 *>(dst) = make_uint2(h0, h1);
                     *reinterpret_cast<uint2 *>(dst + G::kSlabs * G::kSlab) = make_uint2(l0, l1);
                 }
-                unit = bits < 0x7f800000u ? pow2_field(ex - 10u) : __uint_as_float(0x7fc00000u);
             } else {
                 float scale = lane < left ? it.scale : 0.f;
                 const bool bad = !(fabsf(scale) <= 3.4028235e38f);
@@ -354,7 +404,11 @@ static __global__ void __launch_bounds__(kTileThreads, 1)
                         *reinterpret_cast<uint4 *>(slab + swizzled(r, c + 1)) = make_uint4(h[4], h[5], h[6], h[7]);
                     }
                 } else {
-                    const uint32_t ex = exponent_above(__reduce_max_sync(kFullWarpMask, bad ? 0u : __float_as_uint(scale)));
+                    const uint32_t own = bad ? 0u : __float_as_uint(scale);
+                    uint32_t ex = exponent_above(__reduce_max_sync(kFullWarpMask, own));
+                    if (edge) // a row that some nodes do not see takes no bits from the others
+                        each = !__all_sync(kFullWarpMask, own == 0u || exponent_above(own) + kUnlike >= ex);
+                    ex = max(each ? exponent_above(own) : ex, kMinVField);
                     scale = bad ? 0.f : scale * pow2_field(254u - ex + 1u); // at most 2
 #pragma unroll
                     for (int j = 0; j < G::kLoads; ++j) {
@@ -392,13 +446,12 @@ static __global__ void __launch_bounds__(kTileThreads, 1)
                     unit = odd && !edge ? __uint_as_float(0x7fc00000u) : pow2_field(ex - 1u);
                 }
             }
-            if (!v && lane < G::kItemKeys)
-                k_unit[(i & 3) * kTileKeys + row0 + lane] = unit;
+            if (lane < G::kItemKeys && !(G::kWide && each))
+                put_unit(row0 + lane, unit);
             if (lane == 0) {
                 const int at = (v ? stage : i & 3) * 16 + part;
-                if (v) // NaN stays NaN
-                    v_log[at] = unit == unit ? static_cast<float>(static_cast<int>(__float_as_uint(unit) >> 23) - 127) : unit;
                 (v ? v_odd : k_odd)[at] = odd;
+                (v ? v_each : k_each)[at] = each;
             }
             sm100::fence_proxy_async_smem();
             __syncwarp();
@@ -583,7 +636,6 @@ static __global__ void __launch_bounds__(kTileThreads, 1)
         const uint32_t st = tmem + quarter + static_cast<uint32_t>(stream * kTileKeys);
         const uint32_t ot = tmem + quarter + 256u + static_cast<uint32_t>(stream * D);
         float m = kTileNone, l = 0.f;
-        float vlog = kMinVLog; // log2 of a power of two, at least every V unit so far: O is in units of it
         constexpr int kGroup = G::kItemKeys, kGroups = 32 / kGroup; // keys that share their units; such groups in a chunk
         int e = 0; // steps done
         for (; ok; ++e) {
@@ -596,7 +648,7 @@ static __global__ void __launch_bounds__(kTileThreads, 1)
                 break;
             }
             sm100::tc_fence_after();
-            const float *ku = k_unit + (i & 3) * kTileKeys, *vl = v_log + stage * 16;
+            const float *ku = k_unit + (i & 3) * kTileKeys, *vl = v_log + stage * kTileKeys, *vi = v_inv + stage * kTileKeys;
             const bool edge = key0 + kTileKeys > span.ctx; // holds nodes, or places after the last key
             const auto seen_of = [&](int c) {
                 return live ? tree_sees32(a.t, span.row0 + node, node, key0 + 32 * c - span.ctx, keys - span.ctx) : 0u;
@@ -621,13 +673,23 @@ static __global__ void __launch_bounds__(kTileThreads, 1)
             };
             // what two scores of chunk c are multiplied by: 8-bit keys have a factor each, four to
             // a broadcast; the keys of a group of fp32 rows share theirs
-            const auto factors = [&](int c, int n) {
-                if constexpr (G::kWide) {
+            const auto factors = [&](int c, int n, auto each_tag) {
+                if constexpr (G::kWide && !decltype(each_tag)::value) {
                     const float f = rs * ku[32 * c + n / kGroup * kGroup];
                     return make_float2(f, f);
                 } else {
                     const float4 f = *reinterpret_cast<const float4 *>(ku + 32 * c + n / 4 * 4);
                     return __fmul2_rn(n % 4 == 0 ? make_float2(f.x, f.y) : make_float2(f.z, f.w), make_float2(rs, rs));
+                }
+            };
+            // log2 of the V units of two keys of chunk c, less m
+            const auto bases = [&](int c, int n, float m, auto each_tag) {
+                if constexpr (decltype(each_tag)::value) {
+                    const float2 log = *reinterpret_cast<const float2 *>(vl + 32 * c + n);
+                    return make_float2(log.x - m, log.y - m);
+                } else {
+                    const float base = vl[32 * c + n / kGroup * kGroup] - m;
+                    return make_float2(base, base);
                 }
             };
             // two scores of a chunk in log2 units less `m`; masked ones -inf (edge tiles)
@@ -647,10 +709,6 @@ static __global__ void __launch_bounds__(kTileThreads, 1)
                 ok = false;
                 break;
             }
-            float vnew = kMinVLog;
-#pragma unroll
-            for (int c = 0; c < G::kItems; ++c)
-                vnew = fmaxf(vnew, vl[c]);
             // O, where there is one, times fix; the weights of this tile's first `c` chunks too
             const auto rescale = [&](float fix, int c) {
                 if (e > 0) {
@@ -685,13 +743,8 @@ static __global__ void __launch_bounds__(kTileThreads, 1)
                 }
                 tile_tmem_wait_st();
             };
-            if (vnew > vlog) { // the same in every thread of the stream
-                await(xa);
-                rescale(exp2_approx(vlog - vnew), 0);
-                vlog = vnew;
-            }
-            const auto tile = [&](auto edge_tag) {
-                constexpr bool kEdge = decltype(edge_tag)::value;
+            const auto tile = [&](auto edge_tag, auto each_tag) {
+                constexpr bool kEdge = decltype(edge_tag)::value, kEach = decltype(each_tag)::value;
                 // The first reference: the largest score of the first tile of which the row sees
                 // anything. It has to come from the scores: against m's first value every
                 // score is the same number.
@@ -704,7 +757,7 @@ static __global__ void __launch_bounds__(kTileThreads, 1)
                         const uint32_t seen = kEdge ? seen_of(c) : 0u;
 #pragma unroll
                         for (int n = 0; n < 32; n += 2) {
-                            const float2 y = scored(xb, n, factors(c, n), make_float2(0.f, 0.f), seen, 0u, edge_tag);
+                            const float2 y = scored(xb, n, factors(c, n, each_tag), bases(c, n, 0.f, each_tag), seen, 0u, edge_tag);
                             top = fmaxf(top, fmaxf(y.x, y.y));
                         }
                     }
@@ -713,16 +766,6 @@ static __global__ void __launch_bounds__(kTileThreads, 1)
                 }
                 // one chunk of 32 keys, whose scores are in x, the next one's on their way to `next`
                 const auto chunk = [&](int c, uint32_t (&x)[2][16], uint32_t (&next)[2][16]) {
-                    // weights come out as 2^(score - m + shift): the V unit (over vtop) is in the exponent
-                    float shift[kGroups], less_v[kGroups];
-                    bool small = false;
-#pragma unroll
-                    for (int n = 0; n < kGroups; ++n) {
-                        const float log = vl[kGroups * c + n] - vlog;
-                        less_v[n] = log < -kTileShift ? log + kTileShift : 0.f;
-                        shift[n] = log - less_v[n]; // NaN: every weight is
-                        small |= less_v[n] != 0.f;
-                    }
                     await(x);
                     if (c < 3)
                         ask(c + 1, next);
@@ -737,9 +780,7 @@ static __global__ void __launch_bounds__(kTileThreads, 1)
                         float top[4] = {kNegInf, kNegInf, kNegInf, kNegInf};
 #pragma unroll
                         for (int n = 0; n < 32; n += 2) {
-                            const int k = n / kGroup;
-                            const float base = shift[k] - m;
-                            const float2 y = scored(x, n, factors(c, n), make_float2(base, base), seen, odd, edge_tag);
+                            const float2 y = scored(x, n, factors(c, n, each_tag), bases(c, n, m, each_tag), seen, odd, edge_tag);
                             top[n / 2 % 4] = fmaxf(top[n / 2 % 4], fmaxf(y.x, y.y));
                             x[n / 16][n % 16] = __float_as_uint(y.x);
                             x[n / 16][n % 16 + 1] = __float_as_uint(y.y);
@@ -768,21 +809,6 @@ static __global__ void __launch_bounds__(kTileThreads, 1)
                         ask(c, x);
                         await(x);
                     }
-                    float take[kGroups]; // from weights as they come out to l
-#pragma unroll
-                    for (int n = 0; n < kGroups; ++n)
-                        take[n] = exp2_approx(-shift[n]);
-                    if (small) { // V rows that small against others: l first, then the rest of their unit
-#pragma unroll
-                        for (int n = 0; n < 32; ++n) {
-                            const float p = __uint_as_float(x[n / 16][n % 16]);
-                            l = fmaf(p, take[n / kGroup], l);
-                            x[n / 16][n % 16] = __float_as_uint(p * exp2_approx(fmaxf(less_v[n / kGroup], -120.f)));
-                        }
-#pragma unroll
-                        for (int n = 0; n < kGroups; ++n)
-                            take[n] = 0.f;
-                    }
                     float2 sum[kGroups];
 #pragma unroll
                     for (int n = 0; n < kGroups; ++n)
@@ -794,7 +820,10 @@ static __global__ void __launch_bounds__(kTileThreads, 1)
                         for (int n = 0; n < 8; ++n) {
                             const int k = (16 * part + 2 * n) / kGroup;
                             const float2 p = make_float2(__uint_as_float(x[part][2 * n]), __uint_as_float(x[part][2 * n + 1]));
-                            sum[k] = __fadd2_rn(sum[k], p);
+                            if constexpr (kEach)
+                                sum[0] = __ffma2_rn(p, *reinterpret_cast<const float2 *>(vi + 32 * c + 16 * part + 2 * n), sum[0]);
+                            else
+                                sum[k] = __fadd2_rn(sum[k], p);
                             hi[n] = half2_rn(p.x, p.y);
                             if constexpr (G::kQT == 2) {
                                 const float2 w = half2_floats(hi[n]);
@@ -807,8 +836,8 @@ static __global__ void __launch_bounds__(kTileThreads, 1)
                             tile_tmem_st8(st + static_cast<uint32_t>(32 * c + 16 + 8 * part), lo);
                     }
 #pragma unroll
-                    for (int n = 0; n < kGroups; ++n)
-                        l = fmaf(sum[n].x + sum[n].y, take[n], l);
+                    for (int n = 0; n < (kEach ? 1 : kGroups); ++n) // from weights in units of V to l
+                        l = fmaf(sum[n].x + sum[n].y, kEach ? 1.f : vi[32 * c + n * kGroup], l);
                 };
 #pragma unroll 1
                 for (int c = 0; c < 4; c += 2) {
@@ -816,10 +845,18 @@ static __global__ void __launch_bounds__(kTileThreads, 1)
                     chunk(c + 1, xb, xa);
                 }
             };
-            if (edge)
-                tile(std::true_type{});
+            // whether an item of the tile has a unit for each key (edge tiles)
+            const auto any_each = [&] {
+                const uint4 k = *reinterpret_cast<const uint4 *>(k_each + (i & 3) * 16), v = *reinterpret_cast<const uint4 *>(v_each + stage * 16);
+                const uint32_t none = G::kItems < 16 ? 0u : ~0u; // what lies after the items is not theirs
+                return ((k.x | v.x) | (G::kItems >= 8 ? k.y | v.y : 0u) | ((k.z | v.z | k.w | v.w) & none)) != 0u;
+            };
+            if (!edge)
+                tile(std::false_type{}, std::false_type{});
+            else if (!any_each())
+                tile(std::true_type{}, std::false_type{});
             else
-                tile(std::false_type{});
+                tile(std::true_type{}, std::true_type{});
             tile_tmem_wait_st();
             sm100::tc_fence_before();
             __syncwarp();
@@ -831,12 +868,11 @@ static __global__ void __launch_bounds__(kTileThreads, 1)
         if (any && !sm100::mbar_wait_warp(drain, 0)) // all products: O is there, and the tiles are free
             ok = false;
         sm100::tc_fence_after();
-        const float vtop = pow2_field(static_cast<uint32_t>(127 + static_cast<int>(vlog)));
         const bool direct = kM == 2 && splits == 1;
         // where nothing is joined a row goes out as it is; else to shared memory, once all products are done
         if (!direct)
             asm volatile("bar.sync 1, 256;" ::: "memory"); // both streams have waited for that
-        const float inv = l == 0.f ? 0.f : vtop / l;
+        const float inv = l == 0.f ? 0.f : 1.f / l;
         T *dst = out + static_cast<int64_t>(span.row0 + node) * a.out_stride + static_cast<int64_t>(h * rep + row % rep) * D;
         float *part = reinterpret_cast<float *>(smem) + (stream * 128 + r) * G::kPitch;
 #pragma unroll 1
@@ -875,8 +911,7 @@ static __global__ void __launch_bounds__(kTileThreads, 1)
 #pragma unroll
                 for (int k = 0; k < 16; k += 4)
                     *reinterpret_cast<float4 *>(part + c + k) =
-                        make_float4(__uint_as_float(o[k]) * vtop, __uint_as_float(o[k + 1]) * vtop,
-                                    __uint_as_float(o[k + 2]) * vtop, __uint_as_float(o[k + 3]) * vtop);
+                        make_float4(__uint_as_float(o[k]), __uint_as_float(o[k + 1]), __uint_as_float(o[k + 2]), __uint_as_float(o[k + 3]));
             }
         }
         stat[stream * 128 + r] = m;

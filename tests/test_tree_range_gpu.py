@@ -207,3 +207,31 @@ def test_rows_whose_first_tile_is_masked(ops, fmt, kind, dim, shape, ctx, rows, 
     got = attend(ops, cache, q, ctx, rows, sees, 1 / math.sqrt(dim))
     want = expected(cache, q, ctx, rows, sees, 1 / math.sqrt(dim))
     check(got, *want, max(c + n for c, n in zip(ctx, rows)), kind)
+
+
+# ------------------------------------------------------------------ rows of unlike size
+
+
+def hidden_large_rows(ops, fmt, kind, dim, ctx, n, factor, alone):
+    """Nodes whose K and V rows (8-bit: scales) are `factor` times as large as the others': hidden from every node, or
+    (alone) seen by themselves only."""
+    rng = np.random.default_rng(3)
+    cache = plain.Cache([ctx + n], 2, dim, fmt, 11)
+    sees = plain.tree(rng, n)[1]
+    bad = sorted({1, n // 2, n - 1})
+    for j in bad:
+        sees[:, j] = False
+        sees[j, j] = alone
+    scale_rows(cache, 0, [ctx + j for j in bad], factor)
+    q = queries(n, 8, dim, kind, 12)
+    got = attend(ops, cache, q, [ctx], [n], [sees], 1 / math.sqrt(dim))
+    check(got, *expected(cache, q, [ctx], [n], [sees], 1 / math.sqrt(dim)), ctx + n, kind)
+
+
+@pytest.mark.parametrize("fmt,kind,dim", [(0, 0, 64), (0, 0, 128), (0, 1, 64), (0, 1, 128), (1, 0, 64), (1, 1, 64), (1, 1, 128),
+                                          (2, 0, 64), (2, 1, 64), (2, 1, 128)])
+@pytest.mark.parametrize("ctx,n", [(0, 70), (50, 60), (300, 200)])
+@pytest.mark.parametrize("factor", [1e6, 1e20, 1e30])
+@pytest.mark.parametrize("alone", [False, True])
+def test_large_rows_that_a_node_does_not_see(ops, fmt, kind, dim, ctx, n, factor, alone):
+    hidden_large_rows(ops, fmt, kind, dim, ctx, n, factor, alone)
