@@ -147,8 +147,11 @@ __device__ __forceinline__ uint32_t tree_sees32(const TreeBatch &t, int row, int
 constexpr float kLazy = 4.f;  // log2 units a score may pass the reference maximum by
 constexpr float kLift = 10.f; // P is scaled by 2^kLift: at most 2^14
 // V scales below this are not told apart from it (fp16 loses their low bits);
-// lower, and l in their units would leave fp32's range
+// lower, and l in their units would leave fp32's range. The same for the
+// magnitudes of single fp32 V rows.
 constexpr float kMinVLog = -80.f, kMinVTop = 0x1p-80f;
+constexpr int kMinVKey = -60;
+constexpr float kLowV = 0x1p-12f; // V scales this far below their power of two get a new one
 
 // fp16 pair (a, b) as one register, a in the low half
 __device__ __forceinline__ uint32_t half2_rn(float a, float b) {

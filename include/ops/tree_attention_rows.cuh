@@ -36,8 +36,11 @@
 // only: it is raised when a score passes it by kLazy, so most chunks rescale
 // nothing. P is held as 2^kLift times its value, so that fp16 keeps 22 bits of
 // two terms down to 2^-28 of the largest weight. The V scales of 8-bit pools
-// are folded into P, relative to a running power of two that counts as part of
-// the reference (l and O carry it both).
+// are folded into P, and a power of two above them into the reference.
+//
+// Chunks that hold nodes: every K and V row has a power of two of its own there,
+// and the reference of a query row counts those V rows only that it sees, so a
+// row that is masked takes no bits from the others, whatever its size.
 //
 // Measured (kernel time): a decode step of 32 sequences of 1090 to 2180 tokens, 32
 // query and 8 kv heads of 64, int8: 18.8 us, 3.1 TB/s; 4 chains of 5 rows over up
@@ -253,8 +256,8 @@ static __global__ void __launch_bounds__(TreeRowsGeo<T, D, kFmt, kMT>::kThreads,
     float o[kMT][D / 8][4] = {};
     // m: the reference that weights are relative to, 2^(x - m)
     float m[kMT][G::kRPL], l[kMT][G::kRPL];
-    // 8-bit: a power of two above every V scale so far and its log2, part of m.
-    // fp32: the powers of two that K and V are multiplied by (0: not chosen yet)
+    // 8-bit: a power of two next above the V scales of late and its log2, which goes
+    // into m. fp32: the powers of two that K and V are multiplied by (0: not chosen yet)
     float vtop = kMinVTop, vlog = kMinVLog, kmul = 0.f, vmul = 0.f;
 #pragma unroll
     for (int mt = 0; mt < kMT; ++mt)
@@ -286,6 +289,8 @@ static __global__ void __launch_bounds__(TreeRowsGeo<T, D, kFmt, kMT>::kThreads,
         constexpr bool kEdge = decltype(edge_tag)::value;
         float sc[kMT][2 * kC][4];
         float kfac[4 * kC], vfac[4 * kC]; // factors of a lane's scores and weights
+        float vlogs[kEdge ? 4 * kC : 1];  // log2 of the weights' factors, or a little more
+        float vkey[kEdge ? 4 : 1];        // fp32: what V rows are multiplied by
         uint32_t bad = 0;                 // bit i: fp32 row i of the lane holds an infinity or a NaN
         float x[kMT][G::kRPL][4 * kC];
         const auto zero_scores = [&] {
@@ -314,34 +319,65 @@ static __global__ void __launch_bounds__(TreeRowsGeo<T, D, kFmt, kMT>::kThreads,
         };
 
         if constexpr (G::kWide) {
-            if (kEdge) {
-                // rows that are not finite: lanes 4 key .. of a ballot hold a key's eighths
+            float kkey[2] = {kmul, kmul}; // what the lane's two K rows are multiplied by
+            if constexpr (kEdge) {
+                // Rows that are not finite, and each row's largest magnitude: a row that a
+                // node does not see takes no bits from the others. Lanes t, t + 4, .. hold
+                // a row's eighths.
+                if (vmul == 0.f)
+                    vmul = 1.f;
+                uint32_t kex[4];
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
 #pragma unroll
                     for (int part = 0; part < 2; ++part) {
                         const float4 *src = reinterpret_cast<const float4 *>(chunk + (part * kKvPage + 4 * i + t) * D * 4) + g;
                         bool odd = false;
+                        uint32_t top = 0;
 #pragma unroll
                         for (int c = 0; c < D / 32; ++c) {
                             const float4 w = src[8 * c];
-                            odd |= !(fabsf(w.x) <= 3.4028235e38f && fabsf(w.y) <= 3.4028235e38f &&
-                                     fabsf(w.z) <= 3.4028235e38f && fabsf(w.w) <= 3.4028235e38f);
+                            const float y[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                odd |= !(fabsf(y[e]) <= 3.4028235e38f);
+                                top = max(top, __float_as_uint(sane(y[e], 4 * i + t)) & 0x7fffffffu);
+                            }
                         }
                         bad |= ((__ballot_sync(kFullWarpMask, odd) >> t) & 0x11111111u) != 0u ? 1u << i : 0u;
+#pragma unroll
+                        for (int off = 4; off < 32; off <<= 1)
+                            top = max(top, __shfl_xor_sync(kFullWarpMask, top, off));
+                        const uint32_t ex = exponent_above(top);
+                        if (part == 0) {
+                            kex[i] = ex;
+                            kfac[i] = pow2_field(ex - 8u);
+                        } else {
+                            const int log = max(static_cast<int>(ex) - 127, kMinVKey) - 8; // to 2^7 .. 2^8
+                            vkey[i] = pow2_field(static_cast<uint32_t>(127 - log));
+                            vlogs[i] = static_cast<float>(max(-126, min(120, log + static_cast<int>(__float_as_uint(vmul) >> 23) - 127)));
+                            vfac[i] = pow2_field(static_cast<uint32_t>(127 + static_cast<int>(vlogs[i])));
+                        }
                     }
+#pragma unroll
+                for (int j = 0; j < 2; ++j) { // K row 8j + 4 (g & 1) + (g >> 1) is row 4i + t of lane g >> 1, i = 2j + (g & 1)
+                    const uint32_t ex0 = __shfl_sync(kFullWarpMask, kex[2 * j], g >> 1), ex1 = __shfl_sync(kFullWarpMask, kex[2 * j + 1], g >> 1);
+                    kkey[j] = pow2_field(254u - (g & 1 ? ex1 : ex0) + 8u);
+                }
             }
             bool over = kmul == 0.f;
             zero_scores();
 #pragma unroll 1
-            for (int attempt = 0; attempt < 3; ++attempt) { // again after a new kmul
-                if (__any_sync(kFullWarpMask, over)) {
+            for (int attempt = 0; attempt < (kEdge ? 1 : 3); ++attempt) { // again after a new kmul
+                if (kEdge) {
+                    // each row has its own factor
+                } else if (__any_sync(kFullWarpMask, over)) {
                     const uint32_t top = top_of(chunk);
                     if (top >= 0x7f800000u) {
                         poison();
                         break;
                     }
-                    kmul = pow2_field(254u - exponent_above(top) + 8u); // to 2^7 .. 2^8
+                    kkey[0] = kkey[1] = kmul = pow2_field(254u - exponent_above(top) + 8u); // to 2^7 .. 2^8
                 } else if (attempt > 0) {
                     break;
                 }
@@ -361,8 +397,8 @@ static __global__ void __launch_bounds__(TreeRowsGeo<T, D, kFmt, kMT>::kThreads,
                             for (int e = 0; e < 4; ++e)
                                 y[e] = sane(y[e], krow);
                         uint32_t h0, h1, l0, l1;
-                        split_half2(y[0], y[1], kmul, h0, l0, seen_top);
-                        split_half2(y[2], y[3], kmul, h1, l1, seen_top);
+                        split_half2(y[0], y[1], kkey[j], h0, l0, seen_top);
+                        split_half2(y[2], y[3], kkey[j], h1, l1, seen_top);
 #pragma unroll
                         for (int mt = 0; mt < kMT; ++mt) {
                             mma_f16(sc[mt][j], qf[mt][st], h0, h1);
@@ -401,25 +437,32 @@ static __global__ void __launch_bounds__(TreeRowsGeo<T, D, kFmt, kMT>::kThreads,
         float vscale = 0.f;
 #pragma unroll
         for (int i = 0; i < 4 * kC; ++i) {
-            if constexpr (G::kWide) {
+            if constexpr (G::kWide && kEdge) {
+                // set above
+            } else if constexpr (G::kWide) {
                 kfac[i] = pow2_field(254u - (__float_as_uint(kmul) >> 23));
                 vfac[i] = 1.f;
             } else {
                 const uint8_t *page = chunk + i / 4 * G::kPageBytes + 16 * (i % 4) + 4 * t;
                 kfac[i] = *reinterpret_cast<const float *>(page + R::kKScale);
                 vfac[i] = *reinterpret_cast<const float *>(page + R::kVScale);
-                float usable = vfac[i];
-                if (kEdge) { // masked rows may have any scale; places after the last key have none
-                    if (key0 + 4 * i + t >= keys)
-                        vfac[i] = 0.f;
-                    usable = finite_or_zero(vfac[i]);
+                if constexpr (kEdge) { // (places after the last key have none)
+                    const float nan = __uint_as_float(0x7fc00000u);
+                    kfac[i] = fabsf(kfac[i]) <= 3.4028235e38f ? kfac[i] : nan;
+                    vfac[i] = fabsf(vfac[i]) <= 3.4028235e38f ? vfac[i] : nan;
+                    const uint32_t ex = exponent_above(__float_as_uint(key0 + 4 * i + t < keys ? finite_or_zero(vfac[i]) : 0.f));
+                    vlogs[i] = fmaxf(static_cast<float>(static_cast<int>(ex) - 127), kMinVLog);
+                } else {
+                    vscale = fmaxf(vscale, vfac[i]);
                 }
-                vscale = fmaxf(vscale, usable);
             }
         }
-        // scores less their row's scale, masked ones -inf
+        // Scores: less their row's scale; of edge chunks in log2 units, masked ones -inf,
+        // and the V factors of the keys that a row sees enter its own reference
         bool raise = vscale > vtop;
-        const float slack = G::kWide ? kLazy + kLift : kLazy + kLift - vlog;
+        if (!kEdge && !G::kWide) // V far below the chunks before: its own size again
+            raise |= vtop > kMinVTop && !__any_sync(kFullWarpMask, vscale >= vtop * kLowV);
+        const float slack = G::kWide || kEdge ? kLazy + kLift : kLazy + kLift - vlog;
 #pragma unroll
         for (int mt = 0; mt < kMT; ++mt)
 #pragma unroll
@@ -429,46 +472,38 @@ static __global__ void __launch_bounds__(TreeRowsGeo<T, D, kFmt, kMT>::kThreads,
                     const float *c = sc[mt][i >> 1];
                     x[mt][rr][i] = (G::kTwo ? c[i & 1] + c[2 + (i & 1)] : c[2 * rr + (i & 1)]) * kfac[i];
                 }
-                if (kEdge) {
+                float top = kNegInf;
+                if constexpr (kEdge) {
                     const int r = row_base + mt * G::kTileRows + rr * 8 + g;
                     uint32_t seen = 0;
                     if (r < rows)
                         seen = tree_sees32(a.t, span.row0 + r / rep, r / rep, key0 - span.ctx, keys - span.ctx);
 #pragma unroll
                     for (int i = 0; i < 4 * kC; ++i) {
+                        float y = x[mt][rr][i] * row_scale[mt][rr];
                         if (G::kWide && (bad >> i & 1u))
-                            x[mt][rr][i] = __uint_as_float(0x7fc00000u);
+                            y = __uint_as_float(0x7fc00000u);
                         if (!(seen >> (4 * i + t) & 1u))
-                            x[mt][rr][i] = kNegInf;
+                            y = kNegInf;
+                        x[mt][rr][i] = y;
+                        top = fmaxf(top, y + vlogs[i]);
                     }
-                }
-                float top = kNegInf;
+                    raise |= top > m[mt][rr] + slack;
+                } else {
 #pragma unroll
-                for (int i = 0; i < 4 * kC; ++i)
-                    top = fmaxf(top, x[mt][rr][i]);
-                raise |= top * row_scale[mt][rr] > m[mt][rr] + slack;
+                    for (int i = 0; i < 4 * kC; ++i)
+                        top = fmaxf(top, x[mt][rr][i]);
+                    raise |= top * row_scale[mt][rr] > m[mt][rr] + slack;
+                }
             }
         if (__any_sync(kFullWarpMask, raise)) {
-            const uint32_t top = __reduce_max_sync(kFullWarpMask, __float_as_uint(vscale)); // not below zero
-            if (!G::kWide && __uint_as_float(top) > vtop) {
+            if (!kEdge && !G::kWide) {
+                const uint32_t top = __reduce_max_sync(kFullWarpMask, __float_as_uint(vscale)); // not below zero
                 if (top >= 0x7f800000u) {
                     poison();
-                } else {
-                    const uint32_t ex = exponent_above(top);
-                    const float log = static_cast<float>(static_cast<int>(ex) - 127), up = log - vlog;
-                    vtop = pow2_field(ex);
-                    vlog = log;
-#pragma unroll
-                    for (int mt = 0; mt < kMT; ++mt) {
-                        float fix[G::kRPL];
-#pragma unroll
-                        for (int rr = 0; rr < G::kRPL; ++rr) {
-                            fix[rr] = exp2_approx(-up);
-                            m[mt][rr] += up;
-                            l[mt][rr] *= fix[rr];
-                        }
-                        rescale(mt, fix);
-                    }
+                } else if (__uint_as_float(top) > vtop || __uint_as_float(top) < vtop * kLowV) {
+                    vtop = fmaxf(pow2_field(exponent_above(top)), kMinVTop);
+                    vlog = static_cast<float>(static_cast<int>(__float_as_uint(vtop) >> 23) - 127);
                 }
             }
 #pragma unroll
@@ -479,10 +514,10 @@ static __global__ void __launch_bounds__(TreeRowsGeo<T, D, kFmt, kMT>::kThreads,
                     float up = kNegInf;
 #pragma unroll
                     for (int i = 0; i < 4 * kC; ++i)
-                        up = fmaxf(up, x[mt][rr][i]);
+                        up = fmaxf(up, kEdge ? x[mt][rr][i] + vlogs[kEdge ? i : 0] : x[mt][rr][i]);
                     up = fmaxf(up, __shfl_xor_sync(kFullWarpMask, up, 1));
                     up = fmaxf(up, __shfl_xor_sync(kFullWarpMask, up, 2));
-                    up = fmaxf(m[mt][rr], up * row_scale[mt][rr] + (G::kWide ? -kLift : vlog - kLift));
+                    up = fmaxf(m[mt][rr], kEdge ? up - kLift : up * row_scale[mt][rr] + (G::kWide ? -kLift : vlog - kLift));
                     fix[rr] = exp2_approx(m[mt][rr] - up);
                     m[mt][rr] = up;
                     l[mt][rr] *= fix[rr];
@@ -499,12 +534,10 @@ static __global__ void __launch_bounds__(TreeRowsGeo<T, D, kFmt, kMT>::kThreads,
             for (int rr = 0; rr < G::kRPL; ++rr)
 #pragma unroll
                 for (int i = 0; i < 4 * kC; ++i) {
-                    float w = exp2_approx(fmaf(x[mt][rr][i], row_scale[mt][rr], -m[mt][rr]));
+                    const float w = exp2_approx(kEdge ? x[mt][rr][i] - m[mt][rr] : fmaf(x[mt][rr][i], row_scale[mt][rr], -m[mt][rr]));
                     const bool masked = kEdge && x[mt][rr][i] == kNegInf; // no weight, whatever the row's scales
-                    if (masked)
-                        w = 0.f;
                     l[mt][rr] += w;
-                    p[rr][i] = G::kWide || masked ? w : w * vfac[i];
+                    p[rr][i] = (G::kWide && !kEdge) || masked ? w : w * vfac[i];
                 }
 #pragma unroll
             for (int i = 0; i < 2 * kC; ++i) {
@@ -526,14 +559,16 @@ static __global__ void __launch_bounds__(TreeRowsGeo<T, D, kFmt, kMT>::kThreads,
                 uint32_t hi[4][2], lo[4][2]; // of dims 32c + 4g + e, keys (t, 4 + t) and (8 + t, 12 + t)
                 bool over = c == 0 && vmul == 0.f;
 #pragma unroll 1
-                for (int attempt = 0; attempt < 3; ++attempt) {
-                    if (__any_sync(kFullWarpMask, over)) {
+                for (int attempt = 0; attempt < (kEdge ? 1 : 3); ++attempt) {
+                    if (kEdge) {
+                        // each row has its own factor
+                    } else if (__any_sync(kFullWarpMask, over)) {
                         const uint32_t top = top_of(chunk + kKvPage * D * 4);
                         if (top >= 0x7f800000u) {
                             poison();
                             break;
                         }
-                        const float next = pow2_field(254u - exponent_above(top) + 8u); // to 2^7 .. 2^8
+                        const float next = pow2_field(254u - max(exponent_above(top), static_cast<uint32_t>(127 + kMinVKey)) + 8u); // to 2^7 .. 2^8
                         const float up = vmul == 0.f ? 0.f : next * pow2_field(254u - (__float_as_uint(vmul) >> 23));
 #pragma unroll
                         for (int mt = 0; mt < kMT; ++mt) {
@@ -555,17 +590,18 @@ static __global__ void __launch_bounds__(TreeRowsGeo<T, D, kFmt, kMT>::kThreads,
                         if (kEdge)
 #pragma unroll
                             for (int e = 0; e < 4; ++e)
-                                y[i][e] = sane(y[i][e], 4 * i + t);
+                                y[i][e] = sane(y[i][e], 4 * i + t) * vkey[kEdge ? i : 0];
                     }
+                    const float vmul_here = kEdge ? 1.f : vmul;
                     __half2 seen_top = __float2half2_rn(0.f);
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
 #pragma unroll
                         for (int j = 0; j < 2; ++j) {
                             if constexpr (G::kTwo) {
-                                split_half2(y[2 * j][e], y[2 * j + 1][e], vmul, hi[e][j], lo[e][j], seen_top);
+                                split_half2(y[2 * j][e], y[2 * j + 1][e], vmul_here, hi[e][j], lo[e][j], seen_top);
                             } else {
-                                hi[e][j] = half2_rn(y[2 * j][e] * vmul, y[2 * j + 1][e] * vmul);
+                                hi[e][j] = half2_rn(y[2 * j][e] * vmul_here, y[2 * j + 1][e] * vmul_here);
                                 seen_top = __hmax2_nan(seen_top, __habs2(*reinterpret_cast<const __half2 *>(&hi[e][j])));
                             }
                         }

@@ -235,3 +235,19 @@ def hidden_large_rows(ops, fmt, kind, dim, ctx, n, factor, alone):
 @pytest.mark.parametrize("alone", [False, True])
 def test_large_rows_that_a_node_does_not_see(ops, fmt, kind, dim, ctx, n, factor, alone):
     hidden_large_rows(ops, fmt, kind, dim, ctx, n, factor, alone)
+
+
+@pytest.mark.parametrize("fmt", [0, 1, 2])
+@pytest.mark.parametrize("kind", [0, 1])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("ctx,n", [(0, 5), (50, 3), (300, 6)])
+@pytest.mark.parametrize("factor", [1e6, 1e20, 1e30])
+def test_large_rows_that_few_nodes_do_not_see(ops, fmt, kind, dim, ctx, n, factor):
+    hidden_large_rows(ops, fmt, kind, dim, ctx, n, factor, False)
+
+
+@pytest.mark.parametrize("fmt", [1, 2])
+@pytest.mark.parametrize("ctx,n", [(0, 70), (300, 100)])
+@pytest.mark.parametrize("factor", [1e6, 1e20, 1e30])
+def test_large_rows_that_a_node_does_not_see_wide_heads(ops, fmt, ctx, n, factor):
+    hidden_large_rows(ops, fmt, 0, 128, ctx, n, factor, False)
