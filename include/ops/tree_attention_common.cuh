@@ -146,6 +146,14 @@ __device__ __forceinline__ uint32_t tree_sees32(const TreeBatch &t, int row, int
 
 constexpr float kLazy = 4.f;  // log2 units a score may pass the reference maximum by
 constexpr float kLift = 10.f; // P is scaled by 2^kLift: at most 2^14
+constexpr float kNone = -1e30f; // reference of a row that has seen nothing yet
+// A reference above this is so coarse that a weight may come out too large for
+// fp16: from there on weights are cut off.
+constexpr float kWary = 0x1p20f;
+// How far below the largest score `top` the reference lies: by `lift`, but at
+// least by two units in its last place, so that the weight of that score, however
+// the difference is rounded, is not below one.
+__device__ __forceinline__ float reference_lift(float lift, float top) { return fmaxf(lift, fabsf(top) * 0x1p-22f); }
 // V scales below this are not told apart from it (fp16 loses their low bits);
 // lower, and l in their units would leave fp32's range. The same for the
 // magnitudes of single fp32 V rows.

@@ -263,7 +263,8 @@ static __global__ void __launch_bounds__(TreeRowsGeo<T, D, kFmt, kMT>::kThreads,
     for (int mt = 0; mt < kMT; ++mt)
 #pragma unroll
         for (int rr = 0; rr < G::kRPL; ++rr)
-            m[mt][rr] = -1e30f, l[mt][rr] = 0.f;
+            m[mt][rr] = kNone, l[mt][rr] = 0.f;
+    bool wary = false; // the warp has met large scores
     const auto rescale = [&](int mt, const float (&fix)[G::kRPL]) {
 #pragma unroll
         for (int n = 0; n < D / 8; ++n) {
@@ -281,11 +282,13 @@ static __global__ void __launch_bounds__(TreeRowsGeo<T, D, kFmt, kMT>::kThreads,
                 l[mt][rr] = __uint_as_float(0x7fc00000u);
     };
 
-    // One chunk. Edge chunks hold nodes, or places after the last key.
+    // One chunk. Edge chunks hold nodes, or places after the last key; chunks of
+    // large scores are taken in the same way.
     // Score column g of n tile j of a page is key 8j + 4 (g & 1) + g / 2, so that
     // lane t's columns 2t + col are keys 8j + 4 col + t: value i = 2j + col of a
     // lane is key 4i + t.
-    const auto take = [&](const uint8_t *chunk, int key0, auto edge_tag) {
+    // False: not taken, for its scores are large (m is raised; see kWary).
+    const auto take = [&](const uint8_t *chunk, int key0, auto edge_tag) -> bool {
         constexpr bool kEdge = decltype(edge_tag)::value;
         float sc[kMT][2 * kC][4];
         float kfac[4 * kC], vfac[4 * kC]; // factors of a lane's scores and weights
@@ -517,13 +520,19 @@ static __global__ void __launch_bounds__(TreeRowsGeo<T, D, kFmt, kMT>::kThreads,
                         up = fmaxf(up, kEdge ? x[mt][rr][i] + vlogs[kEdge ? i : 0] : x[mt][rr][i]);
                     up = fmaxf(up, __shfl_xor_sync(kFullWarpMask, up, 1));
                     up = fmaxf(up, __shfl_xor_sync(kFullWarpMask, up, 2));
-                    up = fmaxf(m[mt][rr], kEdge ? up - kLift : up * row_scale[mt][rr] + (G::kWide ? -kLift : vlog - kLift));
+                    if (!kEdge)
+                        up = up * row_scale[mt][rr] + (G::kWide ? 0.f : vlog);
+                    up = fmaxf(m[mt][rr], up - reference_lift(kLift, up));
+                    wary |= fabsf(up) > kWary && up > kNone;
                     fix[rr] = exp2_approx(m[mt][rr] - up);
                     m[mt][rr] = up;
                     l[mt][rr] *= fix[rr];
                 }
                 rescale(mt, fix);
             }
+            wary = __any_sync(kFullWarpMask, wary);
+            if (!kEdge && wary)
+                return false;
         }
         // P as A fragments; l sums the weights before they are rounded
         uint32_t pf[kMT][kC][4];
@@ -534,7 +543,12 @@ static __global__ void __launch_bounds__(TreeRowsGeo<T, D, kFmt, kMT>::kThreads,
             for (int rr = 0; rr < G::kRPL; ++rr)
 #pragma unroll
                 for (int i = 0; i < 4 * kC; ++i) {
-                    const float w = exp2_approx(kEdge ? x[mt][rr][i] - m[mt][rr] : fmaf(x[mt][rr][i], row_scale[mt][rr], -m[mt][rr]));
+                    float e = kEdge ? x[mt][rr][i] - m[mt][rr] : fmaf(x[mt][rr][i], row_scale[mt][rr], -m[mt][rr]);
+                    if (kEdge) { // (a NaN stays)
+                        const float cap = kLift + kLazy + 1.f - vlogs[kEdge ? i : 0];
+                        e = e > cap ? cap : e;
+                    }
+                    const float w = exp2_approx(e);
                     const bool masked = kEdge && x[mt][rr][i] == kNegInf; // no weight, whatever the row's scales
                     l[mt][rr] += w;
                     p[rr][i] = (G::kWide && !kEdge) || masked ? w : w * vfac[i];
@@ -651,6 +665,7 @@ static __global__ void __launch_bounds__(TreeRowsGeo<T, D, kFmt, kMT>::kThreads,
                 }
             }
         }
+        return true;
     };
 
     bool ok = true;
@@ -663,10 +678,8 @@ static __global__ void __launch_bounds__(TreeRowsGeo<T, D, kFmt, kMT>::kThreads,
         }
         const uint8_t *chunk = ring + stage * G::kChunkBytes;
         const int key0 = (first + done * step) * kC * kKvPage;
-        if (key0 + kC * kKvPage > span.ctx)
+        if (key0 + kC * kKvPage > span.ctx || wary || !take(chunk, key0, std::false_type{}))
             take(chunk, key0, std::true_type{});
-        else
-            take(chunk, key0, std::false_type{});
         __syncwarp(); // every lane has read the stage
         const int next = done + G::kStages;
         if (next < mine) {
@@ -717,7 +730,7 @@ static __global__ void __launch_bounds__(TreeRowsGeo<T, D, kFmt, kMT>::kThreads,
         const int r = i / D, d = i % D;
         if (r >= live)
             break;
-        float top = -1e30f, L = 0.f, O = 0.f;
+        float top = kNone, L = 0.f, O = 0.f;
 #pragma unroll
         for (int w = 0; w < G::kWarps; ++w)
             top = fmaxf(top, stat[w * G::kRows + r]);
@@ -747,7 +760,7 @@ static __global__ void __launch_bounds__(TreeRowsGeo<T, D, kFmt, kMT>::kThreads,
         const int r = i / D, d = i % D;
         if (r >= live)
             break;
-        float top = -1e30f, L = 0.f, O = 0.f;
+        float top = kNone, L = 0.f, O = 0.f;
         for (int c = 0; c < splits; ++c)
             top = fmaxf(top, peer_load(&joined[r], c));
         for (int c = 0; c < splits; ++c) {

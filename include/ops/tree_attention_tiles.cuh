@@ -60,7 +60,6 @@ constexpr float kTileLift = 8.f, kTileTop = 14.f;
 // see takes no bits from those that it sees. V units are 2^-60 at least (exponent
 // field kMinVField - 1): lower, and l would leave fp32's range beside large rows.
 constexpr uint32_t kUnlike = 12, kMinVField = 68;
-constexpr float kTileNone = -1e30f; // m of a row that has seen nothing yet
 
 template <typename T, int D, KvFormat kFmt, int kM> struct TreeTilesGeo {
     static constexpr bool kWide = kFmt == KvFormat::kF32;
@@ -635,7 +634,7 @@ static __global__ void __launch_bounds__(kTileThreads, 1)
         const uint32_t quarter = static_cast<uint32_t>((warp % 4) * 32) << 16;
         const uint32_t st = tmem + quarter + static_cast<uint32_t>(stream * kTileKeys);
         const uint32_t ot = tmem + quarter + 256u + static_cast<uint32_t>(stream * D);
-        float m = kTileNone, l = 0.f;
+        float m = kNone, l = 0.f;
         constexpr int kGroup = G::kItemKeys, kGroups = 32 / kGroup; // keys that share their units; such groups in a chunk
         int e = 0; // steps done
         for (; ok; ++e) {
@@ -748,7 +747,7 @@ static __global__ void __launch_bounds__(kTileThreads, 1)
                 // The first reference: the largest score of the first tile of which the row sees
                 // anything. It has to come from the scores: against m's first value every
                 // score is the same number.
-                if (__any_sync(kFullWarpMask, live && m == kTileNone)) {
+                if (__any_sync(kFullWarpMask, live && m == kNone)) {
                     float top = kNegInf;
 #pragma unroll 1
                     for (int c = 0; c < 4; ++c) {
@@ -761,8 +760,8 @@ static __global__ void __launch_bounds__(kTileThreads, 1)
                             top = fmaxf(top, fmaxf(y.x, y.y));
                         }
                     }
-                    if (m == kTileNone)
-                        m = fmaxf(m, top - kTileLift);
+                    if (m == kNone)
+                        m = fmaxf(m, top - reference_lift(kTileLift, top));
                 }
                 // one chunk of 32 keys, whose scores are in x, the next one's on their way to `next`
                 const auto chunk = [&](int c, uint32_t (&x)[2][16], uint32_t (&next)[2][16]) {
@@ -800,7 +799,7 @@ static __global__ void __launch_bounds__(kTileThreads, 1)
                             }
                             break;
                         }
-                        const float less = fmaxf(0.f, ceilf(most - kTileLift)), fix = exp2_approx(-less);
+                        const float less = fmaxf(0.f, ceilf(most - reference_lift(kTileLift, 2.f * fmaxf(fabsf(most), fabsf(m))))), fix = exp2_approx(-less);
                         if (c < 3)
                             await(next);
                         rescale(fix, c);
@@ -968,7 +967,7 @@ static __global__ void __launch_bounds__(kTileThreads, 1)
         const int r = i / D, d = i % D;
         if (r >= rows_here)
             break;
-        float top = -1e30f, L = 0.f, O = 0.f;
+        float top = kNone, L = 0.f, O = 0.f;
         for (int c = 0; c < splits; ++c)
             top = fmaxf(top, peer_load(&joined[r], c));
         for (int c = 0; c < splits; ++c) {

@@ -251,3 +251,40 @@ def test_large_rows_that_few_nodes_do_not_see(ops, fmt, kind, dim, ctx, n, facto
 @pytest.mark.parametrize("factor", [1e6, 1e20, 1e30])
 def test_large_rows_that_a_node_does_not_see_wide_heads(ops, fmt, ctx, n, factor):
     hidden_large_rows(ops, fmt, 0, 128, ctx, n, factor, False)
+
+
+@pytest.mark.parametrize("fmt", [0, 1, 2])
+@pytest.mark.parametrize("kind", [0, 1])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("ctx,n", [(0, 5), (50, 3), (300, 6)])
+@pytest.mark.parametrize("factor", [1e6, 1e20, 1e30])
+def test_large_rows_that_few_nodes_see(ops, fmt, kind, dim, ctx, n, factor):
+    hidden_large_rows(ops, fmt, kind, dim, ctx, n, factor, True)
+
+
+@pytest.mark.parametrize("fmt", [0, 1, 2])
+@pytest.mark.parametrize("kind", [0, 1])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("size", [1e3, 1e4, 1e5, 1e6, 1e9])
+@pytest.mark.parametrize("ctx,n", [(500, 2), (20, 12), (500, 50), (0, 140)])
+def test_large_scores_choose_the_largest(ops, fmt, kind, dim, size, ctx, n):
+    """Scores of 2^21 to 2^61: where the largest is ahead by more than the scores' rounding (2^-18 of their mass, and 40),
+    the output is its V row."""
+    cache = plain.Cache([ctx + n], 1, dim, fmt, 5)
+    q = (queries(n, 4, dim, 0, 6) * size).to(TYPES[kind])
+    k, _ = cache.rows(0)
+    set_rows(cache, 0, np.arange(ctx + n), k=k * size)
+    scale = 1 / math.sqrt(dim)
+    got = attend(ops, cache, q, [ctx], [n], None, scale)
+    assert torch.isfinite(got).all()
+    k, v = cache.rows(0)
+    seen = torch.cat([torch.ones(n, ctx, dtype=torch.bool), torch.ones(n, n, dtype=torch.bool).tril()], 1)
+    s = (scale * torch.einsum("nhd,kd->nhk", q.double(), k[:, 0])).masked_fill(~seen[:, None], -math.inf)
+    mass = scale * torch.einsum("nhd,kd->nhk", q.double().abs(), k[:, 0].abs()).amax(-1)
+    top = s.sort(-1, descending=True)
+    gap = top.values[..., 0] - top.values[..., 1] if ctx + n > 1 else torch.full_like(mass, math.inf)
+    sure = gap > 2.0**-18 * mass + 40
+    assert sure.double().mean() > 0.9
+    want = v[:, 0][top.indices[..., 0]]
+    err = (got - want).abs()[sure]
+    assert (err <= (2.0**-7 if kind else 2.0**-18) * v.abs().max()).all(), f"{err.max():.3g}"
