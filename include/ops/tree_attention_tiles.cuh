@@ -771,11 +771,12 @@ static __global__ void __launch_bounds__(kTileThreads, 1)
                     const uint32_t seen = kEdge ? seen_of(c) : 0u, odd = kEdge ? odd_of(c) : 0u;
                     // Scores and weights at once, for weights up to 2^kTileTop fit in
                     // fp16 but for a rare chunk: one with a larger one raises the
-                    // reference and is done again (its scores are still there), once:
-                    // scores of 2^28 and more are rounded by more than kTileTop, so that
-                    // what is still too large then is cut off.
+                    // reference and is done again (its scores are still there). From a
+                    // reference far below, each time brings the rest to 2^-19 of it; scores
+                    // of 2^28 and more are rounded by more than kTileTop, so that what is
+                    // too large in the end is cut off.
 #pragma unroll 1
-                    for (bool again = false;; again = true) {
+                    for (int raises = 0;; ++raises) {
                         float top[4] = {kNegInf, kNegInf, kNegInf, kNegInf};
 #pragma unroll
                         for (int n = 0; n < 32; n += 2) {
@@ -790,7 +791,7 @@ static __global__ void __launch_bounds__(kTileThreads, 1)
                         const float most = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
                         if (!__any_sync(kFullWarpMask, most > kTileTop))
                             break;
-                        if (again) {
+                        if (raises == 6) {
                             const float cap = exp2_approx(kTileTop);
 #pragma unroll
                             for (int n = 0; n < 32; ++n) { // (a NaN stays)

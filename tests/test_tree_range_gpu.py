@@ -288,3 +288,27 @@ def test_large_scores_choose_the_largest(ops, fmt, kind, dim, size, ctx, n):
     want = v[:, 0][top.indices[..., 0]]
     err = (got - want).abs()[sure]
     assert (err <= (2.0**-7 if kind else 2.0**-18) * v.abs().max()).all(), f"{err.max():.3g}"
+
+
+@pytest.mark.parametrize("fmt", [0, 1, 2])
+@pytest.mark.parametrize("kind", [0, 1])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("n", [1, 3, 50])
+@pytest.mark.parametrize("bits,back", [(10, False), (20, False), (30, False), (20, True)])
+def test_small_rows_after_large_ones(ops, fmt, kind, dim, n, bits, back):
+    """Pages whose K and V rows are 2^bits times as large as the others' and weigh nothing (their scores are far below):
+    the small rows, after them (or before), keep the bits that they have on their own."""
+    ctx, large = 2200, 1024
+    cache = plain.Cache([ctx + n], 2, dim, fmt, 13)
+    at = np.arange(ctx - large, ctx) // 16 * 16 if back else np.arange(large)
+    at = np.arange(1168, 1168 + large) if back else at
+    k = opposed(3, large, 2, dim, 3.0).clamp(max=-0.5)
+    set_rows(cache, 0, at, k=k * 2.0**bits, v=queries(large, 2, dim, 0, 14).float() * 2.0**bits)
+    q = (0.2 * queries(n, 4, dim, 0, 8) + 1.0).clamp(min=0.1).to(TYPES[kind])
+    scale = 1 / math.sqrt(dim)
+    got = attend(ops, cache, q, [ctx], [n], None, scale)
+    # what the large rows weigh is 0 in 64 bits too: the others alone give the result and the tolerance
+    want, _, _ = expected(cache, q, [ctx], [n], None, scale)
+    set_rows(cache, 0, at, k=torch.zeros(large, 2, dim), v=torch.zeros(large, 2, dim))
+    _, mass, top = expected(cache, q, [ctx], [n], None, scale)
+    check(got, want, mass, top, ctx + n, kind)
