@@ -26,8 +26,9 @@
 // lower, so one product gives both and a lane adds its own two accumulators.
 // bf16 rows fit in one term: 16 rows to a tile. K and V: 8-bit codes are exact
 // in fp16, their scales are applied to S and folded into P; fp32 pools are two
-// fp16 terms too, after a power of two that the warp shares (of the 8 keys for
-// K, running for V) has brought them into range. tf32 terms took as many
+// fp16 terms too, after a power of two that a page shares (for V, 32 dims of it):
+// kept from page to page while it brings their largest to 2^-3 to 2^14, so that
+// the terms hold 2^-22 of that at least. tf32 terms took as many
 // conversions and twice the tensor time. Contraction indices and output columns
 // are permuted so that a lane's fragments are contiguous bytes of a row (see
 // the index comments below).
@@ -106,9 +107,11 @@ __device__ __forceinline__ void split_half2(float x, float y, float f, uint32_t 
     lo = half2_rn(r.x, r.y);
     top = __hmax2_nan(top, __habs2(*reinterpret_cast<const __half2 *>(&hi)));
 }
-// Whether a magnitude in `top` is over 2^14, infinite or NaN.
-__device__ __forceinline__ bool over_half2(__half2 top) {
-    return !(__low2float(top) <= 16384.f && __high2float(top) <= 16384.f);
+// Whether a lane's magnitudes `top` are over 2^14, infinite or NaN, or all the warp's
+// are below 2^-3 (two terms have 2^-22 of them left). The same in every lane.
+__device__ __forceinline__ bool half2_out_of_range(__half2 top) {
+    const float a = __low2float(top), b = __high2float(top);
+    return __any_sync(kFullWarpMask, !(a <= 16384.f && b <= 16384.f)) || !__any_sync(kFullWarpMask, a >= 0.125f || b >= 0.125f);
 }
 
 template <typename T, int D, KvFormat kFmt, int kMT>
@@ -257,8 +260,9 @@ static __global__ void __launch_bounds__(TreeRowsGeo<T, D, kFmt, kMT>::kThreads,
     // m: the reference that weights are relative to, 2^(x - m)
     float m[kMT][G::kRPL], l[kMT][G::kRPL];
     // 8-bit: a power of two next above the V scales of late and its log2, which goes
-    // into m. fp32: the powers of two that K and V are multiplied by (0: not chosen yet)
-    float vtop = kMinVTop, vlog = kMinVLog, kmul = 0.f, vmul = 0.f;
+    // into m. fp32: the powers of two that K and V (32 dims each) of the last chunk were
+    // multiplied by (0: not chosen yet)
+    float vtop = kMinVTop, vlog = kMinVLog, kmul = 0.f, vmul[D / 32] = {};
 #pragma unroll
     for (int mt = 0; mt < kMT; ++mt)
 #pragma unroll
@@ -273,6 +277,31 @@ static __global__ void __launch_bounds__(TreeRowsGeo<T, D, kFmt, kMT>::kThreads,
             o[mt][n][2] *= fix[G::kRPL - 1];
             o[mt][n][3] *= fix[G::kRPL - 1];
         }
+    };
+    // fp32: columns 32 c .. of O go over to V times `next`
+    const auto resize = [&](int c, float next) {
+        const float up = vmul[c] == 0.f ? 1.f : next * pow2_field(254u - (__float_as_uint(vmul[c]) >> 23));
+#pragma unroll
+        for (int mt = 0; mt < kMT; ++mt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    o[mt][4 * c + e][i] *= up;
+        vmul[c] = next;
+    };
+    // one factor for all of O: the largest rows'. Returns it.
+    const auto one_vmul = [&] {
+        float least = 0.f;
+#pragma unroll
+        for (int c = 0; c < D / 32; ++c)
+            least = vmul[c] == 0.f || (least != 0.f && least < vmul[c]) ? least : vmul[c];
+        least = least == 0.f ? 1.f : least;
+#pragma unroll
+        for (int c = 0; c < D / 32; ++c)
+            if (vmul[c] != least)
+                resize(c, least);
+        return least;
     };
     const auto poison = [&] { // a row that every node sees holds an infinity or a NaN
 #pragma unroll
@@ -327,8 +356,7 @@ static __global__ void __launch_bounds__(TreeRowsGeo<T, D, kFmt, kMT>::kThreads,
                 // Rows that are not finite, and each row's largest magnitude: a row that a
                 // node does not see takes no bits from the others. Lanes t, t + 4, .. hold
                 // a row's eighths.
-                if (vmul == 0.f)
-                    vmul = 1.f;
+                const int unit = static_cast<int>(__float_as_uint(one_vmul()) >> 23) - 127;
                 uint32_t kex[4];
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
@@ -358,7 +386,7 @@ static __global__ void __launch_bounds__(TreeRowsGeo<T, D, kFmt, kMT>::kThreads,
                         } else {
                             const int log = max(static_cast<int>(ex) - 127, kMinVKey) - 8; // to 2^7 .. 2^8
                             vkey[i] = pow2_field(static_cast<uint32_t>(127 - log));
-                            vlogs[i] = static_cast<float>(max(-126, min(120, log + static_cast<int>(__float_as_uint(vmul) >> 23) - 127)));
+                            vlogs[i] = static_cast<float>(max(-126, min(120, log + unit)));
                             vfac[i] = pow2_field(static_cast<uint32_t>(127 + static_cast<int>(vlogs[i])));
                         }
                     }
@@ -368,21 +396,19 @@ static __global__ void __launch_bounds__(TreeRowsGeo<T, D, kFmt, kMT>::kThreads,
                     kkey[j] = pow2_field(254u - (g & 1 ? ex1 : ex0) + 8u);
                 }
             }
-            bool over = kmul == 0.f;
+            bool anew = !kEdge && kmul == 0.f; // (edge chunks: each row has its own factor)
             zero_scores();
 #pragma unroll 1
-            for (int attempt = 0; attempt < (kEdge ? 1 : 3); ++attempt) { // again after a new kmul
-                if (kEdge) {
-                    // each row has its own factor
-                } else if (__any_sync(kFullWarpMask, over)) {
+            for (int attempt = 0;; ++attempt) { // again after a new kmul
+                if (anew) {
                     const uint32_t top = top_of(chunk);
                     if (top >= 0x7f800000u) {
                         poison();
                         break;
                     }
+                    if (attempt > 0 && top == 0u)
+                        break;
                     kkey[0] = kkey[1] = kmul = pow2_field(254u - exponent_above(top) + 8u); // to 2^7 .. 2^8
-                } else if (attempt > 0) {
-                    break;
                 }
                 zero_scores();
                 float small[kMT][2][4] = {}; // the small products: an accumulator is cut off at every step, to its size
@@ -414,7 +440,9 @@ static __global__ void __launch_bounds__(TreeRowsGeo<T, D, kFmt, kMT>::kThreads,
 #pragma unroll
                     for (int n = 0; n < 8; ++n)
                         sc[mt][n / 4][n % 4] += small[mt][n / 4][n % 4];
-                over = over_half2(seen_top);
+                anew = !kEdge && attempt < 2 && half2_out_of_range(seen_top);
+                if (!anew)
+                    break;
             }
         } else {
             zero_scores();
@@ -571,31 +599,9 @@ static __global__ void __launch_bounds__(TreeRowsGeo<T, D, kFmt, kMT>::kThreads,
 #pragma unroll
             for (int c = 0; c < D / 32; ++c) {
                 uint32_t hi[4][2], lo[4][2]; // of dims 32c + 4g + e, keys (t, 4 + t) and (8 + t, 12 + t)
-                bool over = c == 0 && vmul == 0.f;
+                bool anew = !kEdge && vmul[c] == 0.f;
 #pragma unroll 1
-                for (int attempt = 0; attempt < (kEdge ? 1 : 3); ++attempt) {
-                    if (kEdge) {
-                        // each row has its own factor
-                    } else if (__any_sync(kFullWarpMask, over)) {
-                        const uint32_t top = top_of(chunk + kKvPage * D * 4);
-                        if (top >= 0x7f800000u) {
-                            poison();
-                            break;
-                        }
-                        const float next = pow2_field(254u - max(exponent_above(top), static_cast<uint32_t>(127 + kMinVKey)) + 8u); // to 2^7 .. 2^8
-                        const float up = vmul == 0.f ? 0.f : next * pow2_field(254u - (__float_as_uint(vmul) >> 23));
-#pragma unroll
-                        for (int mt = 0; mt < kMT; ++mt) {
-                            float fix[G::kRPL];
-#pragma unroll
-                            for (int rr = 0; rr < G::kRPL; ++rr)
-                                fix[rr] = up;
-                            rescale(mt, fix);
-                        }
-                        vmul = next;
-                    } else if (attempt > 0) {
-                        break;
-                    }
+                for (int attempt = 0;; ++attempt) {
                     float y[4][4]; // value i's key, dim e
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
@@ -606,7 +612,27 @@ static __global__ void __launch_bounds__(TreeRowsGeo<T, D, kFmt, kMT>::kThreads,
                             for (int e = 0; e < 4; ++e)
                                 y[i][e] = sane(y[i][e], 4 * i + t) * vkey[kEdge ? i : 0];
                     }
-                    const float vmul_here = kEdge ? 1.f : vmul;
+                    if (anew) {
+                        uint32_t top = 0;
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e)
+                                top = max(top, __float_as_uint(y[i][e]) & 0x7fffffffu);
+                        top = __reduce_max_sync(kFullWarpMask, top);
+                        if (top >= 0x7f800000u) {
+                            poison();
+                            top = 0u;
+                        }
+                        if (attempt > 0 && top == 0u)
+                            break;
+                        // to 2^7 .. 2^8; what is summed already must not leave fp32's range
+                        float next = pow2_field(254u - max(exponent_above(top), static_cast<uint32_t>(127 + kMinVKey)) + 8u);
+                        if (vmul[c] != 0.f)
+                            next = fminf(next, vmul[c] * 0x1p60f);
+                        resize(c, next);
+                    }
+                    const float vmul_here = kEdge ? 1.f : vmul[c];
                     __half2 seen_top = __float2half2_rn(0.f);
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
@@ -619,7 +645,9 @@ static __global__ void __launch_bounds__(TreeRowsGeo<T, D, kFmt, kMT>::kThreads,
                                 seen_top = __hmax2_nan(seen_top, __habs2(*reinterpret_cast<const __half2 *>(&hi[e][j])));
                             }
                         }
-                    over = over_half2(seen_top);
+                    anew = !kEdge && attempt < 2 && half2_out_of_range(seen_top);
+                    if (!anew)
+                        break;
                 }
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
@@ -701,7 +729,9 @@ static __global__ void __launch_bounds__(TreeRowsGeo<T, D, kFmt, kMT>::kThreads,
 
     // the warps' results over the ring, joined in warp order
     float *part = reinterpret_cast<float *>(smem);
-    const float vunit = G::kWide && vmul != 0.f ? pow2_field(254u - (__float_as_uint(vmul) >> 23)) : 1.f;
+    float vunit = 1.f;
+    if constexpr (G::kWide)
+        vunit = pow2_field(254u - (__float_as_uint(one_vmul()) >> 23));
 #pragma unroll
     for (int mt = 0; mt < kMT; ++mt)
 #pragma unroll

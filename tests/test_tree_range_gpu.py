@@ -312,3 +312,27 @@ def test_small_rows_after_large_ones(ops, fmt, kind, dim, n, bits, back):
     set_rows(cache, 0, at, k=torch.zeros(large, 2, dim), v=torch.zeros(large, 2, dim))
     _, mass, top = expected(cache, q, [ctx], [n], None, scale)
     check(got, want, mass, top, ctx + n, kind)
+
+
+@pytest.mark.parametrize("fmt", [0, 1, 2])
+@pytest.mark.parametrize("kind", [0, 1])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("n", [1, 3, 50])
+@pytest.mark.parametrize("bits", [10, 20, 30])
+def test_small_rows_after_rows_of_large_values(ops, fmt, kind, dim, n, bits):
+    """The same where scores are ordinary: K rows (fp32) with one value of 2^bits that no query looks at, V rows of that
+    size, scores of -60 (in log2 units) below the others'."""
+    ctx, large = 2200, 1024
+    cache = plain.Cache([ctx + n], 2, dim, fmt, 13)
+    k = opposed(3, large, 2, dim, 60 / (math.log2(math.e) * math.sqrt(dim)))
+    if fmt == 0:
+        k[..., 0] = 2.0**bits
+    set_rows(cache, 0, np.arange(large), k=k, v=queries(large, 2, dim, 0, 14).float() * 2.0**bits)
+    q = (0.2 * queries(n, 4, dim, 0, 8) + 1.0).to(TYPES[kind])
+    q[..., 0] = 0
+    scale = 1 / math.sqrt(dim)
+    got = attend(ops, cache, q, [ctx], [n], None, scale)
+    want, _, _ = expected(cache, q, [ctx], [n], None, scale)
+    set_rows(cache, 0, np.arange(large), k=torch.zeros(large, 2, dim), v=torch.zeros(large, 2, dim))
+    _, mass, top = expected(cache, q, [ctx], [n], None, scale)
+    check(got, want, mass, top, ctx + n, kind)
