@@ -198,6 +198,7 @@ static __global__ void __launch_bounds__(kKvThreads)
     constexpr int kLanes = D / V::kN, kItems = 32 / kLanes;
     const int lane = threadIdx.x & 31;
     const int row = static_cast<int>(blockIdx.x) * (kKvThreads / 32) + static_cast<int>(threadIdx.x >> 5);
+    pdl_wait();
     if (row >= a.rows)
         return;
     const int item0 = static_cast<int>(blockIdx.y) * kKvWritePasses * kItems + lane / kLanes;
@@ -262,6 +263,7 @@ static __global__ void __launch_bounds__(kKvThreads)
     constexpr int kLanes = D / V::kN, kItems = 32 / kLanes;
     const int lane = threadIdx.x & 31;
     const int row = static_cast<int>(blockIdx.x) * (kKvThreads / 32) + static_cast<int>(threadIdx.x >> 5);
+    pdl_wait();
     if (row >= a.rows)
         return;
     const int item0 = static_cast<int>(blockIdx.y) * kKvReadPasses * kItems + lane / kLanes;

@@ -91,6 +91,7 @@ static __global__ void __launch_bounds__(kCommitThreads) tree_commit_kernel(Tree
     __shared__ int count_s;
     int *succ = commit_smem, *target = succ + t.max_rows, *path = target + t.max_rows, *place = path + t.max_rows;
     const int b = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    pdl_wait();
     const int row0 = t.row_start[b], ctx = t.ctx_lens[b];
     const int n = min(t.row_start[b + 1] - row0, t.max_rows);
     for (int j = tid; j < n; j += kCommitThreads) {
