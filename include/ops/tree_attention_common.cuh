@@ -118,6 +118,7 @@ __device__ __forceinline__ int sequence_by_work(const TreeBatch &t, int order, i
     }
     __syncthreads();
     const int b = room[0];
+    sm100::fence_proxy_async_smem(); // `room` may lie where bulk copies go next
     __syncthreads();
     return b;
 }

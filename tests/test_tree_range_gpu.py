@@ -336,3 +336,19 @@ def test_small_rows_after_rows_of_large_values(ops, fmt, kind, dim, n, bits):
     set_rows(cache, 0, np.arange(large), k=torch.zeros(large, 2, dim), v=torch.zeros(large, 2, dim))
     _, mass, top = expected(cache, q, [ctx], [n], None, scale)
     check(got, want, mass, top, ctx + n, kind)
+
+
+# ------------------------------------------------------------------ many sequences, long prompts
+
+
+@pytest.mark.parametrize("fmt", [0, 1, 2])
+@pytest.mark.parametrize("kind", [0, 1])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_more_sequences_than_run_at_once(ops, fmt, kind, dim):
+    """Sequences are taken in the order of their work: it is found in the memory that the first pages are copied to."""
+    rng = np.random.default_rng(4)
+    ctx, rows = rng.integers(0, 300, 60).tolist(), rng.integers(0, 4, 60).tolist()
+    cache = plain.Cache([c + n for c, n in zip(ctx, rows)], 4, dim, fmt, 21)
+    q = queries(sum(rows), 8, dim, kind, 22)
+    got = attend(ops, cache, q, ctx, rows, None, 1 / math.sqrt(dim))
+    check(got, *expected(cache, q, ctx, rows, None, 1 / math.sqrt(dim)), 304, kind)
