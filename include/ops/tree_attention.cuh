@@ -13,7 +13,8 @@
 //   o = sum_j softmax_j(scale q . k_j) v_j
 // A node that sees nothing gets zeros. Scores, softmax statistics and sums are
 // fp32. A masked key has no influence, whatever its row holds; an infinity or a
-// NaN in a K or V row that a node does see makes the node's whole output NaN.
+// NaN in a K or V row that a node does see makes the node's whole output NaN,
+// and so does one in its query row.
 
 #include "tree_attention_common.cuh"
 #include "tree_attention_rows.cuh"

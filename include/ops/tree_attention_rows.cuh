@@ -226,6 +226,8 @@ static __global__ void __launch_bounds__(TreeRowsGeo<T, D, kFmt, kMT>::kThreads,
             const uint32_t ex = exponent_above(top);
             const float f = copysignf(pow2_field(254u - ex + 10u), a.scale_log2);
             row_scale[mt][rr] = fabsf(a.scale_log2) * pow2_field(ex - 10u) * (kFmt == KvFormat::kInt8 ? 16777216.f : 1.f);
+            if (top >= 0x7f800000u) // an infinity would be a score like others, or none
+                row_scale[mt][rr] = __uint_as_float(0x7fc00000u);
 #pragma unroll
             for (int e = 0; e < D / 4; ++e)
                 x[rr][e] *= f;

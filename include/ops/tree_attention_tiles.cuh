@@ -601,7 +601,8 @@ static __global__ void __launch_bounds__(kTileThreads, 1)
 #pragma unroll
                 for (int e = 0; e < kE; ++e)
                     top = max(top, __float_as_uint(x[n][e]) & 0x7fffffffu);
-                const uint32_t ex = exponent_above(__reduce_max_sync(kFullWarpMask, top));
+                top = __reduce_max_sync(kFullWarpMask, top);
+                const uint32_t ex = exponent_above(top);
                 const float f = copysignf(pow2_field(254u - ex + 10u), a.scale_log2);
                 const int dim = kE * lane;
                 uint8_t *dst = qs + (dim / 64 * kM + r / 128) * G::kSlab + swizzled(r % 128, dim % 64 / 8) + dim % 8 * 2;
@@ -616,7 +617,7 @@ static __global__ void __launch_bounds__(kTileThreads, 1)
                     }
                 }
                 if (lane == 0)
-                    row_fac[r] = fabsf(a.scale_log2) * pow2_field(ex - 10u);
+                    row_fac[r] = top < 0x7f800000u ? fabsf(a.scale_log2) * pow2_field(ex - 10u) : __uint_as_float(0x7fc00000u);
             }
         }
         sm100::fence_proxy_async_smem();

@@ -352,3 +352,48 @@ def test_more_sequences_than_run_at_once(ops, fmt, kind, dim):
     q = queries(sum(rows), 8, dim, kind, 22)
     got = attend(ops, cache, q, ctx, rows, None, 1 / math.sqrt(dim))
     check(got, *expected(cache, q, ctx, rows, None, 1 / math.sqrt(dim)), 304, kind)
+
+
+# ------------------------------------------------------------------ infinities and NaN
+
+
+@pytest.mark.parametrize("fmt", [0, 1, 2])
+@pytest.mark.parametrize("kind", [0, 1])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("ctx,n", [(0, 3), (300, 3), (0, 60), (300, 60)])
+@pytest.mark.parametrize("bad", [math.inf, -math.inf, math.nan])
+def test_queries_that_are_not_finite(ops, fmt, kind, dim, ctx, n, bad):
+    """Their own rows are NaN (zeros where they see nothing), all others as they were."""
+    cache = plain.Cache([ctx + n], 2, dim, fmt, 23)
+    set_rows(cache, 0, np.arange(ctx + n), k=opposed(5, ctx + n, 2, dim, 4.0).clamp(max=-0.5))  # a score of -inf, too
+    sees = [np.tril(np.ones((n, n), bool))]
+    if ctx == 0:
+        sees[0][2] = False
+    q = queries(n, 4, dim, kind, 24)
+    scale = 1 / math.sqrt(dim)
+    want = expected(cache, q, [ctx], [n], sees, scale)
+    spoiled = q.clone()
+    for i, h in ((0, 1), (1, 2), (2, 0), (n - 1, 3)):
+        spoiled[i, h, (7 * i + h) % dim] = bad
+    got = attend(ops, cache, spoiled, [ctx], [n], sees, scale)
+    hit = ~torch.isfinite(spoiled).all(-1)
+    blind = hit & (want[2] == 0)
+    assert torch.isnan(got[hit & ~blind]).all() and (got[blind] == 0).all()
+    ok = ~hit
+    check(got[ok], want[0][ok], want[1][ok], want[2][ok], ctx + n, kind)
+
+
+@pytest.mark.parametrize("fmt", [0, 1, 2])
+@pytest.mark.parametrize("kind", [0, 1])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("n", [2, 50])
+@pytest.mark.parametrize("at", ["first", "middle", "node"])
+def test_keys_that_are_not_finite(ops, fmt, kind, dim, n, at):
+    """A NaN and an infinity in a row of the context: every node is NaN; in a node's row: those that see it."""
+    ctx = 40
+    bad = {"first": 0, "middle": 21, "node": ctx + 1}[at]
+    cache = plain.Cache([ctx + n], 2, dim, fmt, 25)
+    cache.spoil(0, bad)
+    got = attend(ops, cache, queries(n, 8, dim, kind, 26), [ctx], [n], [np.tril(np.ones((n, n), bool))], 1 / math.sqrt(dim))
+    first = max(0, bad - ctx)
+    assert torch.isnan(got[first:]).all() and torch.isfinite(got[:first]).all()
