@@ -15,6 +15,11 @@
 // fp32. A masked key has no influence, whatever its row holds; an infinity or a
 // NaN in a K or V row that a node does see makes the node's whole output NaN,
 // and so does one in its query row.
+//
+// K and V values may lie anywhere in fp32's range. Those of the context share a
+// power of two, 16 keys (rows kernel; of V 32 dims) or 8 to 32 (tiles), and are
+// held to 2^-22 of the largest of them at least; those of nodes have their own.
+// V rows that one node sees may differ 2^100-fold.
 
 #include "tree_attention_common.cuh"
 #include "tree_attention_rows.cuh"

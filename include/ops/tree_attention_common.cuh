@@ -193,9 +193,10 @@ template <KvFormat kFmt> __device__ __forceinline__ void codes_to_half(uint32_t 
 __device__ __forceinline__ float finite_or_zero(float x) { return fabsf(x) <= 3.4028235e38f ? x : 0.f; }
 
 // The power of two next above magnitude `top` (bits of it) as an exponent
-// field, held where its inverse and its products with 2^10 are normal too.
-__device__ __forceinline__ uint32_t exponent_above(uint32_t top_bits) {
-    return min(max((top_bits >> 23) + 1u, 16u), 240u);
+// field, held where its inverse and its products with 2^10 are normal too (up to
+// `most`: 254 where its inverse times 2^8 or more is all that is wanted).
+__device__ __forceinline__ uint32_t exponent_above(uint32_t top_bits, uint32_t most = 240u) {
+    return min(max((top_bits >> 23) + 1u, 16u), most);
 }
 __device__ __forceinline__ float pow2_field(uint32_t ex) { return __uint_as_float(ex << 23); }
 

@@ -381,14 +381,14 @@ static __global__ void __launch_bounds__(TreeRowsGeo<T, D, kFmt, kMT>::kThreads,
 #pragma unroll
                         for (int off = 4; off < 32; off <<= 1)
                             top = max(top, __shfl_xor_sync(kFullWarpMask, top, off));
-                        const uint32_t ex = exponent_above(top);
+                        const uint32_t ex = exponent_above(top, 254u);
                         if (part == 0) {
                             kex[i] = ex;
                             kfac[i] = pow2_field(ex - 8u);
                         } else {
                             const int log = max(static_cast<int>(ex) - 127, kMinVKey) - 8; // to 2^7 .. 2^8
                             vkey[i] = pow2_field(static_cast<uint32_t>(127 - log));
-                            vlogs[i] = static_cast<float>(max(-126, min(120, log + unit)));
+                            vlogs[i] = static_cast<float>(max(-126, min(126, log + unit)));
                             vfac[i] = pow2_field(static_cast<uint32_t>(127 + static_cast<int>(vlogs[i])));
                         }
                     }
@@ -410,7 +410,7 @@ static __global__ void __launch_bounds__(TreeRowsGeo<T, D, kFmt, kMT>::kThreads,
                     }
                     if (attempt > 0 && top == 0u)
                         break;
-                    kkey[0] = kkey[1] = kmul = pow2_field(254u - exponent_above(top) + 8u); // to 2^7 .. 2^8
+                    kkey[0] = kkey[1] = kmul = pow2_field(254u - exponent_above(top, 254u) + 8u); // to 2^7 .. 2^8
                 }
                 zero_scores();
                 float small[kMT][2][4] = {}; // the small products: an accumulator is cut off at every step, to its size
@@ -473,8 +473,7 @@ static __global__ void __launch_bounds__(TreeRowsGeo<T, D, kFmt, kMT>::kThreads,
             if constexpr (G::kWide && kEdge) {
                 // set above
             } else if constexpr (G::kWide) {
-                kfac[i] = pow2_field(254u - (__float_as_uint(kmul) >> 23));
-                vfac[i] = 1.f;
+                kfac[i] = vfac[i] = 1.f; // K's is the page's, see kunit
             } else {
                 const uint8_t *page = chunk + i / 4 * G::kPageBytes + 16 * (i % 4) + 4 * t;
                 kfac[i] = *reinterpret_cast<const float *>(page + R::kKScale);
@@ -483,13 +482,14 @@ static __global__ void __launch_bounds__(TreeRowsGeo<T, D, kFmt, kMT>::kThreads,
                     const float nan = __uint_as_float(0x7fc00000u);
                     kfac[i] = fabsf(kfac[i]) <= 3.4028235e38f ? kfac[i] : nan;
                     vfac[i] = fabsf(vfac[i]) <= 3.4028235e38f ? vfac[i] : nan;
-                    const uint32_t ex = exponent_above(__float_as_uint(key0 + 4 * i + t < keys ? finite_or_zero(vfac[i]) : 0.f));
+                    const uint32_t ex = exponent_above(__float_as_uint(key0 + 4 * i + t < keys ? finite_or_zero(vfac[i]) : 0.f), 253u);
                     vlogs[i] = fmaxf(static_cast<float>(static_cast<int>(ex) - 127), kMinVLog);
                 } else {
                     vscale = fmaxf(vscale, vfac[i]);
                 }
             }
         }
+        const float kunit = G::kWide && !kEdge ? pow2_field(254u - (__float_as_uint(kmul) >> 23)) : 1.f;
         // Scores: less their row's scale; of edge chunks in log2 units, masked ones -inf,
         // and the V factors of the keys that a row sees enter its own reference
         bool raise = vscale > vtop;
@@ -502,9 +502,10 @@ static __global__ void __launch_bounds__(TreeRowsGeo<T, D, kFmt, kMT>::kThreads,
             for (int rr = 0; rr < G::kRPL; ++rr) {
 #pragma unroll
                 for (int i = 0; i < 4 * kC; ++i) {
-                    const float *c = sc[mt][i >> 1];
-                    x[mt][rr][i] = (G::kTwo ? c[i & 1] + c[2 + (i & 1)] : c[2 * rr + (i & 1)]) * kfac[i];
+                    const float *c = sc[mt][i >> 1], s = G::kTwo ? c[i & 1] + c[2 + (i & 1)] : c[2 * rr + (i & 1)];
+                    x[mt][rr][i] = G::kWide ? s : s * kfac[i];
                 }
+                const float scale = row_scale[mt][rr] * kunit;
                 float top = kNegInf;
                 if constexpr (kEdge) {
                     const int r = row_base + mt * G::kTileRows + rr * 8 + g;
@@ -513,7 +514,7 @@ static __global__ void __launch_bounds__(TreeRowsGeo<T, D, kFmt, kMT>::kThreads,
                         seen = tree_sees32(a.t, span.row0 + r / rep, r / rep, key0 - span.ctx, keys - span.ctx);
 #pragma unroll
                     for (int i = 0; i < 4 * kC; ++i) {
-                        float y = x[mt][rr][i] * row_scale[mt][rr];
+                        float y = G::kWide ? x[mt][rr][i] * scale * kfac[i] : x[mt][rr][i] * scale;
                         if (G::kWide && (bad >> i & 1u))
                             y = __uint_as_float(0x7fc00000u);
                         if (!(seen >> (4 * i + t) & 1u))
@@ -526,7 +527,7 @@ static __global__ void __launch_bounds__(TreeRowsGeo<T, D, kFmt, kMT>::kThreads,
 #pragma unroll
                     for (int i = 0; i < 4 * kC; ++i)
                         top = fmaxf(top, x[mt][rr][i]);
-                    raise |= top * row_scale[mt][rr] > m[mt][rr] + slack;
+                    raise |= top * scale > m[mt][rr] + slack;
                 }
             }
         if (__any_sync(kFullWarpMask, raise)) {
@@ -535,7 +536,7 @@ static __global__ void __launch_bounds__(TreeRowsGeo<T, D, kFmt, kMT>::kThreads,
                 if (top >= 0x7f800000u) {
                     poison();
                 } else if (__uint_as_float(top) > vtop || __uint_as_float(top) < vtop * kLowV) {
-                    vtop = fmaxf(pow2_field(exponent_above(top)), kMinVTop);
+                    vtop = fmaxf(pow2_field(exponent_above(top, 253u)), kMinVTop);
                     vlog = static_cast<float>(static_cast<int>(__float_as_uint(vtop) >> 23) - 127);
                 }
             }
@@ -551,7 +552,7 @@ static __global__ void __launch_bounds__(TreeRowsGeo<T, D, kFmt, kMT>::kThreads,
                     up = fmaxf(up, __shfl_xor_sync(kFullWarpMask, up, 1));
                     up = fmaxf(up, __shfl_xor_sync(kFullWarpMask, up, 2));
                     if (!kEdge)
-                        up = up * row_scale[mt][rr] + (G::kWide ? 0.f : vlog);
+                        up = up * (row_scale[mt][rr] * kunit) + (G::kWide ? 0.f : vlog);
                     up = fmaxf(m[mt][rr], up - reference_lift(kLift, up));
                     wary |= fabsf(up) > kWary && up > kNone;
                     fix[rr] = exp2_approx(m[mt][rr] - up);
@@ -570,10 +571,11 @@ static __global__ void __launch_bounds__(TreeRowsGeo<T, D, kFmt, kMT>::kThreads,
         for (int mt = 0; mt < kMT; ++mt) {
             float p[G::kRPL][4 * kC];
 #pragma unroll
-            for (int rr = 0; rr < G::kRPL; ++rr)
+            for (int rr = 0; rr < G::kRPL; ++rr) {
+                const float scale = row_scale[mt][rr] * kunit;
 #pragma unroll
                 for (int i = 0; i < 4 * kC; ++i) {
-                    float e = kEdge ? x[mt][rr][i] - m[mt][rr] : fmaf(x[mt][rr][i], row_scale[mt][rr], -m[mt][rr]);
+                    float e = kEdge ? x[mt][rr][i] - m[mt][rr] : fmaf(x[mt][rr][i], scale, -m[mt][rr]);
                     if (kEdge) { // (a NaN stays)
                         const float cap = kLift + kLazy + 1.f - vlogs[kEdge ? i : 0];
                         e = e > cap ? cap : e;
@@ -583,6 +585,7 @@ static __global__ void __launch_bounds__(TreeRowsGeo<T, D, kFmt, kMT>::kThreads,
                     l[mt][rr] += w;
                     p[rr][i] = (G::kWide && !kEdge) || masked ? w : w * vfac[i];
                 }
+            }
 #pragma unroll
             for (int i = 0; i < 2 * kC; ++i) {
                 const uint32_t hi = half2_rn(p[0][2 * i], p[0][2 * i + 1]);
@@ -629,7 +632,7 @@ static __global__ void __launch_bounds__(TreeRowsGeo<T, D, kFmt, kMT>::kThreads,
                         if (attempt > 0 && top == 0u)
                             break;
                         // to 2^7 .. 2^8; what is summed already must not leave fp32's range
-                        float next = pow2_field(254u - max(exponent_above(top), static_cast<uint32_t>(127 + kMinVKey)) + 8u);
+                        float next = pow2_field(254u - max(exponent_above(top, 254u), static_cast<uint32_t>(127 + kMinVKey)) + 8u);
                         if (vmul[c] != 0.f)
                             next = fminf(next, vmul[c] * 0x1p60f);
                         resize(c, next);
@@ -731,9 +734,12 @@ static __global__ void __launch_bounds__(TreeRowsGeo<T, D, kFmt, kMT>::kThreads,
 
     // the warps' results over the ring, joined in warp order
     float *part = reinterpret_cast<float *>(smem);
-    float vunit = 1.f;
-    if constexpr (G::kWide)
-        vunit = pow2_field(254u - (__float_as_uint(one_vmul()) >> 23));
+    // fp32: V's unit goes into m and l, for O times it may leave fp32's range
+    float vunit = 1.f, unit_log = 0.f;
+    if constexpr (G::kWide) {
+        vunit = one_vmul();
+        unit_log = static_cast<float>(static_cast<int>(__float_as_uint(vunit) >> 23) - 127);
+    }
 #pragma unroll
     for (int mt = 0; mt < kMT; ++mt)
 #pragma unroll
@@ -749,11 +755,11 @@ static __global__ void __launch_bounds__(TreeRowsGeo<T, D, kFmt, kMT>::kThreads,
                 for (int col = 0; col < 2; ++col) {
                     const float v = G::kTwo ? o[mt][n][col] + o[mt][n][2 + col] : o[mt][n][2 * rr + col];
                     const int d = G::kWide ? 32 * (n / 4) + 4 * (2 * t + col) + n % 4 : (D / 8) * (2 * t + col) + n;
-                    dst[d] = v * vunit;
+                    dst[d] = v;
                 }
             if (t == 0) {
-                stat[warp * G::kRows + r] = m[mt][rr];
-                stat[(G::kWarps + warp) * G::kRows + r] = sum;
+                stat[warp * G::kRows + r] = m[mt][rr] - unit_log;
+                stat[(G::kWarps + warp) * G::kRows + r] = sum * vunit;
             }
         }
     __syncthreads();

@@ -338,7 +338,7 @@ static __global__ void __launch_bounds__(kTileThreads, 1)
                     most = max_abs_nan(max_abs_nan(most, y[j][0], y[j][1]), y[j][2], y[j][3]);
                 }
                 const uint32_t bits = __reduce_max_sync(kFullWarpMask, __float_as_uint(most));
-                const uint32_t ex = max(exponent_above(bits), v ? kMinVField + 9u : 0u);
+                const uint32_t ex = max(exponent_above(bits, 254u), v ? kMinVField + 9u : 0u);
                 const float f = pow2_field(254u - ex + 10u);
                 unit = bits < 0x7f800000u ? pow2_field(ex - 10u) : __uint_as_float(0x7fc00000u);
                 if (edge) { // a row that some nodes do not see takes no bits from the others
@@ -365,7 +365,7 @@ static __global__ void __launch_bounds__(kTileThreads, 1)
 #pragma unroll
                             for (int off = 1; off < kRowLanes; off <<= 1)
                                 t = fmaxf(t, __shfl_xor_sync(kFullWarpMask, t, off));
-                            const uint32_t own = max(exponent_above(__float_as_uint(t)), v ? kMinVField + 9u : 0u);
+                            const uint32_t own = max(exponent_above(__float_as_uint(t), 254u), v ? kMinVField + 9u : 0u);
 #pragma unroll
                             for (int e = 0; e < 4; ++e)
                                 y[j][e] = y[j][e] * pow2_field(254u - own + 10u) * pow2_field(ex - 10u);
@@ -404,10 +404,10 @@ static __global__ void __launch_bounds__(kTileThreads, 1)
                     }
                 } else {
                     const uint32_t own = bad ? 0u : __float_as_uint(scale);
-                    uint32_t ex = exponent_above(__reduce_max_sync(kFullWarpMask, own));
+                    uint32_t ex = exponent_above(__reduce_max_sync(kFullWarpMask, own), 254u);
                     if (edge) // a row that some nodes do not see takes no bits from the others
-                        each = !__all_sync(kFullWarpMask, own == 0u || exponent_above(own) + kUnlike >= ex);
-                    ex = max(each ? exponent_above(own) : ex, kMinVField);
+                        each = !__all_sync(kFullWarpMask, own == 0u || exponent_above(own, 254u) + kUnlike >= ex);
+                    ex = max(each ? exponent_above(own, 254u) : ex, kMinVField);
                     scale = bad ? 0.f : scale * pow2_field(254u - ex + 1u); // at most 2
 #pragma unroll
                     for (int j = 0; j < G::kLoads; ++j) {

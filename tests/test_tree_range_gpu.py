@@ -397,3 +397,21 @@ def test_keys_that_are_not_finite(ops, fmt, kind, dim, n, at):
     got = attend(ops, cache, queries(n, 8, dim, kind, 26), [ctx], [n], [np.tril(np.ones((n, n), bool))], 1 / math.sqrt(dim))
     first = max(0, bad - ctx)
     assert torch.isnan(got[first:]).all() and torch.isfinite(got[:first]).all()
+
+
+# ------------------------------------------------------------------ the range of fp32
+
+
+@pytest.mark.parametrize("fmt", [0, 1, 2])
+@pytest.mark.parametrize("kind", [0, 1])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("ctx,n", [(0, 5), (300, 3), (0, 60), (900, 60)])
+@pytest.mark.parametrize("kexp,vexp", [(100, 0), (-100, 0), (0, 126), (0, -40), (100, 126), (-100, -40)])
+def test_rows_at_the_ends_of_fp32(ops, fmt, kind, dim, ctx, n, kexp, vexp):
+    """K rows of 2^100 and 2^-100 (with queries that make up for them), V rows up to 3 2^126 and down to 2^-40."""
+    cache = plain.Cache([ctx + n], 2, dim, fmt, 27)
+    k, v = (queries(ctx + n, 2, dim, 0, s).clamp(-3, 3) for s in (28, 29))
+    set_rows(cache, 0, np.arange(ctx + n), k=k * 2.0**kexp, v=v * 2.0**vexp)
+    q = queries(n, 8, dim, kind, 30) * 2.0**-kexp
+    got = attend(ops, cache, q, [ctx], [n], None, 1 / math.sqrt(dim))
+    check(got, *expected(cache, q, [ctx], [n], None, 1 / math.sqrt(dim)), ctx + n, kind)
