@@ -60,6 +60,10 @@ SIGNATURES = {
 }
 
 
+# These return a number, below zero for an error; all others 0 or an error.
+VALUES = frozenset(("reduction_workspace_size", "kv_quant_record_bytes"))
+
+
 class OpsLib:
     def __init__(self, lib):
         self.lib = lib
@@ -83,9 +87,11 @@ class OpsLib:
 
         # A call of 20 arguments costs as much here as its launch: numbers go
         # through as they are, and the caller is kept (the next access finds it).
+        value = name in VALUES
+
         def call(*args):
             rc = fn(*[a if a.__class__ in _PLAIN else _arg(a) for a in args])
-            return self.check(rc) if rc else rc
+            return self.check(rc) if rc and not (value and rc > 0) else rc
 
         setattr(self, name, call)
         return call

@@ -66,9 +66,7 @@ class PagedCache:
         self.stride = -(-max_tokens // self.PAGE)
         blocks = batch * self.stride
         if self.format:
-            record = self.ops.raw("kv_quant_record_bytes")(head_dim)
-            if record < 0:
-                raise ValueError(self.ops.last_error())
+            record = self.ops.kv_quant_record_bytes(head_dim)
             self.pool = torch.zeros(layers, blocks, kv_heads, record, dtype=torch.uint8, device=device)
         else:
             self.k = torch.zeros(layers, blocks, kv_heads, self.PAGE, head_dim, device=device)
