@@ -80,13 +80,29 @@ class PagedCache:
     def _stream():
         return torch.cuda.current_stream().cuda_stream
 
+    def _belongs(self, rows):
+        if len(rows.counts) != self.batch or rows.start.device != self.lens.device:
+            raise ValueError("rows: counts of this cache's sequences, on its device")
+
+    def _takes(self, name, t, shape, dtypes):
+        """Refuses a tensor that an operator, which gets its address only, would read or write wrongly."""
+        if t.device != self.lens.device or tuple(t.shape) != tuple(shape) or t.dtype not in dtypes:
+            raise ValueError(f"{name}: {list(shape)} of {' or '.join(str(d) for d in dtypes)} on {self.lens.device}, not "
+                             f"{list(t.shape)} of {t.dtype} on {t.device}")
+
     def _room(self, rows):
         if self.max_len + rows.most > self.stride * self.PAGE:
             raise ValueError("the cache has no room for these rows")
 
     def write(self, layer, k, v, rows):
         """K and V rows [total, kv_heads * head_dim] (any row stride) at positions lens + 0, 1, ... of their sequences."""
+        self._belongs(rows)
+        shape = (rows.total, self.kv_heads * self.head_dim)
+        self._takes("k", k, shape, TYPES)
+        self._takes("v", v, shape, (k.dtype,))
         self._room(rows)
+        if k.stride() != v.stride() or k.stride(1) != 1:  # the operator takes one row stride
+            k, v = k.contiguous(), v.contiguous()
         if self.format:
             self.ops.kv_quant_write(k, v, TYPES[k.dtype], k.stride(0), self.pool[layer], self.format, self.table, self.stride,
                                     self.lens, rows.start, self.batch, rows.total, self.kv_heads, self.head_dim, self._stream())

@@ -14,3 +14,24 @@ def test_record_bytes_through_the_binding():
     assert ops.reduction_workspace_size(1 << 20) > 0
     with pytest.raises(ValueError, match="head_dim"):
         ops.kv_quant_record_bytes(80)
+
+
+def cpu_cache(format="int8", batch=2, tokens=64, **kw):
+    from opworks_b200.tree import PagedCache
+
+    return PagedCache(1, batch, tokens, 2, 64, format, device="cpu", **kw)
+
+
+@pytest.mark.parametrize("format", ["int8", "f32"])
+def test_write_refuses_rows_that_it_would_misread(format):
+    from opworks_b200.tree import Rows
+
+    cache, rows = cpu_cache(format), Rows([3, 2], device="cpu")
+    k = torch.randn(5, 128)
+    for bad_k, bad_v in [(k, k.bfloat16()), (k.double(), k.double()), (k[:4], k[:4]), (k, k[:4]), (k, torch.randn(6, 128)),
+                         (k[:, :64], k[:, :64]), (k.view(5, 2, 64), k.view(5, 2, 64)), (k, k.to("meta")), (k.half(), k.half())]:
+        with pytest.raises(ValueError):
+            cache.write(0, bad_k, bad_v, rows)
+    for counts in ([5], [3, 1, 1]):
+        with pytest.raises(ValueError, match="sequences"):
+            cache.write(0, k, k, Rows(counts, device="cpu"))

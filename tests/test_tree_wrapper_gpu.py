@@ -1,0 +1,26 @@
+"""The torch wrapper of the drafted-token step (opworks_b200/tree.py) against plain torch, on the GPU."""
+
+import math
+
+import pytest
+
+pytestmark = pytest.mark.gpu
+torch = pytest.importorskip("torch")
+
+
+@pytest.mark.parametrize("format", ["int8", "e4m3", "f32"])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_write_takes_k_and_v_of_different_strides(format, dtype):
+    """K a slice of a fused projection and V a tensor of its own, or turned round: as if both lay one row after another."""
+    from opworks_b200.tree import PagedCache, Rows
+
+    rows = Rows([5, 0, 33])
+    wide = torch.randn(rows.total, 384, device="cuda").to(dtype)
+    k, v = wide[:, 128:256], torch.randn(rows.total, 128, device="cuda").to(dtype)
+    turned = v.t().contiguous().t()  # inner stride rows.total
+    caches = []
+    for a, b in ((k.contiguous(), v), (k, v), (k, turned), (v, k)):
+        caches.append(PagedCache(1, 3, 100, 2, 64, format))
+        caches[-1].write(0, a, b, rows)
+    same = lambda x, y: torch.equal(x.pool, y.pool) if format != "f32" else torch.equal(x.k, y.k) and torch.equal(x.v, y.v)  # noqa: E731
+    assert same(caches[0], caches[1]) and same(caches[0], caches[2]) and not same(caches[0], caches[3])
