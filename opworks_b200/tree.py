@@ -126,8 +126,15 @@ class PagedCache:
         return k, v
 
     def attend(self, layer, q, rows, out, scale):
-        """q, out [total, q_heads, head_dim], fp32 or bf16, rows contiguous; the rows' K and V are written already."""
-        heads = q.shape[1]
+        """q, out [total, q_heads, head_dim], both fp32 or both bf16, rows contiguous; the rows' K and V are written already."""
+        self._belongs(rows)
+        heads = q.shape[1] if q.dim() == 3 else 0
+        shape = (rows.total, heads, self.head_dim)
+        self._takes("q", q, shape, TYPES)
+        self._takes("out", out, shape, (q.dtype,))
+        for name, t in (("q", q), ("out", out)):
+            if rows.total and (t.stride(2) != 1 or (heads > 1 and t.stride(1) != self.head_dim)):
+                raise ValueError(f"{name}: the heads of a row lie one after another")
         rest = (self.table, self.stride, self.lens, rows.start, rows.mask, rows.words, self.batch, rows.total, rows.most,
                 self.max_len, heads, self.kv_heads, self.head_dim, scale, out, out.stride(0), self._stream())
         if self.format:

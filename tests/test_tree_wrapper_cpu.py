@@ -35,3 +35,18 @@ def test_write_refuses_rows_that_it_would_misread(format):
     for counts in ([5], [3, 1, 1]):
         with pytest.raises(ValueError, match="sequences"):
             cache.write(0, k, k, Rows(counts, device="cpu"))
+
+
+@pytest.mark.parametrize("format", ["int8", "f32"])
+def test_attend_refuses_what_it_would_misread_or_overrun(format):
+    from opworks_b200.tree import Rows
+
+    cache, rows = cpu_cache(format), Rows([3, 2], device="cpu")
+    q = torch.randn(5, 8, 64)
+    for bad_q, bad_out in [(q, q.bfloat16()), (q.half(), q.half()), (q[:4], q[:4]), (q, q[:4]), (q, q[:, :4]), (q[..., :32], q[..., :32]),
+                           (q.view(5, 512), q.view(5, 512)), (torch.randn(8, 5, 64).transpose(0, 1), q), (q, torch.randn(5, 64, 8).transpose(1, 2)),
+                           (q, q.to("meta"))]:
+        with pytest.raises(ValueError):
+            cache.attend(0, bad_q, rows, bad_out, 0.125)
+    with pytest.raises(ValueError, match="sequences"):
+        cache.attend(0, q, Rows([5], device="cpu"), q, 0.125)

@@ -24,3 +24,23 @@ def test_write_takes_k_and_v_of_different_strides(format, dtype):
         caches[-1].write(0, a, b, rows)
     same = lambda x, y: torch.equal(x.pool, y.pool) if format != "f32" else torch.equal(x.k, y.k) and torch.equal(x.v, y.v)  # noqa: E731
     assert same(caches[0], caches[1]) and same(caches[0], caches[2]) and not same(caches[0], caches[3])
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_attend_over_rows_of_a_wider_tensor(dtype):
+    from opworks_b200.tree import PagedCache, Rows
+
+    rows = Rows([4, 7])
+    cache = PagedCache(1, 2, 64, 2, 64, "f32")
+    k, v = torch.randn(2, rows.total, 128, device="cuda")
+    cache.write(0, k, v, rows)
+    wide = torch.randn(rows.total, 10, 64, device="cuda").to(dtype)
+    out = torch.zeros(rows.total, 10, 64, device="cuda", dtype=dtype)
+    cache.attend(0, wide[:, 1:9], rows, out[:, 1:9], 0.125)
+    assert not out[:, 0].any() and not out[:, 9].any()
+    for b, (lo, hi) in enumerate(((0, 4), (4, 11))):
+        for h in range(8):
+            kk, vv = (x[lo:hi, h // 4 * 64 : h // 4 * 64 + 64].double() for x in (k, v))
+            s = (0.125 * wide[lo:hi, 1 + h].double() @ kk.T).masked_fill(~torch.ones(hi - lo, hi - lo, device="cuda").bool().tril(), -math.inf)
+            want = torch.softmax(s, -1) @ vv
+            assert (out[lo:hi, 1 + h].double() - want).abs().max() <= (2.0**-7 if dtype == torch.bfloat16 else 2.0**-16) * vv.abs().max()
