@@ -26,6 +26,7 @@ from . import ops_lib
 
 FORMATS = {"f32": 0, "int8": 1, "e4m3": 2}
 TYPES = {torch.float32: 0, torch.bfloat16: 1}
+INTEGERS = (torch.int32, torch.int64, torch.int16, torch.uint8, torch.int8)
 
 
 def tree_mask(parents, words):
@@ -148,7 +149,12 @@ class PagedCache:
         self.max_len += rows.most
 
     def commit(self, draft, target, rows):
-        """Keeps each tree's accepted path (all layers). Returns (path, count, next), int32 on the device."""
+        """Keeps each tree's accepted path (all layers). draft, target: whole numbers [total], any integer type. Returns
+        (path, count, next), int32 on the device."""
+        self._belongs(rows)
+        for name, t in (("draft", draft), ("target", target)):
+            self._takes(name, t, (rows.total,), INTEGERS)
+        draft, target = draft.to(torch.int32).contiguous(), target.to(torch.int32).contiguous()
         new = lambda n: torch.empty(n, dtype=torch.int32, device=self.lens.device)  # noqa: E731
         path, count, nxt, lens = new(rows.total), new(self.batch), new(self.batch), new(self.batch)
         head = (draft, target, rows.parents, rows.start, self.lens, self.batch, rows.most)

@@ -50,3 +50,16 @@ def test_attend_refuses_what_it_would_misread_or_overrun(format):
             cache.attend(0, bad_q, rows, bad_out, 0.125)
     with pytest.raises(ValueError, match="sequences"):
         cache.attend(0, q, Rows([5], device="cpu"), q, 0.125)
+
+
+def test_commit_refuses_tokens_that_are_none():
+    from opworks_b200.tree import Rows
+
+    cache, rows = cpu_cache(), Rows([3, 2], [[-1, 0, 0], [-1, 0]], device="cpu")
+    good = torch.zeros(5, dtype=torch.int32)
+    for draft, target in [(good.float(), good), (good, good.float()), (good[:4], good), (good, good[:3]), (good.view(5, 1), good),
+                          (good, good.to("meta"))]:
+        with pytest.raises(ValueError):
+            cache.commit(draft, target, rows)
+    with pytest.raises(ValueError, match="sequences"):
+        cache.commit(good, good, Rows([5], [[-1, 0, 1, 2, 3]], device="cpu"))

@@ -44,3 +44,18 @@ def test_attend_over_rows_of_a_wider_tensor(dtype):
             s = (0.125 * wide[lo:hi, 1 + h].double() @ kk.T).masked_fill(~torch.ones(hi - lo, hi - lo, device="cuda").bool().tril(), -math.inf)
             want = torch.softmax(s, -1) @ vv
             assert (out[lo:hi, 1 + h].double() - want).abs().max() <= (2.0**-7 if dtype == torch.bfloat16 else 2.0**-16) * vv.abs().max()
+
+
+@pytest.mark.parametrize("kind", [torch.int32, torch.int64, torch.int16])
+def test_commit_takes_tokens_of_any_integer_type(kind):
+    from opworks_b200.tree import PagedCache, Rows
+
+    cache = PagedCache(1, 2, 64, 2, 64, "int8")
+    rows = Rows([4, 3], [[-1, 0, 0, 2], [-1, 0, 1]])
+    k, v = torch.randn(2, 7, 128, device="cuda")
+    cache.write(0, k, v, rows)
+    draft = torch.tensor([5, 6, 7, 8, 5, 6, 7], device="cuda").to(kind)
+    target = torch.tensor([7, 0, 8, 9, 1, 2, 3], device="cuda").to(kind)
+    path, count, nxt = cache.commit(draft.repeat_interleave(2)[::2], target, rows)
+    assert path.tolist() == [0, 2, 3, -1, 0, -1, -1] and count.tolist() == [3, 1] and nxt.tolist() == [9, 1]
+    assert cache.lens.tolist() == [3, 1]
