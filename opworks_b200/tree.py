@@ -49,13 +49,22 @@ class Rows:
         start = np.concatenate([[0], np.cumsum(counts)]).astype(np.int32)
         self.counts, self.total, self.most = list(counts), int(start[-1]), max(counts, default=0)
         self.start = torch.from_numpy(start).to(device)
-        self.mask, self.words, self.parents = None, 0, None
+        self.mask, self.words, self._parents = None, 0, None
         if parents is not None:
             if [len(p) for p in parents] != self.counts:
                 raise ValueError("parents: one list per sequence, as long as its rows")
             self.words = max(1, -(-self.most // 32))
             self.mask = torch.from_numpy(np.concatenate([tree_mask(p, self.words) for p in parents])).to(device)
-            self.parents = torch.from_numpy(np.concatenate(parents).astype(np.int32)).to(device)
+            self._parents = torch.from_numpy(np.concatenate(parents).astype(np.int32)).to(device)
+
+    @property
+    def parents(self):
+        """The node that each row follows, int32 on the device: in a chain the one before it."""
+        if self._parents is None:
+            owner = np.repeat(np.arange(len(self.counts)), self.counts)
+            node = np.arange(self.total) - np.concatenate([[0], np.cumsum(self.counts)])[owner]
+            self._parents = torch.from_numpy((node - 1).astype(np.int32)).to(self.start.device)
+        return self._parents
 
 
 class PagedCache:
@@ -149,7 +158,7 @@ class PagedCache:
         self.max_len += rows.most
 
     def commit(self, draft, target, rows):
-        """Keeps each tree's accepted path (all layers). draft, target: whole numbers [total], any integer type. Returns
+        """Keeps each tree's accepted path, each chain's accepted part (all layers). draft, target: whole numbers [total], any integer type. Returns
         (path, count, next), int32 on the device."""
         self._belongs(rows)
         for name, t in (("draft", draft), ("target", target)):

@@ -63,3 +63,11 @@ def test_commit_refuses_tokens_that_are_none():
             cache.commit(draft, target, rows)
     with pytest.raises(ValueError, match="sequences"):
         cache.commit(good, good, Rows([5], [[-1, 0, 1, 2, 3]], device="cpu"))
+
+
+def test_the_parents_of_a_chain():
+    from opworks_b200.tree import Rows
+
+    assert Rows([3, 0, 2], device="cpu").parents.tolist() == [-1, 0, 1, -1, 0]
+    assert Rows([], device="cpu").parents.tolist() == []
+    assert Rows([2, 1], [[-1, 0], [-1]], device="cpu").parents.tolist() == [-1, 0, -1]

@@ -59,3 +59,19 @@ def test_commit_takes_tokens_of_any_integer_type(kind):
     path, count, nxt = cache.commit(draft.repeat_interleave(2)[::2], target, rows)
     assert path.tolist() == [0, 2, 3, -1, 0, -1, -1] and count.tolist() == [3, 1] and nxt.tolist() == [9, 1]
     assert cache.lens.tolist() == [3, 1]
+
+
+@pytest.mark.parametrize("format", ["int8", "f32"])
+def test_commit_of_drafted_chains(format):
+    from opworks_b200.tree import PagedCache, Rows
+
+    cache = PagedCache(2, 3, 64, 2, 64, format)
+    rows = Rows([4, 1, 3])
+    k, v = torch.randn(2, 8, 128, device="cuda")
+    for layer in range(2):
+        cache.write(layer, k, v, rows)
+    draft = torch.tensor([5, 6, 7, 8, 1, 2, 3, 4], device="cuda")
+    target = torch.tensor([6, 7, 1, 9, 4, 3, 4, 11], device="cuda")  # two of three right; nothing drafted; all right
+    path, count, nxt = cache.commit(draft, target, rows)
+    assert path.tolist() == [0, 1, 2, -1, 0, 0, 1, 2] and count.tolist() == [3, 1, 3] and nxt.tolist() == [1, 4, 11]
+    assert cache.lens.tolist() == [3, 1, 3]
