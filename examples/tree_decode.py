@@ -79,7 +79,7 @@ def generate(model, prompts, tokens, format, draft=None, seed=0):
     """Continues the prompts by at least `tokens` tokens. draft: None for one token per step, else the continuations that
     the stand-in for a draft model knows. Returns (tokens of each sequence, steps)."""
     rng, batch = random.Random(seed), len(prompts)
-    room = max(map(len, prompts)) + (tokens + 1) * len(PARENTS) + len(PARENTS)
+    room = max(map(len, prompts)) + tokens + 2 * len(PARENTS)  # what is kept (a path may end past `tokens`), and a tree
     cache = PagedCache(LAYERS, batch, room, KV_HEADS, DIM, format)
     rows = Rows([len(p) for p in prompts])
     _, target = model.step(cache, sum(prompts, []), [i for p in prompts for i in range(len(p))], rows)
@@ -91,7 +91,7 @@ def generate(model, prompts, tokens, format, draft=None, seed=0):
         depth[i] = depth[p] + 1
     while min(map(len, out)) <= tokens:
         steps += 1
-        parents = [PARENTS if draft else [-1]] * batch
+        parents = [[] if len(o) > tokens else PARENTS if draft else [-1] for o in out]  # a sequence that is done has no rows
         rows = Rows([len(p) for p in parents], parents)
         given, positions = [], []
         for b in range(batch):
@@ -106,7 +106,10 @@ def generate(model, prompts, tokens, format, draft=None, seed=0):
         ids, target = model.step(cache, given, positions, rows)
         path, count, nxt = cache.commit(ids, target, rows)
         path, count, nxt, start = path.tolist(), count.tolist(), nxt.tolist(), rows.start.tolist()
+        cache.kept(count)
         for b in range(batch):
+            if count[b] == 0:
+                continue
             kept = [given[start[b] + path[start[b] + i]] for i in range(1, count[b])]
             out[b] += kept + [nxt[b]]
             lens[b] += count[b]

@@ -13,6 +13,7 @@ fp32 or in 8 bits; a step writes the new tokens' K and V, attends, and commits::
     ...
     rows = Rows([n] * 4, parents)                           # a drafted tree per sequence
     path, count, next = cache.commit(draft, target, rows)   # only the accepted path stays
+    cache.kept(count.tolist())                              # once the host has read it: how full the cache is
 
 Everything runs on torch's current stream; nothing here waits for the device.
 """
@@ -41,6 +42,14 @@ def tree_mask(parents, words):
     return (sees.reshape(len(parents), words, 32) << np.arange(32, dtype=np.uint32)).sum(-1, dtype=np.uint32).view(np.int32)
 
 
+def deepest(parents):
+    """Nodes on the longest path of a tree from node 0 on, which is all that can be accepted."""
+    depth = []
+    for i, p in enumerate(parents):
+        depth.append(1 if i == 0 else depth[p] + 1 if p >= 0 and depth[p] else 0)
+    return max(depth, default=0)
+
+
 class Rows:
     """The new tokens of a step: ``counts[b]`` rows of each sequence, one after another. With ``parents`` (a list per
     sequence) they are trees, else chains."""
@@ -50,12 +59,14 @@ class Rows:
         self.counts, self.total, self.most = list(counts), int(start[-1]), max(counts, default=0)
         self.start = torch.from_numpy(start).to(device)
         self.mask, self.words, self._parents = None, 0, None
+        self.depths = list(counts)  # the most nodes on a path
         if parents is not None:
             if [len(p) for p in parents] != self.counts:
                 raise ValueError("parents: one list per sequence, as long as its rows")
             self.words = max(1, -(-self.most // 32))
             self.mask = torch.from_numpy(np.concatenate([tree_mask(p, self.words) for p in parents])).to(device)
             self._parents = torch.from_numpy(np.concatenate(parents).astype(np.int32)).to(device)
+            self.depths = [deepest(p) for p in parents]
 
     @property
     def parents(self):
@@ -84,7 +95,12 @@ class PagedCache:
         # each sequence's pages spread over the pool, as an allocator would leave them
         self.table = torch.arange(blocks, dtype=torch.int32, device=device).view(self.stride, batch).t().contiguous()
         self.lens = torch.zeros(batch, dtype=torch.int32, device=device)
-        self.max_len = 0  # an upper bound of lens that the host knows
+        self.bounds = [0] * batch  # upper bounds of lens that the host knows
+        self._before = None        # those before the last commit
+
+    @property
+    def max_len(self):
+        return max(self.bounds, default=0)
 
     @staticmethod
     def _stream():
@@ -101,7 +117,7 @@ class PagedCache:
                              f"{list(t.shape)} of {t.dtype} on {t.device}")
 
     def _room(self, rows):
-        if self.max_len + rows.most > self.stride * self.PAGE:
+        if any(n and b + n > self.stride * self.PAGE for b, n in zip(self.bounds, rows.counts)):
             raise ValueError("the cache has no room for these rows")
 
     def write(self, layer, k, v, rows):
@@ -154,8 +170,9 @@ class PagedCache:
 
     def advance(self, rows):
         """Keeps all rows (a prompt, or a chain that needs no verification)."""
+        self._belongs(rows)
         self.lens = self.lens + rows.start.diff()
-        self.max_len += rows.most
+        self.bounds, self._before = [b + n for b, n in zip(self.bounds, rows.counts)], None
 
     def commit(self, draft, target, rows):
         """Keeps each tree's accepted path, each chain's accepted part (all layers). draft, target: whole numbers [total], any integer type. Returns
@@ -173,5 +190,16 @@ class PagedCache:
         else:
             self.ops.tree_commit(*head, self.k, self.v, self.k.stride(0), *tail)
         self.lens = lens
-        self.max_len += rows.most
+        self._before, self.bounds = self.bounds, [b + n for b, n in zip(self.bounds, rows.depths)]
         return path, count, nxt
+
+    def kept(self, counts):
+        """Tells the host what the last commit kept: its count, which the caller has read. Without it a sequence is taken
+        to have grown by its tree's deepest path, and the cache seems full before it is."""
+        counts = [int(n) for n in counts]
+        if self._before is None or len(counts) != self.batch:
+            raise ValueError("kept: the counts of a commit, once after it")
+        bounds = [b + n for b, n in zip(self._before, counts)]
+        if any(n < 0 for n in counts) or any(b > most for b, most in zip(bounds, self.bounds)):
+            raise ValueError("kept: no more than the deepest paths of the last commit's trees")
+        self.bounds, self._before = bounds, None

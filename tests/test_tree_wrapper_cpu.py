@@ -71,3 +71,34 @@ def test_the_parents_of_a_chain():
     assert Rows([3, 0, 2], device="cpu").parents.tolist() == [-1, 0, 1, -1, 0]
     assert Rows([], device="cpu").parents.tolist() == []
     assert Rows([2, 1], [[-1, 0], [-1]], device="cpu").parents.tolist() == [-1, 0, -1]
+
+
+def test_deepest_path():
+    from opworks_b200.tree import deepest
+
+    assert deepest([]) == 0 and deepest([-1]) == 1 and deepest([-1, 0, 1, 2]) == 4
+    assert deepest([-1, 0, 0, 1, 1, 3, 3]) == 4
+    assert deepest([-1, -1, 1, 2]) == 1  # what hangs on another root is never accepted
+
+
+def test_the_host_knows_how_full_the_cache_is():
+    from opworks_b200.tree import Rows
+
+    cache = cpu_cache(tokens=64)  # 64 places
+    tree = Rows([4, 3], [[-1, 0, 0, 2], [-1, 0, 1]], device="cpu")
+    cache.advance(Rows([10, 20], device="cpu"))
+    assert cache.bounds == [10, 20] and cache.max_len == 20 and cache.lens.tolist() == [10, 20]
+    # as after a commit: deepest paths, until the host says what was kept
+    cache._before, cache.bounds = cache.bounds, [b + n for b, n in zip(cache.bounds, tree.depths)]
+    assert cache.bounds == [13, 23]
+    for wrong in ([4, 1], [1], [-1, 0]):
+        with pytest.raises(ValueError, match="kept"):
+            cache.kept(wrong)
+    cache.kept([2, 1])
+    assert cache.bounds == [12, 21]
+    with pytest.raises(ValueError, match="kept"):
+        cache.kept([0, 0])
+    cache._room(Rows([52, 43], device="cpu"))
+    cache._room(Rows([52, 0], device="cpu"))
+    with pytest.raises(ValueError, match="room"):
+        cache._room(Rows([1, 44], device="cpu"))

@@ -75,3 +75,30 @@ def test_commit_of_drafted_chains(format):
     path, count, nxt = cache.commit(draft, target, rows)
     assert path.tolist() == [0, 1, 2, -1, 0, 0, 1, 2] and count.tolist() == [3, 1, 3] and nxt.tolist() == [1, 4, 11]
     assert cache.lens.tolist() == [3, 1, 3]
+
+
+@pytest.mark.parametrize("format", ["int8", "f32"])
+@pytest.mark.parametrize("told", [True, False])
+def test_a_cache_lasts_for_what_it_keeps(format, told):
+    """Trees of 20 nodes, 3 deep, of which 2 are kept, in 128 places: each step takes 2 of them where the host says what was
+    kept, else 3, until a tree has no room."""
+    from opworks_b200.tree import PagedCache, Rows
+
+    cache = PagedCache(1, 1, 128, 1, 64, format)
+    parents = [[-1] + [0] * 10 + [1 + i % 9 for i in range(9)]]
+    draft = torch.arange(20, device="cuda")
+    target = torch.full((20,), 77, device="cuda")
+    target[0] = 10  # node 10 has no children
+    k, v = torch.randn(2, 20, 64, device="cuda")
+    steps = 0
+    rows = Rows([20], parents)
+    while True:
+        try:
+            cache.write(0, k, v, rows)
+        except ValueError:
+            break
+        _, count, _ = cache.commit(draft, target, rows)
+        if told:
+            cache.kept(count.tolist())
+        steps += 1
+    assert cache.lens.tolist() == [2 * steps] and steps == (55 if told else 37)  # (128 - 20) // growth + 1
