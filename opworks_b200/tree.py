@@ -50,6 +50,19 @@ def deepest(parents):
     return max(depth, default=0)
 
 
+def to_device(device, *arrays):
+    """int32 arrays as tensors, in one copy that the host does not wait for (from pinned memory, which torch keeps until
+    the copy is done)."""
+    both = torch.from_numpy(np.concatenate([a.ravel() for a in arrays]))
+    if torch.device(device).type == "cuda":
+        both = both.pin_memory().to(device, non_blocking=True)
+    out, at = [], 0
+    for a in arrays:
+        out.append(both[at : at + a.size].view(a.shape))
+        at += a.size
+    return out
+
+
 class Rows:
     """The new tokens of a step: ``counts[b]`` rows of each sequence, one after another. With ``parents`` (a list per
     sequence) they are trees, else chains."""
@@ -57,16 +70,17 @@ class Rows:
     def __init__(self, counts, parents=None, device="cuda"):
         start = np.concatenate([[0], np.cumsum(counts)]).astype(np.int32)
         self.counts, self.total, self.most = list(counts), int(start[-1]), max(counts, default=0)
-        self.start = torch.from_numpy(start).to(device)
-        self.mask, self.words, self._parents = None, 0, None
         self.depths = list(counts)  # the most nodes on a path
-        if parents is not None:
-            if [len(p) for p in parents] != self.counts:
-                raise ValueError("parents: one list per sequence, as long as its rows")
-            self.words = max(1, -(-self.most // 32))
-            self.mask = torch.from_numpy(np.concatenate([tree_mask(p, self.words) for p in parents])).to(device)
-            self._parents = torch.from_numpy(np.concatenate(parents).astype(np.int32)).to(device)
-            self.depths = [deepest(p) for p in parents]
+        self.mask, self.words, self._parents = None, 0, None
+        if parents is None:
+            (self.start,) = to_device(device, start)
+            return
+        if [len(p) for p in parents] != self.counts:
+            raise ValueError("parents: one list per sequence, as long as its rows")
+        self.words = max(1, -(-self.most // 32))
+        mask = np.concatenate([tree_mask(p, self.words) for p in parents])
+        self.depths = [deepest(p) for p in parents]
+        self.start, self.mask, self._parents = to_device(device, start, mask, np.concatenate(parents).astype(np.int32))
 
     @property
     def parents(self):
@@ -74,7 +88,7 @@ class Rows:
         if self._parents is None:
             owner = np.repeat(np.arange(len(self.counts)), self.counts)
             node = np.arange(self.total) - np.concatenate([[0], np.cumsum(self.counts)])[owner]
-            self._parents = torch.from_numpy((node - 1).astype(np.int32)).to(self.start.device)
+            (self._parents,) = to_device(self.start.device, (node - 1).astype(np.int32))
         return self._parents
 
 

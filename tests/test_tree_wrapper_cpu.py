@@ -102,3 +102,17 @@ def test_the_host_knows_how_full_the_cache_is():
     cache._room(Rows([52, 0], device="cpu"))
     with pytest.raises(ValueError, match="room"):
         cache._room(Rows([1, 44], device="cpu"))
+
+
+def test_rows_on_the_device_are_what_they_were_on_the_host():
+    from opworks_b200.tree import Rows, tree_mask
+
+    trees = [[-1, 0, 0, 2] + [3] * 40, [], [-1]]
+    rows = Rows([len(t) for t in trees], trees, device="cpu")
+    assert rows.start.tolist() == [0, 44, 44, 45] and rows.words == 2 and rows.mask.shape == (45, 2)
+    assert np.array_equal(rows.mask.numpy(), np.concatenate([tree_mask(t, 2) for t in trees]))
+    assert rows.parents.tolist() == sum(trees, []) and rows.depths == [4, 0, 1]
+    with pytest.raises(ValueError, match="one list"):
+        Rows([1, 2], [[-1], [-1]], device="cpu")
+    with pytest.raises(ValueError, match="after its parent"):
+        Rows([2], [[-1, 1]], device="cpu")

@@ -102,3 +102,22 @@ def test_a_cache_lasts_for_what_it_keeps(format, told):
             cache.kept(count.tolist())
         steps += 1
     assert cache.lens.tolist() == [2 * steps] and steps == (55 if told else 37)  # (128 - 20) // growth + 1
+
+
+def test_making_rows_does_not_wait_for_the_device():
+    from opworks_b200.tree import Rows
+
+    trees = [[-1] + list(range(63))] * 32
+    Rows([64] * 32, trees)  # pinned memory is there from here on
+    big = torch.empty(1 << 28, device="cuda")
+    torch.cuda.synchronize()
+    done = torch.cuda.Event()
+    for _ in range(200):  # about 60 ms of stores
+        big.fill_(1.0)
+    done.record()
+    rows = Rows([64] * 32, trees)
+    first = rows.start
+    waited = done.query()
+    torch.cuda.synchronize()
+    assert not waited
+    assert first[-1].item() == 2048 and rows.parents[:64].tolist() == trees[0]
