@@ -415,3 +415,34 @@ def test_rows_at_the_ends_of_fp32(ops, fmt, kind, dim, ctx, n, kexp, vexp):
     q = queries(n, 8, dim, kind, 30) * 2.0**-kexp
     got = attend(ops, cache, q, [ctx], [n], None, 1 / math.sqrt(dim))
     check(got, *expected(cache, q, [ctx], [n], None, 1 / math.sqrt(dim)), ctx + n, kind)
+
+
+@pytest.mark.parametrize("fmt", [0, 1, 2])
+@pytest.mark.parametrize("kind", [0, 1])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("kvh,ctx,rows", [(1, [0], [2100]), (2, [1000, 0, 17], [700, 513, 1])])
+def test_prompts(ops, fmt, kind, dim, kvh, ctx, rows):
+    """Chains of hundreds and thousands of rows, on their own and after a context."""
+    cache = plain.Cache([c + n for c, n in zip(ctx, rows)], kvh, dim, fmt, 31)
+    q = queries(sum(rows), 2 * kvh, dim, kind, 32)
+    got = attend(ops, cache, q, ctx, rows, None, 1 / math.sqrt(dim))
+    check(got, *expected(cache, q, ctx, rows, None, 1 / math.sqrt(dim)), max(c + n for c, n in zip(ctx, rows)), kind)
+
+
+@pytest.mark.parametrize("fmt", [1, 2])
+@pytest.mark.parametrize("kind", [0, 1])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_codes_of_rows_that_are_not_finite_are_zero(ops, fmt, kind, dim):
+    x = queries(6, 1, dim, kind, 33).view(6, dim)
+    x[1, 3], x[2, dim - 1], x[4, 0] = math.inf, math.nan, -math.inf
+    cache = plain.Cache([6], 1, dim, fmt, 34)
+    pool, rows = dev(cache.pool), dev(x)
+    table, first, start = dev(cache.table), dev(np.zeros(1, np.int32)), dev(starts([6]))
+    ops.kv_quant_write(rows, rows, kind, dim, pool, fmt, table, cache.stride, first, start, 1, 6, 1, dim, 0)
+    codes_k, codes_v, scale_k, scale_v = plain.views(pool.cpu(), dim, fmt)
+    blk = int(cache.table[0, 0])
+    for codes, scales in ((codes_k, scale_k), (codes_v, scale_v)):
+        c, s = codes.view(torch.uint8)[blk, 0, :6], scales[blk, 0, :6]
+        for i in range(6):
+            bad = i in (1, 2, 4)
+            assert bool(torch.isnan(s[i])) == bad and bool(c[i].any()) == (not bad)
