@@ -52,21 +52,25 @@ template <typename T, int D, KvFormat kFmt>
 inline void tree_attention_launch(const T *q, T *out, const TreeArgs &a, cudaStream_t stream) {
     constexpr int kTile = TreeRowsGeo<T, D, kFmt, 1>::kRows;
     const int64_t rows = static_cast<int64_t>(a.t.max_rows) * (a.qh / a.kvh), tiles = (rows + kTile - 1) / kTile;
-    // The rows kernel's time grows with the rows, that of 128-row tiles does not:
-    // 8 sequences of 4096 tokens, 8 kv heads, us with rows / with tiles
-    //   fp32 rows, 8-bit, D 64    32 rows 44 / 51   64: 55 / 53   128: 90 / 58
-    //   fp32 rows, 8-bit, D 128   64 rows 82 / 98   128: 136 / 106 (e4m3 121 / 115)
-    //   fp32 rows, fp32, D 64     16 rows 39 / 69   32: 81 / 70   128: 197 / 76
-    //   bf16 rows, 8-bit, D 64    32 rows 22 / 37   64: 56 / 39   128: 67 / 45
-    //   bf16 rows, 8-bit, D 128   32 rows 53 / 45   64: 76 / 49   128: 117 / 57
-    // (ragged trees of up to 26 nodes x 4 heads, fp32, e4m3: 54 / 58). fp32 rows of
-    // 128 dims over 8-bit pools stay with rows: their operands as two terms each
-    // leave shared memory for one stage of tiles, and more rounding in the sums.
+    // The rows kernel's time grows with the rows, that of 128-row tiles does not. 8 (32)
+    // sequences of 4096 (2048) tokens with equal trees, 8 kv heads, us with rows / tiles:
+    //   fp32 rows, fp32, D 64     24 rows  52 / 77 (84 / 150)     32   85 / 77 (158 / 150)
+    //   fp32 rows, fp32, D 128    16 rows  97 / 127 (182 / 246)   24  169 / 128 (352 / 247)
+    //   bf16 rows, fp32, D 64     48 rows  55 / 70 (85 / 132)     64   87 / 72 (161 / 135)
+    //   bf16 rows, fp32, D 128    32 rows  94 / 130 (172 / 252)   48  155 / 132 (327 / 255)
+    //   fp32 rows, int8, D 64     48 rows  47 / 56 (74 / 108)     64   64 / 56 (109 / 109)
+    //   fp32 rows, e4m3, D 64     48 rows  45 / 57 (70 / 112)     64   61 / 58 (103 / 113)   80   61 / 59 (132 / 118)
+    //   bf16 rows, int8, D 64     48 rows  44 / 41 (49 / 76)      64   61 / 42 (94 / 77)
+    //   bf16 rows, int8, D 128    32 rows  54 / 52 (80 / 99)      48   75 / 54 (139 / 102)
+    // Where trees differ it is the mean that tells: one sequence of 128 rows among 32 of
+    // 2000 tokens and 4 rows, fp32 rows: fp32 134 / 138, int8 65 / 98; one of 2048 rows:
+    // 519 / 377, 347 / 313. (fp32 rows of 128 dims over 8-bit pools have no tiles.)
     constexpr bool kBf16 = std::is_same_v<T, __nv_bfloat16>, kWide = kFmt == KvFormat::kF32;
     constexpr bool kHasTiles = kBf16 || kWide || D == 64;
-    constexpr int kFrom = kBf16 ? 32 : kWide ? 24 : 104;
+    constexpr int kFrom = kBf16 ? (D == 64 ? 48 : 32) : kWide ? (D == 64 ? 24 : 16) : 60; // rows of a kv head
+    const bool many = static_cast<int64_t>(a.t.rows) * (a.qh / a.kvh) > static_cast<int64_t>(kFrom) * a.t.batch;
     if constexpr (kHasTiles) {
-        if (rows > kFrom) {
+        if (many) {
             // two row tiles to a CTA where shared memory holds both
             constexpr int kPair = D == 64 || (!kWide && kBf16) ? 2 : 1;
             if (rows <= 128 || kPair == 1)
