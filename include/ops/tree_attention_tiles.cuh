@@ -347,7 +347,7 @@ static __global__ void __launch_bounds__(kTileThreads, 1)
                     float least = low;
 #pragma unroll
                     for (int j = 0; j < G::kLoads; ++j)
-                        least = fminf(least, top(j));
+                        least = fminf(least, j * kRowsPerLoad + lrow < left ? top(j) : low);
                     if (__any_sync(kFullWarpMask, least < low)) // (four values of a row that are all small)
 #pragma unroll 1
                         for (int n = 0; n < G::kItemKeys; ++n) {
