@@ -116,8 +116,10 @@ class PagedCache:
     def max_len(self):
         return max(self.bounds, default=0)
 
-    @staticmethod
-    def _stream():
+    def _stream(self):
+        """torch's current stream, where it is one of this cache's device: an operator launches on the current device."""
+        if self.lens.device.type != "cuda" or self.lens.device.index != torch.cuda.current_device():
+            raise ValueError(f"the cache is on {self.lens.device}, which is not the current CUDA device")
         return torch.cuda.current_stream().cuda_stream
 
     def _belongs(self, rows):
@@ -158,6 +160,9 @@ class PagedCache:
         """The rows at positions lens + 0, 1, ... of an 8-bit cache, as [total, kv_heads, head_dim] K and V."""
         if not self.format:
             raise ValueError("read: of an 8-bit cache; the fp32 pools are plain tensors")
+        self._belongs(rows)
+        if dtype not in TYPES:
+            raise ValueError(f"read: as {' or '.join(str(d) for d in TYPES)}, not {dtype}")
         k = torch.empty(rows.total, self.kv_heads, self.head_dim, dtype=dtype, device=self.lens.device)
         v = torch.empty_like(k)
         self.ops.kv_quant_read(self.pool[layer], self.format, self.table, self.stride, self.lens, rows.start, self.batch,

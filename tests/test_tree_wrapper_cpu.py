@@ -116,3 +116,19 @@ def test_rows_on_the_device_are_what_they_were_on_the_host():
         Rows([1, 2], [[-1], [-1]], device="cpu")
     with pytest.raises(ValueError, match="after its parent"):
         Rows([2], [[-1, 1]], device="cpu")
+
+
+def test_a_cache_that_is_not_on_the_current_device_launches_nothing():
+    from opworks_b200.tree import Rows
+
+    cache, rows = cpu_cache(), Rows([3, 2], device="cpu")
+    k, q, tokens = torch.randn(5, 128), torch.randn(5, 8, 64), torch.zeros(5, dtype=torch.int32)
+    for call in (lambda: cache.write(0, k, k, rows), lambda: cache.read(0, rows), lambda: cache.attend(0, q, rows, q.clone(), 0.125),
+                 lambda: cache.commit(tokens, tokens, rows)):
+        with pytest.raises(ValueError, match="current CUDA device"):
+            call()
+    assert cache.bounds == [0, 0]
+    with pytest.raises(ValueError, match="float16"):
+        cache.read(0, rows, torch.float16)
+    with pytest.raises(ValueError, match="sequences"):
+        cache.read(0, Rows([1], device="cpu"))
