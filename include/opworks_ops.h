@@ -187,7 +187,8 @@ OPW_API int opw_kv_quant_read(const uint8_t *pool, int format, const int32_t *bl
  * max_rows: the most rows of one sequence (at most 32 * mask_words with a
  * mask); max_ctx: an upper bound of ctx_lens, which plans the launch only.
  * type: q and out fp32 (0) or bf16 (1); scores are scale * q . k; any number
- * of query heads per kv head; q_stride and out_stride in elements. */
+ * of query heads per kv head; q_stride and out_stride in elements. q, out and
+ * the pools are 16-byte aligned, and the row strides multiples of 16 bytes. */
 OPW_API int opw_tree_attention(const void *q, int type, int64_t q_stride, const float *kpool, const float *vpool,
                                const int32_t *block_table, int table_stride, const int32_t *ctx_lens,
                                const int32_t *row_start, const uint32_t *mask, int mask_words, int batch, int rows,
