@@ -28,9 +28,10 @@
 //
 // Precision as in the rows kernel: fp32 queries and weights are two fp16 terms
 // (a product each), bf16 rows one. The tensor cores cut an accumulator off at
-// every step, so the error of fp32 rows grows with the keys of a CTA: relative to
-// 64 bits 1.1e-6 over 2000 keys, 6.6e-6 over 7000 in one CTA (D = 128, fp32 pools;
-// fp32 sums in torch: 1.2e-6, 1.5e-6). K's 8-bit codes are one exact term, and the
+// every step, so fp32 rows are summed in periods (see kPeriod): relative to 64
+// bits 1.1e-6 over 7000 keys in one CTA, 1.4e-6 over 15,000 (D = 128, fp32 pools;
+// fp32 sums in torch: 1.5e-6, 2.2e-6; one accumulator all along: 6.5e-6, 1.4e-5).
+// K's 8-bit codes are one exact term, and the
 // softmax multiplies a score by its key's scale, four to a shared-memory broadcast
 // (353 us for the case above, 25 less with codes and scale rounded to one term, which
 // left weights of scores near -60 off by 1e-2 and more).
@@ -71,11 +72,15 @@ template <typename T, int D, KvFormat kFmt, int kM> struct TreeTilesGeo {
     static constexpr int kQBytes = kQT * kSlabs * kM * kSlab;
     static constexpr int kKBytes = kKT * kSlabs * kSlab, kVBytes = kVT * kSlabs * kSlab; // of a tile
     static constexpr int kStages = kVT == 2 && D == 128 ? 1 : 2;
-    // O's small products have an accumulator of their own: one is cut off at every
-    // step, to its size. At D = 128 tensor memory has room for that with one
-    // stream (widening is what takes the time there, so that little is lost).
-    static constexpr bool kSplitO = kQT == 2;
-    static constexpr int kStreams = kSplitO && D == 128 ? 1 : 2;
+    // An accumulator is cut off at every step, to its size. So for fp32 rows O is summed
+    // over a few tiles only and then added, rounded, to a sum of its own (kLong, in
+    // columns from O's); at D = 128, with one stream, tensor memory has room for another
+    // accumulator for its small products (widening is what takes the time there, so that
+    // little is lost).
+    static constexpr bool kSplitO = kQT == 2 && D == 128;
+    static constexpr int kPeriod = kQT == 1 ? 1 << 30 : kSplitO ? 4 : 2; // tiles
+    static constexpr int kLong = kSplitO ? -128 : 128;
+    static constexpr int kStreams = kSplitO ? 1 : 2;
     static constexpr int kKvBytes = kStages * (kKBytes + kVBytes);
     static constexpr int kRowBytes = D * (kWide ? 4 : 1);
     // an item: 4 KB of K or of V, but at most 32 keys: a tile has at least as many
@@ -566,7 +571,7 @@ static __global__ void __launch_bounds__(kTileThreads, 1)
                         break;
                     }
                     sm100::tc_fence_after();
-                    weigh(s, i, e > 0);
+                    weigh(s, i, e % G::kPeriod != 0);
                     if (kM == 1 || s == 1)
                         commit(&v_empty[i & 3]);
                     if (next < tiles && (kM == 2 && s == 1 ? true : k_ready(next))) {
@@ -702,6 +707,35 @@ static __global__ void __launch_bounds__(kTileThreads, 1)
                 }
                 return y;
             };
+            // a period's end: O to the long sum (this tile's S is there, so the products
+            // before it are done; the next ones start O anew)
+            if (G::kQT == 2 && e > 0 && e % G::kPeriod == 0) {
+#pragma unroll 1
+                for (int d = 0; d < D; d += 16) {
+                    uint32_t o[16], x[16];
+                    sm100::tmem_ld_32x16(ot + static_cast<uint32_t>(d), o);
+                    if (G::kSplitO)
+                        sm100::tmem_ld_32x16(ot + static_cast<uint32_t>(d + 128), x);
+                    sm100::tmem_wait_ld();
+                    sm100::tmem_reg_fence(o);
+                    if constexpr (G::kSplitO) {
+                        sm100::tmem_reg_fence(x);
+#pragma unroll
+                        for (int k = 0; k < 16; ++k)
+                            o[k] = __float_as_uint(__uint_as_float(o[k]) + __uint_as_float(x[k]));
+                    }
+                    if (e > G::kPeriod) {
+                        sm100::tmem_ld_32x16(ot + static_cast<uint32_t>(d + G::kLong), x);
+                        sm100::tmem_wait_ld();
+                        sm100::tmem_reg_fence(x);
+#pragma unroll
+                        for (int k = 0; k < 16; ++k)
+                            o[k] = __float_as_uint(__uint_as_float(o[k]) + __uint_as_float(x[k]));
+                    }
+                    tile_tmem_st16(ot + static_cast<uint32_t>(d + G::kLong), o);
+                }
+                tile_tmem_wait_st();
+            }
             uint32_t xa[2][16], xb[2][16];
             ask(0, xa);
             if (!sm100::mbar_wait_warp(&v_full[i & 3], phase_of(i))) {
@@ -714,8 +748,9 @@ static __global__ void __launch_bounds__(kTileThreads, 1)
                 if (e > 0) {
                     // (this tile's S is there, so the products before it are done)
 #pragma unroll 1
-                    for (int n = 0; n < (G::kSplitO ? 2 * D : D); n += 16) {
-                        const int d = n < D ? n : n - D + 128; // the small products' columns lie 128 on
+                    for (int n = 0; n < (G::kSplitO ? 2 * D : D) + (G::kQT == 2 && e >= G::kPeriod ? D : 0); n += 16) {
+                        // the small products' columns lie 128 on
+                        const int d = n < D ? n : G::kSplitO && n < 2 * D ? n - D + 128 : n % D + G::kLong;
                         uint32_t o[16];
                         sm100::tmem_ld_32x16(ot + static_cast<uint32_t>(d), o);
                         sm100::tmem_wait_ld();
@@ -884,15 +919,19 @@ static __global__ void __launch_bounds__(kTileThreads, 1)
                 sm100::tmem_ld_32x16(ot + static_cast<uint32_t>(c), o);
                 sm100::tmem_wait_ld();
                 sm100::tmem_reg_fence(o);
-                if constexpr (G::kSplitO) {
-                    uint32_t small[16];
-                    sm100::tmem_ld_32x16(ot + static_cast<uint32_t>(c + 128), small);
+                const auto plus = [&](int from) {
+                    uint32_t x[16];
+                    sm100::tmem_ld_32x16(ot + static_cast<uint32_t>(c + from), x);
                     sm100::tmem_wait_ld();
-                    sm100::tmem_reg_fence(small);
+                    sm100::tmem_reg_fence(x);
 #pragma unroll
                     for (int k = 0; k < 16; ++k)
-                        o[k] = __float_as_uint(__uint_as_float(o[k]) + __uint_as_float(small[k]));
-                }
+                        o[k] = __float_as_uint(__uint_as_float(o[k]) + __uint_as_float(x[k]));
+                };
+                if (G::kSplitO)
+                    plus(128);
+                if (G::kQT == 2 && e > G::kPeriod)
+                    plus(G::kLong);
             } else {
 #pragma unroll
                 for (int k = 0; k < 16; ++k)

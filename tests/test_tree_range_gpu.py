@@ -446,3 +446,31 @@ def test_codes_of_rows_that_are_not_finite_are_zero(ops, fmt, kind, dim):
         for i in range(6):
             bad = i in (1, 2, 4)
             assert bool(torch.isnan(s[i])) == bad and bool(c[i].any()) == (not bad)
+
+
+# ------------------------------------------------------------------ long sums
+
+
+@pytest.mark.parametrize("fmt,dim", [(0, 64), (0, 128), (1, 64), (2, 64)])
+def test_long_sums_keep_their_bits(ops, fmt, dim):
+    """9000 keys of one sign in one CTA (no splits: there are as many sequences as SMs), weights alike: an accumulator that
+    is cut off at each of its 560 steps ends up low by half of 560 2^-23. Here it is the same for all the steps: 2^-18, half
+    of 64 steps."""
+    n, ctx = 33, 9000
+    cache = plain.Cache([ctx + n], 1, dim, fmt, 41)
+    v = queries(ctx + n, 1, dim, 0, 42).abs().clamp(0.5, 2.0)
+    set_rows(cache, 0, np.arange(ctx + n), v=v)
+    q = queries(n, 4, dim, 0, 43) * 0.1
+    # many sequences with the same pages, so that each gets one CTA
+    copies = 150
+    many = type("Pages", (), {})()
+    many.fmt, many.kvh, many.stride, many.table = fmt, 1, cache.stride, np.repeat(cache.table, copies, 0)
+    for name in ("k", "v", "pool"):
+        if hasattr(cache, name):
+            setattr(many, name, getattr(cache, name))
+    got = attend(ops, many, q.repeat(copies, 1, 1), [ctx] * copies, [n] * copies, [np.eye(n, dtype=bool)] * copies, 1 / math.sqrt(dim))
+    want, mass, top = expected(cache, q, [ctx], [n], [np.eye(n, dtype=bool)], 1 / math.sqrt(dim))
+    got = got.view(copies, n, 4, dim)
+    assert (got == got[:1]).all()
+    err = ((got[0] - want).abs() / want).max()
+    assert err <= 2.0**-18, f"{err:.3g}"
