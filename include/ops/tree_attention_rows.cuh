@@ -43,12 +43,18 @@
 // and the reference of a query row counts those V rows only that it sees, so a
 // row that is masked takes no bits from the others, whatever its size.
 //
+// The tensor cores cut an accumulator off at every step, so the O of fp32 rows is
+// summed outside of them, a page's product at a time: two packed additions for
+// each, 3 to 4 % of a decode step's time (10 % at D = 128), and errors over 12,000
+// keys of 5e-7 to 8e-7 relative to 64 bits (fp32 sums in torch 7e-7 to 2e-6) where
+// they were 1.5e-6 to 5.8e-6.
+//
 // Measured (kernel time): a decode step of 32 sequences of 1090 to 2180 tokens, 32
-// query and 8 kv heads of 64, int8: 18.8 us, 3.1 TB/s; 4 chains of 5 rows over up
-// to 8192 tokens, fp32 pools: 48.6 us, 2.2 TB/s; one row over 511 tokens: 7.7 us.
-// What bounds it is instruction latency: 200 instructions per 8-bit page and tile
-// (880 per fp32 page and three tiles), 7 cycles each at the 16 (8) warps per SM
-// that registers leave room for.
+// query and 8 kv heads of 64, int8: 19.6 us, 3.0 TB/s; 4 chains of 5 rows over up
+// to 8192 tokens, fp32 pools: 49.2 us, 2.2 TB/s; one row over 511 tokens: 7.1 us.
+// What bounds it is instruction latency: over 200 instructions per 8-bit page and
+// tile (over 900 per fp32 page and three tiles), 7 cycles each at the 16 (8) warps
+// per SM that registers leave room for.
 
 #include "tree_attention_common.cuh"
 
@@ -82,6 +88,12 @@ __device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], u
                  "{%0, %1, %2, %3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// d += s, rounded: the tensor cores cut a sum off at every step, which over thousands
+// of keys would cost fp32 rows bits
+__device__ __forceinline__ void add4(float (&d)[4], const float (&s)[4]) {
+    const float2 a = __fadd2_rn(make_float2(d[0], d[1]), make_float2(s[0], s[1])), b = __fadd2_rn(make_float2(d[2], d[3]), make_float2(s[2], s[3]));
+    d[0] = a.x, d[1] = a.y, d[2] = b.x, d[3] = b.y;
 }
 // int8 codes as K operands: fp16 subnormals (c + 128) 2^-24, exact too. The
 // offset is taken off by the accumulators' start, -128 sum q: two instructions
@@ -658,9 +670,11 @@ static __global__ void __launch_bounds__(TreeRowsGeo<T, D, kFmt, kMT>::kThreads,
                 for (int e = 0; e < 4; ++e)
 #pragma unroll
                     for (int mt = 0; mt < kMT; ++mt) {
-                        mma_f16(o[mt][4 * c + e], pf[mt][0], hi[e][0], hi[e][1]);
+                        float sum[4] = {};
                         if constexpr (G::kTwo)
-                            mma_f16(o[mt][4 * c + e], pf[mt][0], lo[e][0], lo[e][1]);
+                            mma_f16(sum, pf[mt][0], lo[e][0], lo[e][1]);
+                        mma_f16(sum, pf[mt][0], hi[e][0], hi[e][1]);
+                        add4(o[mt][4 * c + e], sum);
                     }
             }
         } else {
@@ -694,7 +708,13 @@ static __global__ void __launch_bounds__(TreeRowsGeo<T, D, kFmt, kMT>::kThreads,
                     for (int e = 0; e < 4; ++e)
 #pragma unroll
                         for (int mt = 0; mt < kMT; ++mt)
-                            mma_f16(o[mt][4 * c + e], pf[mt][pg], b0[e], b1[e]);
+                            if constexpr (G::kTwo) {
+                                float sum[4] = {};
+                                mma_f16(sum, pf[mt][pg], b0[e], b1[e]);
+                                add4(o[mt][4 * c + e], sum);
+                            } else {
+                                mma_f16(o[mt][4 * c + e], pf[mt][pg], b0[e], b1[e]);
+                            }
                 }
             }
         }

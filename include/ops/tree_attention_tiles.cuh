@@ -5,9 +5,9 @@
 //
 // The floor is the tensor cores' time, nearly level with the exponential unit's.
 // What bounds it now is the chain of a tile: scores, softmax, weights, sum, each
-// waiting for the one before (6,450 cycles for 256 rows x 128 keys, of which the
+// waiting for the one before (6,400 cycles for 256 rows x 128 keys, of which the
 // products are 2,048). Measured: 32 sequences of 4096 to 8192 tokens with up to 64
-// nodes of 32 heads (8 kv heads, D = 128, int8, bf16 rows): 353 us, 0.49 PFLOP/s.
+// nodes of 32 heads (8 kv heads, D = 128, int8, bf16 rows): 348 us, 0.49 PFLOP/s.
 //
 // Two streams per CTA keep both busy: while the softmax of one stream's tile
 // runs, the products of the other's do. With more than 128 query rows (row =
@@ -31,10 +31,9 @@
 // every step, so fp32 rows are summed in periods (see kPeriod): relative to 64
 // bits 1.1e-6 over 7000 keys in one CTA, 1.4e-6 over 15,000 (D = 128, fp32 pools;
 // fp32 sums in torch: 1.5e-6, 2.2e-6; one accumulator all along: 6.5e-6, 1.4e-5).
-// K's 8-bit codes are one exact term, and the
-// softmax multiplies a score by its key's scale, four to a shared-memory broadcast
-// (353 us for the case above, 25 less with codes and scale rounded to one term, which
-// left weights of scores near -60 off by 1e-2 and more).
+// K's 8-bit codes are one exact term, and the softmax multiplies a score by its
+// key's scale, four to a shared-memory broadcast (20 us of the case above; codes and
+// scale rounded to one term left weights of scores near -60 off by 1e-2 and more).
 // V's codes are widened with their scale, and fp32 rows as they are (one term for
 // bf16 queries over 8-bit pools, 11 bits of V being more than the output has;
 // else two: hi hi + hi lo + lo hi), but for a power of two that the keys of an

@@ -474,3 +474,24 @@ def test_long_sums_keep_their_bits(ops, fmt, dim):
     assert (got == got[:1]).all()
     err = ((got[0] - want).abs() / want).max()
     assert err <= 2.0**-18, f"{err:.3g}"
+
+
+@pytest.mark.parametrize("fmt", [0, 1, 2])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("n", [1, 5])
+def test_long_sums_of_few_rows_keep_their_bits(ops, fmt, dim, n):
+    """24,000 keys of one sign in one CTA: 190 (8-bit) to 375 steps of a warp; the bound is that of 64 steps cut off."""
+    ctx, copies = 24000, 300
+    cache = plain.Cache([ctx + n], 1, dim, fmt, 44)
+    set_rows(cache, 0, np.arange(ctx + n), v=queries(ctx + n, 1, dim, 0, 45).abs().clamp(0.5, 2.0))
+    q = queries(n, 2, dim, 0, 46) * 0.1
+    many = type("Pages", (), {})()
+    many.fmt, many.kvh, many.stride, many.table = fmt, 1, cache.stride, np.repeat(cache.table, copies, 0)
+    for name in ("k", "v", "pool"):
+        if hasattr(cache, name):
+            setattr(many, name, getattr(cache, name))
+    got = attend(ops, many, q.repeat(copies, 1, 1), [ctx] * copies, [n] * copies, None, 1 / math.sqrt(dim)).view(copies, n, 2, dim)
+    want, _, _ = expected(cache, q, [ctx], [n], None, 1 / math.sqrt(dim))
+    assert (got == got[:1]).all()
+    err = ((got[0] - want).abs() / want).max()
+    assert err <= 2.0**-18, f"{err:.3g}"
