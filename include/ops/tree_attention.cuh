@@ -54,17 +54,17 @@ inline void tree_attention_launch(const T *q, T *out, const TreeArgs &a, cudaStr
     const int64_t rows = static_cast<int64_t>(a.t.max_rows) * (a.qh / a.kvh), tiles = (rows + kTile - 1) / kTile;
     // The rows kernel's time grows with the rows, that of 128-row tiles does not. 8 (32)
     // sequences of 4096 (2048) tokens with equal trees, 8 kv heads, us with rows / tiles:
-    //   fp32 rows, fp32, D 64     24 rows  52 / 77 (84 / 150)     32   85 / 77 (158 / 150)
-    //   fp32 rows, fp32, D 128    16 rows  97 / 127 (182 / 246)   24  169 / 128 (352 / 247)
-    //   bf16 rows, fp32, D 64     48 rows  55 / 70 (85 / 132)     64   87 / 72 (161 / 135)
-    //   bf16 rows, fp32, D 128    32 rows  94 / 130 (172 / 252)   48  155 / 132 (327 / 255)
-    //   fp32 rows, int8, D 64     48 rows  47 / 56 (74 / 108)     64   64 / 56 (109 / 109)
-    //   fp32 rows, e4m3, D 64     48 rows  45 / 57 (70 / 112)     64   61 / 58 (103 / 113)   80   61 / 59 (132 / 118)
+    //   fp32 rows, fp32, D 64     24 rows  54 / 79 (89 / 147)     32   88 / 80 (167 / 149)
+    //   fp32 rows, fp32, D 128    16 rows 102 / 127 (193 / 242)   24  180 / 126 (374 / 243)
+    //   bf16 rows, fp32, D 64     48 rows  56 / 67 (86 / 126)     64   88 / 68 (162 / 130)
+    //   bf16 rows, fp32, D 128    32 rows  97 / 127 (177 / 247)   48  159 / 129 (339 / 251)
+    //   fp32 rows, int8, D 64     48 rows  53 / 59 (82 / 112)     64   71 / 60 (120 / 113)
+    //   fp32 rows, e4m3, D 64     48 rows  49 / 60 (74 / 114)     64   62 / 61 (109 / 117)   80   62 / 62 (144 / 120)
     //   bf16 rows, int8, D 64     48 rows  44 / 41 (49 / 76)      64   61 / 42 (94 / 77)
-    //   bf16 rows, int8, D 128    32 rows  54 / 52 (80 / 99)      48   75 / 54 (139 / 102)
-    // Where trees differ it is the mean that tells: one sequence of 128 rows among 32 of
-    // 2000 tokens and 4 rows, fp32 rows: fp32 134 / 138, int8 65 / 98; one of 2048 rows:
-    // 519 / 377, 347 / 313. (fp32 rows of 128 dims over 8-bit pools have no tiles.)
+    //   bf16 rows, int8, D 128    32 rows  54 / 53 (80 / 102)     48   75 / 55 (140 / 105)
+    // Where trees differ it is the mean that tells: one sequence of 64 rows among 32 of
+    // 2000 tokens and 4 rows, fp32 rows: fp32 92 / 138, int8 51 / 100; one of 2048 rows:
+    // 545 / 404, 373 / 323. (fp32 rows of 128 dims over 8-bit pools have no tiles.)
     constexpr bool kBf16 = std::is_same_v<T, __nv_bfloat16>, kWide = kFmt == KvFormat::kF32;
     constexpr bool kHasTiles = kBf16 || kWide || D == 64;
     constexpr int kFrom = kBf16 ? (D == 64 ? 48 : 32) : kWide ? (D == 64 ? 24 : 16) : 60; // rows of a kv head
