@@ -29,8 +29,9 @@
 // Precision as in the rows kernel: fp32 queries and weights are two fp16 terms
 // (a product each), bf16 rows one. The tensor cores cut an accumulator off at
 // every step, so fp32 rows are summed in periods (see kPeriod): relative to 64
-// bits 1.1e-6 over 7000 keys in one CTA, 1.4e-6 over 15,000 (D = 128, fp32 pools;
-// fp32 sums in torch: 1.5e-6, 2.2e-6; one accumulator all along: 6.5e-6, 1.4e-5).
+// bits 5.6e-7 (D = 64) and 7.4e-7 (D = 128) over 600 to 4000 keys, fp32 pools, where
+// fp32 sums in torch are 7.6e-7 to 1.5e-6 off; with one accumulator all along 1.5e-6
+// over 1300 keys and 1.4e-5 over 15,000 in one CTA.
 // K's 8-bit codes are one exact term, and the softmax multiplies a score by its
 // key's scale, four to a shared-memory broadcast (20 us of the case above; codes and
 // scale rounded to one term left weights of scores near -60 off by 1e-2 and more).
@@ -72,12 +73,12 @@ template <typename T, int D, KvFormat kFmt, int kM> struct TreeTilesGeo {
     static constexpr int kKBytes = kKT * kSlabs * kSlab, kVBytes = kVT * kSlabs * kSlab; // of a tile
     static constexpr int kStages = kVT == 2 && D == 128 ? 1 : 2;
     // An accumulator is cut off at every step, to its size. So for fp32 rows O is summed
-    // over a few tiles only and then added, rounded, to a sum of its own (kLong, in
+    // over one or two tiles only and then added, rounded, to a sum of its own (kLong, in
     // columns from O's); at D = 128, with one stream, tensor memory has room for another
     // accumulator for its small products (widening is what takes the time there, so that
     // little is lost).
     static constexpr bool kSplitO = kQT == 2 && D == 128;
-    static constexpr int kPeriod = kQT == 1 ? 1 << 30 : kSplitO ? 4 : 2; // tiles
+    static constexpr int kPeriod = kQT == 1 ? 1 << 30 : kSplitO ? 2 : 1; // tiles
     static constexpr int kLong = kSplitO ? -128 : 128;
     static constexpr int kStreams = kSplitO ? 1 : 2;
     static constexpr int kKvBytes = kStages * (kKBytes + kVBytes);
@@ -526,12 +527,13 @@ static __global__ void __launch_bounds__(kTileThreads, 1)
                                    idesc_o, st > 0 ? 1u : first);
                 };
                 if (leader) {
-                    product(Zero{}, Zero{}, d, acc);
+                    // small products first, where they begin a sum
                     if constexpr (G::kQT == 2) {
                         const uint32_t small = G::kSplitO ? tm + 384u + static_cast<uint32_t>(stream * D) : d;
-                        product(Zero{}, One{}, small, G::kSplitO ? acc : 1u);
+                        product(Zero{}, One{}, small, acc);
                         product(One{}, Zero{}, small, 1);
                     }
+                    product(Zero{}, Zero{}, d, G::kQT == 2 && !G::kSplitO ? 1u : acc);
                 }
                 __syncwarp();
             };

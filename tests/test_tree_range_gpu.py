@@ -495,3 +495,17 @@ def test_long_sums_of_few_rows_keep_their_bits(ops, fmt, dim, n):
     assert (got == got[:1]).all()
     err = ((got[0] - want).abs() / want).max()
     assert err <= 2.0**-18, f"{err:.3g}"
+
+
+@pytest.mark.parametrize("fmt", [0, 1, 2])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("ctx,n", [(600, 1), (600, 12), (50, 60), (600, 30), (1300, 40)])
+def test_fp32_rows_are_off_by_a_millionth_at_most(ops, fmt, dim, ctx, n):
+    """Relative 2-norm of the error over all rows: operands and weights to 2^-22, rounded sums: 2^-20 together."""
+    cache = plain.Cache([ctx + n], 2, dim, fmt, 51)
+    q = queries(n, 8, dim, 0, 52)
+    sees = [plain.tree(np.random.default_rng(5), n)[1]]
+    got = attend(ops, cache, q, [ctx], [n], sees, 1 / math.sqrt(dim))
+    want, _, _ = expected(cache, q, [ctx], [n], sees, 1 / math.sqrt(dim))
+    err = (got - want).norm() / want.norm()
+    assert err <= 2.0**-20, f"{err:.3g}"
