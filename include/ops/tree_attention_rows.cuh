@@ -50,8 +50,8 @@
 // they were 1.5e-6 to 5.8e-6.
 //
 // Measured (kernel time): a decode step of 32 sequences of 1090 to 2180 tokens, 32
-// query and 8 kv heads of 64, int8: 19.6 us, 3.0 TB/s; 4 chains of 5 rows over up
-// to 8192 tokens, fp32 pools: 49.2 us, 2.2 TB/s; one row over 511 tokens: 7.1 us.
+// query and 8 kv heads of 64, int8: 19.7 us, 2.9 TB/s; 4 chains of 5 rows over up
+// to 8192 tokens, fp32 pools: 48.5 us, 2.2 TB/s; one row over 511 tokens: 7.0 us.
 // What bounds it is instruction latency: over 200 instructions per 8-bit page and
 // tile (over 900 per fp32 page and three tiles), 7 cycles each at the 16 (8) warps
 // per SM that registers leave room for.
