@@ -645,8 +645,19 @@ static __global__ void __launch_bounds__(TreeRowsGeo<T, D, kFmt, kMT>::kThreads,
                             break;
                         // to 2^7 .. 2^8; what is summed already must not leave fp32's range
                         float next = pow2_field(254u - max(exponent_above(top, 254u), static_cast<uint32_t>(127 + kMinVKey)) + 8u);
-                        if (vmul[c] != 0.f)
-                            next = fminf(next, vmul[c] * 0x1p60f);
+                        if (next > vmul[c] && vmul[c] != 0.f) {
+                            uint32_t most = 0;
+#pragma unroll
+                            for (int mt = 0; mt < kMT; ++mt)
+#pragma unroll
+                                for (int n = 4 * c; n < 4 * c + 4; ++n)
+#pragma unroll
+                                    for (int i = 0; i < 4; ++i)
+                                        most = max(most, __float_as_uint(o[mt][n][i]) & 0x7fffffffu);
+                            most = __reduce_max_sync(kFullWarpMask, most) >> 23;
+                            const uint32_t room = most < 227u ? min(227u - most, 100u) : 0u; // to 2^100
+                            next = fminf(next, vmul[c] * pow2_field(127u + room));
+                        }
                         resize(c, next);
                     }
                     const float vmul_here = kEdge ? 1.f : vmul[c];

@@ -509,3 +509,18 @@ def test_fp32_rows_are_off_by_a_millionth_at_most(ops, fmt, dim, ctx, n):
     want, _, _ = expected(cache, q, [ctx], [n], sees, 1 / math.sqrt(dim))
     err = (got - want).norm() / want.norm()
     assert err <= 2.0**-20, f"{err:.3g}"
+
+
+@pytest.mark.parametrize("kind", [0, 1])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("n", [1, 3, 50])
+@pytest.mark.parametrize("bits", [60, 90, 110, 125])
+@pytest.mark.parametrize("fmt", [0, 1])
+def test_v_rows_that_differ_by_powers_of_two(ops, fmt, kind, dim, n, bits):
+    """Pages of V of 2^bits, then of 1, all weighing alike: the sum stays in fp32's range."""
+    ctx, large = 2200, 1024
+    cache = plain.Cache([ctx + n], 2, dim, fmt, 61)
+    set_rows(cache, 0, np.arange(large), v=queries(large, 2, dim, 0, 62).clamp(-2, 2) * 2.0**bits)
+    q = queries(n, 4, dim, kind, 63) * 0.25
+    got = attend(ops, cache, q, [ctx], [n], None, 1 / math.sqrt(dim))
+    check(got, *expected(cache, q, [ctx], [n], None, 1 / math.sqrt(dim)), ctx + n, kind)
