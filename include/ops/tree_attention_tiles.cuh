@@ -783,8 +783,9 @@ static __global__ void __launch_bounds__(kTileThreads, 1)
                 constexpr bool kEdge = decltype(edge_tag)::value, kEach = decltype(each_tag)::value;
                 // The first reference: the largest score of the first tile of which the row sees
                 // anything. It has to come from the scores: against m's first value every
-                // score is the same number.
-                if (__any_sync(kFullWarpMask, live && m == kNone)) {
+                // score is the same number. (Rows past the last one have scores of the context
+                // too, zeros, and would raise theirs many times over.)
+                if (__any_sync(kFullWarpMask, m == kNone && (live || !kEdge))) {
                     float top = kNegInf;
 #pragma unroll 1
                     for (int c = 0; c < 4; ++c) {
