@@ -7,7 +7,7 @@
 // What bounds it now is the chain of a tile: scores, softmax, weights, sum, each
 // waiting for the one before (6,400 cycles for 256 rows x 128 keys, of which the
 // products are 2,048). Measured: 32 sequences of 4096 to 8192 tokens with up to 64
-// nodes of 32 heads (8 kv heads, D = 128, int8, bf16 rows): 346 us, 0.50 PFLOP/s.
+// nodes of 32 heads (8 kv heads, D = 128, int8, bf16 rows): 344 us, 0.50 PFLOP/s.
 //
 // Two streams per CTA keep both busy: while the softmax of one stream's tile
 // runs, the products of the other's do. With more than 128 query rows (row =
