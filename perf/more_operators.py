@@ -10,9 +10,9 @@ Four operators, in the order in which a step of a serving program calls them:
   other over the 4-bit cache.
 
 Pages hold 16 tokens, a slot is 16 * block + place in the page. The 4-bit pool has one record of 576 G bytes per block
-and kv head, G = D / 32 groups of 32 dims: K codes [G][16 tokens][16 bytes], V codes the same, K scales bf16 [G][16], V
-scales bf16 [G][16]. Byte i of a group's 16 holds dims 2 i (low half) and 2 i + 1. A value is (code - 8) * scale, the
-scale max|x| / 7 of the group rounded to 5 significant bits, so that every value is a bf16 number.
+and kv head, G = D / 32 groups of 32 dims: K codes [G][16 tokens][16 bytes], V codes the same, K scales fp16 [G][16], V
+scales fp16 [G][16]. Byte i of a group's 16 holds dims 2 i (low half) and 2 i + 1. A value is (code - 8) * scale, the
+scale max|x| / 7 of the group rounded to an fp16 number of 5 significant bits, so that every value is an fp16 number too.
 
 ``run`` computes the plain form with elementary torch operations, or calls the framework where ``own`` is true.
 """
@@ -146,16 +146,17 @@ def _quantise(x):
     top = g.abs().amax(-1) * torch.tensor(1.0 / 7.0, dtype=torch.float32, device=x.device)
     bits = top.view(torch.int32)
     scale = ((bits + 0x3FFFF + ((bits >> 19) & 1)) & ~0x7FFFF).view(torch.float32)
+    scale = torch.where(top < 2.0**-20, (top * 2.0**24).round() * 2.0**-24, scale)  # fp16 has no finer step
     y = torch.where(scale[..., None] > 0, g / scale[..., None], torch.zeros_like(g))
     return (y.round().clamp_(-7, 7) + 8).to(torch.int32).flatten(-2), scale
 
 
 def _views(pool, dim):
-    """K codes, V codes [..., G, 16, 16 bytes] and K, V scales bf16 [..., G, 16] of a pool [..., record]."""
+    """K codes, V codes [..., G, 16, 16 bytes] and K, V scales fp16 [..., G, 16] of a pool [..., record]."""
     g = dim // GROUP
     n = g * PAGE * 16
     k, v = (pool[..., i * n : (i + 1) * n].unflatten(-1, (g, PAGE, 16)) for i in (0, 1))
-    s = pool[..., 2 * n :].view(torch.bfloat16)
+    s = pool[..., 2 * n :].view(torch.float16)
     return k, v, s[..., : g * PAGE].unflatten(-1, (g, PAGE)), s[..., g * PAGE :].unflatten(-1, (g, PAGE))
 
 
@@ -166,7 +167,7 @@ def _store(codes, scales, where, x):
     packed = (c[..., 0] | (c[..., 1] << 4)).to(torch.uint8)  # [n, kvh, G, 16]
     block, slot = where
     codes[block, :, :, slot] = packed
-    scales[block, :, :, slot] = s.to(torch.bfloat16)
+    scales[block, :, :, slot] = s.to(torch.float16)
 
 
 def _fetch(codes, scales, where):
@@ -499,7 +500,7 @@ def _exact_rows(s):
     for name in ("k", "v"):
         x = s[name].double().view(s["total"], -1, GROUP) if s[name].is_contiguous() else s[name].double().reshape(s["total"], -1, GROUP)
         want = torch.linalg.vector_norm(x, ord=math.inf, dim=-1) / 7.0
-        unit = torch.exp2(torch.floor(torch.log2(want.clamp_min(2.0**-100))) - 4)  # of a scale's fifth bit
+        unit = torch.exp2((torch.floor(torch.log2(want.clamp_min(2.0**-100))) - 4).clamp_min(-24))  # of a scale's last bit
         scale = (torch.round(want / unit) * unit)[..., None]
         out[name] = (torch.round(x / scale.clamp_min(2.0**-200)).clamp(-7, 7) * scale).view(s["total"], s["width"])
     return out
@@ -517,8 +518,8 @@ def _exact_tokens(s, which, slots):
     at = 2 * g * 256 + which * g * 32 + torch.arange(g, device="cuda")[None, :] * 32 + place[:, None] * 2
     lo, hi = (rec.gather(2, (at + i)[:, None, :].expand(-1, rec.shape[1], -1)) for i in (0, 1))
     bits = lo + 256 * hi
-    exponent, fraction = (bits >> 7) & 255, (bits & 127).double()
-    scale = torch.where(exponent == 0, fraction * 2.0**-133, (128.0 + fraction) * torch.exp2((exponent - 134).double()))
+    exponent, fraction = (bits >> 10) & 31, (bits & 1023).double()
+    scale = torch.where(exponent == 0, fraction * 2.0**-24, (1024.0 + fraction) * torch.exp2((exponent - 25).double()))
     return c * scale.repeat_interleave(GROUP, 2)
 
 
