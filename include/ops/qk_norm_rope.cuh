@@ -1,0 +1,192 @@
+#pragma once
+
+// ops::qk_norm_rope — queries and keys of a step: the root-mean-square norm of
+// each head, and the rotation by the row's position, in one pass. The reference
+// has a row norm (include/ops/rms_norm.cuh) and a rotation of rows at positions
+// one after another (include/ops/rope.cuh), and no norm of heads.
+//
+// For head x of D values, weight w (none: the head is not normalised), position p:
+//   y_i = x_i / sqrt(mean(x^2) + eps) * w_i
+//   pairs (i, i + rot / 2) of the first rot values: a cos - b sin, b cos + a sin
+//   with the angle p * inv_freq[i]
+// and the values from rot on as they are. Norms, angles and rotation are fp32 with
+// one rounding to the output's type at the end; the angle is reduced to an eighth
+// of a turn in 64 bits, so that far positions keep their bits (fp32 products of
+// position 100,000 are off by 0.004 rad).
+//
+// The kernel is bound by HBM: each value is read and written once, 16 bytes a
+// lane, a head on D / 32 (fp32) or D / 16 (bf16) lanes. A lane has the same pairs
+// in every head, so cos and sin of the row are computed once by the block and stay
+// in registers.
+
+#include <algorithm>
+#include <cstdint>
+#include <cuda_bf16.h>
+
+#include "../core/cuda_utils.cuh"
+#include "kv_quant.cuh"
+
+namespace opworks {
+
+// Queries and keys of `rows` rows: head h of row r at r * stride + h * head_dim.
+// The outputs may be the inputs (same strides); else nothing overlaps.
+template <typename T> struct QkNormRope {
+    const T *q;
+    int64_t q_stride;
+    const T *k;
+    int64_t k_stride;
+    const float *q_weight, *k_weight; // [head_dim], null: no norm
+    float eps;
+    const int *positions;  // [rows]
+    const float *inv_freq; // [rot_dim / 2]
+    int rot_dim;
+    int rows, q_heads, kv_heads, head_dim;
+    T *q_out;
+    int64_t q_out_stride;
+    T *k_out;
+    int64_t k_out_stride;
+};
+
+namespace detail {
+
+constexpr int kNormRopeMaxWarps = 12, kNormRopeMaxDim = 256;
+
+// cos and sin of position * frequency.
+__device__ __forceinline__ void turn(int position, float frequency, float &c, float &s) {
+    constexpr double kTurns = 0.15915494309189533577; // 1 / (2 pi)
+    const double turns = static_cast<double>(position) * static_cast<double>(frequency) * kTurns;
+    const double eighths = rint(turns * 4.0);
+    float sn, cs;
+    sincospif(static_cast<float>((turns - eighths * 0.25) * 2.0), &sn, &cs);
+    const int quarter = static_cast<int>(static_cast<long long>(eighths) & 3);
+    s = quarter == 0 ? sn : quarter == 1 ? cs : quarter == 2 ? -sn : -cs;
+    c = quarter == 0 ? cs : quarter == 1 ? -sn : quarter == 2 ? -cs : sn;
+}
+
+template <typename T, int D>
+static __global__ void __launch_bounds__(32 * kNormRopeMaxWarps) qk_norm_rope_kernel(QkNormRope<T> a) {
+    using V = KvVec<T>;
+    constexpr int kN = V::kN, kLanes = D / (2 * kN), kPer = 32 / kLanes; // heads of a warp at a time
+    __shared__ float table[2][kNormRopeMaxDim / 2];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, warps = blockDim.x >> 5;
+    const int half = a.rot_dim / 2, j = lane % kLanes;
+    // the lane's two vectors of a head: a pair of rotated ones, or two of the rest
+    const bool turned = j * kN < half;
+    const int at0 = turned ? j * kN : a.rot_dim + (j - half / kN) * 2 * kN;
+    const int at1 = turned ? half + j * kN : at0 + kN;
+    const int heads = a.q_heads + a.kv_heads;
+    pdl_trigger();
+    pdl_wait();
+    for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+        const int head0 = warp * kPer + lane / kLanes;
+        const auto source = [&](int h) { return h < a.q_heads ? a.q + row * a.q_stride + h * D : a.k + row * a.k_stride + (h - a.q_heads) * D; };
+        uint4 r0{}, r1{};
+        if (head0 < heads) {
+            const T *src = source(head0);
+            r0 = *reinterpret_cast<const uint4 *>(src + at0), r1 = *reinterpret_cast<const uint4 *>(src + at1);
+        }
+        if (half > 0) {
+            const int position = a.positions[row];
+            __syncthreads(); // the row before has read the table
+            for (int i = tid; i < half; i += blockDim.x)
+                turn(position, a.inv_freq[i], table[0][i], table[1][i]);
+            __syncthreads();
+        }
+        float c[kN], s[kN];
+#pragma unroll
+        for (int i = 0; i < kN; ++i) {
+            c[i] = turned ? table[0][at0 + i] : 1.f;
+            s[i] = turned ? table[1][at0 + i] : 0.f;
+        }
+        const float *have = nullptr; // the weights that the lane holds its part of
+        float w0[kN], w1[kN];
+        for (int h = head0; h - lane / kLanes < heads; h += warps * kPer) { // whole warps
+            float x[kN], y[kN];
+            V::unpack(r0, x), V::unpack(r1, y);
+            const int next = h + warps * kPer;
+            if (next < heads) {
+                const T *src = source(next);
+                r0 = *reinterpret_cast<const uint4 *>(src + at0), r1 = *reinterpret_cast<const uint4 *>(src + at1);
+            }
+            float sum = 0.f;
+#pragma unroll
+            for (int i = 0; i < kN; ++i)
+                sum += x[i] * x[i] + y[i] * y[i];
+#pragma unroll
+            for (int off = 1; off < kLanes; off <<= 1)
+                sum += __shfl_xor_sync(kFullWarpMask, sum, off);
+            const float *w = h < a.q_heads ? a.q_weight : a.k_weight;
+            if (h >= heads)
+                continue;
+            if (w != nullptr) {
+                if (w != have) { // at the first head, and where the queries end
+                    have = w;
+#pragma unroll
+                    for (int i = 0; i < kN; ++i)
+                        w0[i] = __ldg(w + at0 + i), w1[i] = __ldg(w + at1 + i);
+                }
+                const float inv = rsqrtf(sum / D + a.eps);
+#pragma unroll
+                for (int i = 0; i < kN; ++i) {
+                    x[i] = x[i] * inv * w0[i];
+                    y[i] = y[i] * inv * w1[i];
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < kN; ++i) {
+                const float u = x[i], v = y[i];
+                x[i] = turned ? u * c[i] - v * s[i] : u;
+                y[i] = turned ? v * c[i] + u * s[i] : v;
+            }
+            T *dst = h < a.q_heads ? a.q_out + row * a.q_out_stride + h * D : a.k_out + row * a.k_out_stride + (h - a.q_heads) * D;
+            *reinterpret_cast<uint4 *>(dst + at0) = V::pack(x);
+            *reinterpret_cast<uint4 *>(dst + at1) = V::pack(y);
+        }
+    }
+}
+
+template <typename T, int D> inline void qk_norm_rope_launch(const QkNormRope<T> &a, cudaStream_t stream) {
+    constexpr int kPer = 32 / (D / (2 * KvVec<T>::kN));
+    // as many warps as share the heads out evenly, in as few rounds as 12 warps allow
+    const int pieces = (a.q_heads + a.kv_heads + kPer - 1) / kPer;
+    const int rounds = (pieces + kNormRopeMaxWarps - 1) / kNormRopeMaxWarps;
+    const int warps = (pieces + rounds - 1) / rounds;
+    launch_ex(qk_norm_rope_kernel<T, D>, dim3(static_cast<unsigned>(a.rows)), dim3(static_cast<unsigned>(32 * warps)), 0, stream, a);
+}
+
+} // namespace detail
+
+namespace ops {
+
+template <typename T> inline void qk_norm_rope(const QkNormRope<T> &a, cudaStream_t stream = nullptr) {
+    const int D = a.head_dim;
+    detail::require(a.rows >= 0, "qk_norm_rope: rows must be nonnegative");
+    detail::require(a.q_heads >= 0 && a.kv_heads >= 0 && a.q_heads <= 65535 && a.kv_heads <= 65535,
+                    "qk_norm_rope: 0 to 65535 heads of each kind");
+    detail::require(D == 32 || D == 64 || D == 128 || D == 256, "qk_norm_rope: head_dim must be 32, 64, 128 or 256");
+    detail::require(a.rot_dim >= 0 && a.rot_dim <= D && a.rot_dim % 16 == 0,
+                    "qk_norm_rope: rot_dim must be a multiple of 16 up to head_dim");
+    detail::require((a.q_weight == nullptr && a.k_weight == nullptr) || a.eps > 0.f, "qk_norm_rope: eps must be positive");
+    if (a.rows == 0 || a.q_heads + a.kv_heads == 0)
+        return;
+    detail::require(a.rot_dim == 0 || (a.positions && a.inv_freq), "qk_norm_rope: null pointer");
+    constexpr int64_t kElem = sizeof(T);
+    const auto check = [&](const void *p, int64_t stride, int heads) {
+        if (heads == 0)
+            return;
+        detail::require(p != nullptr, "qk_norm_rope: null pointer");
+        detail::require(stride >= static_cast<int64_t>(heads) * D, "qk_norm_rope: rows overlap (stride below heads * head_dim)");
+        detail::require(detail::aligned16(p) && stride * kElem % 16 == 0, "qk_norm_rope: rows must be 16-byte aligned");
+    };
+    check(a.q, a.q_stride, a.q_heads), check(a.q_out, a.q_out_stride, a.q_heads);
+    check(a.k, a.k_stride, a.kv_heads), check(a.k_out, a.k_out_stride, a.kv_heads);
+    switch (D) {
+    case 32: detail::qk_norm_rope_launch<T, 32>(a, stream); break;
+    case 64: detail::qk_norm_rope_launch<T, 64>(a, stream); break;
+    case 128: detail::qk_norm_rope_launch<T, 128>(a, stream); break;
+    default: detail::qk_norm_rope_launch<T, 256>(a, stream); break;
+    }
+}
+
+} // namespace ops
+} // namespace opworks

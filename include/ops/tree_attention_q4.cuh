@@ -1,0 +1,35 @@
+#pragma once
+
+// ops::tree_attention_q4 — attention of several new tokens per sequence
+// (ops/tree_attention.cuh has the definition of the operator: rows, contexts,
+// masks, and what a masked key may hold) over the 4-bit pool of ops/kv4.cuh. No
+// reference counterpart.
+//
+// What is held there is an fp16 number, so K and V enter the tensor cores' fp16
+// products exactly, with no units and no factors behind them: scores are q . k as
+// they are, weights times V too. A query row is scaled by a power of two, to a
+// largest magnitude of 2^14 to 2^15, and is one fp16 term where it comes in bf16
+// (exact down to 2^-29 of the largest), two where it comes in fp32 (22 bits).
+
+#include "tree_attention.cuh"
+#include "kv4.cuh"
+#include "tree_attention_q4_rows.cuh"
+
+namespace opworks {
+namespace ops {
+
+// Over the 4-bit pool [blocks][kv_heads][record] of ops/kv4.cuh. q row r, head h at
+// r * q_stride + h * head_dim; T fp32 or bf16; out in the same form and type.
+template <typename T>
+inline void tree_attention_q4(const T *q, int64_t q_stride, const uint8_t *pool, const TreeBatch &t, int q_heads, int kv_heads,
+                              int head_dim, float scale, T *out, int64_t out_stride, cudaStream_t stream = nullptr) {
+    using namespace detail;
+    validate_tree(t, q, out, q_stride, out_stride, sizeof(T), q_heads, kv_heads, head_dim, pool, pool);
+    if (t.batch == 0 || t.max_rows == 0)
+        return;
+    const TreeArgs a{t, pool, nullptr, q_heads, kv_heads, scale * kLog2e, q_stride, out_stride};
+    head_dim == 64 ? q4_rows_call<T, 64>(q, out, a, stream) : q4_rows_call<T, 128>(q, out, a, stream);
+}
+
+} // namespace ops
+} // namespace opworks

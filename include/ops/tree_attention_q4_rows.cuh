@@ -1,0 +1,488 @@
+#pragma once
+
+// Attention over the 4-bit cache, kernel for few query rows per KV head
+// (ops/tree_attention_q4.cuh has the definition): mma.sync, K and V widened in
+// registers.
+//
+// The rows of a KV head (row = node * rep + head in group) are the M side of the
+// products, the keys of a step (32: two pages) the N side of the scores, the dims
+// that of the output. Every warp of the CTA has the same rows and takes every
+// n-th step; the steps of a sequence go round the warps of a cluster, and what
+// they have is joined at the end through shared memory, in rank order.
+//
+// A page record comes with 16-byte asynchronous copies into a ring that only this
+// warp uses, so nothing in the loop waits for another warp. ldmatrix hands out its
+// codes as fragments, four codes to a 16-bit element: of K eight dims of a key (the
+// four k slots of two products, in an order that Q follows), of V, transposed, four
+// dims of two keys each.
+//
+// fp32 rows are two fp16 terms, and so are their weights. With up to 8 rows both
+// terms share a tile (rows g and g + 8 of the fragments), so one product does both;
+// above that a tile has 16 rows and a product for each term, in one accumulator.
+// The tensor cores cut an accumulator off at every step, so fp32 rows add up O
+// outside of them, rounded, once a step.
+
+#include <type_traits>
+
+#include "tree_attention_common.cuh"
+#include "tree_attention_rows.cuh"
+#include "kv4.cuh"
+
+namespace opworks::detail {
+
+template <typename T, int D, bool kSplit> struct Q4RowsGeo {
+    static constexpr bool kWide = std::is_same_v<T, float>;
+    static_assert(kWide || !kSplit, "bf16 rows are one term");
+    static constexpr int kGroups = D / kKv4Group;
+    static constexpr int kRows = kSplit ? 8 : 16;              // of a tile
+    static constexpr int kRPL = kSplit ? 1 : 2;                // rows that a lane has scores of
+    static constexpr int kSets = kWide && !kSplit ? 2 : 1;     // products of a k step
+    static constexpr int kWarps = 4, kThreads = 32 * kWarps;
+    static constexpr int kStepPages = 2, kStepKeys = kStepPages * kKvPage;
+    static constexpr int kStages = 3;
+    static constexpr int kPageBytes = Kv4Record<D>::kBytes, kStage = kStepPages * kPageBytes;
+    static constexpr int kRing = kWarps * kStages * kStage;
+    static constexpr int kPitch = D + 4; // floats of a row of partial sums
+    // O of the warps, then of the CTA; m and l of the warps, then of the CTA
+    static constexpr int kJoin = 4 * ((kWarps + 1) * kRows * kPitch + 2 * (kWarps + 1) * kRows);
+    static constexpr int kBytes = kRing > kJoin ? kRing : kJoin;
+};
+
+// Scores may pass a row's reference by this many log2 units before it is raised:
+// weights are 2^(x - reference), 2^10 for the largest score when it is set.
+constexpr float kQ4Top = 14.f, kQ4Lift = 10.f;
+constexpr float kQ4None = -3.4028235e38f; // reference of a row that has seen nothing yet
+constexpr uint32_t kQ4BadScale = 0x7000u; // fp16 8,192: above every scale that is written; junk, infinity, NaN
+
+__device__ __forceinline__ void q4_copy16(uint32_t dst, const void *src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void q4_copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int kLeft> __device__ __forceinline__ void q4_copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(kLeft) : "memory"); }
+
+template <bool kTrans> __device__ __forceinline__ void q4_ldmatrix(uint32_t at, uint32_t (&r)[4]) {
+    if constexpr (kTrans)
+        asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+                     : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                     : "r"(at)
+                     : "memory");
+    else
+        asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+                     : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                     : "r"(at)
+                     : "memory");
+}
+
+// x as an fp16 pair, and what that leaves
+__device__ __forceinline__ uint32_t q4_term(float &x, float &y) {
+    const uint32_t h = half2_rn(x, y);
+    const float2 f = half2_floats(h);
+    x -= f.x, y -= f.y;
+    return h;
+}
+
+__device__ __forceinline__ float4 peer_load4(const float *p, int rank) {
+    uint32_t at;
+    float4 v;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(sm100::smem_u32(p)), "r"(rank));
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(at) : "memory");
+    return v;
+}
+
+__device__ __forceinline__ void q4_store4(float *p, const float (&x)[4]) {
+    *reinterpret_cast<float4 *>(p) = make_float4(x[0], x[1], x[2], x[3]);
+}
+__device__ __forceinline__ void q4_store4(__nv_bfloat16 *p, const float (&x)[4]) {
+    const __nv_bfloat162 a = __floats2bfloat162_rn(x[0], x[1]), b = __floats2bfloat162_rn(x[2], x[3]);
+    *reinterpret_cast<uint2 *>(p) = make_uint2(*reinterpret_cast<const uint32_t *>(&a), *reinterpret_cast<const uint32_t *>(&b));
+}
+
+// The scale of a query row (a power of two that brings its largest magnitude `top`
+// to 2^14 .. 2^15, held where its inverse is a normal number) and what scores are
+// multiplied by. NaN where the row holds one, or an infinity. The latter is held to
+// 2^88, where scores stay finite; what differs at all differs by far more than a
+// weight can tell, then.
+__device__ __forceinline__ float q4_row_scale(float top, float scale_log2, float &factor) {
+    const int e = min(max(static_cast<int>(__float_as_uint(top) >> 23) - 127, -106), 127);
+    const float up = __uint_as_float(static_cast<uint32_t>(127 + 14 - e) << 23), down = __uint_as_float(static_cast<uint32_t>(127 + e - 14) << 23);
+    factor = fminf(fmaxf(scale_log2 * down, -0x1p88f), 0x1p88f);
+    if (!(top <= 3.4028235e38f))
+        factor = __uint_as_float(0x7fc00000u);
+    return up;
+}
+
+template <typename T, int D, bool kSplit>
+static __global__ void __launch_bounds__(Q4RowsGeo<T, D, kSplit>::kThreads)
+    q4_rows_kernel(const T *__restrict__ q, T *__restrict__ out, TreeArgs a, int groups, int splits, bool sorted) {
+    using G = Q4RowsGeo<T, D, kSplit>;
+    using R = Kv4Record<D>;
+    extern __shared__ __align__(128) uint8_t q4_smem[];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
+    const int rank = blockIdx.x % splits, unit = blockIdx.x / splits;
+    const int group = unit % groups, h = unit / groups, rep = a.qh / a.kvh;
+    pdl_trigger();
+    pdl_wait();
+    const int b = sorted ? sequence_by_work(a.t, blockIdx.y, reinterpret_cast<int *>(q4_smem)) : blockIdx.y;
+    const TreeSpan span(a.t, b);
+    const int row_base = group * G::kRows, rows = span.n * rep;
+    if (row_base >= rows)
+        return; // the whole cluster
+    int keys = span.keys;
+    if (a.t.mask == nullptr) // a chain: nothing after the tile's last node is seen
+        keys = min(keys, span.ctx + (min(row_base + G::kRows, rows) + rep - 1) / rep);
+    const int steps = (keys + G::kStepKeys - 1) / G::kStepKeys;
+    const int first = rank * G::kWarps + warp, stride = splits * G::kWarps;
+    const int mine = steps > first ? (steps - first + stride - 1) / stride : 0;
+
+    // ---- copies
+    const int *table = a.t.block_table + static_cast<int64_t>(b) * a.t.table_stride;
+    const int pages = (keys + kKvPage - 1) / kKvPage;
+    uint8_t *ring = q4_smem + warp * G::kStages * G::kStage;
+    int ids = 0; // a lane has the block of one page of the next 16 steps
+    const auto fetch = [&](int i) {
+        if (i < mine) {
+            if (i % 16 == 0) {
+                const int page = (first + (i + lane / 2) * stride) * G::kStepPages + lane % 2;
+                ids = i + lane / 2 < mine && page < pages ? table[page] : -1;
+            }
+            const uint32_t dst = sm100::smem_u32(ring + i % G::kStages * G::kStage);
+#pragma unroll
+            for (int pg = 0; pg < G::kStepPages; ++pg) {
+                const int64_t id = __shfl_sync(kFullWarpMask, ids, i % 16 * 2 + pg);
+                if (id < 0)
+                    continue; // after the last page: what the ring holds is masked
+                const uint8_t *src = static_cast<const uint8_t *>(a.k) + (id * a.kvh + h) * R::kBytes;
+#pragma unroll
+                for (int c = 0; c < G::kPageBytes; c += 512)
+                    if (c + lane * 16 < G::kPageBytes)
+                        q4_copy16(dst + pg * G::kPageBytes + c + lane * 16, src + c + lane * 16);
+            }
+        }
+        q4_copy_commit();
+    };
+#pragma unroll
+    for (int i = 0; i < G::kStages - 1; ++i)
+        fetch(i);
+
+    // ---- queries: fragments of the first product (k slots 2t, 2t + 1, 2t + 8, 2t + 9 of step u: dims
+    // 8t + 2u, + 4, + 1, + 5 of the group), and the row's factor
+    uint32_t qf[G::kSets][G::kGroups][2][4];
+    float factor[G::kRPL];
+#pragma unroll
+    for (int rr = 0; rr < G::kRPL; ++rr) {
+        const int r = row_base + rr * 8 + g;
+        float x[G::kGroups][8];
+        float top = 0.f;
+#pragma unroll
+        for (int c = 0; c < G::kGroups; ++c) {
+            if (r < rows) {
+                const T *src = q + static_cast<int64_t>(span.row0 + r / rep) * a.q_stride + static_cast<int64_t>(h * rep + r % rep) * D + 32 * c + 8 * t;
+#pragma unroll
+                for (int i = 0; i < 8 / KvVec<T>::kN; ++i) {
+                    float y[KvVec<T>::kN];
+                    KvVec<T>::unpack(*reinterpret_cast<const uint4 *>(src + i * KvVec<T>::kN), y);
+#pragma unroll
+                    for (int j = 0; j < KvVec<T>::kN; ++j)
+                        x[c][i * KvVec<T>::kN + j] = y[j];
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    x[c][i] = 0.f;
+            }
+#pragma unroll
+            for (int i = 0; i < 8; i += 2)
+                top = max_abs_nan(top, x[c][i], x[c][i + 1]);
+        }
+        top = max_abs_nan(top, __shfl_xor_sync(kFullWarpMask, top, 1), 0.f);
+        top = max_abs_nan(top, __shfl_xor_sync(kFullWarpMask, top, 2), 0.f);
+        const float up = q4_row_scale(top, a.scale_log2, factor[rr]);
+#pragma unroll
+        for (int c = 0; c < G::kGroups; ++c)
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    float v0 = x[c][2 * u + i] * up, v1 = x[c][2 * u + i + 4] * up;
+                    const uint32_t hi = q4_term(v0, v1);
+                    if constexpr (kSplit) {
+                        qf[0][c][u][2 * i] = hi;
+                        qf[0][c][u][2 * i + 1] = half2_rn(v0, v1);
+                    } else {
+                        qf[0][c][u][2 * i + rr] = hi;
+                        if constexpr (G::kSets == 2)
+                            qf[1][c][u][2 * i + rr] = half2_rn(v0, v1);
+                    }
+                }
+    }
+
+    float o[G::kGroups][4][2 * G::kRPL] = {}; // of n tile i, the dims 32 c + 8 t + i and + 4 of the lane's rows
+    float m[G::kRPL], l[G::kRPL];
+#pragma unroll
+    for (int rr = 0; rr < G::kRPL; ++rr)
+        m[rr] = kQ4None, l[rr] = 0.f;
+
+    const uint32_t lane_at = (lane / 16) * G::kPageBytes + lane % 16 * 16; // both pages' rows of a group
+    for (int i = 0; i < mine; ++i) {
+        q4_copy_wait<G::kStages - 2>();
+        __syncwarp(); // all lanes' copies are there; all have done with the stage that is filled next
+        fetch(i + G::kStages - 1);
+        const uint8_t *stage = ring + i % G::kStages * G::kStage;
+        const uint32_t stage_at = sm100::smem_u32(stage) + lane_at;
+        const int key0 = (first + i * stride) * G::kStepKeys;
+        const bool edge = key0 + G::kStepKeys > span.ctx;
+
+        // ---- scores
+        float sc[4][4] = {};
+#pragma unroll
+        for (int c = 0; c < G::kGroups; ++c) {
+            uint32_t w[4];
+            q4_ldmatrix<false>(stage_at + c * 256, w);
+#pragma unroll
+            for (int n = 0; n < 4; ++n) {
+                const __half s = *reinterpret_cast<const __half *>(stage + n / 2 * G::kPageBytes + R::kKScale + (c * kKvPage + n % 2 * 8 + g) * 2);
+                uint32_t k[4];
+                kv4_widen(w[n], __half2half2(s), k);
+#pragma unroll
+                for (int set = G::kSets - 1; set >= 0; --set) {
+                    mma_f16(sc[n], qf[set][c][0], k[0], k[1]);
+                    mma_f16(sc[n], qf[set][c][1], k[2], k[3]);
+                }
+            }
+        }
+        float x[G::kRPL][8]; // of key 8 n + 2 t + e: place 2 n + e
+#pragma unroll
+        for (int rr = 0; rr < G::kRPL; ++rr)
+#pragma unroll
+            for (int n = 0; n < 8; ++n)
+                x[rr][n] = (kSplit ? sc[n / 2][n % 2] + sc[n / 2][2 + n % 2] : sc[n / 2][2 * rr + n % 2]) * factor[rr];
+        if (edge) {
+            uint32_t bad = 0; // keys whose V is no number: a row that sees one gets NaN, the others nothing of it
+#pragma unroll
+            for (int n = 0; n < 4; ++n)
+#pragma unroll
+                for (int c = 0; c < G::kGroups; ++c) {
+                    const uint32_t v = *reinterpret_cast<const uint32_t *>(stage + n / 2 * G::kPageBytes + R::kVScale + (c * kKvPage + n % 2 * 8 + 2 * t) * 2);
+                    bad |= ((v & 0x7fffu) >= kQ4BadScale ? 1u : 0u) << (2 * n) | ((v >> 16 & 0x7fffu) >= kQ4BadScale ? 2u : 0u) << (2 * n);
+                }
+#pragma unroll
+            for (int rr = 0; rr < G::kRPL; ++rr) {
+                const int r = row_base + rr * 8 + g;
+                uint32_t seen = 0;
+                if (r < rows)
+                    seen = tree_sees32(a.t, span.row0 + r / rep, r / rep, key0 - span.ctx, keys - span.ctx);
+#pragma unroll
+                for (int n = 0; n < 8; ++n) {
+                    if (bad >> n & 1u)
+                        x[rr][n] = __uint_as_float(0x7fc00000u);
+                    if (!(seen >> (n / 2 * 8 + 2 * t + n % 2) & 1u))
+                        x[rr][n] = kNegInf;
+                }
+            }
+        }
+
+        // ---- weights
+        bool raise = false;
+        float top[G::kRPL];
+#pragma unroll
+        for (int rr = 0; rr < G::kRPL; ++rr) {
+            top[rr] = x[rr][0];
+#pragma unroll
+            for (int n = 1; n < 8; ++n)
+                top[rr] = fmaxf(top[rr], x[rr][n]);
+            raise |= top[rr] - m[rr] > kQ4Top;
+        }
+        if (__any_sync(kFullWarpMask, raise)) {
+#pragma unroll
+            for (int rr = 0; rr < G::kRPL; ++rr) {
+                top[rr] = fmaxf(top[rr], __shfl_xor_sync(kFullWarpMask, top[rr], 1));
+                top[rr] = fmaxf(top[rr], __shfl_xor_sync(kFullWarpMask, top[rr], 2));
+                if (top[rr] - m[rr] > kQ4Top) {
+                    // below scores that are large a lift would be lost in the rounding, or grow by it
+                    const float up = fabsf(top[rr]) < 0x1p20f ? top[rr] - kQ4Lift : top[rr];
+                    const float fix = exp2_approx(m[rr] - up);
+                    m[rr] = up;
+                    l[rr] *= fix;
+#pragma unroll
+                    for (int c = 0; c < G::kGroups; ++c)
+#pragma unroll
+                        for (int n = 0; n < 4; ++n)
+                            o[c][n][2 * rr] *= fix, o[c][n][2 * rr + 1] *= fix;
+                }
+            }
+        }
+        uint32_t pf[G::kSets][2][4]; // of page pg: rows g and g + 8 of keys 2t.., then of keys 8 + 2t..
+#pragma unroll
+        for (int rr = 0; rr < G::kRPL; ++rr)
+#pragma unroll
+            for (int n = 0; n < 4; ++n) {
+                float p0 = exp2_approx(x[rr][2 * n] - m[rr]), p1 = exp2_approx(x[rr][2 * n + 1] - m[rr]);
+                l[rr] += p0 + p1;
+                if constexpr (kSplit) {
+                    pf[0][n / 2][n % 2 * 2] = q4_term(p0, p1);
+                    pf[0][n / 2][n % 2 * 2 + 1] = half2_rn(p0, p1);
+                } else if constexpr (G::kSets == 2) {
+                    pf[0][n / 2][n % 2 * 2 + rr] = q4_term(p0, p1);
+                    pf[1][n / 2][n % 2 * 2 + rr] = half2_rn(p0, p1);
+                } else {
+                    pf[0][n / 2][n % 2 * 2 + rr] = half2_rn(p0, p1);
+                }
+            }
+
+        // ---- output
+#pragma unroll
+        for (int c = 0; c < G::kGroups; ++c) {
+            uint32_t w[4];
+            q4_ldmatrix<true>(stage_at + R::kCodes + c * 256, w);
+            float sum[4][4] = {};
+#pragma unroll
+            for (int pg = 0; pg < 2; ++pg) {
+                uint32_t v[2][4];
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    uint32_t s = *reinterpret_cast<const uint32_t *>(stage + pg * G::kPageBytes + R::kVScale + (c * kKvPage + j * 8 + 2 * t) * 2);
+                    if (edge) // (times a weight of zero it would be NaN)
+                        s &= ((s & 0x7fffu) >= kQ4BadScale ? 0u : 0xffffu) | ((s >> 16 & 0x7fffu) >= kQ4BadScale ? 0u : 0xffff0000u);
+                    kv4_widen(w[2 * pg + j], *reinterpret_cast<const __half2 *>(&s), v[j]);
+                }
+#pragma unroll
+                for (int n = 0; n < 4; ++n)
+#pragma unroll
+                    for (int set = G::kSets - 1; set >= 0; --set) {
+                        if constexpr (G::kWide)
+                            mma_f16(sum[n], pf[set][pg], v[0][n], v[1][n]);
+                        else
+                            mma_f16(o[c][n], pf[set][pg], v[0][n], v[1][n]);
+                    }
+            }
+            if constexpr (G::kWide)
+#pragma unroll
+                for (int n = 0; n < 4; ++n) {
+                    if constexpr (kSplit) {
+                        o[c][n][0] += sum[n][0] + sum[n][2];
+                        o[c][n][1] += sum[n][1] + sum[n][3];
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            o[c][n][e] += sum[n][e];
+                    }
+                }
+        }
+    }
+    q4_copy_wait<0>();
+
+    // ---- joining: the warps, then the cluster
+    __syncthreads(); // the rings are done with
+    float *part = reinterpret_cast<float *>(q4_smem), *joined = part + G::kWarps * G::kRows * G::kPitch;
+    float *stat = joined + G::kRows * G::kPitch, *joined_stat = stat + 2 * G::kWarps * G::kRows; // m, l by warp; of the CTA
+#pragma unroll
+    for (int rr = 0; rr < G::kRPL; ++rr) {
+        l[rr] += __shfl_xor_sync(kFullWarpMask, l[rr], 1);
+        l[rr] += __shfl_xor_sync(kFullWarpMask, l[rr], 2);
+        const int r = rr * 8 + g;
+        if (t == 0) {
+            stat[warp * G::kRows + r] = m[rr];
+            stat[(G::kWarps + warp) * G::kRows + r] = l[rr];
+        }
+#pragma unroll
+        for (int c = 0; c < G::kGroups; ++c) {
+            float *p = part + (warp * G::kRows + r) * G::kPitch + 32 * c + 8 * t;
+            *reinterpret_cast<float4 *>(p) = make_float4(o[c][0][2 * rr], o[c][1][2 * rr], o[c][2][2 * rr], o[c][3][2 * rr]);
+            *reinterpret_cast<float4 *>(p + 4) =
+                make_float4(o[c][0][2 * rr + 1], o[c][1][2 * rr + 1], o[c][2][2 * rr + 1], o[c][3][2 * rr + 1]);
+        }
+    }
+    __syncthreads();
+    const int live = min(G::kRows, rows - row_base);
+    const auto put = [&](int r, int d, float L, const float (&y)[4]) {
+        const int row = row_base + r;
+        const float inv = L == 0.f ? 0.f : 1.f / L;
+        const float z[4] = {L == 0.f ? 0.f : y[0] * inv, L == 0.f ? 0.f : y[1] * inv, L == 0.f ? 0.f : y[2] * inv, L == 0.f ? 0.f : y[3] * inv};
+        q4_store4(out + static_cast<int64_t>(span.row0 + row / rep) * a.out_stride + static_cast<int64_t>(h * rep + row % rep) * D + d, z);
+    };
+    for (int i = tid; i < live * (D / 4); i += G::kThreads) {
+        const int r = i / (D / 4), d = i % (D / 4) * 4;
+        float M = kQ4None, L = 0.f, y[4] = {};
+#pragma unroll
+        for (int w = 0; w < G::kWarps; ++w)
+            M = fmaxf(M, stat[w * G::kRows + r]);
+#pragma unroll
+        for (int w = 0; w < G::kWarps; ++w) {
+            const float f = exp2_approx(stat[w * G::kRows + r] - M);
+            const float4 p = *reinterpret_cast<const float4 *>(part + (w * G::kRows + r) * G::kPitch + d);
+            L += f * stat[(G::kWarps + w) * G::kRows + r];
+            y[0] += f * p.x, y[1] += f * p.y, y[2] += f * p.z, y[3] += f * p.w;
+        }
+        if (splits == 1) {
+            put(r, d, L, y);
+        } else {
+            *reinterpret_cast<float4 *>(joined + r * G::kPitch + d) = make_float4(y[0], y[1], y[2], y[3]);
+            if (d == 0)
+                joined_stat[r] = M, joined_stat[G::kRows + r] = L;
+        }
+    }
+    if (splits == 1)
+        return;
+    __syncthreads();
+    cluster_sync_all();
+    for (int i = rank * G::kThreads + tid; i < live * (D / 4); i += splits * G::kThreads) {
+        const int r = i / (D / 4), d = i % (D / 4) * 4;
+        float M = kQ4None, L = 0.f, y[4] = {};
+        for (int c = 0; c < splits; ++c)
+            M = fmaxf(M, peer_load(&joined_stat[r], c));
+        for (int c = 0; c < splits; ++c) {
+            const float f = exp2_approx(peer_load(&joined_stat[r], c) - M);
+            const float4 p = peer_load4(joined + r * G::kPitch + d, c);
+            L += f * peer_load(&joined_stat[G::kRows + r], c);
+            y[0] += f * p.x, y[1] += f * p.y, y[2] += f * p.z, y[3] += f * p.w;
+        }
+        put(r, d, L, y);
+    }
+    cluster_sync_all(); // peers read this CTA's shared memory until here
+}
+
+// CTAs of a kernel that run at once on the current device, asked once.
+template <typename... P> inline int q4_slots(void (*kernel)(P...), int threads, int bytes) {
+    struct Known {
+        const void *kernel;
+        int device, slots;
+    };
+    static thread_local std::vector<Known> mine;
+    const int device = device_facts().device;
+    for (const Known &k : mine)
+        if (k.kernel == reinterpret_cast<const void *>(kernel) && k.device == device)
+            return k.slots;
+    int per_sm = 0;
+    OPWORKS_CUDA_CHECK(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, threads, bytes));
+    mine.push_back({reinterpret_cast<const void *>(kernel), device, std::max(1, per_sm) * device_facts().sm_count});
+    return mine.back().slots;
+}
+
+template <typename T, int D, bool kSplit> inline void q4_rows_launch(const T *q, T *out, const TreeArgs &a, cudaStream_t stream) {
+    using G = Q4RowsGeo<T, D, kSplit>;
+    const auto kernel = q4_rows_kernel<T, D, kSplit>;
+    const int most = allow_shared_bytes(kernel, G::kThreads, G::kBytes);
+    const int64_t slots = q4_slots(kernel, G::kThreads, G::kBytes);
+    const int64_t rows = static_cast<int64_t>(a.t.max_rows) * (a.qh / a.kvh);
+    const int64_t groups = (rows + G::kRows - 1) / G::kRows, units = groups * a.kvh, all = units * a.t.batch;
+    const int64_t keys = static_cast<int64_t>(a.t.max_ctx) + a.t.max_rows;
+    // As many splits as all CTAs still run at once, and as leave each warp two steps or more.
+    const int64_t cap = std::min<int64_t>(most, keys / (2 * G::kStepKeys * G::kWarps));
+    const int splits = static_cast<int>(std::max<int64_t>(1, std::min(cap, slots / all)));
+    require(units * splits <= 0x7fffffff, "tree attention: too many rows for one call");
+    const bool sort = a.t.batch > 1 && a.t.batch < G::kThreads && all * splits > slots / 2;
+    launch_ex_cluster(kernel, dim3(static_cast<unsigned>(units * splits), a.t.batch), dim3(splits), dim3(G::kThreads), G::kBytes, stream,
+                      q, out, a, static_cast<int>(groups), splits, sort);
+}
+
+template <typename T, int D> inline void q4_rows_call(const T *q, T *out, const TreeArgs &a, cudaStream_t stream) {
+    if constexpr (std::is_same_v<T, float>) {
+        if (static_cast<int64_t>(a.t.max_rows) * (a.qh / a.kvh) <= 8) {
+            q4_rows_launch<T, D, true>(q, out, a, stream);
+            return;
+        }
+    }
+    q4_rows_launch<T, D, false>(q, out, a, stream);
+}
+
+} // namespace opworks::detail

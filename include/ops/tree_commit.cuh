@@ -28,6 +28,7 @@
 #include <cstdint>
 
 #include "../core/cuda_utils.cuh"
+#include "kv4.cuh"
 #include "kv_quant.cuh"
 
 namespace opworks {
@@ -83,15 +84,18 @@ template <int kBytes> struct LaneBytes { // what a lane moves of one row: kBytes
     }
 };
 
-// kRowBytes: a K or V row of one head. Lanes 0-15 move K, 16-31 V. A lane reads
-// and writes the same bytes of every row, so its own program order is enough.
-template <int kRowBytes, bool kScales>
-static __global__ void __launch_bounds__(kCommitThreads) tree_commit_kernel(TreeVerify t, CommitCache c) {
+// The walk of sequence blockIdx.y, by the whole block: its results (from block x =
+// 0), the accepted nodes' count, and the places that path row i is moved from and
+// to: block * 16 + slot, -1 for a row that stays or lies outside the table.
+struct CommitMoves {
+    const int *from, *to;
+    int count;
+};
+__device__ __forceinline__ CommitMoves commit_walk(const TreeVerify &t, const CommitCache &c) {
     extern __shared__ int commit_smem[]; // succ | target | path | place of each path row
     __shared__ int count_s;
     int *succ = commit_smem, *target = succ + t.max_rows, *path = target + t.max_rows, *place = path + t.max_rows;
-    const int b = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    pdl_wait();
+    const int b = blockIdx.y, tid = threadIdx.x;
     const int row0 = t.row_start[b], ctx = t.ctx_lens[b];
     const int n = min(t.row_start[b + 1] - row0, t.max_rows);
     for (int j = tid; j < n; j += kCommitThreads) {
@@ -117,8 +121,7 @@ static __global__ void __launch_bounds__(kCommitThreads) tree_commit_kernel(Tree
     const int count = count_s;
     const int64_t tokens = static_cast<int64_t>(c.table_stride) * kKvPage;
     const int *table = c.table + static_cast<int64_t>(b) * c.table_stride;
-    // place of path row i (block * 16 + slot, -1 outside the table), and over
-    // succ, which is done, the place that it moves to
+    // place of path row i, and over succ, which is done, the place that it moves to
     for (int i = tid; i < count; i += kCommitThreads) {
         const int64_t from = static_cast<int64_t>(ctx) + path[i], to = static_cast<int64_t>(ctx) + i;
         const bool in = to >= 0 && from < tokens && from != to;
@@ -135,6 +138,17 @@ static __global__ void __launch_bounds__(kCommitThreads) tree_commit_kernel(Tree
         }
     }
     __syncthreads();
+    return {place, succ, count};
+}
+
+// kRowBytes: a K or V row of one head. Lanes 0-15 move K, 16-31 V. A lane reads
+// and writes the same bytes of every row, so its own program order is enough.
+template <int kRowBytes, bool kScales>
+static __global__ void __launch_bounds__(kCommitThreads) tree_commit_kernel(TreeVerify t, CommitCache c) {
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    pdl_wait();
+    const CommitMoves moves = commit_walk(t, c);
+    const int *place = moves.from, *succ = moves.to, count = moves.count;
     constexpr int kLane = kRowBytes / 16; // bytes per lane
     const int units = c.layers * c.kvh;
     for (int u = blockIdx.x * (kCommitThreads / 32) + warp; u < units; u += gridDim.x * (kCommitThreads / 32)) {
@@ -163,6 +177,48 @@ static __global__ void __launch_bounds__(kCommitThreads) tree_commit_kernel(Tree
                 x[i].store(rows + at + (to % kKvPage) * kRowBytes + (lane & 15) * min(kLane, 16));
                 if (kScales && lane < 2)
                     *reinterpret_cast<float *>(scales + at + 4 * (to % kKvPage)) = s[i];
+            }
+        }
+    }
+}
+
+// Records of ops/kv4.cuh, from c.k: a row is 2 G pieces of 16 bytes (K's groups,
+// then V's) and as many fp16 scales, a lane each, so a warp moves a row of 4 (D = 64)
+// or 2 heads at a time. The same bytes of every row again.
+template <int D> static __global__ void __launch_bounds__(kCommitThreads) tree_commit_q4_kernel(TreeVerify t, CommitCache c) {
+    using R = Kv4Record<D>;
+    constexpr int kPieces = 2 * R::kGroups, kLanes = 2 * kPieces;
+    const int tid = threadIdx.x, part = tid % kLanes;
+    pdl_wait();
+    const CommitMoves moves = commit_walk(t, c);
+    const bool codes = part < kPieces;
+    const int64_t at0 = codes ? part * kKvPage * 16 : R::kKScale + (part - kPieces) * kKvPage * 2, step = codes ? 16 : 2;
+    const int units = c.layers * c.kvh;
+    for (int u = (blockIdx.x * kCommitThreads + tid) / kLanes; u < units; u += gridDim.x * kCommitThreads / kLanes) {
+        uint8_t *base = c.k + (u / c.kvh) * c.layer_bytes + (u % c.kvh) * c.head_bytes + at0;
+        for (int i0 = 1; i0 < moves.count; i0 += kCommitBatch) {
+            uint4 x[kCommitBatch];
+#pragma unroll
+            for (int i = 0; i < kCommitBatch; ++i) {
+                const int from = i0 + i < moves.count ? moves.from[i0 + i] : -1;
+                if (from < 0)
+                    continue;
+                const uint8_t *src = base + static_cast<int64_t>(from / kKvPage) * c.kvh * c.head_bytes + from % kKvPage * step;
+                if (codes)
+                    x[i] = *reinterpret_cast<const uint4 *>(src);
+                else
+                    x[i].x = *reinterpret_cast<const uint16_t *>(src);
+            }
+#pragma unroll
+            for (int i = 0; i < kCommitBatch; ++i) {
+                const int to = i0 + i < moves.count ? moves.to[i0 + i] : -1;
+                if (to < 0)
+                    continue;
+                uint8_t *dst = base + static_cast<int64_t>(to / kKvPage) * c.kvh * c.head_bytes + to % kKvPage * step;
+                if (codes)
+                    *reinterpret_cast<uint4 *>(dst) = x[i];
+                else
+                    *reinterpret_cast<uint16_t *>(dst) = static_cast<uint16_t>(x[i].x);
             }
         }
     }
@@ -222,6 +278,20 @@ inline void tree_commit_q8(const TreeVerify &t, uint8_t *pool, int64_t layer_str
     if (t.batch == 0)
         return;
     head_dim == 64 ? detail::commit_launch<64, true>(t, c, stream) : detail::commit_launch<128, true>(t, c, stream);
+}
+
+// Over 4-bit pools [layers][blocks][kvh][record]; layer_stride in bytes.
+inline void tree_commit_q4(const TreeVerify &t, uint8_t *pool, int64_t layer_stride, int layers, const int *block_table,
+                           int table_stride, int kv_heads, int head_dim, cudaStream_t stream = nullptr) {
+    const detail::CommitCache c{pool, pool, pool, 18 * static_cast<int64_t>(head_dim), layer_stride, layers, kv_heads, block_table, table_stride};
+    detail::validate_commit(t, c, head_dim, layer_stride);
+    if (t.batch == 0)
+        return;
+    const int units = layers * kv_heads, per_block = detail::kCommitThreads / (head_dim == 64 ? 8 : 16);
+    const int want = (units + per_block - 1) / per_block, room = (4 * detail::device_facts().sm_count + t.batch - 1) / t.batch;
+    launch_ex(head_dim == 64 ? detail::tree_commit_q4_kernel<64> : detail::tree_commit_q4_kernel<128>,
+              dim3(want < room ? want : room, t.batch), dim3(detail::kCommitThreads), sizeof(int) * 4 * static_cast<size_t>(t.max_rows),
+              stream, t, c);
 }
 
 } // namespace ops

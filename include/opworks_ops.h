@@ -220,6 +220,72 @@ OPW_API int opw_tree_commit_q8(const int32_t *draft, const int32_t *target, cons
                                int table_stride, int num_kv_heads, int head_dim, int32_t *path, int32_t *count,
                                int32_t *next, int32_t *new_lens, void *stream);
 
+/* ---- Block tables and slot maps built on the GPU (include/ops/pages.cuh).
+ * Extensions of this library.
+ *
+ * Sequence b holds lens[b] tokens in the first ceil(lens[b] / 16) pages of its
+ * table row and gets rows [row_start[b], row_start[b + 1]) (device int32, batch +
+ * 1 of them). free_blocks is a stack of free_count[0] block ids, taken from its
+ * end, sequence by sequence. Writes the new ids into the table, position lens[b] +
+ * i and slot 16 * block + position % 16 of every row (rows past the last
+ * sequence's: position 0, slot -1) and what is left of the stack (free_left may be
+ * free_count). free_blocks NULL: the table is complete; positions and slots only.
+ * status[0]: 0; the pages missing; or -1 where a length is below zero, a sequence
+ * longer than its table row, or a row past `rows`. Unless it is 0 nothing is taken
+ * and every slot is -1. */
+OPW_API int opw_page_take(const int32_t *lens, const int32_t *row_start, int batch, int rows, int32_t *block_table,
+                          int table_stride, const int32_t *free_blocks, const int32_t *free_count, int32_t *positions,
+                          int64_t *slots, int32_t *free_left, int32_t *status, void *stream);
+/* The other way round: pages ceil(new / 16) .. ceil(old / 16) - 1 of each sequence
+ * go onto the stack (room for `capacity` ids), in order; new >= old gives none.
+ * status[0]: 0, or -1 (a length below zero or past the table row, a stack without
+ * room), and then nothing is given. */
+OPW_API int opw_page_give(const int32_t *old_lens, const int32_t *new_lens, int batch, const int32_t *block_table,
+                          int table_stride, int32_t *free_blocks, int capacity, const int32_t *free_count,
+                          int32_t *free_left, int32_t *status, void *stream);
+
+/* ---- Norms of queries and keys for each head, and their rotation, in one pass
+ * (include/ops/qk_norm_rope.cuh). Extension of this library.
+ *
+ * Head h of row r lies at r * stride + h * head_dim (head_dim 32, 64, 128 or 256),
+ * type 0 fp32 or 1 bf16; x / sqrt(mean(x^2) + eps) * weight (fp32 [head_dim]; NULL:
+ * that side is not normalised), then the pairs (i, i + rot_dim / 2) are turned by
+ * positions[r] * inv_freq[i] (rot_dim a multiple of 16 up to head_dim; 0: no
+ * rotation). The outputs may be the inputs. Rows are 16-byte aligned, strides too. */
+OPW_API int opw_qk_norm_rope(const void *q, int64_t q_stride, const void *k, int64_t k_stride, int type,
+                             const float *q_weight, const float *k_weight, float eps, const int32_t *positions,
+                             const float *inv_freq, int rot_dim, int rows, int q_heads, int kv_heads, int head_dim,
+                             void *q_out, int64_t q_out_stride, void *k_out, int64_t k_out_stride, void *stream);
+
+/* ---- 4-bit paged KV cache (include/ops/kv4.cuh). Extensions of this library.
+ *
+ * One record of 18 * head_dim bytes per (block, kv head), G = head_dim / 32 groups
+ * of 32 dims: K codes [G][16 tokens][16 bytes], V codes the same, K scales fp16
+ * [G][16], V scales fp16 [G][16]; byte i of a group's 16 holds dims 2 i (low half)
+ * and 2 i + 1. A value is (code - 8) * scale; scale = max|x| / 7 of the group,
+ * rounded to 5 significant bits, code = 8 + x / scale rounded to nearest even, 1 to
+ * 15. A group with a value above 55,552 (whose scale would be above 7,936), an
+ * infinity or a NaN has scale NaN and codes 8. Row r of K and V goes to (comes
+ * from) slot slots[r] = 16 * block + place of a pool of `blocks` blocks; rows with a
+ * slot outside of it are left out. No two rows written have the same slot. type,
+ * alignment and head_dim as in the 8-bit cache; K and V have a stride each. */
+OPW_API int opw_kv4_record_bytes(int head_dim); /* -1: not a supported head_dim */
+OPW_API int opw_kv4_write(const void *k, int64_t k_stride, const void *v, int64_t v_stride, int type, uint8_t *pool,
+                          int blocks, const int64_t *slots, int rows, int num_kv_heads, int head_dim, void *stream);
+OPW_API int opw_kv4_read(const uint8_t *pool, int blocks, const int64_t *slots, int rows, int num_kv_heads,
+                         int head_dim, void *k, int64_t k_stride, void *v, int64_t v_stride, int type, void *stream);
+/* opw_tree_attention and opw_tree_commit over the 4-bit pool (layer_stride in bytes). */
+OPW_API int opw_tree_attention_q4(const void *q, int type, int64_t q_stride, const uint8_t *pool,
+                                  const int32_t *block_table, int table_stride, const int32_t *ctx_lens,
+                                  const int32_t *row_start, const uint32_t *mask, int mask_words, int batch, int rows,
+                                  int max_rows, int max_ctx, int num_q_heads, int num_kv_heads, int head_dim,
+                                  float scale, void *out, int64_t out_stride, void *stream);
+OPW_API int opw_tree_commit_q4(const int32_t *draft, const int32_t *target, const int32_t *parent,
+                               const int32_t *row_start, const int32_t *ctx_lens, int batch, int max_rows,
+                               uint8_t *pool, int64_t layer_stride, int layers, const int32_t *block_table,
+                               int table_stride, int num_kv_heads, int head_dim, int32_t *path, int32_t *count,
+                               int32_t *next, int32_t *new_lens, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -57,11 +57,19 @@ SIGNATURES = {
     "opw_tree_attention_q8": [P, I, I64, P, I, P, I, P, P, P, I, I, I, I, I, I, I, I, F, P, I64, P],
     "opw_tree_commit": [P, P, P, P, P, I, I, P, P, I64, I, P, I, I, I, P, P, P, P, P],
     "opw_tree_commit_q8": [P, P, P, P, P, I, I, P, I64, I, P, I, I, I, P, P, P, P, P],
+    "opw_page_take": [P, P, I, I, P, I, P, P, P, P, P, P, P],
+    "opw_page_give": [P, P, I, P, I, P, I, P, P, P, P],
+    "opw_qk_norm_rope": [P, I64, P, I64, I, P, P, F, P, P, I, I, I, I, I, P, I64, P, I64, P],
+    "opw_kv4_record_bytes": [I],
+    "opw_kv4_write": [P, I64, P, I64, I, P, I, P, I, I, I, P],
+    "opw_kv4_read": [P, I, P, I, I, I, P, I64, P, I64, I, P],
+    "opw_tree_attention_q4": [P, I, I64, P, P, I, P, P, P, I, I, I, I, I, I, I, I, F, P, I64, P],
+    "opw_tree_commit_q4": [P, P, P, P, P, I, I, P, I64, I, P, I, I, I, P, P, P, P, P],
 }
 
 
 # These return a number, below zero for an error; all others 0 or an error.
-VALUES = frozenset(("reduction_workspace_size", "kv_quant_record_bytes"))
+VALUES = frozenset(("reduction_workspace_size", "kv_quant_record_bytes", "kv4_record_bytes"))
 
 
 class OpsLib:
