@@ -4,23 +4,27 @@
 // (ops/tree_attention_q4.cuh has the definition): mma.sync, K and V widened in
 // registers.
 //
-// The rows of a KV head (row = node * rep + head in group) are the M side of the
-// products, the keys of a step (32: two pages) the N side of the scores, the dims
-// that of the output. Every warp of the CTA has the same rows and takes every
-// n-th step; the steps of a sequence go round the warps of a cluster, and what
-// they have is joined at the end through shared memory, in rank order.
+// The keys of a step (32: two pages) are the M side of the scores, the dims that of
+// the output, and the rows of a KV head (row = node * rep + head in group) the N
+// side of both, 8 columns a tile: so few rows waste little, and a lane holds the
+// scores of few rows and many keys. Every warp of the CTA has the same rows and
+// takes every n-th step; the steps of a sequence go round the warps of a cluster,
+// and what they have is joined at the end through shared memory, in rank order.
 //
 // A page record comes with 16-byte asynchronous copies into a ring that only this
 // warp uses, so nothing in the loop waits for another warp. ldmatrix hands out its
 // codes as fragments, four codes to a 16-bit element: of K eight dims of a key (the
 // four k slots of two products, in an order that Q follows), of V, transposed, four
-// dims of two keys each.
+// dims of two keys each. Widening them is most of what the loop does. K's stay
+// integers, one operation a pair of codes, and their scale multiplies the sum over
+// the group's dims; V's are multiplied out, since a scale is a key's there, which
+// the product sums over.
 //
-// fp32 rows are two fp16 terms, and so are their weights. With up to 8 rows both
-// terms share a tile (rows g and g + 8 of the fragments), so one product does both;
-// above that a tile has 16 rows and a product for each term, in one accumulator.
-// The tensor cores cut an accumulator off at every step, so fp32 rows add up O
-// outside of them, rounded, once a step.
+// fp32 rows are two fp16 terms, and so are their weights. Up to 4 rows have two
+// columns each, which are the two terms (bf16 rows: of the weights only, which
+// costs nothing); above that fp32 rows take a product for each term, in one
+// accumulator. The tensor cores cut an accumulator off at every step, so fp32 rows
+// add up O outside of them, rounded, once a step.
 
 #include <type_traits>
 
@@ -30,22 +34,28 @@
 
 namespace opworks::detail {
 
-template <typename T, int D, bool kSplit> struct Q4RowsGeo {
-    static constexpr bool kWide = std::is_same_v<T, float>;
-    static_assert(kWide || !kSplit, "bf16 rows are one term");
+// kNT: tiles of 8 columns; 0: one tile with two columns a row.
+template <typename T, int D, int kNT> struct Q4RowsGeo {
+    static constexpr bool kWide = std::is_same_v<T, float>, kPair = kNT == 0;
+    static constexpr int kTiles = kPair ? 1 : kNT;
     static constexpr int kGroups = D / kKv4Group;
-    static constexpr int kRows = kSplit ? 8 : 16;              // of a tile
-    static constexpr int kRPL = kSplit ? 1 : 2;                // rows that a lane has scores of
-    static constexpr int kSets = kWide && !kSplit ? 2 : 1;     // products of a k step
+    static constexpr int kRows = kPair ? 4 : 8 * kNT;
+    static constexpr int kRPL = kPair ? 1 : 2 * kNT;         // rows that a lane has scores of
+    static constexpr int kSets = kWide && !kPair ? 2 : 1;    // products of a k step
+    // c + 8 as it is, with 8 sum(q) taken off the sums from the start, costs fp32 rows bits
+    // (the sum is 3 times as large as what is left) and two registers a group and tile
+    static constexpr bool kSigned = kWide || kNT > 1;
+    static constexpr bool kQShared = kSets * kTiles * D > 256; // queries in shared memory, not in registers
     static constexpr int kWarps = 4, kThreads = 32 * kWarps;
     static constexpr int kStepPages = 2, kStepKeys = kStepPages * kKvPage;
     static constexpr int kStages = 3;
     static constexpr int kPageBytes = Kv4Record<D>::kBytes, kStage = kStepPages * kPageBytes;
+    static constexpr int kQBytes = kQShared ? kSets * kTiles * kGroups * 2 * 32 * 8 : 0;
     static constexpr int kRing = kWarps * kStages * kStage;
     static constexpr int kPitch = D + 4; // floats of a row of partial sums
     // O of the warps, then of the CTA; m and l of the warps, then of the CTA
     static constexpr int kJoin = 4 * ((kWarps + 1) * kRows * kPitch + 2 * (kWarps + 1) * kRows);
-    static constexpr int kBytes = kRing > kJoin ? kRing : kJoin;
+    static constexpr int kBytes = kQBytes + kRing > kJoin ? kQBytes + kRing : kJoin;
 };
 
 // Scores may pass a row's reference by this many log2 units before it is raised:
@@ -72,13 +82,24 @@ template <bool kTrans> __device__ __forceinline__ void q4_ldmatrix(uint32_t at, 
                      : "r"(at)
                      : "memory");
 }
+// An 8 x 8 matrix of 16-bit elements, two of a row to a lane, turned round.
+__device__ __forceinline__ uint32_t q4_transposed(uint32_t x) {
+    uint32_t y;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
 
-// x as an fp16 pair, and what that leaves
+// x, y as an fp16 pair, and what that leaves of them
 __device__ __forceinline__ uint32_t q4_term(float &x, float &y) {
     const uint32_t h = half2_rn(x, y);
     const float2 f = half2_floats(h);
     x -= f.x, y -= f.y;
     return h;
+}
+// both terms of x as a pair
+__device__ __forceinline__ uint32_t q4_terms(float x) {
+    const __half hi = __float2half_rn(x);
+    return kv4_bits(__halves2half2(hi, __float2half_rn(x - __half2float(hi))));
 }
 
 __device__ __forceinline__ float4 peer_load4(const float *p, int rank) {
@@ -98,24 +119,25 @@ __device__ __forceinline__ void q4_store4(__nv_bfloat16 *p, const float (&x)[4])
 }
 
 // The scale of a query row (a power of two that brings its largest magnitude `top`
-// to 2^14 .. 2^15, held where its inverse is a normal number) and what scores are
-// multiplied by. NaN where the row holds one, or an infinity. The latter is held to
-// 2^88, where scores stay finite; what differs at all differs by far more than a
-// weight can tell, then.
+// to 2^14 .. 2^15, held where its inverse is a normal number) and what scores, in
+// units of 2^-24 for the codes, are multiplied by. NaN where the row holds one, or an
+// infinity. The latter is held to 2^110, where scores stay finite; what differs at
+// all differs by far more than a weight can tell, then.
 __device__ __forceinline__ float q4_row_scale(float top, float scale_log2, float &factor) {
     const int e = min(max(static_cast<int>(__float_as_uint(top) >> 23) - 127, -106), 127);
     const float up = __uint_as_float(static_cast<uint32_t>(127 + 14 - e) << 23), down = __uint_as_float(static_cast<uint32_t>(127 + e - 14) << 23);
-    factor = fminf(fmaxf(scale_log2 * down, -0x1p88f), 0x1p88f);
+    factor = fminf(fmaxf(scale_log2 * down, -0x1p86f), 0x1p86f) * 0x1p24f;
     if (!(top <= 3.4028235e38f))
         factor = __uint_as_float(0x7fc00000u);
     return up;
 }
 
-template <typename T, int D, bool kSplit>
-static __global__ void __launch_bounds__(Q4RowsGeo<T, D, kSplit>::kThreads)
+template <typename T, int D, int kNT>
+static __global__ void __launch_bounds__(Q4RowsGeo<T, D, kNT>::kThreads)
     q4_rows_kernel(const T *__restrict__ q, T *__restrict__ out, TreeArgs a, int groups, int splits, bool sorted) {
-    using G = Q4RowsGeo<T, D, kSplit>;
+    using G = Q4RowsGeo<T, D, kNT>;
     using R = Kv4Record<D>;
+    constexpr bool kPair = G::kPair;
     extern __shared__ __align__(128) uint8_t q4_smem[];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
     const int rank = blockIdx.x % splits, unit = blockIdx.x / splits;
@@ -137,15 +159,15 @@ static __global__ void __launch_bounds__(Q4RowsGeo<T, D, kSplit>::kThreads)
     // ---- copies
     const int *table = a.t.block_table + static_cast<int64_t>(b) * a.t.table_stride;
     const int pages = (keys + kKvPage - 1) / kKvPage;
-    uint8_t *ring = q4_smem + warp * G::kStages * G::kStage;
+    uint8_t *ring = q4_smem + G::kQBytes + warp * G::kStages * G::kStage;
     int ids = 0; // a lane has the block of one page of the next 16 steps
-    const auto fetch = [&](int i) {
+    const auto fetch = [&](int i, int to) {
         if (i < mine) {
             if (i % 16 == 0) {
                 const int page = (first + (i + lane / 2) * stride) * G::kStepPages + lane % 2;
                 ids = i + lane / 2 < mine && page < pages ? table[page] : -1;
             }
-            const uint32_t dst = sm100::smem_u32(ring + i % G::kStages * G::kStage);
+            const uint32_t dst = sm100::smem_u32(ring + to * G::kStage);
 #pragma unroll
             for (int pg = 0; pg < G::kStepPages; ++pg) {
                 const int64_t id = __shfl_sync(kFullWarpMask, ids, i % 16 * 2 + pg);
@@ -162,15 +184,17 @@ static __global__ void __launch_bounds__(Q4RowsGeo<T, D, kSplit>::kThreads)
     };
 #pragma unroll
     for (int i = 0; i < G::kStages - 1; ++i)
-        fetch(i);
+        fetch(i, i);
 
-    // ---- queries: fragments of the first product (k slots 2t, 2t + 1, 2t + 8, 2t + 9 of step u: dims
-    // 8t + 2u, + 4, + 1, + 5 of the group), and the row's factor
-    uint32_t qf[G::kSets][G::kGroups][2][4];
+    // ---- queries, as fragments: column g of a tile, k slots 2t, 2t + 1 and 2t + 8, 2t + 9 of product u: dims 8t + 2u, + 4
+    // and 8t + 2u + 1, + 5 of the group. The latter ones meet codes that are 16 times as large.
+    constexpr int kInRegs = G::kQShared ? 1 : G::kGroups; // (not used where they are shared)
+    uint32_t qf[G::kSets][G::kTiles][kInRegs][2][2];
+    uint2 *q_shared = reinterpret_cast<uint2 *>(q4_smem); // [set][tile][group][u][lane]
     float factor[G::kRPL];
 #pragma unroll
-    for (int rr = 0; rr < G::kRPL; ++rr) {
-        const int r = row_base + rr * 8 + g;
+    for (int nt = 0; nt < G::kTiles; ++nt) {
+        const int r = row_base + (kPair ? g / 2 : nt * 8 + g);
         float x[G::kGroups][8];
         float top = 0.f;
 #pragma unroll
@@ -196,86 +220,144 @@ static __global__ void __launch_bounds__(Q4RowsGeo<T, D, kSplit>::kThreads)
         }
         top = max_abs_nan(top, __shfl_xor_sync(kFullWarpMask, top, 1), 0.f);
         top = max_abs_nan(top, __shfl_xor_sync(kFullWarpMask, top, 2), 0.f);
-        const float up = q4_row_scale(top, a.scale_log2, factor[rr]);
+        float mine_f; // of row r: lanes 4 g ..; wanted by the lanes that have its scores
+        const float up = q4_row_scale(top, a.scale_log2, mine_f);
+        if constexpr (kPair) {
+            factor[0] = __shfl_sync(kFullWarpMask, mine_f, t * 8);
+        } else {
+            factor[2 * nt] = __shfl_sync(kFullWarpMask, mine_f, t * 8);
+            factor[2 * nt + 1] = __shfl_sync(kFullWarpMask, mine_f, t * 8 + 4);
+        }
 #pragma unroll
         for (int c = 0; c < G::kGroups; ++c)
 #pragma unroll
-            for (int u = 0; u < 2; ++u)
+            for (int u = 0; u < 2; ++u) {
+                uint32_t f[2][2]; // [term][slots]
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
-                    float v0 = x[c][2 * u + i] * up, v1 = x[c][2 * u + i + 4] * up;
-                    const uint32_t hi = q4_term(v0, v1);
-                    if constexpr (kSplit) {
-                        qf[0][c][u][2 * i] = hi;
-                        qf[0][c][u][2 * i + 1] = half2_rn(v0, v1);
+                    const float less = i == 0 ? up : up * 0.0625f;
+                    float v0 = x[c][2 * u + i] * less, v1 = x[c][2 * u + i + 4] * less;
+                    f[0][i] = q4_term(v0, v1);
+                    f[1][i] = half2_rn(v0, v1);
+                    if constexpr (kPair)
+                        f[0][i] = g & 1 ? f[1][i] : f[0][i];
+                }
+#pragma unroll
+                for (int set = 0; set < G::kSets; ++set) {
+                    if constexpr (G::kQShared) {
+                        if (warp == 0)
+                            q_shared[(((set * G::kTiles + nt) * G::kGroups + c) * 2 + u) * 32 + lane] = make_uint2(f[set][0], f[set][1]);
                     } else {
-                        qf[0][c][u][2 * i + rr] = hi;
-                        if constexpr (G::kSets == 2)
-                            qf[1][c][u][2 * i + rr] = half2_rn(v0, v1);
+                        qf[set][nt][c][u][0] = f[set][0], qf[set][nt][c][u][1] = f[set][1];
                     }
                 }
+            }
+    }
+    if constexpr (G::kQShared)
+        __syncthreads();
+    // what codes of 8 everywhere would sum to: where the sums start when codes come with 8 added
+    float start[G::kSigned ? 1 : G::kGroups][2];
+    if constexpr (!G::kSigned) {
+        const uint32_t eight[4] = {0x00080008u, 0x00080008u, 0x00800080u, 0x00800080u};
+#pragma unroll
+        for (int c = 0; c < G::kGroups; ++c) {
+            float sum[4] = {};
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+                mma_f16(sum, eight, qf[0][0][c][u][0], qf[0][0][c][u][1]);
+            start[c][0] = -sum[0], start[c][1] = -sum[1];
+        }
     }
 
-    float o[G::kGroups][4][2 * G::kRPL] = {}; // of n tile i, the dims 32 c + 8 t + i and + 4 of the lane's rows
+    float o[G::kGroups][2][G::kTiles][kPair && G::kWide ? 2 : 4] = {}; // dims 32 c + 4 g + 2 i and + 1 of the lane's rows
     float m[G::kRPL], l[G::kRPL];
 #pragma unroll
     for (int rr = 0; rr < G::kRPL; ++rr)
         m[rr] = kQ4None, l[rr] = 0.f;
 
-    const uint32_t lane_at = (lane / 16) * G::kPageBytes + lane % 16 * 16; // both pages' rows of a group
+    const uint32_t ring_at = sm100::smem_u32(ring) + (lane / 16) * G::kPageBytes + lane % 16 * 16; // both pages' rows of a group
+    int at = 0;
     for (int i = 0; i < mine; ++i) {
         q4_copy_wait<G::kStages - 2>();
         __syncwarp(); // all lanes' copies are there; all have done with the stage that is filled next
-        fetch(i + G::kStages - 1);
-        const uint8_t *stage = ring + i % G::kStages * G::kStage;
-        const uint32_t stage_at = sm100::smem_u32(stage) + lane_at;
+        fetch(i + G::kStages - 1, at == 0 ? G::kStages - 1 : at - 1);
+        const uint8_t *stage = ring + at * G::kStage;
+        const uint32_t stage_at = ring_at + at * G::kStage;
+        at = at + 1 == G::kStages ? 0 : at + 1;
         const int key0 = (first + i * stride) * G::kStepKeys;
         const bool edge = key0 + G::kStepKeys > span.ctx;
 
-        // ---- scores
-        float sc[4][4] = {};
+        // ---- scores: of key 16 p + 8 e + g at place 2 p + e
+        float x[G::kRPL][4] = {};
 #pragma unroll
         for (int c = 0; c < G::kGroups; ++c) {
-            uint32_t w[4];
+            uint32_t w[4], k[4][4];
             q4_ldmatrix<false>(stage_at + c * 256, w);
 #pragma unroll
-            for (int n = 0; n < 4; ++n) {
-                const __half s = *reinterpret_cast<const __half *>(stage + n / 2 * G::kPageBytes + R::kKScale + (c * kKvPage + n % 2 * 8 + g) * 2);
-                uint32_t k[4];
-                kv4_widen(w[n], __half2half2(s), k);
+            for (int j = 0; j < 4; ++j)
+                kv4_integers<G::kSigned>(w[j], k[j]);
+            float sum[2][G::kTiles][4];
 #pragma unroll
-                for (int set = G::kSets - 1; set >= 0; --set) {
-                    mma_f16(sc[n], qf[set][c][0], k[0], k[1]);
-                    mma_f16(sc[n], qf[set][c][1], k[2], k[3]);
+            for (int p = 0; p < 2; ++p)
+#pragma unroll
+                for (int nt = 0; nt < G::kTiles; ++nt)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        sum[p][nt][e] = G::kSigned ? 0.f : start[G::kSigned ? 0 : c][e & 1];
+#pragma unroll
+            for (int set = G::kSets - 1; set >= 0; --set)
+#pragma unroll
+                for (int u = 0; u < 2; ++u)
+#pragma unroll
+                    for (int nt = 0; nt < G::kTiles; ++nt) {
+                        uint32_t b0, b1;
+                        if constexpr (G::kQShared) {
+                            const uint2 f = q_shared[(((set * G::kTiles + nt) * G::kGroups + c) * 2 + u) * 32 + lane];
+                            b0 = f.x, b1 = f.y;
+                        } else {
+                            b0 = qf[set][nt][G::kQShared ? 0 : c][u][0], b1 = qf[set][nt][G::kQShared ? 0 : c][u][1];
+                        }
+#pragma unroll
+                        for (int p = 0; p < 2; ++p) {
+                            const uint32_t f[4] = {k[2 * p][2 * u], k[2 * p + 1][2 * u], k[2 * p][2 * u + 1], k[2 * p + 1][2 * u + 1]};
+                            mma_f16(sum[p][nt], f, b0, b1);
+                        }
+                    }
+#pragma unroll
+            for (int p = 0; p < 2; ++p)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const float s = __half2float(*reinterpret_cast<const __half *>(stage + p * G::kPageBytes + R::kKScale + (c * kKvPage + e * 8 + g) * 2));
+#pragma unroll
+                    for (int rr = 0; rr < G::kRPL; ++rr)
+                        x[rr][2 * p + e] += s * (kPair ? sum[p][0][2 * e] + sum[p][0][2 * e + 1] : sum[p][rr / 2][2 * e + rr % 2]);
                 }
-            }
         }
-        float x[G::kRPL][8]; // of key 8 n + 2 t + e: place 2 n + e
 #pragma unroll
         for (int rr = 0; rr < G::kRPL; ++rr)
 #pragma unroll
-            for (int n = 0; n < 8; ++n)
-                x[rr][n] = (kSplit ? sc[n / 2][n % 2] + sc[n / 2][2 + n % 2] : sc[n / 2][2 * rr + n % 2]) * factor[rr];
+            for (int n = 0; n < 4; ++n)
+                x[rr][n] *= factor[rr];
         if (edge) {
             uint32_t bad = 0; // keys whose V is no number: a row that sees one gets NaN, the others nothing of it
 #pragma unroll
             for (int n = 0; n < 4; ++n)
 #pragma unroll
                 for (int c = 0; c < G::kGroups; ++c) {
-                    const uint32_t v = *reinterpret_cast<const uint32_t *>(stage + n / 2 * G::kPageBytes + R::kVScale + (c * kKvPage + n % 2 * 8 + 2 * t) * 2);
-                    bad |= ((v & 0x7fffu) >= kQ4BadScale ? 1u : 0u) << (2 * n) | ((v >> 16 & 0x7fffu) >= kQ4BadScale ? 2u : 0u) << (2 * n);
+                    const uint32_t v = *reinterpret_cast<const uint16_t *>(stage + n / 2 * G::kPageBytes + R::kVScale + (c * kKvPage + n % 2 * 8 + g) * 2);
+                    bad |= ((v & 0x7fffu) >= kQ4BadScale ? 1u : 0u) << n;
                 }
 #pragma unroll
             for (int rr = 0; rr < G::kRPL; ++rr) {
-                const int r = row_base + rr * 8 + g;
+                const int r = row_base + (kPair ? t : rr / 2 * 8 + 2 * t + rr % 2);
                 uint32_t seen = 0;
                 if (r < rows)
                     seen = tree_sees32(a.t, span.row0 + r / rep, r / rep, key0 - span.ctx, keys - span.ctx);
 #pragma unroll
-                for (int n = 0; n < 8; ++n) {
+                for (int n = 0; n < 4; ++n) {
                     if (bad >> n & 1u)
                         x[rr][n] = __uint_as_float(0x7fc00000u);
-                    if (!(seen >> (n / 2 * 8 + 2 * t + n % 2) & 1u))
+                    if (!(seen >> (n * 8 + g) & 1u))
                         x[rr][n] = kNegInf;
                 }
             }
@@ -286,17 +368,15 @@ static __global__ void __launch_bounds__(Q4RowsGeo<T, D, kSplit>::kThreads)
         float top[G::kRPL];
 #pragma unroll
         for (int rr = 0; rr < G::kRPL; ++rr) {
-            top[rr] = x[rr][0];
-#pragma unroll
-            for (int n = 1; n < 8; ++n)
-                top[rr] = fmaxf(top[rr], x[rr][n]);
+            top[rr] = fmaxf(fmaxf(x[rr][0], x[rr][1]), fmaxf(x[rr][2], x[rr][3]));
             raise |= top[rr] - m[rr] > kQ4Top;
         }
         if (__any_sync(kFullWarpMask, raise)) {
 #pragma unroll
             for (int rr = 0; rr < G::kRPL; ++rr) {
-                top[rr] = fmaxf(top[rr], __shfl_xor_sync(kFullWarpMask, top[rr], 1));
-                top[rr] = fmaxf(top[rr], __shfl_xor_sync(kFullWarpMask, top[rr], 2));
+#pragma unroll
+                for (int off = 4; off < 32; off <<= 1)
+                    top[rr] = fmaxf(top[rr], __shfl_xor_sync(kFullWarpMask, top[rr], off));
                 if (top[rr] - m[rr] > kQ4Top) {
                     // below scores that are large a lift would be lost in the rounding, or grow by it
                     const float up = fabsf(top[rr]) < 0x1p20f ? top[rr] - kQ4Lift : top[rr];
@@ -306,67 +386,78 @@ static __global__ void __launch_bounds__(Q4RowsGeo<T, D, kSplit>::kThreads)
 #pragma unroll
                     for (int c = 0; c < G::kGroups; ++c)
 #pragma unroll
-                        for (int n = 0; n < 4; ++n)
-                            o[c][n][2 * rr] *= fix, o[c][n][2 * rr + 1] *= fix;
+                        for (int n = 0; n < 2; ++n) {
+                            if constexpr (kPair) {
+                                for (float &y : o[c][n][0])
+                                    y *= fix;
+                            } else {
+                                o[c][n][rr / 2][rr % 2] *= fix, o[c][n][rr / 2][2 + rr % 2] *= fix;
+                            }
+                        }
                 }
             }
         }
-        uint32_t pf[G::kSets][2][4]; // of page pg: rows g and g + 8 of keys 2t.., then of keys 8 + 2t..
+        uint32_t pf[G::kSets][G::kTiles][2][2]; // of page p: keys 2t, 2t + 1, and 8 more, of column g
 #pragma unroll
-        for (int rr = 0; rr < G::kRPL; ++rr)
+        for (int n = 0; n < 4; ++n) {
+            if constexpr (kPair) {
+                const float p = exp2_approx(x[0][n] - m[0]);
+                l[0] += p;
+                pf[0][0][n / 2][n % 2] = q4_transposed(q4_terms(p));
+            } else {
 #pragma unroll
-            for (int n = 0; n < 4; ++n) {
-                float p0 = exp2_approx(x[rr][2 * n] - m[rr]), p1 = exp2_approx(x[rr][2 * n + 1] - m[rr]);
-                l[rr] += p0 + p1;
-                if constexpr (kSplit) {
-                    pf[0][n / 2][n % 2 * 2] = q4_term(p0, p1);
-                    pf[0][n / 2][n % 2 * 2 + 1] = half2_rn(p0, p1);
-                } else if constexpr (G::kSets == 2) {
-                    pf[0][n / 2][n % 2 * 2 + rr] = q4_term(p0, p1);
-                    pf[1][n / 2][n % 2 * 2 + rr] = half2_rn(p0, p1);
-                } else {
-                    pf[0][n / 2][n % 2 * 2 + rr] = half2_rn(p0, p1);
+                for (int nt = 0; nt < G::kTiles; ++nt) {
+                    float p0 = exp2_approx(x[2 * nt][n] - m[2 * nt]), p1 = exp2_approx(x[2 * nt + 1][n] - m[2 * nt + 1]);
+                    l[2 * nt] += p0, l[2 * nt + 1] += p1;
+                    if constexpr (G::kSets == 2) {
+                        pf[0][nt][n / 2][n % 2] = q4_transposed(q4_term(p0, p1));
+                        pf[1][nt][n / 2][n % 2] = q4_transposed(half2_rn(p0, p1));
+                    } else {
+                        pf[0][nt][n / 2][n % 2] = q4_transposed(half2_rn(p0, p1));
+                    }
                 }
             }
+        }
 
         // ---- output
 #pragma unroll
         for (int c = 0; c < G::kGroups; ++c) {
-            uint32_t w[4];
+            uint32_t w[4], v[4][4];
             q4_ldmatrix<true>(stage_at + R::kCodes + c * 256, w);
-            float sum[4][4] = {};
 #pragma unroll
-            for (int pg = 0; pg < 2; ++pg) {
-                uint32_t v[2][4];
-#pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    uint32_t s = *reinterpret_cast<const uint32_t *>(stage + pg * G::kPageBytes + R::kVScale + (c * kKvPage + j * 8 + 2 * t) * 2);
-                    if (edge) // (times a weight of zero it would be NaN)
-                        s &= ((s & 0x7fffu) >= kQ4BadScale ? 0u : 0xffffu) | ((s >> 16 & 0x7fffu) >= kQ4BadScale ? 0u : 0xffff0000u);
-                    kv4_widen(w[2 * pg + j], *reinterpret_cast<const __half2 *>(&s), v[j]);
-                }
-#pragma unroll
-                for (int n = 0; n < 4; ++n)
-#pragma unroll
-                    for (int set = G::kSets - 1; set >= 0; --set) {
-                        if constexpr (G::kWide)
-                            mma_f16(sum[n], pf[set][pg], v[0][n], v[1][n]);
-                        else
-                            mma_f16(o[c][n], pf[set][pg], v[0][n], v[1][n]);
-                    }
+            for (int j = 0; j < 4; ++j) {
+                uint32_t s = *reinterpret_cast<const uint32_t *>(stage + j / 2 * G::kPageBytes + R::kVScale + (c * kKvPage + j % 2 * 8 + 2 * t) * 2);
+                if (edge) // (times a weight of zero it would be NaN)
+                    s &= ((s & 0x7fffu) >= kQ4BadScale ? 0u : 0xffffu) | ((s >> 16 & 0x7fffu) >= kQ4BadScale ? 0u : 0xffff0000u);
+                kv4_widen(w[j], kv4_half2(s), v[j]);
             }
-            if constexpr (G::kWide)
 #pragma unroll
-                for (int n = 0; n < 4; ++n) {
-                    if constexpr (kSplit) {
-                        o[c][n][0] += sum[n][0] + sum[n][2];
-                        o[c][n][1] += sum[n][1] + sum[n][3];
-                    } else {
+            for (int n = 0; n < 2; ++n) {
+                float sum[G::kTiles][4] = {};
+#pragma unroll
+                for (int set = G::kSets - 1; set >= 0; --set)
+#pragma unroll
+                    for (int p = 0; p < 2; ++p) {
+                        const uint32_t f[4] = {v[2 * p][2 * n], v[2 * p][2 * n + 1], v[2 * p + 1][2 * n], v[2 * p + 1][2 * n + 1]};
+#pragma unroll
+                        for (int nt = 0; nt < G::kTiles; ++nt) {
+                            if constexpr (G::kWide)
+                                mma_f16(sum[nt], f, pf[set][nt][p][0], pf[set][nt][p][1]);
+                            else
+                                mma_f16(o[c][n][nt], f, pf[set][nt][p][0], pf[set][nt][p][1]);
+                        }
+                    }
+                if constexpr (G::kWide && kPair) {
+                    o[c][n][0][0] += sum[0][0] + sum[0][1];
+                    o[c][n][0][1] += sum[0][2] + sum[0][3];
+                } else if constexpr (G::kWide) {
+#pragma unroll
+                    for (int nt = 0; nt < G::kTiles; ++nt)
 #pragma unroll
                         for (int e = 0; e < 4; ++e)
-                            o[c][n][e] += sum[n][e];
-                    }
+                            o[c][n][nt][e] += sum[nt][e];
                 }
+            }
         }
     }
     q4_copy_wait<0>();
@@ -377,19 +468,32 @@ static __global__ void __launch_bounds__(Q4RowsGeo<T, D, kSplit>::kThreads)
     float *stat = joined + G::kRows * G::kPitch, *joined_stat = stat + 2 * G::kWarps * G::kRows; // m, l by warp; of the CTA
 #pragma unroll
     for (int rr = 0; rr < G::kRPL; ++rr) {
-        l[rr] += __shfl_xor_sync(kFullWarpMask, l[rr], 1);
-        l[rr] += __shfl_xor_sync(kFullWarpMask, l[rr], 2);
-        const int r = rr * 8 + g;
-        if (t == 0) {
-            stat[warp * G::kRows + r] = m[rr];
-            stat[(G::kWarps + warp) * G::kRows + r] = l[rr];
-        }
+        const int r = kPair ? t : rr / 2 * 8 + 2 * t + rr % 2;
+        float any = 0.f;
 #pragma unroll
         for (int c = 0; c < G::kGroups; ++c) {
-            float *p = part + (warp * G::kRows + r) * G::kPitch + 32 * c + 8 * t;
-            *reinterpret_cast<float4 *>(p) = make_float4(o[c][0][2 * rr], o[c][1][2 * rr], o[c][2][2 * rr], o[c][3][2 * rr]);
-            *reinterpret_cast<float4 *>(p + 4) =
-                make_float4(o[c][0][2 * rr + 1], o[c][1][2 * rr + 1], o[c][2][2 * rr + 1], o[c][3][2 * rr + 1]);
+            float y[4];
+#pragma unroll
+            for (int n = 0; n < 2; ++n) {
+                if constexpr (kPair && G::kWide) {
+                    y[2 * n] = o[c][n][0][0], y[2 * n + 1] = o[c][n][0][1];
+                } else if constexpr (kPair) {
+                    y[2 * n] = o[c][n][0][0] + o[c][n][0][1], y[2 * n + 1] = o[c][n][0][2] + o[c][n][0][3];
+                } else {
+                    y[2 * n] = o[c][n][rr / 2][rr % 2], y[2 * n + 1] = o[c][n][rr / 2][2 + rr % 2];
+                }
+            }
+            any = max_abs_nan(max_abs_nan(any, y[0], y[1]), y[2], y[3]);
+            q4_store4(part + (warp * G::kRows + r) * G::kPitch + 32 * c + 4 * g, y);
+        }
+        // a V row that is no number, in a group of some dims, makes the whole output none
+        l[rr] = any == any ? l[rr] : any;
+#pragma unroll
+        for (int off = 4; off < 32; off <<= 1)
+            l[rr] += __shfl_xor_sync(kFullWarpMask, l[rr], off);
+        if (g == 0) {
+            stat[warp * G::kRows + r] = m[rr];
+            stat[(G::kWarps + warp) * G::kRows + r] = l[rr];
         }
     }
     __syncthreads();
@@ -458,9 +562,9 @@ template <typename... P> inline int q4_slots(void (*kernel)(P...), int threads, 
     return mine.back().slots;
 }
 
-template <typename T, int D, bool kSplit> inline void q4_rows_launch(const T *q, T *out, const TreeArgs &a, cudaStream_t stream) {
-    using G = Q4RowsGeo<T, D, kSplit>;
-    const auto kernel = q4_rows_kernel<T, D, kSplit>;
+template <typename T, int D, int kNT> inline void q4_rows_launch(const T *q, T *out, const TreeArgs &a, cudaStream_t stream) {
+    using G = Q4RowsGeo<T, D, kNT>;
+    const auto kernel = q4_rows_kernel<T, D, kNT>;
     const int most = allow_shared_bytes(kernel, G::kThreads, G::kBytes);
     const int64_t slots = q4_slots(kernel, G::kThreads, G::kBytes);
     const int64_t rows = static_cast<int64_t>(a.t.max_rows) * (a.qh / a.kvh);
@@ -476,13 +580,15 @@ template <typename T, int D, bool kSplit> inline void q4_rows_launch(const T *q,
 }
 
 template <typename T, int D> inline void q4_rows_call(const T *q, T *out, const TreeArgs &a, cudaStream_t stream) {
-    if constexpr (std::is_same_v<T, float>) {
-        if (static_cast<int64_t>(a.t.max_rows) * (a.qh / a.kvh) <= 8) {
-            q4_rows_launch<T, D, true>(q, out, a, stream);
-            return;
-        }
-    }
-    q4_rows_launch<T, D, false>(q, out, a, stream);
+    const int64_t rows = static_cast<int64_t>(a.t.max_rows) * (a.qh / a.kvh);
+    if (rows <= 4)
+        q4_rows_launch<T, D, 0>(q, out, a, stream);
+    else if (rows <= 8)
+        q4_rows_launch<T, D, 1>(q, out, a, stream);
+    else if (rows <= 16 || (D == 128 && std::is_same_v<T, float>))
+        q4_rows_launch<T, D, 2>(q, out, a, stream);
+    else
+        q4_rows_launch<T, D, 4>(q, out, a, stream);
 }
 
 } // namespace opworks::detail
