@@ -14,8 +14,25 @@
 #include "tree_attention.cuh"
 #include "kv4.cuh"
 #include "tree_attention_q4_rows.cuh"
+#include "tree_attention_q4_tiles.cuh"
 
 namespace opworks {
+namespace detail {
+
+template <typename T, int D> inline void q4_call(const T *q, T *out, const TreeArgs &a, cudaStream_t stream) {
+    constexpr bool kHasTiles = D == 64 || std::is_same_v<T, __nv_bfloat16>;
+    constexpr int kFrom = 64; // rows of a kv head
+    const bool many = static_cast<int64_t>(a.t.rows) * (a.qh / a.kvh) > static_cast<int64_t>(kFrom) * a.t.batch;
+    if constexpr (kHasTiles)
+        if (many) {
+            q4_tiles_call<T, D>(q, out, a, stream);
+            return;
+        }
+    q4_rows_call<T, D>(q, out, a, stream);
+}
+
+} // namespace detail
+
 namespace ops {
 
 // Over the 4-bit pool [blocks][kv_heads][record] of ops/kv4.cuh. q row r, head h at
@@ -28,7 +45,7 @@ inline void tree_attention_q4(const T *q, int64_t q_stride, const uint8_t *pool,
     if (t.batch == 0 || t.max_rows == 0)
         return;
     const TreeArgs a{t, pool, nullptr, q_heads, kv_heads, scale * kLog2e, q_stride, out_stride};
-    head_dim == 64 ? q4_rows_call<T, 64>(q, out, a, stream) : q4_rows_call<T, 128>(q, out, a, stream);
+    head_dim == 64 ? q4_call<T, 64>(q, out, a, stream) : q4_call<T, 128>(q, out, a, stream);
 }
 
 } // namespace ops

@@ -21,8 +21,7 @@
 // the product sums over.
 //
 // fp32 rows are two fp16 terms, and so are their weights. Up to 4 rows have two
-// columns each, which are the two terms (bf16 rows: of the weights only, which
-// costs nothing); above that fp32 rows take a product for each term, in one
+// columns each, which are the two terms (bf16 rows: one is empty); above that fp32 rows take a product for each term, in one
 // accumulator. The tensor cores cut an accumulator off at every step, so fp32 rows
 // add up O outside of them, rounded, once a step.
 
@@ -39,6 +38,7 @@ template <typename T, int D, int kNT> struct Q4RowsGeo {
     static constexpr bool kWide = std::is_same_v<T, float>, kPair = kNT == 0;
     static constexpr int kTiles = kPair ? 1 : kNT;
     static constexpr int kGroups = D / kKv4Group;
+    static constexpr float kLift = kWide ? 6.f : 0.f; // see kQ4Top
     static constexpr int kRows = kPair ? 4 : 8 * kNT;
     static constexpr int kRPL = kPair ? 1 : 2 * kNT;         // rows that a lane has scores of
     static constexpr int kSets = kWide && !kPair ? 2 : 1;    // products of a k step
@@ -46,21 +46,27 @@ template <typename T, int D, int kNT> struct Q4RowsGeo {
     // (the sum is 3 times as large as what is left) and two registers a group and tile
     static constexpr bool kSigned = kWide || kNT > 1;
     static constexpr bool kQShared = kSets * kTiles * D > 256; // queries in shared memory, not in registers
-    static constexpr int kWarps = 4, kThreads = 32 * kWarps;
-    static constexpr int kStepPages = 2, kStepKeys = kStepPages * kKvPage;
-    static constexpr int kStages = 3;
+    static constexpr int kWarps = kNT <= 2 ? 8 : 4, kThreads = 32 * kWarps;
+    // a step: 64 keys where registers and shared memory have room, since what is done once a
+    // step is a third of the instructions of 32
+    static constexpr int kPairs = D == 64 && kNT <= 1 ? 2 : 1; // of pages
+    static constexpr int kStepPages = 2 * kPairs, kStepKeys = kStepPages * kKvPage;
+    static constexpr int kStages = kPairs == 2 ? 2 : 3;
     static constexpr int kPageBytes = Kv4Record<D>::kBytes, kStage = kStepPages * kPageBytes;
     static constexpr int kQBytes = kQShared ? kSets * kTiles * kGroups * 2 * 32 * 8 : 0;
-    static constexpr int kRing = kWarps * kStages * kStage;
+    static constexpr int kRing = kStages * kStage; // of a warp
     static constexpr int kPitch = D + 4; // floats of a row of partial sums
     // O of the warps, then of the CTA; m and l of the warps, then of the CTA
     static constexpr int kJoin = 4 * ((kWarps + 1) * kRows * kPitch + 2 * (kWarps + 1) * kRows);
-    static constexpr int kBytes = kQBytes + kRing > kJoin ? kQBytes + kRing : kJoin;
+    static constexpr int kLoop = kQBytes + kWarps * kRing;
+    static constexpr int kBytes = kLoop > kJoin ? kLoop : kJoin;
 };
 
-// Scores may pass a row's reference by this many log2 units before it is raised:
-// weights are 2^(x - reference), 2^10 for the largest score when it is set.
-constexpr float kQ4Top = 14.f, kQ4Lift = 10.f;
+// Weights are 2^(x - reference). Scores may pass a row's reference by kQ4Top log2
+// units before it is raised, to kLift below the largest: fp16 keeps steps of 2^-24, so
+// 2^-25 of the largest weight is what a bf16 row's may be off by, 2^-31 an fp32 row's.
+// (Raised to 8 below it, prompts did so for some row of a warp in every few tiles.)
+constexpr float kQ4Top = 15.f;
 constexpr float kQ4None = -3.4028235e38f; // reference of a row that has seen nothing yet
 constexpr uint32_t kQ4BadScale = 0x7000u; // fp16 8,192: above every scale that is written; junk, infinity, NaN
 
@@ -96,10 +102,10 @@ __device__ __forceinline__ uint32_t q4_term(float &x, float &y) {
     x -= f.x, y -= f.y;
     return h;
 }
-// both terms of x as a pair
-__device__ __forceinline__ uint32_t q4_terms(float x) {
-    const __half hi = __float2half_rn(x);
-    return kv4_bits(__halves2half2(hi, __float2half_rn(x - __half2float(hi))));
+// both terms of x, and of y, as pairs
+__device__ __forceinline__ void q4_terms(float x, float y, uint32_t &px, uint32_t &py) {
+    const uint32_t hi = q4_term(x, y), lo = half2_rn(x, y);
+    px = __byte_perm(hi, lo, 0x5410), py = __byte_perm(hi, lo, 0x7632);
 }
 
 __device__ __forceinline__ float4 peer_load4(const float *p, int rank) {
@@ -132,45 +138,78 @@ __device__ __forceinline__ float q4_row_scale(float top, float scale_log2, float
     return up;
 }
 
+// The span of the sequence with the `order`-th most work (the longest context, equal
+// ones by index): CTAs come longest first, and those that share an SM differ. Every
+// thread of the block calls it; `room` is shared memory for 4 ints and one more a
+// sequence, batch <= the block's threads.
+__device__ __forceinline__ TreeSpan q4_span_by_work(const TreeBatch &t, int order, int *room) {
+    const int tid = threadIdx.x;
+    TreeSpan mine{};
+    if (tid < t.batch) {
+        mine = TreeSpan(t, tid);
+        room[4 + tid] = mine.n > 0 ? mine.ctx : -1;
+    }
+    __syncthreads();
+    if (tid < t.batch) {
+        const int work = room[4 + tid];
+        int before = 0;
+        for (int i = 0; i < t.batch; ++i)
+            before += room[4 + i] > work || (room[4 + i] == work && i < tid) ? 1 : 0;
+        if (before == order)
+            room[0] = mine.b, room[1] = mine.row0, room[2] = mine.n, room[3] = mine.ctx;
+    }
+    __syncthreads();
+    TreeSpan s{};
+    s.b = room[0], s.row0 = room[1], s.n = room[2], s.ctx = room[3];
+    s.set_keys(t);
+    __syncthreads(); // `room` may lie where copies go next
+    return s;
+}
+
 template <typename T, int D, int kNT>
 static __global__ void __launch_bounds__(Q4RowsGeo<T, D, kNT>::kThreads)
-    q4_rows_kernel(const T *__restrict__ q, T *__restrict__ out, TreeArgs a, int groups, int splits, bool sorted) {
+    q4_rows_kernel(const T *__restrict__ q, T *__restrict__ out, TreeArgs a, int rep, int splits, bool sorted) {
     using G = Q4RowsGeo<T, D, kNT>;
     using R = Kv4Record<D>;
     constexpr bool kPair = G::kPair;
     extern __shared__ __align__(128) uint8_t q4_smem[];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
-    const int rank = blockIdx.x % splits, unit = blockIdx.x / splits;
-    const int group = unit % groups, h = unit / groups, rep = a.qh / a.kvh;
+    constexpr int threads = G::kThreads, warps = G::kWarps;
+    const int h = blockIdx.y;
+    int rank = blockIdx.x, group = 0; // groups of rows side by side, the CTAs of a cluster each
+    if (gridDim.x != splits)
+        group = rank / splits, rank -= group * splits;
     pdl_trigger();
     pdl_wait();
-    const int b = sorted ? sequence_by_work(a.t, blockIdx.y, reinterpret_cast<int *>(q4_smem)) : blockIdx.y;
-    const TreeSpan span(a.t, b);
-    const int row_base = group * G::kRows, rows = span.n * rep;
+    const TreeSpan span = sorted ? q4_span_by_work(a.t, blockIdx.z, reinterpret_cast<int *>(q4_smem)) : TreeSpan(a.t, blockIdx.z);
+    const int b = span.b, row_base = group * G::kRows, rows = span.n * rep;
     if (row_base >= rows)
         return; // the whole cluster
     int keys = span.keys;
     if (a.t.mask == nullptr) // a chain: nothing after the tile's last node is seen
         keys = min(keys, span.ctx + (min(row_base + G::kRows, rows) + rep - 1) / rep);
     const int steps = (keys + G::kStepKeys - 1) / G::kStepKeys;
-    const int first = rank * G::kWarps + warp, stride = splits * G::kWarps;
+    const int first = rank * warps + warp, stride = splits * warps;
     const int mine = steps > first ? (steps - first + stride - 1) / stride : 0;
+
+    const auto node_of = [&](int r) { return span.n == 1 ? 0 : r / rep; };
 
     // ---- copies
     const int *table = a.t.block_table + static_cast<int64_t>(b) * a.t.table_stride;
     const int pages = (keys + kKvPage - 1) / kKvPage;
-    uint8_t *ring = q4_smem + G::kQBytes + warp * G::kStages * G::kStage;
-    int ids = 0; // a lane has the block of one page of the next 16 steps
+    uint8_t *ring = q4_smem + G::kQBytes + warp * G::kRing;
+    int ids = 0; // a lane has the block of one page of the next steps
     const auto fetch = [&](int i, int to) {
+        constexpr int kAhead = 32 / G::kStepPages; // steps whose pages are looked up at once
         if (i < mine) {
-            if (i % 16 == 0) {
-                const int page = (first + (i + lane / 2) * stride) * G::kStepPages + lane % 2;
-                ids = i + lane / 2 < mine && page < pages ? table[page] : -1;
+            if (i % kAhead == 0) {
+                const int s = i + lane / G::kStepPages, page = (first + s * stride) * G::kStepPages + lane % G::kStepPages;
+                ids = s < mine && page < pages ? table[page] : -1;
             }
             const uint32_t dst = sm100::smem_u32(ring + to * G::kStage);
 #pragma unroll
             for (int pg = 0; pg < G::kStepPages; ++pg) {
-                const int64_t id = __shfl_sync(kFullWarpMask, ids, i % 16 * 2 + pg);
+                const int64_t id = __shfl_sync(kFullWarpMask, ids, i % kAhead * G::kStepPages + pg);
                 if (id < 0)
                     continue; // after the last page: what the ring holds is masked
                 const uint8_t *src = static_cast<const uint8_t *>(a.k) + (id * a.kvh + h) * R::kBytes;
@@ -194,13 +233,13 @@ static __global__ void __launch_bounds__(Q4RowsGeo<T, D, kNT>::kThreads)
     float factor[G::kRPL];
 #pragma unroll
     for (int nt = 0; nt < G::kTiles; ++nt) {
-        const int r = row_base + (kPair ? g / 2 : nt * 8 + g);
+        const int r = row_base + (kPair ? g / 2 : nt * 8 + g), node = node_of(r);
         float x[G::kGroups][8];
         float top = 0.f;
 #pragma unroll
         for (int c = 0; c < G::kGroups; ++c) {
             if (r < rows) {
-                const T *src = q + static_cast<int64_t>(span.row0 + r / rep) * a.q_stride + static_cast<int64_t>(h * rep + r % rep) * D + 32 * c + 8 * t;
+                const T *src = q + static_cast<int64_t>(span.row0 + node) * a.q_stride + static_cast<int64_t>(h * rep + r - node * rep) * D + 32 * c + 8 * t;
 #pragma unroll
                 for (int i = 0; i < 8 / KvVec<T>::kN; ++i) {
                     float y[KvVec<T>::kN];
@@ -288,60 +327,63 @@ static __global__ void __launch_bounds__(Q4RowsGeo<T, D, kNT>::kThreads)
         const bool edge = key0 + G::kStepKeys > span.ctx;
 
         // ---- scores: of key 16 p + 8 e + g at place 2 p + e
-        float x[G::kRPL][4] = {};
+        float x[G::kRPL][2 * G::kStepPages] = {};
 #pragma unroll
-        for (int c = 0; c < G::kGroups; ++c) {
-            uint32_t w[4], k[4][4];
-            q4_ldmatrix<false>(stage_at + c * 256, w);
+        for (int pp = 0; pp < G::kPairs; ++pp)
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-                kv4_integers<G::kSigned>(w[j], k[j]);
-            float sum[2][G::kTiles][4];
+            for (int c = 0; c < G::kGroups; ++c) {
+                uint32_t w[4], k[4][4];
+                q4_ldmatrix<false>(stage_at + pp * 2 * G::kPageBytes + c * 256, w);
 #pragma unroll
-            for (int p = 0; p < 2; ++p)
+                for (int j = 0; j < 4; ++j)
+                    kv4_integers<G::kSigned>(w[j], k[j]);
+                float sum[2][G::kTiles][4];
 #pragma unroll
-                for (int nt = 0; nt < G::kTiles; ++nt)
+                for (int p = 0; p < 2; ++p)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        sum[p][nt][e] = G::kSigned ? 0.f : start[G::kSigned ? 0 : c][e & 1];
+                    for (int nt = 0; nt < G::kTiles; ++nt)
 #pragma unroll
-            for (int set = G::kSets - 1; set >= 0; --set)
+                        for (int e = 0; e < 4; ++e)
+                            sum[p][nt][e] = G::kSigned ? 0.f : start[G::kSigned ? 0 : c][e & 1];
 #pragma unroll
-                for (int u = 0; u < 2; ++u)
+                for (int set = G::kSets - 1; set >= 0; --set)
 #pragma unroll
-                    for (int nt = 0; nt < G::kTiles; ++nt) {
-                        uint32_t b0, b1;
-                        if constexpr (G::kQShared) {
-                            const uint2 f = q_shared[(((set * G::kTiles + nt) * G::kGroups + c) * 2 + u) * 32 + lane];
-                            b0 = f.x, b1 = f.y;
-                        } else {
-                            b0 = qf[set][nt][G::kQShared ? 0 : c][u][0], b1 = qf[set][nt][G::kQShared ? 0 : c][u][1];
+                    for (int u = 0; u < 2; ++u)
+#pragma unroll
+                        for (int nt = 0; nt < G::kTiles; ++nt) {
+                            uint32_t b0, b1;
+                            if constexpr (G::kQShared) {
+                                const uint2 f = q_shared[(((set * G::kTiles + nt) * G::kGroups + c) * 2 + u) * 32 + lane];
+                                b0 = f.x, b1 = f.y;
+                            } else {
+                                b0 = qf[set][nt][G::kQShared ? 0 : c][u][0], b1 = qf[set][nt][G::kQShared ? 0 : c][u][1];
+                            }
+#pragma unroll
+                            for (int p = 0; p < 2; ++p) {
+                                const uint32_t f[4] = {k[2 * p][2 * u], k[2 * p + 1][2 * u], k[2 * p][2 * u + 1], k[2 * p + 1][2 * u + 1]};
+                                mma_f16(sum[p][nt], f, b0, b1);
+                            }
                         }
 #pragma unroll
-                        for (int p = 0; p < 2; ++p) {
-                            const uint32_t f[4] = {k[2 * p][2 * u], k[2 * p + 1][2 * u], k[2 * p][2 * u + 1], k[2 * p + 1][2 * u + 1]};
-                            mma_f16(sum[p][nt], f, b0, b1);
-                        }
+                for (int p = 0; p < 2; ++p)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const float s = __half2float(
+                            *reinterpret_cast<const __half *>(stage + (2 * pp + p) * G::kPageBytes + R::kKScale + (c * kKvPage + e * 8 + g) * 2));
+#pragma unroll
+                        for (int rr = 0; rr < G::kRPL; ++rr)
+                            x[rr][4 * pp + 2 * p + e] += s * (kPair ? sum[p][0][2 * e] + sum[p][0][2 * e + 1] : sum[p][rr / 2][2 * e + rr % 2]);
                     }
-#pragma unroll
-            for (int p = 0; p < 2; ++p)
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    const float s = __half2float(*reinterpret_cast<const __half *>(stage + p * G::kPageBytes + R::kKScale + (c * kKvPage + e * 8 + g) * 2));
-#pragma unroll
-                    for (int rr = 0; rr < G::kRPL; ++rr)
-                        x[rr][2 * p + e] += s * (kPair ? sum[p][0][2 * e] + sum[p][0][2 * e + 1] : sum[p][rr / 2][2 * e + rr % 2]);
-                }
-        }
+            }
 #pragma unroll
         for (int rr = 0; rr < G::kRPL; ++rr)
 #pragma unroll
-            for (int n = 0; n < 4; ++n)
+            for (int n = 0; n < 2 * G::kStepPages; ++n)
                 x[rr][n] *= factor[rr];
         if (edge) {
             uint32_t bad = 0; // keys whose V is no number: a row that sees one gets NaN, the others nothing of it
 #pragma unroll
-            for (int n = 0; n < 4; ++n)
+            for (int n = 0; n < 2 * G::kStepPages; ++n)
 #pragma unroll
                 for (int c = 0; c < G::kGroups; ++c) {
                     const uint32_t v = *reinterpret_cast<const uint16_t *>(stage + n / 2 * G::kPageBytes + R::kVScale + (c * kKvPage + n % 2 * 8 + g) * 2);
@@ -350,15 +392,18 @@ static __global__ void __launch_bounds__(Q4RowsGeo<T, D, kNT>::kThreads)
 #pragma unroll
             for (int rr = 0; rr < G::kRPL; ++rr) {
                 const int r = row_base + (kPair ? t : rr / 2 * 8 + 2 * t + rr % 2);
-                uint32_t seen = 0;
-                if (r < rows)
-                    seen = tree_sees32(a.t, span.row0 + r / rep, r / rep, key0 - span.ctx, keys - span.ctx);
 #pragma unroll
-                for (int n = 0; n < 4; ++n) {
-                    if (bad >> n & 1u)
-                        x[rr][n] = __uint_as_float(0x7fc00000u);
-                    if (!(seen >> (n * 8 + g) & 1u))
-                        x[rr][n] = kNegInf;
+                for (int pp = 0; pp < G::kPairs; ++pp) {
+                    uint32_t seen = 0;
+                    if (r < rows)
+                        seen = tree_sees32(a.t, span.row0 + node_of(r), node_of(r), key0 + 32 * pp - span.ctx, keys - span.ctx);
+#pragma unroll
+                    for (int n = 0; n < 4; ++n) {
+                        if (bad >> (4 * pp + n) & 1u)
+                            x[rr][4 * pp + n] = __uint_as_float(0x7fc00000u);
+                        if (!(seen >> (n * 8 + g) & 1u))
+                            x[rr][4 * pp + n] = kNegInf;
+                    }
                 }
             }
         }
@@ -368,7 +413,10 @@ static __global__ void __launch_bounds__(Q4RowsGeo<T, D, kNT>::kThreads)
         float top[G::kRPL];
 #pragma unroll
         for (int rr = 0; rr < G::kRPL; ++rr) {
-            top[rr] = fmaxf(fmaxf(x[rr][0], x[rr][1]), fmaxf(x[rr][2], x[rr][3]));
+            top[rr] = x[rr][0];
+#pragma unroll
+            for (int n = 1; n < 2 * G::kStepPages; ++n)
+                top[rr] = fmaxf(top[rr], x[rr][n]);
             raise |= top[rr] - m[rr] > kQ4Top;
         }
         if (__any_sync(kFullWarpMask, raise)) {
@@ -379,7 +427,7 @@ static __global__ void __launch_bounds__(Q4RowsGeo<T, D, kNT>::kThreads)
                     top[rr] = fmaxf(top[rr], __shfl_xor_sync(kFullWarpMask, top[rr], off));
                 if (top[rr] - m[rr] > kQ4Top) {
                     // below scores that are large a lift would be lost in the rounding, or grow by it
-                    const float up = fabsf(top[rr]) < 0x1p20f ? top[rr] - kQ4Lift : top[rr];
+                    const float up = fabsf(top[rr]) < 0x1p20f ? top[rr] - G::kLift : top[rr];
                     const float fix = exp2_approx(m[rr] - up);
                     m[rr] = up;
                     l[rr] *= fix;
@@ -397,13 +445,20 @@ static __global__ void __launch_bounds__(Q4RowsGeo<T, D, kNT>::kThreads)
                 }
             }
         }
-        uint32_t pf[G::kSets][G::kTiles][2][2]; // of page p: keys 2t, 2t + 1, and 8 more, of column g
+        uint32_t pf[G::kSets][G::kTiles][G::kStepPages][2]; // of page p: keys 2t, 2t + 1, and 8 more, of column g
 #pragma unroll
-        for (int n = 0; n < 4; ++n) {
+        for (int n = 0; n < 2 * G::kStepPages; ++n) {
             if constexpr (kPair) {
-                const float p = exp2_approx(x[0][n] - m[0]);
-                l[0] += p;
-                pf[0][0][n / 2][n % 2] = q4_transposed(q4_terms(p));
+                if (n % 2)
+                    continue;
+                const float p0 = exp2_approx(x[0][n] - m[0]), p1 = exp2_approx(x[0][n + 1] - m[0]);
+                l[0] += p0 + p1;
+                uint32_t t0, t1;
+                if constexpr (G::kWide)
+                    q4_terms(p0, p1, t0, t1);
+                else
+                    t0 = half2_rn(p0, 0.f), t1 = half2_rn(p1, 0.f);
+                pf[0][0][n / 2][0] = q4_transposed(t0), pf[0][0][n / 2][1] = q4_transposed(t1);
             } else {
 #pragma unroll
                 for (int nt = 0; nt < G::kTiles; ++nt) {
@@ -422,14 +477,19 @@ static __global__ void __launch_bounds__(Q4RowsGeo<T, D, kNT>::kThreads)
         // ---- output
 #pragma unroll
         for (int c = 0; c < G::kGroups; ++c) {
-            uint32_t w[4], v[4][4];
-            q4_ldmatrix<true>(stage_at + R::kCodes + c * 256, w);
+            uint32_t v[2 * G::kStepPages][4];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                uint32_t s = *reinterpret_cast<const uint32_t *>(stage + j / 2 * G::kPageBytes + R::kVScale + (c * kKvPage + j % 2 * 8 + 2 * t) * 2);
-                if (edge) // (times a weight of zero it would be NaN)
-                    s &= ((s & 0x7fffu) >= kQ4BadScale ? 0u : 0xffffu) | ((s >> 16 & 0x7fffu) >= kQ4BadScale ? 0u : 0xffff0000u);
-                kv4_widen(w[j], kv4_half2(s), v[j]);
+            for (int pp = 0; pp < G::kPairs; ++pp) {
+                uint32_t w[4];
+                q4_ldmatrix<true>(stage_at + pp * 2 * G::kPageBytes + R::kCodes + c * 256, w);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    uint32_t s = *reinterpret_cast<const uint32_t *>(stage + (2 * pp + j / 2) * G::kPageBytes + R::kVScale +
+                                                                     (c * kKvPage + j % 2 * 8 + 2 * t) * 2);
+                    if (edge) // (times a weight of zero it would be NaN)
+                        s &= ((s & 0x7fffu) >= kQ4BadScale ? 0u : 0xffffu) | ((s >> 16 & 0x7fffu) >= kQ4BadScale ? 0u : 0xffff0000u);
+                    kv4_widen(w[j], kv4_half2(s), v[4 * pp + j]);
+                }
             }
 #pragma unroll
             for (int n = 0; n < 2; ++n) {
@@ -437,7 +497,7 @@ static __global__ void __launch_bounds__(Q4RowsGeo<T, D, kNT>::kThreads)
 #pragma unroll
                 for (int set = G::kSets - 1; set >= 0; --set)
 #pragma unroll
-                    for (int p = 0; p < 2; ++p) {
+                    for (int p = 0; p < G::kStepPages; ++p) {
                         const uint32_t f[4] = {v[2 * p][2 * n], v[2 * p][2 * n + 1], v[2 * p + 1][2 * n], v[2 * p + 1][2 * n + 1]};
 #pragma unroll
                         for (int nt = 0; nt < G::kTiles; ++nt) {
@@ -464,8 +524,8 @@ static __global__ void __launch_bounds__(Q4RowsGeo<T, D, kNT>::kThreads)
 
     // ---- joining: the warps, then the cluster
     __syncthreads(); // the rings are done with
-    float *part = reinterpret_cast<float *>(q4_smem), *joined = part + G::kWarps * G::kRows * G::kPitch;
-    float *stat = joined + G::kRows * G::kPitch, *joined_stat = stat + 2 * G::kWarps * G::kRows; // m, l by warp; of the CTA
+    float *part = reinterpret_cast<float *>(q4_smem), *joined = part + warps * G::kRows * G::kPitch;
+    float *stat = joined + G::kRows * G::kPitch, *joined_stat = stat + 2 * warps * G::kRows; // m, l by warp; of the CTA
 #pragma unroll
     for (int rr = 0; rr < G::kRPL; ++rr) {
         const int r = kPair ? t : rr / 2 * 8 + 2 * t + rr % 2;
@@ -493,28 +553,26 @@ static __global__ void __launch_bounds__(Q4RowsGeo<T, D, kNT>::kThreads)
             l[rr] += __shfl_xor_sync(kFullWarpMask, l[rr], off);
         if (g == 0) {
             stat[warp * G::kRows + r] = m[rr];
-            stat[(G::kWarps + warp) * G::kRows + r] = l[rr];
+            stat[(warps + warp) * G::kRows + r] = l[rr];
         }
     }
     __syncthreads();
     const int live = min(G::kRows, rows - row_base);
     const auto put = [&](int r, int d, float L, const float (&y)[4]) {
-        const int row = row_base + r;
+        const int row = row_base + r, node = node_of(row);
         const float inv = L == 0.f ? 0.f : 1.f / L;
         const float z[4] = {L == 0.f ? 0.f : y[0] * inv, L == 0.f ? 0.f : y[1] * inv, L == 0.f ? 0.f : y[2] * inv, L == 0.f ? 0.f : y[3] * inv};
-        q4_store4(out + static_cast<int64_t>(span.row0 + row / rep) * a.out_stride + static_cast<int64_t>(h * rep + row % rep) * D + d, z);
+        q4_store4(out + static_cast<int64_t>(span.row0 + node) * a.out_stride + static_cast<int64_t>(h * rep + row - node * rep) * D + d, z);
     };
-    for (int i = tid; i < live * (D / 4); i += G::kThreads) {
+    for (int i = tid; i < live * (D / 4); i += threads) {
         const int r = i / (D / 4), d = i % (D / 4) * 4;
         float M = kQ4None, L = 0.f, y[4] = {};
-#pragma unroll
-        for (int w = 0; w < G::kWarps; ++w)
+        for (int w = 0; w < warps; ++w)
             M = fmaxf(M, stat[w * G::kRows + r]);
-#pragma unroll
-        for (int w = 0; w < G::kWarps; ++w) {
+        for (int w = 0; w < warps; ++w) {
             const float f = exp2_approx(stat[w * G::kRows + r] - M);
             const float4 p = *reinterpret_cast<const float4 *>(part + (w * G::kRows + r) * G::kPitch + d);
-            L += f * stat[(G::kWarps + w) * G::kRows + r];
+            L += f * stat[(warps + w) * G::kRows + r];
             y[0] += f * p.x, y[1] += f * p.y, y[2] += f * p.z, y[3] += f * p.w;
         }
         if (splits == 1) {
@@ -529,7 +587,7 @@ static __global__ void __launch_bounds__(Q4RowsGeo<T, D, kNT>::kThreads)
         return;
     __syncthreads();
     cluster_sync_all();
-    for (int i = rank * G::kThreads + tid; i < live * (D / 4); i += splits * G::kThreads) {
+    for (int i = rank * threads + tid; i < live * (D / 4); i += splits * threads) {
         const int r = i / (D / 4), d = i % (D / 4) * 4;
         float M = kQ4None, L = 0.f, y[4] = {};
         for (int c = 0; c < splits; ++c)
@@ -545,7 +603,7 @@ static __global__ void __launch_bounds__(Q4RowsGeo<T, D, kNT>::kThreads)
     cluster_sync_all(); // peers read this CTA's shared memory until here
 }
 
-// CTAs of a kernel that run at once on the current device, asked once.
+// CTAs of a kernel that run at once on the current device. Asked once.
 template <typename... P> inline int q4_slots(void (*kernel)(P...), int threads, int bytes) {
     struct Known {
         const void *kernel;
@@ -566,17 +624,21 @@ template <typename T, int D, int kNT> inline void q4_rows_launch(const T *q, T *
     using G = Q4RowsGeo<T, D, kNT>;
     const auto kernel = q4_rows_kernel<T, D, kNT>;
     const int most = allow_shared_bytes(kernel, G::kThreads, G::kBytes);
-    const int64_t slots = q4_slots(kernel, G::kThreads, G::kBytes);
+    const int64_t slots = q4_slots(kernel, G::kThreads, G::kBytes), sms = device_facts().sm_count;
     const int64_t rows = static_cast<int64_t>(a.t.max_rows) * (a.qh / a.kvh);
-    const int64_t groups = (rows + G::kRows - 1) / G::kRows, units = groups * a.kvh, all = units * a.t.batch;
-    const int64_t keys = static_cast<int64_t>(a.t.max_ctx) + a.t.max_rows;
-    // As many splits as all CTAs still run at once, and as leave each warp two steps or more.
-    const int64_t cap = std::min<int64_t>(most, keys / (2 * G::kStepKeys * G::kWarps));
-    const int splits = static_cast<int>(std::max<int64_t>(1, std::min(cap, slots / all)));
-    require(units * splits <= 0x7fffffff, "tree attention: too many rows for one call");
-    const bool sort = a.t.batch > 1 && a.t.batch < G::kThreads && all * splits > slots / 2;
-    launch_ex_cluster(kernel, dim3(static_cast<unsigned>(units * splits), a.t.batch), dim3(splits), dim3(G::kThreads), G::kBytes, stream,
-                      q, out, a, static_cast<int>(groups), splits, sort);
+    const int64_t groups = (rows + G::kRows - 1) / G::kRows, all = groups * a.kvh * a.t.batch;
+    const int64_t keys = static_cast<int64_t>(a.t.max_ctx) + a.t.max_rows, steps = (keys + G::kStepKeys - 1) / G::kStepKeys;
+    // A cluster costs 2 us and more (32 sequences x 8 heads with nothing to do: 5.3 us, 7 with
+    // clusters of two), so keys are split only where there are SMs to spare or each warp has 16
+    // steps and more; then into a third more CTAs than run at once, since sequences differ in
+    // length (12 x 8 of 32,000 tokens, 296 at once: 99.6 us with 3 splits, 90.4 with 4).
+    const bool split = all < sms || steps >= 16 * G::kWarps;
+    const int64_t cap = std::min<int64_t>(most, steps / (2 * G::kWarps));
+    int splits = split ? static_cast<int>(std::max<int64_t>(1, std::min(cap, slots * 4 / 3 / all))) : 1;
+    require(groups * splits <= 0x7fffffff, "tree attention: too many rows for one call");
+    const bool sort = a.t.batch > 1 && a.t.batch <= G::kThreads && all * splits > sms;
+    launch_ex_cluster(kernel, dim3(static_cast<unsigned>(groups * splits), a.kvh, a.t.batch), dim3(splits), dim3(G::kThreads), G::kBytes, stream,
+                      q, out, a, a.qh / a.kvh, splits, sort);
 }
 
 template <typename T, int D> inline void q4_rows_call(const T *q, T *out, const TreeArgs &a, cudaStream_t stream) {
