@@ -327,36 +327,41 @@ static __global__ void __launch_bounds__(kTileThreads, 1)
         // ---- softmax warps. First Q: 8 dims a lane, scaled to 2^14 .. 2^15 and split into
         // terms. The sign of the scale goes with it, so that larger products are larger scores.
         constexpr int kLanes = D / 8, kPer = 32 / kLanes, kAll = G::kRows / (8 * kPer); // rows of a warp at a time; times
-        constexpr int kBatch = kAll < 8 ? kAll : 8;                                    // in flight
+        constexpr int kBatch = kAll < 16 / (8 / KvVec<T>::kN) ? kAll : 16 / (8 / KvVec<T>::kN); // in flight
         static_assert(G::kRows % (8 * kPer * kBatch) == 0, "rows of the tiles");
 #pragma unroll 1
         for (int r0 = warp * kPer; r0 < G::kRows; r0 += 8 * kPer * kBatch) {
-            float x[kBatch][8];
+            constexpr int kVecs = 8 / KvVec<T>::kN;
+            uint4 raw[kBatch][kVecs];
 #pragma unroll
             for (int n = 0; n < kBatch; ++n) {
                 const int row = row_base + r0 + 8 * kPer * n + lane / kLanes, node = row / rep;
 #pragma unroll
-                for (int e = 0; e < 8; ++e)
-                    x[n][e] = 0.f;
+                for (int k = 0; k < kVecs; ++k)
+                    raw[n][k] = make_uint4(0, 0, 0, 0);
                 if (row < rows) {
                     const T *src = q + static_cast<int64_t>(span.row0 + node) * a.q_stride + static_cast<int64_t>(h * rep + row - node * rep) * D + lane % kLanes * 8;
 #pragma unroll
-                    for (int e = 0; e < 8; e += KvVec<T>::kN) {
-                        float y[KvVec<T>::kN];
-                        KvVec<T>::unpack(__ldg(reinterpret_cast<const uint4 *>(src + e)), y);
-#pragma unroll
-                        for (int k = 0; k < KvVec<T>::kN; ++k)
-                            x[n][e + k] = y[k];
-                    }
+                    for (int k = 0; k < kVecs; ++k)
+                        raw[n][k] = __ldg(reinterpret_cast<const uint4 *>(src) + k);
                 }
             }
 #pragma unroll
             for (int n = 0; n < kBatch; ++n) {
                 const int r = r0 + 8 * kPer * n + lane / kLanes;
+                float x[8];
+#pragma unroll
+                for (int k = 0; k < kVecs; ++k) {
+                    float y[KvVec<T>::kN];
+                    KvVec<T>::unpack(raw[n][k], y);
+#pragma unroll
+                    for (int e = 0; e < KvVec<T>::kN; ++e)
+                        x[k * KvVec<T>::kN + e] = y[e];
+                }
                 float top = 0.f;
 #pragma unroll
                 for (int e = 0; e < 8; e += 2)
-                    top = max_abs_nan(top, x[n][e], x[n][e + 1]);
+                    top = max_abs_nan(top, x[e], x[e + 1]);
 #pragma unroll
                 for (int off = 1; off < kLanes; off <<= 1)
                     top = max_abs_nan(top, __shfl_xor_sync(kFullWarpMask, top, off), 0.f);
@@ -366,7 +371,7 @@ static __global__ void __launch_bounds__(kTileThreads, 1)
                 uint32_t hi[4], lo[4];
 #pragma unroll
                 for (int k = 0; k < 4; ++k) { // pairs (k, k + 4), as K's
-                    float u = x[n][k] * up, v = x[n][k + 4] * up;
+                    float u = x[k] * up, v = x[k + 4] * up;
                     hi[k] = q4_term(u, v);
                     lo[k] = half2_rn(u, v);
                 }
@@ -622,20 +627,13 @@ static __global__ void __launch_bounds__(kTileThreads, 1)
                     o[k] = 0;
             }
         };
-        // a V row that is no number, in a group of some dims, makes the whole output none
-        float odd = 0.f;
-#pragma unroll 1
-        for (int c = 0; c < D; c += 16) {
-            uint32_t o[16];
-            load(c, o);
-#pragma unroll
-            for (int k = 0; k < 16; k += 2)
-                odd = max_abs_nan(odd, __uint_as_float(o[k]), __uint_as_float(o[k + 1]));
-        }
-        l = odd == odd ? l : odd;
+        // Rows leave through shared memory, which is free now: finished, and written out 16 bytes a
+        // lane along the row, or as they are, to be joined.
         const float inv = l == 0.f ? 0.f : 1.f / l;
-        T *dst = out + static_cast<int64_t>(span.row0 + node) * a.out_stride + static_cast<int64_t>(h * rep + row - node * rep) * D;
+        constexpr int kOutPitch = D * static_cast<int>(sizeof(T)) + 16; // bytes
+        uint8_t *done = smem + (stream * 128 + r) * kOutPitch;
         float *part = reinterpret_cast<float *>(smem) + (stream * 128 + r) * G::kPitch;
+        float odd = 0.f;
 #pragma unroll 1
         for (int c = 0; c < D; c += 16) {
             uint32_t o[16];
@@ -646,18 +644,42 @@ static __global__ void __launch_bounds__(kTileThreads, 1)
 #pragma unroll
                 for (int n = 0; n < 8; ++n)
                     y[n] = __uint_as_float(o[k + n % 4 * 2 + n / 4]);
-                if (direct) {
-                    if (live)
 #pragma unroll
-                        for (int n = 0; n < 8; n += 4) {
-                            const float z[4] = {l == 0.f ? 0.f : y[n] * inv, l == 0.f ? 0.f : y[n + 1] * inv, l == 0.f ? 0.f : y[n + 2] * inv,
-                                                l == 0.f ? 0.f : y[n + 3] * inv};
-                            q4_store4(dst + c + k + n, z);
-                        }
+                for (int n = 0; n < 8; n += 2)
+                    odd = max_abs_nan(odd, y[n], y[n + 1]);
+                if (direct) {
+#pragma unroll
+                    for (int n = 0; n < 8; n += KvVec<T>::kN) {
+                        float z[KvVec<T>::kN];
+#pragma unroll
+                        for (int j = 0; j < KvVec<T>::kN; ++j)
+                            z[j] = l == 0.f ? 0.f : y[n + j] * inv;
+                        *reinterpret_cast<uint4 *>(done + (c + k + n) * sizeof(T)) = KvVec<T>::pack(z);
+                    }
                 } else {
                     *reinterpret_cast<float4 *>(part + c + k) = make_float4(y[0], y[1], y[2], y[3]);
                     *reinterpret_cast<float4 *>(part + c + k + 4) = make_float4(y[4], y[5], y[6], y[7]);
                 }
+            }
+        }
+        // a V row that is no number, in a group of some dims, makes the whole output none
+        l = odd == odd ? l : odd;
+        if (direct) {
+            if (odd != odd)
+                for (int c = 0; c < D; ++c)
+                    reinterpret_cast<T *>(done)[c] = static_cast<T>(odd);
+            __syncwarp();
+            const uint64_t dst = reinterpret_cast<uint64_t>(out + static_cast<int64_t>(span.row0 + node) * a.out_stride +
+                                                            static_cast<int64_t>(h * rep + row - node * rep) * D);
+            constexpr int kChunks = D * static_cast<int>(sizeof(T)) / 16; // of a row: 8 or 16
+            const int live_rows = min(32, rows - (row - lane));
+#pragma unroll 4
+            for (int n = 0; n < kChunks; ++n) {
+                const int at = n * (32 / kChunks) + lane / kChunks; // of the warp's rows
+                const uint64_t to = __shfl_sync(kFullWarpMask, dst, at);
+                if (at < live_rows)
+                    reinterpret_cast<uint4 *>(to)[lane % kChunks] =
+                        *reinterpret_cast<const uint4 *>(smem + (stream * 128 + r - lane + at) * kOutPitch + lane % kChunks * 16);
             }
         }
         stat[stream * 128 + r] = m;
