@@ -16,8 +16,8 @@
 //
 // The kernel is bound by HBM: each value is read and written once, 16 bytes a
 // lane, a head on D / 32 (fp32) or D / 16 (bf16) lanes. A lane has the same pairs
-// in every head, so cos and sin of the row are computed once by the block and stay
-// in registers.
+// in every head, so a warp computes cos and sin of its row once, each lane some of
+// them, and keeps them in registers; no warp waits for another one.
 
 #include <algorithm>
 #include <cstdint>
@@ -49,7 +49,7 @@ template <typename T> struct QkNormRope {
 
 namespace detail {
 
-constexpr int kNormRopeMaxWarps = 12, kNormRopeMaxDim = 256;
+constexpr int kNormRopeThreads = 128, kNormRopeAhead = 2; // rounds of heads whose loads are on their way
 
 // cos and sin of position * frequency.
 __device__ __forceinline__ void turn(int position, float frequency, float &c, float &s) {
@@ -63,81 +63,95 @@ __device__ __forceinline__ void turn(int position, float frequency, float &c, fl
     c = quarter == 0 ? cs : quarter == 1 ? -sn : quarter == 2 ? -cs : sn;
 }
 
+// A warp takes one of `parts` equal parts of a row's heads, 32 / kLanes at a time.
 template <typename T, int D>
-static __global__ void __launch_bounds__(32 * kNormRopeMaxWarps) qk_norm_rope_kernel(QkNormRope<T> a) {
+static __global__ void __launch_bounds__(kNormRopeThreads) qk_norm_rope_kernel(QkNormRope<T> a, int parts) {
     using V = KvVec<T>;
     constexpr int kN = V::kN, kLanes = D / (2 * kN), kPer = 32 / kLanes; // heads of a warp at a time
-    __shared__ float table[2][kNormRopeMaxDim / 2];
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, warps = blockDim.x >> 5;
-    const int half = a.rot_dim / 2, j = lane % kLanes;
+    const int lane = threadIdx.x & 31, j = lane % kLanes, sub = lane / kLanes;
+    const int64_t task = static_cast<int64_t>(blockIdx.x) * (kNormRopeThreads / 32) + (threadIdx.x >> 5);
+    const int64_t row = task / parts;
+    const int heads = a.q_heads + a.kv_heads, half = a.rot_dim / 2;
+    const int rounds = ((heads + kPer - 1) / kPer + parts - 1) / parts; // of a part
+    pdl_trigger();
+    pdl_wait();
+    if (row >= a.rows)
+        return;
+    const int first = static_cast<int>(task - row * parts) * rounds * kPer;
     // the lane's two vectors of a head: a pair of rotated ones, or two of the rest
     const bool turned = j * kN < half;
     const int at0 = turned ? j * kN : a.rot_dim + (j - half / kN) * 2 * kN;
     const int at1 = turned ? half + j * kN : at0 + kN;
-    const int heads = a.q_heads + a.kv_heads;
-    pdl_trigger();
-    pdl_wait();
-    for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
-        const int head0 = warp * kPer + lane / kLanes;
-        const auto source = [&](int h) { return h < a.q_heads ? a.q + row * a.q_stride + h * D : a.k + row * a.k_stride + (h - a.q_heads) * D; };
-        uint4 r0{}, r1{};
-        if (head0 < heads) {
-            const T *src = source(head0);
-            r0 = *reinterpret_cast<const uint4 *>(src + at0), r1 = *reinterpret_cast<const uint4 *>(src + at1);
+    uint4 r0[kNormRopeAhead], r1[kNormRopeAhead];
+    const auto load = [&](int round, uint4 &u, uint4 &v) {
+        const int h = first + round * kPer + sub;
+        if (round < rounds && h < heads) {
+            const T *src = h < a.q_heads ? a.q + row * a.q_stride + h * D : a.k + row * a.k_stride + (h - a.q_heads) * D;
+            u = *reinterpret_cast<const uint4 *>(src + at0), v = *reinterpret_cast<const uint4 *>(src + at1);
         }
-        if (half > 0) {
-            const int position = a.positions[row];
-            __syncthreads(); // the row before has read the table
-            for (int i = tid; i < half; i += blockDim.x)
-                turn(position, a.inv_freq[i], table[0][i], table[1][i]);
-            __syncthreads();
+    };
+#pragma unroll
+    for (int i = 0; i < kNormRopeAhead; ++i)
+        load(i, r0[i], r1[i]);
+    // cos and sin of the lane's pairs: the lanes that have the same ones share the work
+    float c[kN], s[kN];
+    if (half > 0) {
+        constexpr int kEach = kN > kPer ? kN / kPer : 1;
+        const int position = a.positions[row];
+        float mc[kEach], ms[kEach];
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) {
+            mc[i] = 1.f, ms[i] = 0.f;
+            if (turned && sub * kEach + i < kN)
+                turn(position, __ldg(a.inv_freq + at0 + sub * kEach + i), mc[i], ms[i]);
         }
-        float c[kN], s[kN];
 #pragma unroll
         for (int i = 0; i < kN; ++i) {
-            c[i] = turned ? table[0][at0 + i] : 1.f;
-            s[i] = turned ? table[1][at0 + i] : 0.f;
+            c[i] = __shfl_sync(kFullWarpMask, mc[i % kEach], i / kEach * kLanes + j);
+            s[i] = __shfl_sync(kFullWarpMask, ms[i % kEach], i / kEach * kLanes + j);
         }
-        const float *have = nullptr; // the weights that the lane holds its part of
-        float w0[kN], w1[kN];
-        for (int h = head0; h - lane / kLanes < heads; h += warps * kPer) { // whole warps
-            float x[kN], y[kN];
-            V::unpack(r0, x), V::unpack(r1, y);
-            const int next = h + warps * kPer;
-            if (next < heads) {
-                const T *src = source(next);
-                r0 = *reinterpret_cast<const uint4 *>(src + at0), r1 = *reinterpret_cast<const uint4 *>(src + at1);
-            }
-            float sum = 0.f;
+    } else {
+#pragma unroll
+        for (int i = 0; i < kN; ++i)
+            c[i] = 1.f, s[i] = 0.f;
+    }
+    const float *have = nullptr; // the weights that the lane holds its part of
+    float w0[kN], w1[kN];
+#pragma unroll kNormRopeAhead
+    for (int round = 0; round < rounds; ++round) {
+        const int h = first + round * kPer + sub;
+        float x[kN], y[kN];
+        V::unpack(r0[round % kNormRopeAhead], x), V::unpack(r1[round % kNormRopeAhead], y);
+        load(round + kNormRopeAhead, r0[round % kNormRopeAhead], r1[round % kNormRopeAhead]);
+        const float *w = h < a.q_heads ? a.q_weight : a.k_weight;
+        if (w != nullptr && w != have) { // at the first head, and where the queries end
+            have = w;
 #pragma unroll
             for (int i = 0; i < kN; ++i)
-                sum += x[i] * x[i] + y[i] * y[i];
+                w0[i] = __ldg(w + at0 + i), w1[i] = __ldg(w + at1 + i);
+        }
+        float sum = 0.f;
 #pragma unroll
-            for (int off = 1; off < kLanes; off <<= 1)
-                sum += __shfl_xor_sync(kFullWarpMask, sum, off);
-            const float *w = h < a.q_heads ? a.q_weight : a.k_weight;
-            if (h >= heads)
-                continue;
-            if (w != nullptr) {
-                if (w != have) { // at the first head, and where the queries end
-                    have = w;
+        for (int i = 0; i < kN; ++i)
+            sum += x[i] * x[i] + y[i] * y[i];
 #pragma unroll
-                    for (int i = 0; i < kN; ++i)
-                        w0[i] = __ldg(w + at0 + i), w1[i] = __ldg(w + at1 + i);
-                }
-                const float inv = rsqrtf(sum / D + a.eps);
-#pragma unroll
-                for (int i = 0; i < kN; ++i) {
-                    x[i] = x[i] * inv * w0[i];
-                    y[i] = y[i] * inv * w1[i];
-                }
-            }
+        for (int off = 1; off < kLanes; off <<= 1)
+            sum += __shfl_xor_sync(kFullWarpMask, sum, off);
+        if (w != nullptr) {
+            const float inv = rsqrtf(sum / D + a.eps);
 #pragma unroll
             for (int i = 0; i < kN; ++i) {
-                const float u = x[i], v = y[i];
-                x[i] = turned ? u * c[i] - v * s[i] : u;
-                y[i] = turned ? v * c[i] + u * s[i] : v;
+                x[i] = x[i] * inv * w0[i];
+                y[i] = y[i] * inv * w1[i];
             }
+        }
+#pragma unroll
+        for (int i = 0; i < kN; ++i) { // (the rest as it is: zero times an infinity would be NaN)
+            const float u = x[i], v = y[i];
+            x[i] = turned ? u * c[i] - v * s[i] : u;
+            y[i] = turned ? v * c[i] + u * s[i] : v;
+        }
+        if (h < heads) {
             T *dst = h < a.q_heads ? a.q_out + row * a.q_out_stride + h * D : a.k_out + row * a.k_out_stride + (h - a.q_heads) * D;
             *reinterpret_cast<uint4 *>(dst + at0) = V::pack(x);
             *reinterpret_cast<uint4 *>(dst + at1) = V::pack(y);
@@ -146,12 +160,13 @@ static __global__ void __launch_bounds__(32 * kNormRopeMaxWarps) qk_norm_rope_ke
 }
 
 template <typename T, int D> inline void qk_norm_rope_launch(const QkNormRope<T> &a, cudaStream_t stream) {
-    constexpr int kPer = 32 / (D / (2 * KvVec<T>::kN));
-    // as many warps as share the heads out evenly, in as few rounds as 12 warps allow
+    constexpr int kPer = 32 / (D / (2 * KvVec<T>::kN)), kWarps = kNormRopeThreads / 32;
+    // few rows: parts of a row's heads, as long as that brings warps to SMs that have fewer than 16
     const int pieces = (a.q_heads + a.kv_heads + kPer - 1) / kPer;
-    const int rounds = (pieces + kNormRopeMaxWarps - 1) / kNormRopeMaxWarps;
-    const int warps = (pieces + rounds - 1) / rounds;
-    launch_ex(qk_norm_rope_kernel<T, D>, dim3(static_cast<unsigned>(a.rows)), dim3(static_cast<unsigned>(32 * warps)), 0, stream, a);
+    const int64_t want = 16LL * device_facts().sm_count / a.rows;
+    const int parts = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(pieces, want)));
+    const int64_t blocks = (static_cast<int64_t>(a.rows) * parts + kWarps - 1) / kWarps;
+    launch_ex(qk_norm_rope_kernel<T, D>, dim3(static_cast<unsigned>(blocks)), dim3(kNormRopeThreads), 0, stream, a, parts);
 }
 
 } // namespace detail
