@@ -61,42 +61,27 @@ __device__ __forceinline__ float kv4_scale(float top) {
     return __uint_as_float(s <= kKv4MaxScale && top <= 3.4028235e38f ? s : 0x7fc00000u);
 }
 
-// Eight codes + 8 of x / s, the first in the lowest bits; inv is about 1 / s.
-// The quotient's nearest integer r is found with x * inv, which is 2^-22 off at
-// most: so r can be wrong only where the rest x - r s, which is exact, is half of
-// s or more, and then the rest decides.
+// Eight codes + 8 of x / s, the first in the lowest bits; inv = 1 / s, rounded to
+// nearest. The quotients are correctly rounded (Markstein, IBM J. Res. Dev. 34, 1990:
+// from such a reciprocal y, q = x y, then q + (x - q s) y is): a code is that of an
+// IEEE division, ties included, which half-way numbers of bf16 rows often are. Sums
+// of codes times powers of 16 are exact in fp32, four codes to a sum.
 __device__ __forceinline__ uint32_t kv4_encode8(const float (&x)[8], float s, float inv) {
-    constexpr float kRound = 12582920.f; // 1.5 2^23 + 8: the sum's low bits are the nearest integer, plus 8
-    const float2 i2 = make_float2(inv, inv), up = make_float2(kRound, kRound), down = make_float2(-kRound, -kRound);
-    const float2 s2 = make_float2(-s, -s);
-    float2 t[4], rest[4];
-    float most = 0.f;
+    constexpr float kRound = 12582912.f, kBias = kRound + 0x8888; // 1.5 2^23: what is added to it is rounded to an integer
+    const float2 y = make_float2(inv, inv), less = make_float2(-s, -s), up = make_float2(kRound, kRound), down = make_float2(-kRound, -kRound);
+    float2 r[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        const float2 v = make_float2(x[2 * i], x[2 * i + 1]);
-        // (the sum is rounded once: 8 + x inv to an integer, ties to an even one)
-        t[i] = __ffma2_rn(v, i2, up);
-        rest[i] = __ffma2_rn(__fadd2_rn(t[i], down), s2, v);
-        most = max_abs_nan(most, rest[i].x, rest[i].y);
+        const float2 v = make_float2(x[2 * i], x[2 * i + 1]), q = __fmul2_rn(v, y);
+        r[i] = __fadd2_rn(__fadd2_rn(__ffma2_rn(__ffma2_rn(q, less, v), y, q), up), down);
     }
-    uint32_t c[8];
+    uint32_t w[2];
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-        c[2 * i] = __float_as_uint(t[i].x), c[2 * i + 1] = __float_as_uint(t[i].y);
-    if (!(most < 0.5f * s)) {
-        const float half = 0.5f * s;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const float d = i & 1 ? rest[i / 2].y : rest[i / 2].x, a = fabsf(d);
-            if (a > half || (a == half && (c[i] & 1u)))
-                c[i] += d > 0.f ? 1u : -1u;
-        }
+    for (int i = 0; i < 2; ++i) {
+        const float2 e = __ffma2_rn(r[2 * i + 1], make_float2(256.f, 256.f), r[2 * i]);
+        w[i] = __float_as_uint(fmaf(e.y, 16.f, e.x + kBias));
     }
-    uint32_t w = 0;
-#pragma unroll
-    for (int i = 7; i >= 0; --i)
-        w = (w << 4) | (c[i] & 15u);
-    return w;
+    return __byte_perm(w[0], w[1], 0x5410);
 }
 
 // The same for scales near or below the smallest normal numbers, and none (0, NaN).
@@ -212,7 +197,7 @@ static __global__ void __launch_bounds__(kKv4Threads)
         if (at >= groups)
             continue;
         const float s = kv4_scale(top);
-        const uint32_t w = s >= 0x1p-20f ? kv4_encode8(y, s, rcp_approx(s)) : kv4_encode8_small(y, s);
+        const uint32_t w = s >= 0x1p-20f ? kv4_encode8(y, s, __frcp_rn(s)) : kv4_encode8_small(y, s);
         uint8_t *rec = recs + at / R::kGroups * R::kBytes;
         const int g = at % R::kGroups;
         *reinterpret_cast<uint32_t *>(rec + (p & 1 ? R::kCodes : 0) + (g * kKvPage + slot) * 16 + lane % 4 * 4) = w;

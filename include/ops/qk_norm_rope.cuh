@@ -17,7 +17,11 @@
 // The kernel is bound by HBM: each value is read and written once, 16 bytes a
 // lane, a head on D / 32 (fp32) or D / 16 (bf16) lanes. A lane has the same pairs
 // in every head, so a warp computes cos and sin of its row once, each lane some of
-// them, and keeps them in registers; no warp waits for another one.
+// them, and keeps them in registers; no warp waits for another one. 32 warps an SM
+// (64 registers, weights in shared memory) hide the loads better than loads further
+// ahead do (two rounds ahead: 61.6 us for 57.9; weights in registers, 20 warps: 73.5).
+// Measured: 16,384 rows of 40 heads x 128, bf16: 57.9 us, 5.8 TB/s (copy rate 6.46);
+// 32 rows, fp32: 2.6 us, launch included.
 
 #include <algorithm>
 #include <cstdint>
@@ -49,7 +53,7 @@ template <typename T> struct QkNormRope {
 
 namespace detail {
 
-constexpr int kNormRopeThreads = 128, kNormRopeAhead = 2; // rounds of heads whose loads are on their way
+constexpr int kNormRopeThreads = 128;
 
 // cos and sin of position * frequency.
 __device__ __forceinline__ void turn(int position, float frequency, float &c, float &s) {
@@ -65,7 +69,7 @@ __device__ __forceinline__ void turn(int position, float frequency, float &c, fl
 
 // A warp takes one of `parts` equal parts of a row's heads, 32 / kLanes at a time.
 template <typename T, int D>
-static __global__ void __launch_bounds__(kNormRopeThreads) qk_norm_rope_kernel(QkNormRope<T> a, int parts) {
+static __global__ void __launch_bounds__(kNormRopeThreads, 8) qk_norm_rope_kernel(QkNormRope<T> a, int parts) {
     using V = KvVec<T>;
     constexpr int kN = V::kN, kLanes = D / (2 * kN), kPer = 32 / kLanes; // heads of a warp at a time
     const int lane = threadIdx.x & 31, j = lane % kLanes, sub = lane / kLanes;
@@ -75,24 +79,28 @@ static __global__ void __launch_bounds__(kNormRopeThreads) qk_norm_rope_kernel(Q
     const int rounds = ((heads + kPer - 1) / kPer + parts - 1) / parts; // of a part
     pdl_trigger();
     pdl_wait();
-    if (row >= a.rows)
-        return;
     const int first = static_cast<int>(task - row * parts) * rounds * kPer;
     // the lane's two vectors of a head: a pair of rotated ones, or two of the rest
     const bool turned = j * kN < half;
     const int at0 = turned ? j * kN : a.rot_dim + (j - half / kN) * 2 * kN;
     const int at1 = turned ? half + j * kN : at0 + kN;
-    uint4 r0[kNormRopeAhead], r1[kNormRopeAhead];
-    const auto load = [&](int round, uint4 &u, uint4 &v) {
+    uint4 r0{}, r1{}; // of the next round
+    const auto load = [&](int round) {
         const int h = first + round * kPer + sub;
-        if (round < rounds && h < heads) {
+        if (row < a.rows && round < rounds && h < heads) {
             const T *src = h < a.q_heads ? a.q + row * a.q_stride + h * D : a.k + row * a.k_stride + (h - a.q_heads) * D;
-            u = *reinterpret_cast<const uint4 *>(src + at0), v = *reinterpret_cast<const uint4 *>(src + at1);
+            r0 = *reinterpret_cast<const uint4 *>(src + at0), r1 = *reinterpret_cast<const uint4 *>(src + at1);
         }
     };
-#pragma unroll
-    for (int i = 0; i < kNormRopeAhead; ++i)
-        load(i, r0[i], r1[i]);
+    load(0);
+    __shared__ __align__(16) float weights[2][D];
+    for (int i = threadIdx.x; i < D; i += kNormRopeThreads) {
+        weights[0][i] = a.q_weight != nullptr ? __ldg(a.q_weight + i) : 1.f;
+        weights[1][i] = a.k_weight != nullptr ? __ldg(a.k_weight + i) : 1.f;
+    }
+    __syncthreads();
+    if (row >= a.rows)
+        return;
     // cos and sin of the lane's pairs: the lanes that have the same ones share the work
     float c[kN], s[kN];
     if (half > 0) {
@@ -115,21 +123,11 @@ static __global__ void __launch_bounds__(kNormRopeThreads) qk_norm_rope_kernel(Q
         for (int i = 0; i < kN; ++i)
             c[i] = 1.f, s[i] = 0.f;
     }
-    const float *have = nullptr; // the weights that the lane holds its part of
-    float w0[kN], w1[kN];
-#pragma unroll kNormRopeAhead
     for (int round = 0; round < rounds; ++round) {
         const int h = first + round * kPer + sub;
         float x[kN], y[kN];
-        V::unpack(r0[round % kNormRopeAhead], x), V::unpack(r1[round % kNormRopeAhead], y);
-        load(round + kNormRopeAhead, r0[round % kNormRopeAhead], r1[round % kNormRopeAhead]);
-        const float *w = h < a.q_heads ? a.q_weight : a.k_weight;
-        if (w != nullptr && w != have) { // at the first head, and where the queries end
-            have = w;
-#pragma unroll
-            for (int i = 0; i < kN; ++i)
-                w0[i] = __ldg(w + at0 + i), w1[i] = __ldg(w + at1 + i);
-        }
+        V::unpack(r0, x), V::unpack(r1, y);
+        load(round + 1);
         float sum = 0.f;
 #pragma unroll
         for (int i = 0; i < kN; ++i)
@@ -137,12 +135,14 @@ static __global__ void __launch_bounds__(kNormRopeThreads) qk_norm_rope_kernel(Q
 #pragma unroll
         for (int off = 1; off < kLanes; off <<= 1)
             sum += __shfl_xor_sync(kFullWarpMask, sum, off);
-        if (w != nullptr) {
+        const bool key = h >= a.q_heads;
+        if ((key ? a.k_weight : a.q_weight) != nullptr) {
             const float inv = rsqrtf(sum / D + a.eps);
 #pragma unroll
-            for (int i = 0; i < kN; ++i) {
-                x[i] = x[i] * inv * w0[i];
-                y[i] = y[i] * inv * w1[i];
+            for (int i = 0; i < kN; i += 4) {
+                const float4 w0 = *reinterpret_cast<const float4 *>(&weights[key][at0 + i]), w1 = *reinterpret_cast<const float4 *>(&weights[key][at1 + i]);
+                x[i] = x[i] * inv * w0.x, x[i + 1] = x[i + 1] * inv * w0.y, x[i + 2] = x[i + 2] * inv * w0.z, x[i + 3] = x[i + 3] * inv * w0.w;
+                y[i] = y[i] * inv * w1.x, y[i + 1] = y[i + 1] * inv * w1.y, y[i + 2] = y[i + 2] * inv * w1.z, y[i + 3] = y[i + 3] * inv * w1.w;
             }
         }
 #pragma unroll
