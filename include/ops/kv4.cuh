@@ -148,17 +148,6 @@ template <typename T> __device__ __forceinline__ void kv4_load8(const T *p, floa
             x[i * KvVec<T>::kN + j] = y[j];
     }
 }
-template <typename T> __device__ __forceinline__ void kv4_store8(T *p, const float (&x)[8]) {
-#pragma unroll
-    for (int i = 0; i < 8 / KvVec<T>::kN; ++i) {
-        float y[KvVec<T>::kN];
-#pragma unroll
-        for (int j = 0; j < KvVec<T>::kN; ++j)
-            y[j] = x[i * KvVec<T>::kN + j];
-        __stcs(reinterpret_cast<uint4 *>(p) + i, KvVec<T>::pack(y));
-    }
-}
-
 // A warp takes one row and 8 * kKv4Passes of its kvh * G groups, K and V of each:
 // four lanes a group, eight dims a lane.
 template <typename T, int D>
@@ -206,11 +195,14 @@ static __global__ void __launch_bounds__(kKv4Threads)
     }
 }
 
+// The other way round, 16 bytes of the output a lane: 4 (fp32) or 8 lanes' worth of a
+// group's 32 dims, so that a warp's store is one run of 512 bytes.
 template <typename T, int D>
 static __global__ void __launch_bounds__(kKv4Threads)
     kv4_read_kernel(const uint8_t *__restrict__ pool, T *__restrict__ k, int64_t k_stride, T *__restrict__ v, int64_t v_stride,
                     Kv4Rows a) {
     using R = Kv4Record<D>;
+    constexpr int kN = KvVec<T>::kN, kLanes = kKv4Group / kN, kPer = 32 / kLanes, kPasses = kKv4Passes * 8 / kPer;
     const int lane = threadIdx.x & 31;
     const int64_t row = static_cast<int64_t>(blockIdx.x) * (kKv4Threads / 32) + (threadIdx.x >> 5);
     pdl_wait();
@@ -221,27 +213,37 @@ static __global__ void __launch_bounds__(kKv4Threads)
         return;
     const int slot = static_cast<int>(place % kKvPage);
     const uint8_t *recs = pool + place / kKvPage * a.kvh * R::kBytes;
-    const int groups = a.kvh * R::kGroups, group0 = static_cast<int>(blockIdx.y) * kKv4Passes * 8 + lane / 4;
-    uint32_t w[2 * kKv4Passes];
-    __half s[2 * kKv4Passes];
+    const int groups = a.kvh * R::kGroups, group0 = static_cast<int>(blockIdx.y) * kKv4Passes * 8 + lane / kLanes, part = lane % kLanes;
+    uint32_t w[2 * kPasses];
+    __half s[2 * kPasses];
 #pragma unroll
-    for (int p = 0; p < 2 * kKv4Passes; ++p) {
-        const int at = min(group0 + 8 * (p / 2), groups - 1), g = at % R::kGroups;
+    for (int p = 0; p < 2 * kPasses; ++p) {
+        const int at = min(group0 + kPer * (p / 2), groups - 1), g = at % R::kGroups;
         const uint8_t *rec = recs + at / R::kGroups * R::kBytes;
-        w[p] = *reinterpret_cast<const uint32_t *>(rec + (p & 1 ? R::kCodes : 0) + (g * kKvPage + slot) * 16 + lane % 4 * 4);
+        const uint8_t *codes = rec + (p & 1 ? R::kCodes : 0) + (g * kKvPage + slot) * 16;
+        if constexpr (kN == 8)
+            w[p] = reinterpret_cast<const uint32_t *>(codes)[part];
+        else
+            w[p] = reinterpret_cast<const uint16_t *>(codes)[part];
         s[p] = *reinterpret_cast<const __half *>(rec + (p & 1 ? R::kVScale : R::kKScale) + (g * kKvPage + slot) * 2);
     }
 #pragma unroll
-    for (int p = 0; p < 2 * kKv4Passes; ++p) {
-        const int at = group0 + 8 * (p / 2);
+    for (int p = 0; p < 2 * kPasses; ++p) {
+        const int at = group0 + kPer * (p / 2);
         if (at >= groups)
             continue;
-        const float scale = __half2float(s[p]);
-        float x[8];
+        uint32_t h[4];
+        kv4_widen(w[p], __half2half2(s[p]), h); // codes (0, 4), (1, 5), (2, 6), (3, 7)
+        float x[kN];
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-            x[i] = static_cast<float>(static_cast<int>(w[p] >> (4 * i) & 15u) - 8) * scale;
-        kv4_store8((p & 1 ? v + row * v_stride : k + row * k_stride) + at * kKv4Group + lane % 4 * 8, x);
+        for (int i = 0; i < 4; ++i) {
+            const float2 f = __half22float2(kv4_half2(h[i]));
+            x[i] = f.x;
+            if constexpr (kN == 8)
+                x[i + 4] = f.y;
+        }
+        T *dst = (p & 1 ? v + row * v_stride : k + row * k_stride) + at * kKv4Group + part * kN;
+        __stcs(reinterpret_cast<uint4 *>(dst), KvVec<T>::pack(x));
     }
 }
 
