@@ -1,8 +1,9 @@
-"""Drafted-token decoding over a paged cache: the torch-side wrapper of
-``kv_quant_*``, ``tree_attention*`` and ``tree_commit*`` (include/opworks_ops.h).
+"""Decoding over a paged cache, drafted tokens included: the torch-side wrapper of
+``kv_quant_*``, ``kv4_*``, ``page_*``, ``qk_norm_rope``, ``tree_attention*`` and
+``tree_commit*`` (include/opworks_ops.h).
 
 ``PagedCache`` owns the pools of all layers and the block table of a batch, in
-fp32 or in 8 bits; a step writes the new tokens' K and V, attends, and commits::
+fp32, in 8 bits or in 4; a step writes the new tokens' K and V, attends, and commits::
 
     cache = PagedCache(layers=2, batch=4, max_tokens=512, kv_heads=2, head_dim=64, format="int8")
     rows = Rows([len(p) for p in prompts])                 # ragged: a chain per sequence
@@ -15,6 +16,17 @@ fp32 or in 8 bits; a step writes the new tokens' K and V, attends, and commits::
     path, count, next = cache.commit(draft, target, rows)   # only the accepted path stays
     cache.kept(count.tolist())                              # once the host has read it: how full the cache is
 
+With ``blocks`` the sequences share that many pages: a step takes what its new
+tokens need, a commit gives back what its drafts did not, and ``release`` all that
+sequences hold. ``place`` says where the new tokens go; ``qk_norm_rope`` takes their
+positions::
+
+    cache = PagedCache(layers=2, batch=64, max_tokens=4096, kv_heads=2, head_dim=64, format="int4", blocks=1000)
+    positions, slots = cache.place(rows)
+    q, k = qk_norm_rope(q, k, positions, inv_freq, q_weight, k_weight)
+    ...
+    cache.release([3, 7])                                   # sequences that are done
+
 Everything runs on torch's current stream; nothing here waits for the device.
 """
 
@@ -25,7 +37,8 @@ import torch
 
 from . import ops_lib
 
-FORMATS = {"f32": 0, "int8": 1, "e4m3": 2}
+FORMATS = {"f32": 0, "int8": 1, "e4m3": 2, "int4": 4}
+INT4 = FORMATS["int4"]
 TYPES = {torch.float32: 0, torch.bfloat16: 1}
 INTEGERS = (torch.int32, torch.int64, torch.int16, torch.uint8, torch.int8)
 
@@ -92,22 +105,67 @@ class Rows:
         return self._parents
 
 
+def _current(device):
+    """torch's current stream, where it is one of `device`: an operator launches on the current device."""
+    if device.type != "cuda" or device.index != torch.cuda.current_device():
+        raise ValueError(f"these tensors are on {device}, which is not the current CUDA device")
+    return torch.cuda.current_stream().cuda_stream
+
+
+def qk_norm_rope(q, k, positions, inv_freq=None, q_weight=None, k_weight=None, eps=1e-5, out=None):
+    """Queries [rows, q_heads, D] and keys [rows, kv_heads, D] (fp32 or bf16, any row stride), each head normalised (root mean
+    square, fp32 weights [D]; None: that side is not) and its first 2 * len(inv_freq) dims rotated by its row's position (int32;
+    inv_freq None: no rotation). Returns new tensors, or writes into ``out`` = (q_out, k_out), which may be (q, k)."""
+    rows, dim = (q.shape[0], q.shape[2]) if q.dim() == 3 else (-1, -1)
+    if k.dim() != 3 or k.shape[0] != rows or k.shape[2] != dim or q.dtype not in TYPES or k.dtype != q.dtype or k.device != q.device:
+        raise ValueError("q and k: [rows, heads, D], both fp32 or both bf16, on one device")
+    new = (torch.empty(q.shape, dtype=q.dtype, device=q.device), torch.empty(k.shape, dtype=k.dtype, device=k.device)) if out is None else tuple(out)
+    for name, t, like in (("q_out", new[0], q), ("k_out", new[1], k)):
+        if t.shape != like.shape or t.dtype != like.dtype or t.device != like.device:
+            raise ValueError(f"{name}: as its input, {list(like.shape)} of {like.dtype} on {like.device}")
+    for name, t in (("q", q), ("k", k), ("q_out", new[0]), ("k_out", new[1])):
+        if rows and t.shape[1] and (t.stride(2) != 1 or (t.shape[1] > 1 and t.stride(1) != dim)):
+            raise ValueError(f"{name}: the heads of a row lie one after another")
+    rot = 0 if inv_freq is None else 2 * inv_freq.numel()
+    plain = [("q_weight", q_weight, torch.float32, dim), ("k_weight", k_weight, torch.float32, dim)]
+    if rot:
+        plain += [("inv_freq", inv_freq, torch.float32, rot // 2), ("positions", positions, torch.int32, rows)]
+    for name, t, kind, n in plain:
+        if t is not None and (t.dtype != kind or t.numel() != n or not t.is_contiguous() or t.device != q.device):
+            raise ValueError(f"{name}: {n} of {kind} on {q.device}, one after another")
+    if rot and positions is None:
+        raise ValueError("positions: a rotation needs them")
+    stride = lambda t: t.stride(0) if rows > 1 else t.shape[1] * dim  # noqa: E731
+    ops_lib().qk_norm_rope(q, stride(q), k, stride(k), TYPES[q.dtype], q_weight, k_weight, eps, positions if rot else None, inv_freq if rot else None,
+                           rot, rows, q.shape[1], k.shape[1], dim, new[0], stride(new[0]), new[1], stride(new[1]), _current(q.device))
+    return new
+
+
 class PagedCache:
     PAGE = 16
 
-    def __init__(self, layers, batch, max_tokens, kv_heads, head_dim, format="int8", device="cuda"):
+    def __init__(self, layers, batch, max_tokens, kv_heads, head_dim, format="int8", device="cuda", blocks=None):
         self.ops, self.format = ops_lib(), FORMATS[format]
         self.layers, self.batch, self.kv_heads, self.head_dim = layers, batch, kv_heads, head_dim
         self.stride = -(-max_tokens // self.PAGE)
-        blocks = batch * self.stride
+        self.shared = blocks is not None  # pages are taken as sequences grow, and given back
+        blocks = batch * self.stride if blocks is None else blocks
+        self.blocks = blocks
         if self.format:
-            record = self.ops.kv_quant_record_bytes(head_dim)
+            record = self.ops.kv4_record_bytes(head_dim) if self.format == INT4 else self.ops.kv_quant_record_bytes(head_dim)
             self.pool = torch.zeros(layers, blocks, kv_heads, record, dtype=torch.uint8, device=device)
         else:
             self.k = torch.zeros(layers, blocks, kv_heads, self.PAGE, head_dim, device=device)
             self.v = torch.zeros_like(self.k)
         # each sequence's pages spread over the pool, as an allocator would leave them
-        self.table = torch.arange(blocks, dtype=torch.int32, device=device).view(self.stride, batch).t().contiguous()
+        if self.shared:
+            self.table = torch.zeros(batch, self.stride, dtype=torch.int32, device=device)
+            self.free = torch.arange(blocks - 1, -1, -1, dtype=torch.int32, device=device)
+            self.free_count = torch.full((1,), blocks, dtype=torch.int32, device=device)
+        else:
+            self.table = torch.arange(blocks, dtype=torch.int32, device=device).view(self.stride, batch).t().contiguous()
+        self.status = torch.zeros(1, dtype=torch.int32, device=device)  # of the last pages taken or given: 0
+        self._placed = None        # the step that has been given its places: (rows, lens, its version, positions, slots)
         self.lens = torch.zeros(batch, dtype=torch.int32, device=device)
         self.bounds = [0] * batch  # upper bounds of lens that the host knows
         self._before = None        # those before the last commit
@@ -122,6 +180,9 @@ class PagedCache:
             raise ValueError(f"the cache is on {self.lens.device}, which is not the current CUDA device")
         return torch.cuda.current_stream().cuda_stream
 
+    def _pages(self, tokens):
+        return sum(-(-n // self.PAGE) for n in tokens)
+
     def _belongs(self, rows):
         if len(rows.counts) != self.batch or rows.start.device != self.lens.device:
             raise ValueError("rows: counts of this cache's sequences, on its device")
@@ -135,6 +196,58 @@ class PagedCache:
     def _room(self, rows):
         if any(n and b + n > self.stride * self.PAGE for b, n in zip(self.bounds, rows.counts)):
             raise ValueError("the cache has no room for these rows")
+        if self.shared and self._pages(b + n for b, n in zip(self.bounds, rows.counts)) > self.blocks:
+            raise ValueError("the cache has no pages for these rows")
+
+    def _where(self, rows, take):
+        """Positions (int32) and slots (int64) of the rows; with ``take`` their pages come off the stack."""
+        positions = torch.empty(rows.total, dtype=torch.int32, device=self.lens.device)
+        slots = torch.empty(rows.total, dtype=torch.int64, device=self.lens.device)
+        stack = (self.free, self.free_count) if take else (None, None)
+        self.ops.page_take(self.lens, rows.start, self.batch, rows.total, self.table, self.stride, *stack, positions, slots, stack[1],
+                           self.status, self._stream())
+        return positions, slots
+
+    def place(self, rows):
+        """Where the rows of a step go: positions (int32, lens + 0, 1, ...) and slots (int64, 16 * block + place in the page). With
+        shared pages those that the step needs are taken, once, whoever asks first: this, or the step's first write."""
+        self._belongs(rows)
+        self._room(rows)
+        if not self._has_places(rows):
+            if self._placed is not None and self.shared:
+                raise ValueError("place: the step before has been given its places and is neither kept nor dropped (advance, commit, drop)")
+            self._placed = (rows, self.lens, self.lens._version, *self._where(rows, self.shared))
+        return self._placed[3:]
+
+    def _has_places(self, rows):
+        p = self._placed  # (lens: a program that sets it itself has moved the rows)
+        return p is not None and p[0] is rows and p[1] is self.lens and p[2] == self.lens._version
+
+    def drop(self):
+        """Forgets the rows of the step that was placed: their pages go back."""
+        if self._placed is not None and self.shared:
+            self._give(self.lens + self._placed[0].start.diff(), self.lens)
+        self._placed = None
+
+    def _give(self, old, new):
+        self.ops.page_give(old, new, self.batch, self.table, self.stride, self.free, self.blocks, self.free_count, self.free_count,
+                           self.status, self._stream())
+
+    def release(self, sequences):
+        """Ends sequences (their numbers): their lengths become zero, and with shared pages their pages go back."""
+        gone = np.zeros(self.batch, np.int32)
+        for b in sequences:
+            if not 0 <= int(b) < self.batch:
+                raise ValueError(f"release: sequences 0 to {self.batch - 1}, not {b}")
+            gone[int(b)] = 1
+        if self._placed is not None and self.shared:
+            raise ValueError("release: between steps, not within one (advance, commit, drop)")
+        (mask,) = to_device(self.lens.device, gone)
+        lens = torch.where(mask != 0, torch.zeros_like(self.lens), self.lens)
+        if self.shared:
+            self._give(self.lens, lens)
+        self.lens, self._placed = lens, None
+        self.bounds, self._before = [0 if g else n for n, g in zip(self.bounds, gone)], None
 
     def write(self, layer, k, v, rows):
         """K and V rows [total, kv_heads * head_dim] (any row stride) at positions lens + 0, 1, ... of their sequences."""
@@ -143,6 +256,14 @@ class PagedCache:
         self._takes("k", k, shape, TYPES)
         self._takes("v", v, shape, (k.dtype,))
         self._room(rows)
+        if self.shared or self.format == INT4:
+            _, slots = self.place(rows)
+        if self.format == INT4:
+            k, v = (x if x.stride(1) == 1 else x.contiguous() for x in (k, v))
+            stride = lambda x: x.stride(0) if rows.total > 1 else shape[1]  # noqa: E731
+            self.ops.kv4_write(k, stride(k), v, stride(v), TYPES[k.dtype], self.pool[layer], self.blocks, slots, rows.total, self.kv_heads,
+                               self.head_dim, self._stream())
+            return
         if k.stride() != v.stride() or k.stride(1) != 1:  # the operator takes one row stride
             k, v = k.contiguous(), v.contiguous()
         if self.format:
@@ -157,14 +278,20 @@ class PagedCache:
         self.v[layer][block, :, slot] = v.float().view(shape)
 
     def read(self, layer, rows, dtype=torch.float32):
-        """The rows at positions lens + 0, 1, ... of an 8-bit cache, as [total, kv_heads, head_dim] K and V."""
+        """The rows at positions lens + 0, 1, ... of an 8-bit or 4-bit cache, as [total, kv_heads, head_dim] K and V."""
         if not self.format:
-            raise ValueError("read: of an 8-bit cache; the fp32 pools are plain tensors")
+            raise ValueError("read: of an 8-bit or 4-bit cache; the fp32 pools are plain tensors")
         self._belongs(rows)
         if dtype not in TYPES:
             raise ValueError(f"read: as {' or '.join(str(d) for d in TYPES)}, not {dtype}")
         k = torch.empty(rows.total, self.kv_heads, self.head_dim, dtype=dtype, device=self.lens.device)
         v = torch.empty_like(k)
+        if self.format == INT4:
+            _, slots = self._placed[3:] if self._has_places(rows) else self._where(rows, False)
+            width = self.kv_heads * self.head_dim
+            self.ops.kv4_read(self.pool[layer], self.blocks, slots, rows.total, self.kv_heads, self.head_dim, k, width, v, width, TYPES[dtype],
+                              self._stream())
+            return k, v
         self.ops.kv_quant_read(self.pool[layer], self.format, self.table, self.stride, self.lens, rows.start, self.batch,
                                rows.total, self.kv_heads, self.head_dim, k, v, TYPES[dtype], self.kv_heads * self.head_dim,
                                self._stream())
@@ -182,7 +309,9 @@ class PagedCache:
                 raise ValueError(f"{name}: the heads of a row lie one after another")
         rest = (self.table, self.stride, self.lens, rows.start, rows.mask, rows.words, self.batch, rows.total, rows.most,
                 self.max_len, heads, self.kv_heads, self.head_dim, scale, out, out.stride(0), self._stream())
-        if self.format:
+        if self.format == INT4:
+            self.ops.tree_attention_q4(q, TYPES[q.dtype], q.stride(0), self.pool[layer], *rest)
+        elif self.format:
             self.ops.tree_attention_q8(q, TYPES[q.dtype], q.stride(0), self.pool[layer], self.format, *rest)
         else:
             self.ops.tree_attention(q, TYPES[q.dtype], q.stride(0), self.k[layer], self.v[layer], *rest)
@@ -190,6 +319,9 @@ class PagedCache:
     def advance(self, rows):
         """Keeps all rows (a prompt, or a chain that needs no verification)."""
         self._belongs(rows)
+        if self.shared:
+            self.place(rows)
+        self._placed = None
         self.lens = self.lens + rows.start.diff()
         self.bounds, self._before = [b + n for b, n in zip(self.bounds, rows.counts)], None
 
@@ -204,11 +336,16 @@ class PagedCache:
         path, count, nxt, lens = new(rows.total), new(self.batch), new(self.batch), new(self.batch)
         head = (draft, target, rows.parents, rows.start, self.lens, self.batch, rows.most)
         tail = (self.layers, self.table, self.stride, self.kv_heads, self.head_dim, path, count, nxt, lens, self._stream())
+        if self.shared:
+            self.place(rows)
         if self.format:
-            self.ops.tree_commit_q8(*head, self.pool, self.pool.stride(0), *tail)
+            call = self.ops.tree_commit_q4 if self.format == INT4 else self.ops.tree_commit_q8
+            call(*head, self.pool, self.pool.stride(0), *tail)
         else:
             self.ops.tree_commit(*head, self.k, self.v, self.k.stride(0), *tail)
-        self.lens = lens
+        if self.shared:  # pages that the drafts had and the kept path does not need
+            self._give(self.lens + rows.start.diff(), lens)
+        self.lens, self._placed = lens, None
         self._before, self.bounds = self.bounds, [b + n for b, n in zip(self.bounds, rows.depths)]
         return path, count, nxt
 
