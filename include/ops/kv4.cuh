@@ -105,30 +105,34 @@ template <uint32_t kMask, uint32_t kOr> __device__ __forceinline__ uint32_t kv4_
 __device__ __forceinline__ __half2 kv4_half2(uint32_t u) { return *reinterpret_cast<const __half2 *>(&u); }
 __device__ __forceinline__ uint32_t kv4_bits(__half2 h) { return *reinterpret_cast<const uint32_t *>(&h); }
 
-// Four pairs of fp16 numbers from the eight codes of a word: (0, 4), (1, 5), (2,
-// 6), (3, 7), times the pair `scale`. Exact: a code goes into the low bits of fp16
-// 1024 .. 1039 (or, 16-fold, 1024 .. 1264), from which 1032 (72) is taken away.
-__device__ __forceinline__ void kv4_widen(uint32_t w, __half2 scale, uint32_t (&h)[4]) {
+// Four pairs of codes from the eight of a word, as fp16 numbers: (0, 4), (1, 5), (2,
+// 6), (3, 7). A code + 8 goes into the low bits of fp16 1024 .. 1039 (or, 16-fold, 1024
+// .. 1264), from which 1032 (72) is taken away.
+__device__ __forceinline__ void kv4_integers(uint32_t w, __half2 (&h)[4]) {
     const uint32_t hi = w >> 8;
-    const auto low = [&](uint32_t u) {
-        return kv4_bits(__hmul2(__hsub2(kv4_half2(kv4_pick<0x000f000fu, 0x64006400u>(u)), kv4_half2(0x64086408u)), scale));
-    };
-    const auto high = [&](uint32_t u) { // 1 / 16, -72
-        return kv4_bits(__hmul2(__hfma2(kv4_half2(kv4_pick<0x00f000f0u, 0x64006400u>(u)), kv4_half2(0x2c002c00u), kv4_half2(0xd480d480u)), scale));
+    const auto low = [](uint32_t u) { return __hsub2(kv4_half2(kv4_pick<0x000f000fu, 0x64006400u>(u)), kv4_half2(0x64086408u)); };
+    const auto high = [](uint32_t u) { // 1 / 16, -72
+        return __hfma2(kv4_half2(kv4_pick<0x00f000f0u, 0x64006400u>(u)), kv4_half2(0x2c002c00u), kv4_half2(0xd480d480u));
     };
     h[0] = low(w), h[1] = high(w), h[2] = low(hi), h[3] = high(hi);
 }
 
-// The same without a scale, as the integers that they are: pairs 0 and 2 of c
-// 2^-24, 1 and 3 of c 2^-20 (fp16's subnormal numbers are integers times 2^-24), less
-// 8 of them where kSigned, else c + 8 as it is stored.
-template <bool kSigned> __device__ __forceinline__ void kv4_integers(uint32_t w, uint32_t (&h)[4]) {
+// The same times the pair `scale`. Exact.
+__device__ __forceinline__ void kv4_widen(uint32_t w, __half2 scale, uint32_t (&h)[4]) {
+    __half2 c[4];
+    kv4_integers(w, c);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        h[i] = kv4_bits(__hmul2(c[i], scale));
+}
+
+// Half the operations: code + 8 as it is stored, pairs 0 and 2 times 2^-24, 1 and 3
+// times 2^-20 (fp16's subnormal numbers are integers times 2^-24). Sums of products with
+// subnormal factors are good to 2^-19 only: the tensor cores line products up as if
+// their factors were normal.
+__device__ __forceinline__ void kv4_subnormals(uint32_t w, uint32_t (&h)[4]) {
     const uint32_t hi = w >> 8;
     h[0] = w & 0x000f000fu, h[1] = w & 0x00f000f0u, h[2] = hi & 0x000f000fu, h[3] = hi & 0x00f000f0u;
-    if constexpr (kSigned)
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-            h[i] = kv4_bits(__hsub2(kv4_half2(h[i]), kv4_half2(i & 1 ? 0x00800080u : 0x00080008u)));
 }
 
 struct Kv4Rows {

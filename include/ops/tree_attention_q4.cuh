@@ -20,8 +20,15 @@ namespace opworks {
 namespace detail {
 
 template <typename T, int D> inline void q4_call(const T *q, T *out, const TreeArgs &a, cudaStream_t stream) {
-    constexpr bool kHasTiles = D == 64 || std::is_same_v<T, __nv_bfloat16>;
-    constexpr int kFrom = 64; // rows of a kv head
+    // The rows kernel's time grows with the rows, that of 128-row tiles does not. 8 (32)
+    // sequences of 4096 (2048) tokens with up to n rows of a kv head, 0.8 n on average, 8 kv
+    // heads, us with rows / tiles:
+    //   fp32 rows, D 64     n = 32  37 / 44 (40 / 67)   48  49 / 45 (66 / 68)   64  52 / 45 (70 / 69)
+    //   bf16 rows, D 64     n = 32  30 / 31 (29 / 48)   48  37 / 31 (48 / 49)   64  39 / 32 (51 / 51)
+    //   bf16 rows, D 128    n = 24  43 / 40 (46 / 61)   32  44 / 40 (48 / 62)   48  59 / 41 (78 / 63)
+    // It is the mean that tells. (fp32 rows of 128 dims have no tiles.)
+    constexpr bool kBf16 = std::is_same_v<T, __nv_bfloat16>, kHasTiles = D == 64 || kBf16;
+    constexpr int kFrom = !kBf16 ? 40 : D == 64 ? 36 : 30; // rows of a kv head
     const bool many = static_cast<int64_t>(a.t.rows) * (a.qh / a.kvh) > static_cast<int64_t>(kFrom) * a.t.batch;
     if constexpr (kHasTiles)
         if (many) {

@@ -16,8 +16,8 @@
 // codes as fragments, four codes to a 16-bit element: of K eight dims of a key (the
 // four k slots of two products, in an order that Q follows), of V, transposed, four
 // dims of two keys each. Widening them is most of what the loop does. K's stay
-// integers, one operation a pair of codes, and their scale multiplies the sum over
-// the group's dims; V's are multiplied out, since a scale is a key's there, which
+// integers, one or two operations a pair of codes, and their scale multiplies the sum
+// over the group's dims; V's are multiplied out, since a scale is a key's there, which
 // the product sums over.
 //
 // fp32 rows are two fp16 terms, and so are their weights. Up to 4 rows have two
@@ -42,9 +42,10 @@ template <typename T, int D, int kNT> struct Q4RowsGeo {
     static constexpr int kRows = kPair ? 4 : 8 * kNT;
     static constexpr int kRPL = kPair ? 1 : 2 * kNT;         // rows that a lane has scores of
     static constexpr int kSets = kWide && !kPair ? 2 : 1;    // products of a k step
-    // c + 8 as it is, with 8 sum(q) taken off the sums from the start, costs fp32 rows bits
-    // (the sum is 3 times as large as what is left) and two registers a group and tile
-    static constexpr bool kSigned = kWide || kNT > 1;
+    // K's codes as stored (kv4_subnormals), with 8 sum(q) taken off the sums from the start, take
+    // half the operations of signed ones, two registers a group and tile, and cost accuracy: of
+    // fp32 rows 3.5e-6 for 4e-7
+    static constexpr bool kSigned = kNT > 1 || kWide;
     static constexpr bool kQShared = kSets * kTiles * D > 256; // queries in shared memory, not in registers
     static constexpr int kWarps = kNT <= 2 ? 8 : 4, kThreads = 32 * kWarps;
     // a step: 64 keys where registers and shared memory have room, since what is done once a
@@ -53,7 +54,7 @@ template <typename T, int D, int kNT> struct Q4RowsGeo {
     static constexpr int kStepPages = 2 * kPairs, kStepKeys = kStepPages * kKvPage;
     static constexpr int kStages = kPairs == 2 ? 2 : 3;
     static constexpr int kPageBytes = Kv4Record<D>::kBytes, kStage = kStepPages * kPageBytes;
-    static constexpr int kQBytes = kQShared ? kSets * kTiles * kGroups * 2 * 32 * 8 : 0;
+    static constexpr int kQBytes = kSets * kTiles * kGroups * 2 * 32 * 8 + 128; // fragments; a factor a row
     static constexpr int kRing = kStages * kStage; // of a warp
     static constexpr int kPitch = D + 4; // floats of a row of partial sums
     // O of the warps, then of the CTA; m and l of the warps, then of the CTA
@@ -125,14 +126,14 @@ __device__ __forceinline__ void q4_store4(__nv_bfloat16 *p, const float (&x)[4])
 }
 
 // The scale of a query row (a power of two that brings its largest magnitude `top`
-// to 2^14 .. 2^15, held where its inverse is a normal number) and what scores, in
-// units of 2^-24 for the codes, are multiplied by. NaN where the row holds one, or an
-// infinity. The latter is held to 2^110, where scores stay finite; what differs at
-// all differs by far more than a weight can tell, then.
+// to 2^14 .. 2^15, held where its inverse is a normal number) and what scores are
+// multiplied by. NaN where the row holds one, or an infinity. The latter is held to 2^86,
+// where scores stay finite; what differs at all differs by far more than a weight can
+// tell, then.
 __device__ __forceinline__ float q4_row_scale(float top, float scale_log2, float &factor) {
     const int e = min(max(static_cast<int>(__float_as_uint(top) >> 23) - 127, -106), 127);
     const float up = __uint_as_float(static_cast<uint32_t>(127 + 14 - e) << 23), down = __uint_as_float(static_cast<uint32_t>(127 + e - 14) << 23);
-    factor = fminf(fmaxf(scale_log2 * down, -0x1p86f), 0x1p86f) * 0x1p24f;
+    factor = fminf(fmaxf(scale_log2 * down, -0x1p86f), 0x1p86f);
     if (!(top <= 3.4028235e38f))
         factor = __uint_as_float(0x7fc00000u);
     return up;
@@ -226,13 +227,15 @@ static __global__ void __launch_bounds__(Q4RowsGeo<T, D, kNT>::kThreads)
         fetch(i, i);
 
     // ---- queries, as fragments: column g of a tile, k slots 2t, 2t + 1 and 2t + 8, 2t + 9 of product u: dims 8t + 2u, + 4
-    // and 8t + 2u + 1, + 5 of the group. The latter ones meet codes that are 16 times as large.
-    constexpr int kInRegs = G::kQShared ? 1 : G::kGroups; // (not used where they are shared)
+    // and 8t + 2u + 1, + 5 of the group. Every warp wants the same ones: the tiles are shared out, and handed round through
+    // shared memory.
+    constexpr int kInRegs = G::kQShared ? 1 : G::kGroups; // (not used where they stay in shared memory)
     uint32_t qf[G::kSets][G::kTiles][kInRegs][2][2];
     uint2 *q_shared = reinterpret_cast<uint2 *>(q4_smem); // [set][tile][group][u][lane]
+    float *factors = reinterpret_cast<float *>(q4_smem + G::kQBytes - 4 * G::kRows); // of the scores of each row
     float factor[G::kRPL];
-#pragma unroll
-    for (int nt = 0; nt < G::kTiles; ++nt) {
+#pragma unroll 1
+    for (int nt = warp; nt < G::kTiles; nt += warps) {
         const int r = row_base + (kPair ? g / 2 : nt * 8 + g), node = node_of(r);
         float x[G::kGroups][8];
         float top = 0.f;
@@ -259,14 +262,10 @@ static __global__ void __launch_bounds__(Q4RowsGeo<T, D, kNT>::kThreads)
         }
         top = max_abs_nan(top, __shfl_xor_sync(kFullWarpMask, top, 1), 0.f);
         top = max_abs_nan(top, __shfl_xor_sync(kFullWarpMask, top, 2), 0.f);
-        float mine_f; // of row r: lanes 4 g ..; wanted by the lanes that have its scores
+        float mine_f;
         const float up = q4_row_scale(top, a.scale_log2, mine_f);
-        if constexpr (kPair) {
-            factor[0] = __shfl_sync(kFullWarpMask, mine_f, t * 8);
-        } else {
-            factor[2 * nt] = __shfl_sync(kFullWarpMask, mine_f, t * 8);
-            factor[2 * nt + 1] = __shfl_sync(kFullWarpMask, mine_f, t * 8 + 4);
-        }
+        if (t == 0)
+            factors[kPair ? g / 2 : nt * 8 + g] = G::kSigned ? mine_f : mine_f * 0x1p24f; // (pairs: the same number twice)
 #pragma unroll
         for (int c = 0; c < G::kGroups; ++c)
 #pragma unroll
@@ -274,7 +273,7 @@ static __global__ void __launch_bounds__(Q4RowsGeo<T, D, kNT>::kThreads)
                 uint32_t f[2][2]; // [term][slots]
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
-                    const float less = i == 0 ? up : up * 0.0625f;
+                    const float less = i == 0 || G::kSigned ? up : up * 0.0625f; // stored codes: these are 16 times as large
                     float v0 = x[c][2 * u + i] * less, v1 = x[c][2 * u + i + 4] * less;
                     f[0][i] = q4_term(v0, v1);
                     f[1][i] = half2_rn(v0, v1);
@@ -282,18 +281,26 @@ static __global__ void __launch_bounds__(Q4RowsGeo<T, D, kNT>::kThreads)
                         f[0][i] = g & 1 ? f[1][i] : f[0][i];
                 }
 #pragma unroll
-                for (int set = 0; set < G::kSets; ++set) {
-                    if constexpr (G::kQShared) {
-                        if (warp == 0)
-                            q_shared[(((set * G::kTiles + nt) * G::kGroups + c) * 2 + u) * 32 + lane] = make_uint2(f[set][0], f[set][1]);
-                    } else {
-                        qf[set][nt][c][u][0] = f[set][0], qf[set][nt][c][u][1] = f[set][1];
-                    }
-                }
+                for (int set = 0; set < G::kSets; ++set)
+                    q_shared[(((set * G::kTiles + nt) * G::kGroups + c) * 2 + u) * 32 + lane] = make_uint2(f[set][0], f[set][1]);
             }
     }
-    if constexpr (G::kQShared)
-        __syncthreads();
+    __syncthreads();
+#pragma unroll
+    for (int rr = 0; rr < G::kRPL; ++rr)
+        factor[rr] = factors[kPair ? t : rr / 2 * 8 + 2 * t + rr % 2];
+    if constexpr (!G::kQShared)
+#pragma unroll
+        for (int set = 0; set < G::kSets; ++set)
+#pragma unroll
+            for (int nt = 0; nt < G::kTiles; ++nt)
+#pragma unroll
+                for (int c = 0; c < G::kGroups; ++c)
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) {
+                        const uint2 f = q_shared[(((set * G::kTiles + nt) * G::kGroups + c) * 2 + u) * 32 + lane];
+                        qf[set][nt][c][u][0] = f.x, qf[set][nt][c][u][1] = f.y;
+                    }
     // what codes of 8 everywhere would sum to: where the sums start when codes come with 8 added
     float start[G::kSigned ? 1 : G::kGroups][2];
     if constexpr (!G::kSigned) {
@@ -335,8 +342,17 @@ static __global__ void __launch_bounds__(Q4RowsGeo<T, D, kNT>::kThreads)
                 uint32_t w[4], k[4][4];
                 q4_ldmatrix<false>(stage_at + pp * 2 * G::kPageBytes + c * 256, w);
 #pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    kv4_integers<G::kSigned>(w[j], k[j]);
+                for (int j = 0; j < 4; ++j) {
+                    if constexpr (G::kSigned) {
+                        __half2 c4[4];
+                        kv4_integers(w[j], c4);
+#pragma unroll
+                        for (int i4 = 0; i4 < 4; ++i4)
+                            k[j][i4] = kv4_bits(c4[i4]);
+                    } else {
+                        kv4_subnormals(w[j], k[j]);
+                    }
+                }
                 float sum[2][G::kTiles][4];
 #pragma unroll
                 for (int p = 0; p < 2; ++p)

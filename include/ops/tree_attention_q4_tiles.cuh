@@ -380,7 +380,7 @@ static __global__ void __launch_bounds__(kTileThreads, 1)
                 if constexpr (G::kWide)
                     *reinterpret_cast<uint4 *>(dst + G::kSlabs * kM * G::kSlab) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
                 if (lane % kLanes == 0)
-                    row_fac[r] = factor * 0x1p-24f; // codes are themselves here, not integers times 2^-24
+                    row_fac[r] = factor;
             }
         }
         sm100::fence_proxy_async_smem();
