@@ -139,37 +139,42 @@ __device__ __forceinline__ float q4_row_scale(float top, float scale_log2, float
     return up;
 }
 
-// The span of the sequence with the `order`-th most work (the longest context, equal
-// ones by index): CTAs come longest first, and those that share an SM differ. Every
-// thread of the block calls it; `room` is shared memory for 4 ints and one more a
-// sequence, batch <= the block's threads.
-__device__ __forceinline__ TreeSpan q4_span_by_work(const TreeBatch &t, int order, int *room) {
+// The span of the sequence that CTAs with z = `order` take: the one with the
+// order-th most work (the longest context, equal ones by index) up to `descending`,
+// from there on the one with the least first. So CTAs come longest first, or, where
+// all run at once and each SM gets some of the first and of the second kind, long ones
+// share an SM with short ones. Every thread of the block calls it; `room` is shared
+// memory for 4 ints and one more a sequence.
+__device__ __forceinline__ TreeSpan q4_span_by_work(const TreeBatch &t, int order, int descending, int *room) {
     const int tid = threadIdx.x;
-    TreeSpan mine{};
-    if (tid < t.batch) {
-        mine = TreeSpan(t, tid);
-        room[4 + tid] = mine.n > 0 ? mine.ctx : -1;
+    if (order >= descending)
+        order = t.batch - 1 - (order - descending);
+    for (int b = tid; b < t.batch; b += blockDim.x) {
+        const TreeSpan s(t, b);
+        room[4 + b] = s.n > 0 ? s.ctx : -1;
     }
     __syncthreads();
-    if (tid < t.batch) {
-        const int work = room[4 + tid];
+    for (int b0 = 0; b0 < t.batch; b0 += blockDim.x / 8) { // eight threads a sequence
+        const int b = b0 + tid / 8, work = b < t.batch ? room[4 + b] : 0;
         int before = 0;
-        for (int i = 0; i < t.batch; ++i)
-            before += room[4 + i] > work || (room[4 + i] == work && i < tid) ? 1 : 0;
-        if (before == order)
-            room[0] = mine.b, room[1] = mine.row0, room[2] = mine.n, room[3] = mine.ctx;
+        if (b < t.batch)
+            for (int i = tid % 8; i < t.batch; i += 8)
+                before += room[4 + i] > work || (room[4 + i] == work && i < b) ? 1 : 0;
+#pragma unroll
+        for (int off = 1; off < 8; off <<= 1)
+            before += __shfl_xor_sync(kFullWarpMask, before, off);
+        if (b < t.batch && before == order && tid % 8 == 0)
+            room[0] = b;
     }
     __syncthreads();
-    TreeSpan s{};
-    s.b = room[0], s.row0 = room[1], s.n = room[2], s.ctx = room[3];
-    s.set_keys(t);
+    const TreeSpan s(t, room[0]);
     __syncthreads(); // `room` may lie where copies go next
     return s;
 }
 
 template <typename T, int D, int kNT>
 static __global__ void __launch_bounds__(Q4RowsGeo<T, D, kNT>::kThreads)
-    q4_rows_kernel(const T *__restrict__ q, T *__restrict__ out, TreeArgs a, int rep, int splits, bool sorted) {
+    q4_rows_kernel(const T *__restrict__ q, T *__restrict__ out, TreeArgs a, int rep, int splits, int descending) {
     using G = Q4RowsGeo<T, D, kNT>;
     using R = Kv4Record<D>;
     constexpr bool kPair = G::kPair;
@@ -182,7 +187,7 @@ static __global__ void __launch_bounds__(Q4RowsGeo<T, D, kNT>::kThreads)
         group = rank / splits, rank -= group * splits;
     pdl_trigger();
     pdl_wait();
-    const TreeSpan span = sorted ? q4_span_by_work(a.t, blockIdx.z, reinterpret_cast<int *>(q4_smem)) : TreeSpan(a.t, blockIdx.z);
+    const TreeSpan span = descending > 0 ? q4_span_by_work(a.t, blockIdx.z, descending, reinterpret_cast<int *>(q4_smem)) : TreeSpan(a.t, blockIdx.z);
     const int b = span.b, row_base = group * G::kRows, rows = span.n * rep;
     if (row_base >= rows)
         return; // the whole cluster
@@ -315,7 +320,7 @@ static __global__ void __launch_bounds__(Q4RowsGeo<T, D, kNT>::kThreads)
         }
     }
 
-    float o[G::kGroups][2][G::kTiles][kPair && G::kWide ? 2 : 4] = {}; // dims 32 c + 4 g + 2 i and + 1 of the lane's rows
+    float o[G::kGroups][2][G::kTiles][kPair ? 2 : 4] = {}; // dims 32 c + 4 g + 2 i and + 1 of the lane's rows
     float m[G::kRPL], l[G::kRPL];
 #pragma unroll
     for (int rr = 0; rr < G::kRPL; ++rr)
@@ -517,15 +522,15 @@ static __global__ void __launch_bounds__(Q4RowsGeo<T, D, kNT>::kThreads)
                         const uint32_t f[4] = {v[2 * p][2 * n], v[2 * p][2 * n + 1], v[2 * p + 1][2 * n], v[2 * p + 1][2 * n + 1]};
 #pragma unroll
                         for (int nt = 0; nt < G::kTiles; ++nt) {
-                            if constexpr (G::kWide)
+                            if constexpr (G::kWide || kPair)
                                 mma_f16(sum[nt], f, pf[set][nt][p][0], pf[set][nt][p][1]);
                             else
                                 mma_f16(o[c][n][nt], f, pf[set][nt][p][0], pf[set][nt][p][1]);
                         }
                     }
-                if constexpr (G::kWide && kPair) {
-                    o[c][n][0][0] += sum[0][0] + sum[0][1];
-                    o[c][n][0][1] += sum[0][2] + sum[0][3];
+                if constexpr (kPair) { // (the second column of bf16 rows is zero)
+                    o[c][n][0][0] += G::kWide ? sum[0][0] + sum[0][1] : sum[0][0];
+                    o[c][n][0][1] += G::kWide ? sum[0][2] + sum[0][3] : sum[0][2];
                 } else if constexpr (G::kWide) {
 #pragma unroll
                     for (int nt = 0; nt < G::kTiles; ++nt)
@@ -551,10 +556,8 @@ static __global__ void __launch_bounds__(Q4RowsGeo<T, D, kNT>::kThreads)
             float y[4];
 #pragma unroll
             for (int n = 0; n < 2; ++n) {
-                if constexpr (kPair && G::kWide) {
+                if constexpr (kPair) {
                     y[2 * n] = o[c][n][0][0], y[2 * n + 1] = o[c][n][0][1];
-                } else if constexpr (kPair) {
-                    y[2 * n] = o[c][n][0][0] + o[c][n][0][1], y[2 * n + 1] = o[c][n][0][2] + o[c][n][0][3];
                 } else {
                     y[2 * n] = o[c][n][rr / 2][rr % 2], y[2 * n + 1] = o[c][n][rr / 2][2 + rr % 2];
                 }
@@ -652,9 +655,14 @@ template <typename T, int D, int kNT> inline void q4_rows_launch(const T *q, T *
     const int64_t cap = std::min<int64_t>(most, steps / (2 * G::kWarps));
     int splits = split ? static_cast<int>(std::max<int64_t>(1, std::min(cap, slots * 4 / 3 / all))) : 1;
     require(groups * splits <= 0x7fffffff, "tree attention: too many rows for one call");
-    const bool sort = a.t.batch > 1 && a.t.batch <= G::kThreads && all * splits > sms;
+    // sequences in the order of their length, where SMs have more than one CTA (their list is short
+    // beside the rings)
+    const int64_t per_sequence = groups * splits * a.kvh, total = per_sequence * a.t.batch;
+    int descending = 0;
+    if (a.t.batch > 1 && a.t.batch <= 1024 && total > sms)
+        descending = total <= slots ? static_cast<int>(std::min<int64_t>(a.t.batch, (sms + per_sequence - 1) / per_sequence)) : a.t.batch;
     launch_ex_cluster(kernel, dim3(static_cast<unsigned>(groups * splits), a.kvh, a.t.batch), dim3(splits), dim3(G::kThreads), G::kBytes, stream,
-                      q, out, a, a.qh / a.kvh, splits, sort);
+                      q, out, a, a.qh / a.kvh, splits, descending);
 }
 
 template <typename T, int D> inline void q4_rows_call(const T *q, T *out, const TreeArgs &a, cudaStream_t stream) {

@@ -130,7 +130,7 @@ static __global__ void __launch_bounds__(kTileThreads, 1)
     sm100::tc_fence_after();
     const uint32_t tmem = *tmem_slot;
     pdl_wait();
-    const TreeSpan span = sorted ? q4_span_by_work(a.t, blockIdx.z, reinterpret_cast<int *>(row_fac)) : TreeSpan(a.t, blockIdx.z);
+    const TreeSpan span = sorted ? q4_span_by_work(a.t, blockIdx.z, a.t.batch, reinterpret_cast<int *>(row_fac)) : TreeSpan(a.t, blockIdx.z);
     const int b = span.b, row_base = group * G::kRows, rows = span.n * rep;
     int keys = span.keys;
     if (a.t.mask == nullptr) // a chain: nothing after the group's last node is seen
