@@ -586,7 +586,7 @@ static __global__ void __launch_bounds__(kTileThreads, 1)
             };
             await(xa); // (both)
             high = scored(xa);
-#pragma unroll 1
+#pragma unroll
             for (int c = 0; c < 4; c += 2) {
                 chunk(c, xa, xb);
                 chunk(c + 1, xb, xa);

@@ -587,6 +587,26 @@ def test_blocks_whose_offsets_pass_32_bits(ops, dim):
     assert torch.equal(back[0].cpu().double(), q4_plain.dequantise(*q4_plain.quantise(x.cpu()))) and torch.equal(back[0], back[1])
 
 
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("n,rep", [(1, 4), (1, 8), (6, 4), (30, 4)])
+def test_fp32_rows_are_as_near_to_64_bits_as_fp32_sums_are(ops, dim, n, rep):
+    """The 2-norm of the error against that of the same attention in fp32 torch, over 2 heads of 800 keys."""
+    ctx, kvh = 800, 2
+    cache = q4_plain.Cache4([ctx + n], kvh, dim, 3)
+    q = torch.randn(n, kvh * rep * dim, generator=torch.Generator().manual_seed(1))
+    got = attention_case(ops, 0, dim, kvh, rep, [ctx], [n], cache=cache, q=q, trees="chain")
+    sees = [plain.tree(None, n, "chain")[1]]
+    want, _, _ = plain.attention(cache, q.view(n, kvh * rep, dim), [ctx], [0, n], sees, 1 / math.sqrt(dim))
+    k, v = (x.float() for x in cache.rows(0))
+    rows32 = torch.empty_like(want)
+    for i in range(n):
+        for h in range(kvh * rep):
+            p = (k[: ctx + i + 1, h // rep] @ q[i].view(-1, dim)[h]) / math.sqrt(dim)
+            p = (p - p.max()).exp()
+            rows32[i, h] = (p @ v[: ctx + i + 1, h // rep]) / p.sum()
+    assert (got - want).norm() <= 1.5 * (rows32 - want).norm()
+
+
 # ------------------------------------------------------------------ commit
 
 
