@@ -126,15 +126,6 @@ __device__ __forceinline__ void kv4_widen(uint32_t w, __half2 scale, uint32_t (&
         h[i] = kv4_bits(__hmul2(c[i], scale));
 }
 
-// Half the operations: code + 8 as it is stored, pairs 0 and 2 times 2^-24, 1 and 3
-// times 2^-20 (fp16's subnormal numbers are integers times 2^-24). Sums of products with
-// subnormal factors are good to 2^-19 only: the tensor cores line products up as if
-// their factors were normal.
-__device__ __forceinline__ void kv4_subnormals(uint32_t w, uint32_t (&h)[4]) {
-    const uint32_t hi = w >> 8;
-    h[0] = w & 0x000f000fu, h[1] = w & 0x00f000f0u, h[2] = hi & 0x000f000fu, h[3] = hi & 0x00f000f0u;
-}
-
 struct Kv4Rows {
     const int64_t *slots;
     int rows, kvh;

@@ -16,8 +16,8 @@
 // codes as fragments, four codes to a 16-bit element: of K eight dims of a key (the
 // four k slots of two products, in an order that Q follows), of V, transposed, four
 // dims of two keys each. Widening them is most of what the loop does. K's stay
-// integers, one or two operations a pair of codes, and their scale multiplies the sum
-// over the group's dims; V's are multiplied out, since a scale is a key's there, which
+// integers, two operations a pair of codes, and their scale multiplies the sum over
+// the group's dims; V's are multiplied out, since a scale is a key's there, which
 // the product sums over.
 //
 // fp32 rows are two fp16 terms, and so are their weights. Up to 4 rows have two
@@ -42,10 +42,6 @@ template <typename T, int D, int kNT> struct Q4RowsGeo {
     static constexpr int kRows = kPair ? 4 : 8 * kNT;
     static constexpr int kRPL = kPair ? 1 : 2 * kNT;         // rows that a lane has scores of
     static constexpr int kSets = kWide && !kPair ? 2 : 1;    // products of a k step
-    // K's codes as stored (kv4_subnormals), with 8 sum(q) taken off the sums from the start, take
-    // half the operations of signed ones, two registers a group and tile, and cost accuracy: of
-    // fp32 rows 3.5e-6 for 4e-7
-    static constexpr bool kSigned = kNT > 1 || kWide;
     static constexpr bool kQShared = kSets * kTiles * D > 256; // queries in shared memory, not in registers
     static constexpr int kWarps = kNT <= 2 ? 8 : 4, kThreads = 32 * kWarps;
     // a step: 64 keys where registers and shared memory have room, since what is done once a
@@ -173,7 +169,7 @@ __device__ __forceinline__ TreeSpan q4_span_by_work(const TreeBatch &t, int orde
 }
 
 template <typename T, int D, int kNT>
-static __global__ void __launch_bounds__(Q4RowsGeo<T, D, kNT>::kThreads)
+static __global__ void __launch_bounds__(Q4RowsGeo<T, D, kNT>::kThreads, kNT <= 1 ? 2 : 1)
     q4_rows_kernel(const T *__restrict__ q, T *__restrict__ out, TreeArgs a, int rep, int splits, int descending) {
     using G = Q4RowsGeo<T, D, kNT>;
     using R = Kv4Record<D>;
@@ -270,7 +266,7 @@ static __global__ void __launch_bounds__(Q4RowsGeo<T, D, kNT>::kThreads)
         float mine_f;
         const float up = q4_row_scale(top, a.scale_log2, mine_f);
         if (t == 0)
-            factors[kPair ? g / 2 : nt * 8 + g] = G::kSigned ? mine_f : mine_f * 0x1p24f; // (pairs: the same number twice)
+            factors[kPair ? g / 2 : nt * 8 + g] = mine_f; // (pairs: the same number twice)
 #pragma unroll
         for (int c = 0; c < G::kGroups; ++c)
 #pragma unroll
@@ -278,8 +274,7 @@ static __global__ void __launch_bounds__(Q4RowsGeo<T, D, kNT>::kThreads)
                 uint32_t f[2][2]; // [term][slots]
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
-                    const float less = i == 0 || G::kSigned ? up : up * 0.0625f; // stored codes: these are 16 times as large
-                    float v0 = x[c][2 * u + i] * less, v1 = x[c][2 * u + i + 4] * less;
+                    float v0 = x[c][2 * u + i] * up, v1 = x[c][2 * u + i + 4] * up;
                     f[0][i] = q4_term(v0, v1);
                     f[1][i] = half2_rn(v0, v1);
                     if constexpr (kPair)
@@ -306,20 +301,6 @@ static __global__ void __launch_bounds__(Q4RowsGeo<T, D, kNT>::kThreads)
                         const uint2 f = q_shared[(((set * G::kTiles + nt) * G::kGroups + c) * 2 + u) * 32 + lane];
                         qf[set][nt][c][u][0] = f.x, qf[set][nt][c][u][1] = f.y;
                     }
-    // what codes of 8 everywhere would sum to: where the sums start when codes come with 8 added
-    float start[G::kSigned ? 1 : G::kGroups][2];
-    if constexpr (!G::kSigned) {
-        const uint32_t eight[4] = {0x00080008u, 0x00080008u, 0x00800080u, 0x00800080u};
-#pragma unroll
-        for (int c = 0; c < G::kGroups; ++c) {
-            float sum[4] = {};
-#pragma unroll
-            for (int u = 0; u < 2; ++u)
-                mma_f16(sum, eight, qf[0][0][c][u][0], qf[0][0][c][u][1]);
-            start[c][0] = -sum[0], start[c][1] = -sum[1];
-        }
-    }
-
     float o[G::kGroups][2][G::kTiles][kPair ? 2 : 4] = {}; // dims 32 c + 4 g + 2 i and + 1 of the lane's rows
     float m[G::kRPL], l[G::kRPL];
 #pragma unroll
@@ -348,15 +329,11 @@ static __global__ void __launch_bounds__(Q4RowsGeo<T, D, kNT>::kThreads)
                 q4_ldmatrix<false>(stage_at + pp * 2 * G::kPageBytes + c * 256, w);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    if constexpr (G::kSigned) {
-                        __half2 c4[4];
-                        kv4_integers(w[j], c4);
+                    __half2 codes[4];
+                    kv4_integers(w[j], codes);
 #pragma unroll
-                        for (int i4 = 0; i4 < 4; ++i4)
-                            k[j][i4] = kv4_bits(c4[i4]);
-                    } else {
-                        kv4_subnormals(w[j], k[j]);
-                    }
+                    for (int n = 0; n < 4; ++n)
+                        k[j][n] = kv4_bits(codes[n]);
                 }
                 float sum[2][G::kTiles][4];
 #pragma unroll
@@ -365,7 +342,7 @@ static __global__ void __launch_bounds__(Q4RowsGeo<T, D, kNT>::kThreads)
                     for (int nt = 0; nt < G::kTiles; ++nt)
 #pragma unroll
                         for (int e = 0; e < 4; ++e)
-                            sum[p][nt][e] = G::kSigned ? 0.f : start[G::kSigned ? 0 : c][e & 1];
+                            sum[p][nt][e] = 0.f;
 #pragma unroll
                 for (int set = G::kSets - 1; set >= 0; --set)
 #pragma unroll
