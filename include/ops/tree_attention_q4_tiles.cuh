@@ -27,6 +27,13 @@
 // O and the tile's weights so far are multiplied down in place. So scores are looked
 // at once.
 //
+// What bounds it is the chain of a tile: scores, softmax, weights, sum, each waiting for
+// the one before: 5,300 cycles for 256 rows x 128 keys, of which the products are 2,048
+// and the exponentials as much, side by side (tensor pipe 37 % busy, exponentials 38 %).
+// Measured (kernel time, one B200): 3 prompts' pieces of up to 2048 rows x 32 heads behind
+// up to 2100 tokens, 8 x 128 bf16: 324 us, 0.70 PFLOP/s; 8 trees of up to 26 nodes x 32
+// heads over up to 4099 tokens, 8 x 64 fp32: 41 us.
+//
 // fp32 rows have two fp16 terms of Q and P. The tensor cores cut an accumulator off
 // at every step, so for them O is the sum over one tile and is added, rounded, to a
 // sum of its own in tensor memory, which has room for that at D = 64 only.
