@@ -6,8 +6,8 @@
 // reference counterpart.
 //
 // What is held there is an fp16 number, so K and V enter the tensor cores' fp16
-// products exactly, with no units and no factors behind them: scores are q . k as
-// they are, weights times V too. A query row is scaled by a power of two, to a
+// products exactly, with no units and no factors behind them (the rows kernel takes
+// K's codes, and multiplies the sum over a group's dims by the scale in fp32). A query row is scaled by a power of two, to a
 // largest magnitude of 2^14 to 2^15, and is one fp16 term where it comes in bf16
 // (exact down to 2^-29 of the largest), two where it comes in fp32 (22 bits).
 
@@ -23,12 +23,12 @@ template <typename T, int D> inline void q4_call(const T *q, T *out, const TreeA
     // The rows kernel's time grows with the rows, that of 128-row tiles does not. 8 (32)
     // sequences of 4096 (2048) tokens with up to n rows of a kv head, 0.8 n on average, 8 kv
     // heads, us with rows / tiles:
-    //   fp32 rows, D 64     n = 32  37 / 44 (40 / 67)   48  49 / 45 (66 / 68)   64  52 / 45 (70 / 69)
-    //   bf16 rows, D 64     n = 32  30 / 31 (29 / 48)   48  37 / 31 (48 / 49)   64  39 / 32 (51 / 51)
-    //   bf16 rows, D 128    n = 24  43 / 40 (46 / 61)   32  44 / 40 (48 / 62)   48  59 / 41 (78 / 63)
+    //   fp32 rows, D 64     n = 32  34 / 40 (39 / 61)   48  46 / 40 (62 / 63)   64  49 / 40 (65 / 64)   96  64 / 41 (93 / 64)
+    //   bf16 rows, D 64     n = 32  28 / 31 (28 / 48)   48  36 / 31 (45 / 49)   64  37 / 31 (47 / 50)   96  48 / 32 (68 / 52)
+    //   bf16 rows, D 128    n = 24  39 / 41 (44 / 63)   32  40 / 42 (45 / 63)   48  55 / 43 (73 / 64)   64  59 / 43 (77 / 65)
     // It is the mean that tells. (fp32 rows of 128 dims have no tiles.)
     constexpr bool kBf16 = std::is_same_v<T, __nv_bfloat16>, kHasTiles = D == 64 || kBf16;
-    constexpr int kFrom = !kBf16 ? 40 : D == 64 ? 36 : 30; // rows of a kv head
+    constexpr int kFrom = !kBf16 ? 37 : D == 64 ? 40 : 32; // rows of a kv head
     const bool many = static_cast<int64_t>(a.t.rows) * (a.qh / a.kvh) > static_cast<int64_t>(kFrom) * a.t.batch;
     if constexpr (kHasTiles)
         if (many) {

@@ -131,14 +131,14 @@ __device__ __forceinline__ void q4_store4(__nv_bfloat16 *p, const float (&x)[4])
 
 // The scale of a query row (a power of two that brings its largest magnitude `top`
 // to 2^14 .. 2^15, held where its inverse is a normal number) and what scores are
-// multiplied by. NaN where the row holds one, or an infinity. The latter is held to 2^86,
+// multiplied by. NaN where the row holds one, or an infinity, or the scale is one. The latter is held to 2^86,
 // where scores stay finite; what differs at all differs by far more than a weight can
 // tell, then.
 __device__ __forceinline__ float q4_row_scale(float top, float scale_log2, float &factor) {
     const int e = min(max(static_cast<int>(__float_as_uint(top) >> 23) - 127, -106), 127);
     const float up = __uint_as_float(static_cast<uint32_t>(127 + 14 - e) << 23), down = __uint_as_float(static_cast<uint32_t>(127 + e - 14) << 23);
     factor = fminf(fmaxf(scale_log2 * down, -0x1p86f), 0x1p86f);
-    if (!(top <= 3.4028235e38f))
+    if (!(top <= 3.4028235e38f) || scale_log2 != scale_log2)
         factor = __uint_as_float(0x7fc00000u);
     return up;
 }
@@ -656,7 +656,9 @@ template <typename T, int D> inline void q4_rows_call(const T *q, T *out, const 
         q4_rows_launch<T, D, 0>(q, out, a, stream);
     else if (rows <= 8)
         q4_rows_launch<T, D, 1>(q, out, a, stream);
-    else if (rows <= 16 || (D == 128 && std::is_same_v<T, float>))
+    else if constexpr (D == 128 && std::is_same_v<T, float>) // (four tiles do not fit into registers)
+        q4_rows_launch<T, D, 2>(q, out, a, stream);
+    else if (rows <= 16)
         q4_rows_launch<T, D, 2>(q, out, a, stream);
     else
         q4_rows_launch<T, D, 4>(q, out, a, stream);

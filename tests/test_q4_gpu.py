@@ -531,6 +531,38 @@ def test_two_calls_give_the_same_bits(ops, kind, n):
 
 @pytest.mark.parametrize("kind", [0, 1])
 @pytest.mark.parametrize("n", [1, 40])
+def test_a_scale_that_is_no_number_gives_nan(ops, kind, n):
+    cache = q4_plain.Cache4([90 + n], 1, 64, 3)
+    q = torch.randn(n, 256, device="cuda").to(TYPES[kind])
+    out = torch.zeros(n, 256, dtype=TYPES[kind], device="cuda")
+    ops.tree_attention_q4(q, kind, 256, dev(cache.pool), dev(cache.table), cache.stride, ints([90]), ints([0, n]), None, 0, 1, n, n, 90, 4, 1, 64, float("nan"), out, 256, 0)
+    assert out.isnan().all()
+
+
+@pytest.mark.parametrize("kind", [0, 1])
+@pytest.mark.parametrize("n", [1, 6, 60])
+def test_calls_on_two_streams_at_once(ops, kind, n):
+    """Many calls on two streams, of their own inputs over one pool: each gives what it gives alone."""
+    cache = q4_plain.Cache4([700 + n, 300 + n], 2, 64, 3)
+    pool, table, lens, start = dev(cache.pool), dev(cache.table), ints([700, 300]), ints([0, n, 2 * n])
+    q = [torch.randn(2 * n, 512, generator=torch.Generator().manual_seed(i)).to(TYPES[kind]).cuda() for i in range(2)]
+    call = lambda x, out, s: ops.tree_attention_q4(x, kind, 512, pool, table, cache.stride, lens, start, None, 0, 2, 2 * n, n, 700, 8, 2, 64, 0.125, out, 512, s)  # noqa: E731
+    alone = [torch.empty_like(x) for x in q]
+    for x, out in zip(q, alone):
+        call(x, out, 0)
+    both = [[torch.empty_like(x) for _ in range(20)] for x in q]
+    streams = [torch.cuda.Stream() for _ in q]
+    torch.cuda.synchronize()
+    for i in range(20):
+        for x, outs, s in zip(q, both, streams):
+            call(x, outs[i], s.cuda_stream)
+    torch.cuda.synchronize()
+    for a, outs in zip(alone, both):
+        assert all(torch.equal(a, out) for out in outs)
+
+
+@pytest.mark.parametrize("kind", [0, 1])
+@pytest.mark.parametrize("n", [1, 40])
 def test_bounds_that_are_larger_than_the_lengths(ops, kind, n):
     """Plans for more rows and a longer context than there are: padded steps of a captured graph."""
     attention_case(ops, kind, 64, 2, 4, [50, 700], [n, 3], max_ctx=30000, seed=2)
