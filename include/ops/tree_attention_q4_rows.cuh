@@ -634,11 +634,16 @@ template <typename T, int D, int kNT> inline void q4_rows_launch(const T *q, T *
     const int64_t keys = static_cast<int64_t>(a.t.max_ctx) + a.t.max_rows, steps = (keys + G::kStepKeys - 1) / G::kStepKeys;
     // A cluster costs 2 us and more (32 sequences x 8 heads with nothing to do: 5.3 us, 7 with
     // clusters of two), so keys are split only where there are SMs to spare or each warp has 16
-    // steps and more; then into a third more CTAs than run at once, since sequences differ in
-    // length (12 x 8 of 32,000 tokens, 296 at once: 99.6 us with 3 splits, 90.4 with 4).
-    const bool split = all < sms || steps >= 16 * G::kWarps;
-    const int64_t cap = std::min<int64_t>(most, steps / (2 * G::kWarps));
-    int splits = split ? static_cast<int>(std::max<int64_t>(1, std::min(cap, slots * 4 / 3 / all))) : 1;
+    // steps and more; then into up to a third more CTAs than run at once, since sequences differ
+    // in length, while each warp keeps one or two steps. By powers of two, which fill the device's
+    // groups of SMs: 12 x 8 of 32,000 tokens, 296 CTAs at once: 113 us with 2 splits, 109 with 3,
+    // 87 with 4, 91 with 5; 16 x 8 of 4,000: 16.1 with 1, 14.5 with 2, 20.9 with 3; 4 x 8 of
+    // 32,000: 48 with 4 and 12, 41 with 8.
+    const int64_t cap = std::min<int64_t>(most, 2 * steps / (3 * G::kWarps));
+    int64_t splits = 1;
+    if (all < sms || steps >= 16 * G::kWarps)
+        while (2 * splits <= cap && 2 * splits * all * 3 <= slots * 4)
+            splits *= 2;
     require(groups * splits <= 0x7fffffff, "tree attention: too many rows for one call");
     // sequences in the order of their length, where SMs have more than one CTA (their list is short
     // beside the rings)
@@ -646,8 +651,8 @@ template <typename T, int D, int kNT> inline void q4_rows_launch(const T *q, T *
     int descending = 0;
     if (a.t.batch > 1 && a.t.batch <= 1024 && total > sms)
         descending = total <= slots ? static_cast<int>(std::min<int64_t>(a.t.batch, (sms + per_sequence - 1) / per_sequence)) : a.t.batch;
-    launch_ex_cluster(kernel, dim3(static_cast<unsigned>(groups * splits), a.kvh, a.t.batch), dim3(splits), dim3(G::kThreads), G::kBytes, stream,
-                      q, out, a, a.qh / a.kvh, splits, descending);
+    launch_ex_cluster(kernel, dim3(static_cast<unsigned>(groups * splits), a.kvh, a.t.batch), dim3(static_cast<unsigned>(splits)), dim3(G::kThreads), G::kBytes, stream,
+                      q, out, a, a.qh / a.kvh, static_cast<int>(splits), descending);
 }
 
 template <typename T, int D> inline void q4_rows_call(const T *q, T *out, const TreeArgs &a, cudaStream_t stream) {

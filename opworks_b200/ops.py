@@ -113,9 +113,10 @@ _PLAIN = frozenset((int, float, type(None)))
 
 
 def _arg(a):
-    if hasattr(a, "data_ptr"):
+    try:
         return a.data_ptr()
-    return a
+    except AttributeError:
+        return a
 
 
 _cache = {}
