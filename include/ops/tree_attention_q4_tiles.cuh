@@ -757,6 +757,35 @@ static __global__ void __launch_bounds__(kTileThreads, 1)
     cluster_sync_all(); // peers read this CTA's shared memory until here
 }
 
+// Clusters of `size` CTAs that run at once on the current device. Asked once.
+template <typename... P> inline int q4_clusters(void (*kernel)(P...), int threads, int bytes, int size) {
+    struct Known {
+        const void *kernel;
+        int device, size, clusters;
+    };
+    static thread_local std::vector<Known> mine;
+    const int device = device_facts().device;
+    for (const Known &k : mine)
+        if (k.kernel == reinterpret_cast<const void *>(kernel) && k.device == device && k.size == size)
+            return k.clusters;
+    cudaLaunchConfig_t cfg{};
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = static_cast<unsigned>(size), attr.val.clusterDim.y = 1, attr.val.clusterDim.z = 1;
+    cfg.gridDim = dim3(static_cast<unsigned>(size));
+    cfg.blockDim = dim3(static_cast<unsigned>(threads));
+    cfg.dynamicSmemBytes = static_cast<size_t>(bytes);
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    int clusters = 0;
+    if (cudaOccupancyMaxActiveClusters(&clusters, kernel, &cfg) != cudaSuccess) {
+        cudaGetLastError(); // no more than an answer to the question
+        clusters = 0;
+    }
+    mine.push_back({reinterpret_cast<const void *>(kernel), device, size, clusters});
+    return clusters;
+}
+
 template <typename T, int D, int kM> inline void q4_tiles_launch(const T *q, T *out, const TreeArgs &a, cudaStream_t stream) {
     using G = Q4TilesGeo<T, D, kM>;
     static_assert(G::kBytes <= 232448, "shared memory");
@@ -765,8 +794,10 @@ template <typename T, int D, int kM> inline void q4_tiles_launch(const T *q, T *
     const int64_t rows = static_cast<int64_t>(a.t.max_rows) * (a.qh / a.kvh);
     const int64_t groups = (rows + G::kRows - 1) / G::kRows, all = groups * a.kvh * a.t.batch;
     const int64_t tiles = (static_cast<int64_t>(a.t.max_ctx) + a.t.max_rows + kTileKeys - 1) / kTileKeys;
-    // as many splits as all CTAs still run at once and each has four tiles
-    const int splits = static_cast<int>(std::max<int64_t>(1, std::min(std::min<int64_t>(8, tiles / 4), device_facts().sm_count / all)));
+    // splits (powers of two) while all clusters still run at once and each CTA has four tiles
+    int splits = 1;
+    while (2 * splits <= 8 && 8 * splits <= tiles && all <= q4_clusters(kernel, kTileThreads, G::kBytes, 2 * splits))
+        splits *= 2;
     require(groups * splits <= 0x7fffffff, "tree attention: too many rows for one call");
     // more CTAs than places: sequences in the order of their length (the list of them lies over row_fac, stat and joined)
     const bool sorted = a.t.batch > 1 && a.t.batch <= kTileThreads && all * splits > device_facts().sm_count;
