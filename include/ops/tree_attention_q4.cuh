@@ -49,6 +49,7 @@ inline void tree_attention_q4(const T *q, int64_t q_stride, const uint8_t *pool,
                               int head_dim, float scale, T *out, int64_t out_stride, cudaStream_t stream = nullptr) {
     using namespace detail;
     validate_tree(t, q, out, q_stride, out_stride, sizeof(T), q_heads, kv_heads, head_dim, pool, pool);
+    require(static_cast<int64_t>(t.max_rows) * (q_heads / kv_heads) <= 0x7fffffff, "tree attention: too many rows for one call");
     if (t.batch == 0 || t.max_rows == 0)
         return;
     const TreeArgs a{t, pool, nullptr, q_heads, kv_heads, scale * kLog2e, q_stride, out_stride};

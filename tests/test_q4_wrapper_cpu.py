@@ -64,7 +64,7 @@ def test_attention_and_commit_refuse(ops):
     refuses(ops.tree_attention_q4, good, [dict(type=2), dict(q=None), dict(out=None), dict(pool=None), dict(table=None), dict(ctx=None), dict(start=None),
                                           dict(stride=0), dict(words=0), dict(batch=-1), dict(batch=70000), dict(rows=-1), dict(most=6), dict(most_ctx=-1),
                                           dict(qh=7), dict(kvh=0), dict(dim=32), dict(dim=256), dict(qs=500), dict(os=511), dict(qs=514), dict(q=A + 4),
-                                          dict(pool=A + 8), dict(out=A + 8)])
+                                          dict(pool=A + 8), dict(out=A + 8), dict(mask=None, rows=2**30, most=2**30)])
     good = dict(draft=A, target=A, parent=A, start=A, ctx=A, batch=2, most=5, pool=A, layer=1024, layers=2, table=A, stride=4, kvh=2, dim=64, path=A, count=A,
                 next=A, new=A + 64, stream=0)
     refuses(ops.tree_commit_q4, good, [dict(draft=None), dict(parent=None), dict(pool=None), dict(most=4000), dict(layers=0), dict(layer=0), dict(layer=1000),
