@@ -23,12 +23,12 @@ template <typename T, int D> inline void q4_call(const T *q, T *out, const TreeA
     // The rows kernel's time grows with the rows, that of 128-row tiles does not. 8 (32)
     // sequences of 4096 (2048) tokens with up to n rows of a kv head, 0.8 n on average, 8 kv
     // heads, us with rows / tiles:
-    //   fp32 rows, D 64     n = 32  34 / 40 (39 / 61)   48  46 / 40 (62 / 63)   64  49 / 40 (65 / 64)   96  64 / 41 (93 / 64)
-    //   bf16 rows, D 64     n = 32  28 / 31 (28 / 48)   48  36 / 31 (45 / 49)   64  37 / 31 (47 / 50)   96  48 / 32 (68 / 52)
-    //   bf16 rows, D 128    n = 24  39 / 41 (44 / 63)   32  40 / 42 (45 / 63)   48  55 / 43 (73 / 64)   64  59 / 43 (77 / 65)
+    //   fp32 rows, D 64     n = 32  25 / 40 (38 / 61)   48  40 / 41 (61 / 63)   64  40 / 41 (65 / 64)   80  58 / 42 (89 / 65)
+    //   bf16 rows, D 64     n = 32  19 / 31 (28 / 48)   48  29 / 32 (45 / 49)   64  29 / 31 (47 / 50)   80  43 / 32 (65 / 51)
+    //   bf16 rows, D 128    n = 32  29 / 41 (45 / 63)   48  47 / 42 (72 / 64)   64  47 / 43 (76 / 65)   80  68 / 44 (102 / 66)
     // It is the mean that tells. (fp32 rows of 128 dims have no tiles.)
-    constexpr bool kBf16 = std::is_same_v<T, __nv_bfloat16>, kHasTiles = D == 64 || kBf16;
-    constexpr int kFrom = !kBf16 ? 37 : D == 64 ? 40 : 32; // rows of a kv head
+    constexpr bool kHasTiles = D == 64 || std::is_same_v<T, __nv_bfloat16>;
+    constexpr int kFrom = D == 128 ? 32 : 53; // rows of a kv head
     const bool many = static_cast<int64_t>(a.t.rows) * (a.qh / a.kvh) > static_cast<int64_t>(kFrom) * a.t.batch;
     if constexpr (kHasTiles)
         if (many) {

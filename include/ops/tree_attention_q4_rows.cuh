@@ -51,7 +51,9 @@ template <typename T, int D, int kNT> struct Q4RowsGeo {
     static constexpr int kRPL = kPair ? 1 : 2 * kNT;         // rows that a lane has scores of
     static constexpr int kSets = kWide && !kPair ? 2 : 1;    // products of a k step
     static constexpr bool kQShared = kSets * kTiles * D > 256; // queries in shared memory, not in registers
-    static constexpr int kWarps = kNT <= 2 ? 8 : 4, kThreads = 32 * kWarps;
+    // 8 warps, as long as two CTAs of them fit on an SM; else 4 (16 rows, 32 sequences of 2180
+    // tokens: fp32 27.7 us with 8, 25.7 with 4; bf16, D 128 33.2, 31.2; bf16, D 64 23.1, 26.9)
+    static constexpr int kWarps = kNT <= 1 || (kNT == 2 && D == 64 && !kWide) ? 8 : 4, kThreads = 32 * kWarps;
     // a step: 64 keys where registers and shared memory have room, since what is done once a
     // step is a third of the instructions of 32
     static constexpr int kPairs = D == 64 && kNT <= 1 ? 2 : 1; // of pages
