@@ -83,7 +83,7 @@ def test_page_take(ops, lens, counts, stride, pad, in_place):
     assert run_take(ops, lens, counts, stride, pad=pad, in_place=in_place) == 0
 
 
-@pytest.mark.parametrize("batch,most", [(513, 9), (600, 200), (1500, 3), (48, 2048)])
+@pytest.mark.parametrize("batch,most", [(513, 9), (600, 200), (1500, 3), (48, 2048), (5000, 4), (4096, 2)])
 def test_page_take_of_large_batches(ops, batch, most):
     rng = np.random.default_rng(batch)
     lens, counts = rng.integers(0, 500, batch), rng.integers(0, most, batch)
@@ -123,7 +123,7 @@ def test_block_ids_whose_slots_pass_32_bits(ops):
 
 
 @pytest.mark.parametrize("old,new", [([0], [0]), ([16], [15]), ([17, 16, 40], [0, 16, 33]), ([100] * 40, list(range(5, 205, 5))),
-                                     (list(range(700)), [0] * 700)])
+                                     (list(range(700)), [0] * 700), ([17] * 5000, [i % 18 for i in range(5000)])])
 @pytest.mark.parametrize("in_place", [False, True])
 def test_page_give(ops, old, new, in_place):
     rng = np.random.default_rng(len(old))
@@ -192,7 +192,7 @@ def norm_case(ops, kind, dim, rot, rows, qh, kvh, weights=(True, True), pad=0, i
 
 @pytest.mark.parametrize("kind", [0, 1])
 @pytest.mark.parametrize("dim,rot", [(32, 32), (64, 64), (64, 32), (64, 0), (128, 128), (128, 48), (256, 256), (256, 64)])
-@pytest.mark.parametrize("rows,qh,kvh,pad", [(1, 1, 1, 0), (5, 32, 8, 0), (33, 7, 1, 16), (2, 96, 3, 8), (3, 0, 2, 0), (3, 2, 0, 8)])
+@pytest.mark.parametrize("rows,qh,kvh,pad", [(1, 1, 1, 0), (5, 32, 8, 0), (33, 7, 1, 16), (2, 96, 3, 8), (3, 0, 2, 0), (3, 2, 0, 8), (2500, 5, 2, 0)])
 def test_norm_and_rotation(ops, kind, dim, rot, rows, qh, kvh, pad):
     norm_case(ops, kind, dim, rot, rows, qh, kvh, pad=pad, seed=dim + rows)
 
@@ -402,9 +402,9 @@ def test_long_contexts(ops, kind, dim, kvh, rep, ctx, rows):
 
 @pytest.mark.parametrize("kind", [0, 1])
 def test_many_sequences(ops, kind):
-    """More sequences than fit at once, longest first; more than a block has threads."""
+    """More sequences than fit at once, longest first; more than a block has threads; more than are put in order."""
     rng = np.random.default_rng(3)
-    for batch in (70, 300):
+    for batch in (70, 300, 1100):
         attention_case(ops, kind, 64, 8, 2, rng.integers(0, 120, batch).tolist(), [1] * batch, trees="chain", seed=batch)
 
 
