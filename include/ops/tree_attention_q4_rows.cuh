@@ -29,8 +29,8 @@
 // of 64 dims about 490 a warp, of which widening is 176, products 16, scales and softmax
 // 90, copies and the rest of the loop the others. Per warp 600 more come before and after
 // (lengths, queries, joining). Measured (kernel time, one B200): 32 sequences of up to
-// 2180 tokens, one token each, 8 x 64 fp32, 4 rows a head 13.8 us (with nothing to attend
-// to 5; floor 4.8); 12 of up to 32,000 tokens, 8 x 128 bf16 87 us, 3.9 TB/s (floor 52).
+// 2180 tokens, one token each, 8 x 64 fp32, 4 rows a head 13.2 us (with nothing to attend
+// to 5; floor 4.8); 12 of up to 32,000 tokens, 8 x 128 bf16 86 us, 3.9 TB/s (floor 52).
 // Rows on the M side of the products, 16 to a tile, took 20.6 and 135.8 us.
 
 #include <type_traits>
@@ -216,14 +216,12 @@ static __global__ void __launch_bounds__(Q4RowsGeo<T, D, kNT>::kThreads, kNT <= 
         if (i < mine) {
             if (i % kAhead == 0) {
                 const int s = i + lane / G::kStepPages, page = (first + s * stride) * G::kStepPages + lane % G::kStepPages;
-                ids = s < mine && page < pages ? table[page] : -1;
+                ids = s < mine && page < pages ? max(0, table[page]) : 0; // after the last page: block 0, and masked
             }
             const uint32_t dst = sm100::smem_u32(ring + to * G::kStage);
 #pragma unroll
             for (int pg = 0; pg < G::kStepPages; ++pg) {
                 const int64_t id = __shfl_sync(kFullWarpMask, ids, i % kAhead * G::kStepPages + pg);
-                if (id < 0)
-                    continue; // after the last page: what the ring holds is masked
                 const uint8_t *src = static_cast<const uint8_t *>(a.k) + (id * a.kvh + h) * R::kBytes;
 #pragma unroll
                 for (int c = 0; c < G::kPageBytes; c += 512)
