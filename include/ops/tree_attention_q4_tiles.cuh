@@ -79,6 +79,40 @@ __device__ __forceinline__ bool q4_elect() {
     return one != 0;
 }
 
+// The stored weights of 32 keys (a chunk's columns: 16 of each term) times the factor that their
+// sum takes: in fp32, and split again. fp16 has few bits of a factor below 2^-14, or none (32
+// keys could so vanish from the output and stay in the sum), and lo corrects hi only as they were
+// split.
+template <int kTerms> __device__ __forceinline__ void q4_lower_weights(uint32_t at, float fix) {
+    uint32_t o[kTerms][16];
+#pragma unroll
+    for (int t = 0; t < kTerms; ++t)
+        sm100::tmem_ld_32x16(at + 16u * t, o[t]);
+    sm100::tmem_wait_ld();
+#pragma unroll
+    for (int t = 0; t < kTerms; ++t)
+        sm100::tmem_reg_fence(o[t]);
+#pragma unroll
+    for (int k = 0; k < 16; ++k) {
+        float2 p = half2_floats(o[0][k]);
+        if constexpr (kTerms == 2) {
+            const float2 rest = half2_floats(o[1][k]);
+            p.x += rest.x, p.y += rest.y;
+        }
+        p.x *= fix, p.y *= fix;
+        o[0][k] = q4_term(p.x, p.y);
+        if constexpr (kTerms == 2)
+            o[1][k] = half2_rn(p.x, p.y);
+    }
+#pragma unroll
+    for (int t = 0; t < kTerms; ++t)
+        tile_tmem_st16(at + 16u * t, o[t]);
+}
+// The same as a call, for bf16 rows: inlined into the four chunks of a tile it costs prompts 10 %
+// (3 x 2048 rows, D 128: 363 us, 326 so), though it hardly ever runs. (fp32 rows, D 64: 409 us
+// inlined, 433 with a call.)
+__device__ __noinline__ void q4_lower_weights_apart(uint32_t at, float fix) { q4_lower_weights<1>(at, fix); }
+
 template <typename T, int D, int kM>
 static __global__ void __launch_bounds__(kTileThreads, 1)
     q4_tiles_kernel(const T *__restrict__ q, T *__restrict__ out, TreeArgs a, int rep, int splits, bool sorted, int *err) {
@@ -495,17 +529,10 @@ static __global__ void __launch_bounds__(kTileThreads, 1)
                 tile_tmem_wait_st(); // the chunks' weights are stored before they are read
 #pragma unroll 1
                 for (int n = second ? 2 : 0; n < c; ++n) {
-                    uint32_t o[2][16];
-                    ask(n, o); // hi, and lo or what is not used
-                    await(o);
-#pragma unroll
-                    for (int t = 0; t < G::kTerms; ++t)
-#pragma unroll
-                        for (int k = 0; k < 16; ++k)
-                            o[t][k] = kv4_bits(__hmul2(kv4_half2(o[t][k]), __float2half2_rn(fix)));
-#pragma unroll
-                    for (int t = 0; t < G::kTerms; ++t)
-                        tile_tmem_st16(st + static_cast<uint32_t>(32 * n + 16 * t), o[t]);
+                    if constexpr (G::kWide)
+                        q4_lower_weights<G::kTerms>(st + static_cast<uint32_t>(32 * n), fix);
+                    else
+                        q4_lower_weights_apart(st + static_cast<uint32_t>(32 * n), fix);
                 }
                 tile_tmem_wait_st();
             };
