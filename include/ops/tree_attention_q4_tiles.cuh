@@ -462,7 +462,7 @@ static __global__ void __launch_bounds__(kTileThreads, 1)
             }
             if (edge && a.t.mask == nullptr) { // a chain, whose rows of this warp see all of the tile
                 const uint4 odd = *reinterpret_cast<const uint4 *>(v_bad + (i & 3) * 8);
-                edge = key0 + kTileKeys > span.ctx + first_node + 1 || (odd.x | odd.y | odd.z | odd.w) != 0;
+                edge = key0 + kTileKeys > min(keys, span.ctx + first_node + 1) || (odd.x | odd.y | odd.z | odd.w) != 0;
             }
             const auto ask = [&](int c, uint32_t (&x)[2][16]) {
                 sm100::tmem_ld_32x16(st + static_cast<uint32_t>(32 * c), x[0]);
