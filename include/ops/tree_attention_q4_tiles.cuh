@@ -202,7 +202,7 @@ static __global__ void __launch_bounds__(kTileThreads, 1)
             const int step = (item - (warp - 8)) / kWidenWarps % 32;
             if (step == 0) {
                 const int mine = item + lane * kWidenWarps, page = key_of(mine / G::kItems) / kKvPage + mine % G::kPages;
-                ids = mine < items && page < pages ? table[page] : 0;
+                ids = mine < items && page < pages ? max(0, table[page]) : 0;
             }
             const int64_t rec = __shfl_sync(kFullWarpMask, ids, step);
             const uint8_t *src = static_cast<const uint8_t *>(a.k) + (rec * a.kvh + h) * R::kBytes;

@@ -1,4 +1,4 @@
-"""Attention over the 4-bit cache where the block table ends before the sequence does."""
+"""Attention over the 4-bit cache where the block table ends before the sequence does, or has no block for a page."""
 
 import math
 
@@ -6,6 +6,7 @@ import numpy as np
 import pytest
 
 import q4_plain
+import tree_cache_plain as plain
 
 pytestmark = pytest.mark.gpu
 torch = pytest.importorskip("torch")
@@ -51,4 +52,26 @@ def test_a_chain_that_is_longer_than_its_table_row(ops, kind, dim, ctx, n, pages
                           rep * dim, 0)
     err, top = (out.cpu().double() - want).abs(), v.abs().max()
     tol = 2.0**-14 * top + (2.0**-8 * want.abs() + 2.0**-10 * top if kind else 0)
+    assert (err <= tol).all(), f"error {err.max():.3g}"
+
+
+@pytest.mark.parametrize("kind", [0, 1])
+@pytest.mark.parametrize("n", [3, 40, 90])
+def test_a_page_that_no_row_sees_may_have_no_block(ops, kind, n):
+    """The last nodes' page has the id -1, and the mask hides all of it: nothing in front of the pool is read, in any kernel."""
+    rep, dim, ctx = 4, 64, 48 - n % 16 if n > 16 else 32  # the last page holds nodes only
+    cache = q4_plain.Cache4([ctx + n + 16], 1, dim, 5)
+    sees = [plain.tree(np.random.default_rng(1), n)[1]]
+    hidden = np.arange(n) + ctx >= 16 * ((ctx + n - 1) // 16)
+    sees[0][:, hidden] = False
+    scale = 1 / math.sqrt(dim)
+    q = torch.randn(n, rep, dim, generator=torch.Generator().manual_seed(1)).to(TYPES[kind])
+    want, mass, top = plain.attention(cache, q, [ctx], [0, n], sees, scale)
+    cache.table[0, (ctx + n - 1) // 16 :] = -1
+    words = -(-n // 32)
+    out = torch.empty(n, rep, dim, dtype=TYPES[kind], device="cuda")
+    ops.tree_attention_q4(q.cuda(), kind, rep * dim, cache.pool.cuda(), torch.from_numpy(cache.table).cuda(), cache.stride, ints([ctx]), ints([0, n]),
+                          torch.from_numpy(plain.pack_mask(sees[0], words)).cuda(), words, 1, n, n, ctx, rep, 1, dim, scale, out, rep * dim, 0)
+    err = (out.cpu().double() - want).abs()
+    tol = (2.0**-17 * mass * top + 24 * 2.0**-23 * top)[..., None] + (2.0**-8 * want.abs() + 2.0**-10 * top[..., None] if kind else 0)
     assert (err <= tol).all(), f"error {err.max():.3g}"
