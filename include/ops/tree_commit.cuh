@@ -85,16 +85,19 @@ template <int kBytes> struct LaneBytes { // what a lane moves of one row: kBytes
 };
 
 // The walk of sequence blockIdx.y, by the whole block: its results (from block x =
-// 0), the accepted nodes' count, and the places that path row i is moved from and
-// to: block * 16 + slot, -1 for a row that stays or lies outside the table.
+// 0), the accepted nodes' count, and the blocks that path row i is moved from and
+// to, -1 for a row that stays or lies outside the table. (A block and its slot are no
+// one int: 16 times an id is above one from 2^27 blocks on.)
 struct CommitMoves {
-    const int *from, *to;
-    int count;
+    const int *from, *to, *path;
+    int ctx, count;
+    __device__ int from_slot(int i) const { return static_cast<int>((static_cast<unsigned>(ctx) + path[i]) % kKvPage); }
+    __device__ int to_slot(int i) const { return static_cast<int>((static_cast<unsigned>(ctx) + i) % kKvPage); }
 };
 __device__ __forceinline__ CommitMoves commit_walk(const TreeVerify &t, const CommitCache &c) {
-    extern __shared__ int commit_smem[]; // succ | target | path | place of each path row
+    extern __shared__ int commit_smem[]; // succ | target | path | block of each path row
     __shared__ int count_s;
-    int *succ = commit_smem, *target = succ + t.max_rows, *path = target + t.max_rows, *place = path + t.max_rows;
+    int *succ = commit_smem, *target = succ + t.max_rows, *path = target + t.max_rows, *block = path + t.max_rows;
     const int b = blockIdx.y, tid = threadIdx.x;
     const int row0 = t.row_start[b], ctx = t.ctx_lens[b];
     const int n = min(t.row_start[b + 1] - row0, t.max_rows);
@@ -121,12 +124,13 @@ __device__ __forceinline__ CommitMoves commit_walk(const TreeVerify &t, const Co
     const int count = count_s;
     const int64_t tokens = static_cast<int64_t>(c.table_stride) * kKvPage;
     const int *table = c.table + static_cast<int64_t>(b) * c.table_stride;
-    // place of path row i, and over succ, which is done, the place that it moves to
+    // block of path row i, and over succ, which is done, the block that it moves to
     for (int i = tid; i < count; i += kCommitThreads) {
         const int64_t from = static_cast<int64_t>(ctx) + path[i], to = static_cast<int64_t>(ctx) + i;
         const bool in = to >= 0 && from < tokens && from != to;
-        place[i] = in ? table[from / kKvPage] * kKvPage + static_cast<int>(from % kKvPage) : -1;
-        succ[i] = in ? table[to / kKvPage] * kKvPage + static_cast<int>(to % kKvPage) : -1;
+        const int from_block = in ? table[from / kKvPage] : -1, to_block = in ? table[to / kKvPage] : -1;
+        block[i] = to_block < 0 ? -1 : from_block;
+        succ[i] = from_block < 0 ? -1 : to_block;
     }
     if (blockIdx.x == 0) {
         for (int i = tid; i < n; i += kCommitThreads)
@@ -138,7 +142,7 @@ __device__ __forceinline__ CommitMoves commit_walk(const TreeVerify &t, const Co
         }
     }
     __syncthreads();
-    return {place, succ, count};
+    return {block, succ, path, ctx, count};
 }
 
 // kRowBytes: a K or V row of one head. Lanes 0-15 move K, 16-31 V. A lane reads
@@ -148,7 +152,7 @@ static __global__ void __launch_bounds__(kCommitThreads) tree_commit_kernel(Tree
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     pdl_wait();
     const CommitMoves moves = commit_walk(t, c);
-    const int *place = moves.from, *succ = moves.to, count = moves.count;
+    const int count = moves.count;
     constexpr int kLane = kRowBytes / 16; // bytes per lane
     const int units = c.layers * c.kvh;
     for (int u = blockIdx.x * (kCommitThreads / 32) + warp; u < units; u += gridDim.x * (kCommitThreads / 32)) {
@@ -160,23 +164,25 @@ static __global__ void __launch_bounds__(kCommitThreads) tree_commit_kernel(Tree
             float s[kCommitBatch];
 #pragma unroll
             for (int i = 0; i < kCommitBatch; ++i) {
-                const int from = i0 + i < count ? place[i0 + i] : -1;
+                const int from = i0 + i < count ? moves.from[i0 + i] : -1;
                 if (from < 0)
                     continue;
-                const int64_t at = static_cast<int64_t>(from / kKvPage) * c.kvh * c.head_bytes;
-                x[i].load(rows + at + (from % kKvPage) * kRowBytes + (lane & 15) * min(kLane, 16));
+                const int64_t at = static_cast<int64_t>(from) * c.kvh * c.head_bytes;
+                const int slot = moves.from_slot(i0 + i);
+                x[i].load(rows + at + slot * kRowBytes + (lane & 15) * min(kLane, 16));
                 if (kScales && lane < 2)
-                    s[i] = *reinterpret_cast<const float *>(scales + at + 4 * (from % kKvPage));
+                    s[i] = *reinterpret_cast<const float *>(scales + at + 4 * slot);
             }
 #pragma unroll
             for (int i = 0; i < kCommitBatch; ++i) {
-                const int to = i0 + i < count ? succ[i0 + i] : -1;
+                const int to = i0 + i < count ? moves.to[i0 + i] : -1;
                 if (to < 0)
                     continue;
-                const int64_t at = static_cast<int64_t>(to / kKvPage) * c.kvh * c.head_bytes;
-                x[i].store(rows + at + (to % kKvPage) * kRowBytes + (lane & 15) * min(kLane, 16));
+                const int64_t at = static_cast<int64_t>(to) * c.kvh * c.head_bytes;
+                const int slot = moves.to_slot(i0 + i);
+                x[i].store(rows + at + slot * kRowBytes + (lane & 15) * min(kLane, 16));
                 if (kScales && lane < 2)
-                    *reinterpret_cast<float *>(scales + at + 4 * (to % kKvPage)) = s[i];
+                    *reinterpret_cast<float *>(scales + at + 4 * slot) = s[i];
             }
         }
     }
@@ -203,7 +209,7 @@ template <int D> static __global__ void __launch_bounds__(kCommitThreads) tree_c
                 const int from = i0 + i < moves.count ? moves.from[i0 + i] : -1;
                 if (from < 0)
                     continue;
-                const uint8_t *src = base + static_cast<int64_t>(from / kKvPage) * c.kvh * c.head_bytes + from % kKvPage * step;
+                const uint8_t *src = base + static_cast<int64_t>(from) * c.kvh * c.head_bytes + moves.from_slot(i0 + i) * step;
                 if (codes)
                     x[i] = *reinterpret_cast<const uint4 *>(src);
                 else
@@ -214,7 +220,7 @@ template <int D> static __global__ void __launch_bounds__(kCommitThreads) tree_c
                 const int to = i0 + i < moves.count ? moves.to[i0 + i] : -1;
                 if (to < 0)
                     continue;
-                uint8_t *dst = base + static_cast<int64_t>(to / kKvPage) * c.kvh * c.head_bytes + to % kKvPage * step;
+                uint8_t *dst = base + static_cast<int64_t>(to) * c.kvh * c.head_bytes + moves.to_slot(i0 + i) * step;
                 if (codes)
                     *reinterpret_cast<uint4 *>(dst) = x[i];
                 else
