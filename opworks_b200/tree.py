@@ -112,6 +112,11 @@ def _current(device):
     return torch.cuda.current_stream().cuda_stream
 
 
+def _version(t):
+    """The number of changes in place of a tensor; None where nothing counts them (made in inference mode)."""
+    return None if t.is_inference() else t._version
+
+
 def qk_norm_rope(q, k, positions, inv_freq=None, q_weight=None, k_weight=None, eps=1e-5, out=None):
     """Queries [rows, q_heads, D] and keys [rows, kv_heads, D] (fp32 or bf16, any row stride), each head normalised (root mean
     square, fp32 weights [D]; None: that side is not) and its first 2 * len(inv_freq) dims rotated by its row's position (int32;
@@ -166,7 +171,8 @@ class PagedCache:
             self.table = torch.arange(blocks, dtype=torch.int32, device=device).view(self.stride, batch).t().contiguous()
         self.status = torch.zeros(1, dtype=torch.int32, device=device)  # of the last pages taken or given: 0
         self._placed = None        # the step that has been given its places: (rows, lens, its version, positions, slots)
-        self.lens = torch.zeros(batch, dtype=torch.int32, device=device)
+        with torch.inference_mode(False):  # (lens is a plain tensor in that mode too, so that its changes are counted)
+            self.lens = torch.zeros(batch, dtype=torch.int32, device=device)
         self.bounds = [0] * batch  # upper bounds of lens that the host knows
         self._before = None        # those before the last commit
 
@@ -216,12 +222,12 @@ class PagedCache:
         if not self._has_places(rows):
             if self._placed is not None and self.shared:
                 raise ValueError("place: the step before has been given its places and is neither kept nor dropped (advance, commit, drop)")
-            self._placed = (rows, self.lens, self.lens._version, *self._where(rows, self.shared))
+            self._placed = (rows, self.lens, _version(self.lens), *self._where(rows, self.shared))
         return self._placed[3:]
 
     def _has_places(self, rows):
         p = self._placed  # (lens: a program that sets it itself has moved the rows)
-        return p is not None and p[0] is rows and p[1] is self.lens and p[2] == self.lens._version
+        return p is not None and p[0] is rows and p[1] is self.lens and p[2] is not None and p[2] == _version(self.lens)
 
     def drop(self):
         """Forgets the rows of the step that was placed: their pages go back."""
@@ -243,7 +249,8 @@ class PagedCache:
         if self._placed is not None and self.shared:
             raise ValueError("release: between steps, not within one (advance, commit, drop)")
         (mask,) = to_device(self.lens.device, gone)
-        lens = torch.where(mask != 0, torch.zeros_like(self.lens), self.lens)
+        with torch.inference_mode(False):
+            lens = torch.where(mask != 0, torch.zeros_like(self.lens), self.lens)
         if self.shared:
             self._give(self.lens, lens)
         self.lens, self._placed = lens, None
@@ -322,7 +329,8 @@ class PagedCache:
         if self.shared:
             self.place(rows)
         self._placed = None
-        self.lens = self.lens + rows.start.diff()
+        with torch.inference_mode(False):
+            self.lens = self.lens + rows.start.diff()
         self.bounds, self._before = [b + n for b, n in zip(self.bounds, rows.counts)], None
 
     def commit(self, draft, target, rows):
@@ -333,7 +341,9 @@ class PagedCache:
             self._takes(name, t, (rows.total,), INTEGERS)
         draft, target = draft.to(torch.int32).contiguous(), target.to(torch.int32).contiguous()
         new = lambda n: torch.empty(n, dtype=torch.int32, device=self.lens.device)  # noqa: E731
-        path, count, nxt, lens = new(rows.total), new(self.batch), new(self.batch), new(self.batch)
+        path, count, nxt = new(rows.total), new(self.batch), new(self.batch)
+        with torch.inference_mode(False):
+            lens = new(self.batch)
         head = (draft, target, rows.parents, rows.start, self.lens, self.batch, rows.most)
         tail = (self.layers, self.table, self.stride, self.kv_heads, self.head_dim, path, count, nxt, lens, self._stream())
         if self.shared:

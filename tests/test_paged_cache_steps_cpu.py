@@ -1,0 +1,51 @@
+"""What PagedCache (opworks_b200/tree.py) keeps from call to call of a step, with a stand-in for the operators: nothing here launches."""
+
+import pytest
+
+torch = pytest.importorskip("torch")
+
+
+class Ops:
+    """Counts the operators' calls and answers none of them."""
+
+    def __init__(self):
+        self.calls = []
+
+    def __getattr__(self, name):
+        return lambda *args: self.calls.append(name)
+
+
+def cache(format="int4", batch=2, tokens=96, **kw):
+    from opworks_b200.tree import PagedCache
+
+    c = PagedCache(2, batch, tokens, 1, 64, format, device="cpu", **kw)
+    c.ops, c._stream = Ops(), lambda: 0
+    return c
+
+
+@pytest.mark.parametrize("made", [False, True])
+@pytest.mark.parametrize("format,blocks", [("int4", None), ("int4", 12), ("int8", 12), ("f32", 12)])
+def test_a_step_in_inference_mode(made, format, blocks):
+    from opworks_b200.tree import Rows
+
+    with torch.inference_mode(made):
+        c = cache(format, blocks=blocks)
+    with torch.inference_mode():
+        for counts in ([5, 2], [1, 1]):
+            rows = Rows(counts, device="cpu")
+            first = c.place(rows)
+            assert all(a is b for a, b in zip(first, c.place(rows)))
+            assert c.ops.calls.count("page_take") == 1
+            c.ops.calls.clear()
+            c.advance(rows)
+        assert c.lens.tolist() == [6, 3] and c.bounds == [6, 3]
+        c.commit(torch.zeros(2, dtype=torch.int32), torch.zeros(2, dtype=torch.int32), rows)
+        c.lens.fill_(0)
+        if blocks is None:
+            first = c.place(rows)
+            c.lens += 20
+            assert c.place(rows)[0] is not first[0]
+            c.lens = c.lens + 1  # nothing counts the changes of this one
+            second = c.place(rows)
+            c.lens += 1
+            assert c.place(rows)[0] is not second[0]
