@@ -60,7 +60,7 @@ class Model:
         n, s = len(tokens), torch.cuda.current_stream().cuda_stream
         x = torch.empty(n, HIDDEN, device="cuda")
         ids = torch.tensor(tokens, dtype=torch.int32).cuda()
-        at = torch.tensor(positions, dtype=torch.int32).cuda()  # a drafted token's is its depth's, not its row's
+        at = None if self.norms is None else cache.positions(rows)  # a drafted token's is its depth's, not its row's
         self.ops.embedding_f32(self.embed, ids, x, n, HIDDEN, s)
         for i, w in enumerate(self.layers):
             h = self.norm(x, s)

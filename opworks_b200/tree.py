@@ -18,12 +18,11 @@ fp32, in 8 bits or in 4; a step writes the new tokens' K and V, attends, and com
 
 With ``blocks`` the sequences share that many pages: a step takes what its new
 tokens need, a commit gives back what its drafts did not, and ``release`` all that
-sequences hold. ``place`` says where the new tokens go; ``qk_norm_rope`` takes their
-positions::
+sequences hold. ``place`` says where the new tokens go, ``positions`` what
+``qk_norm_rope`` rotates them by::
 
     cache = PagedCache(layers=2, batch=64, max_tokens=4096, kv_heads=2, head_dim=64, format="int4", blocks=1000)
-    positions, slots = cache.place(rows)
-    q, k = qk_norm_rope(q, k, positions, inv_freq, q_weight, k_weight)
+    q, k = qk_norm_rope(q, k, cache.positions(rows), inv_freq, q_weight, k_weight)
     ...
     cache.release([3, 7])                                   # sequences that are done
 
@@ -63,6 +62,14 @@ def deepest(parents):
     return max(depth, default=0)
 
 
+def depths(parents):
+    """How far each node of a tree is from its root."""
+    depth = []
+    for p in parents:
+        depth.append(depth[p] + 1 if p >= 0 else 0)
+    return depth
+
+
 def to_device(device, *arrays):
     """int32 arrays as tensors, in one copy that the host does not wait for (from pinned memory, which torch keeps until
     the copy is done)."""
@@ -85,6 +92,7 @@ class Rows:
         self.counts, self.total, self.most = list(counts), int(start[-1]), max(counts, default=0)
         self.depths = list(counts)  # the most nodes on a path
         self.mask, self.words, self._parents = None, 0, None
+        self.lift = None  # of a tree: a node's depth less its number
         if parents is None:
             (self.start,) = to_device(device, start)
             return
@@ -93,7 +101,8 @@ class Rows:
         self.words = max(1, -(-self.most // 32))
         mask = np.concatenate([tree_mask(p, self.words) for p in parents])
         self.depths = [deepest(p) for p in parents]
-        self.start, self.mask, self._parents = to_device(device, start, mask, np.concatenate(parents).astype(np.int32))
+        lift = np.concatenate([np.subtract(depths(p), range(len(p))) for p in parents]).astype(np.int32)
+        self.start, self.mask, self._parents, self.lift = to_device(device, start, mask, np.concatenate(parents).astype(np.int32), lift)
 
     @property
     def parents(self):
@@ -215,7 +224,8 @@ class PagedCache:
         return positions, slots
 
     def place(self, rows):
-        """Where the rows of a step go: positions (int32, lens + 0, 1, ...) and slots (int64, 16 * block + place in the page). With
+        """Where the rows of a step go: positions (int32, lens + 0, 1, ..., in a tree too: until commit every node has its own;
+        ``positions`` is what rows are rotated by) and slots (int64, 16 * block + place in the page). With
         shared pages those that the step needs are taken, once, whoever asks first: this, or the step's first write."""
         self._belongs(rows)
         self._room(rows)
@@ -224,6 +234,13 @@ class PagedCache:
                 raise ValueError("place: the step before has been given its places and is neither kept nor dropped (advance, commit, drop)")
             self._placed = (rows, self.lens, _version(self.lens), *self._where(rows, self.shared))
         return self._placed[3:]
+
+    def positions(self, rows):
+        """The positions that the rows are rotated by, int32: of a chain lens + 0, 1, ..., of a tree lens + the node's depth, so that
+        siblings have one, and a path that commit keeps has those of the places that it moves to. Takes the step's pages as
+        ``place`` does, which has one place for every node."""
+        at, _ = self.place(rows)
+        return at if rows.lift is None else at + rows.lift
 
     def _has_places(self, rows):
         p = self._placed  # (lens: a program that sets it itself has moved the rows)

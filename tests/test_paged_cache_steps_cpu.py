@@ -49,3 +49,14 @@ def test_a_step_in_inference_mode(made, format, blocks):
             second = c.place(rows)
             c.lens += 1
             assert c.place(rows)[0] is not second[0]
+
+
+def test_depths_of_drafted_rows():
+    from opworks_b200.tree import Rows
+
+    rows = Rows([7, 0, 3, 1], [[-1, 0, 0, 1, 1, 3, 2], [], [-1, 0, -1], [-1]], device="cpu")
+    assert rows.lift.dtype == torch.int32
+    node = [*range(7), *range(3), 0]
+    assert [n + x for n, x in zip(node, rows.lift.tolist())] == [0, 1, 1, 2, 2, 3, 2, 0, 1, 0, 0]
+    chain = [-1, 0, 1, 2]
+    assert Rows([4], [chain], device="cpu").lift.tolist() == [0, 0, 0, 0] and Rows([4], device="cpu").lift is None

@@ -76,3 +76,28 @@ def test_a_length_moved_in_inference_mode_moves_the_rows():
         cache.lens -= 30
         cache.write(0, x * 3, x, rows)
         assert torch.equal(held(cache, 0, 0, 10, 2), of(x * 3))
+
+
+def test_drafted_rows_are_rotated_by_their_depth():
+    """Siblings have one position; a kept path's rows then lie where their positions are."""
+    from opworks_b200.tree import PagedCache, Rows
+
+    for blocks in (None, 9):
+        cache = PagedCache(1, 3, 64, 1, 64, "int4", blocks=blocks)
+        prompt = Rows([7, 0, 20])
+        assert cache.positions(prompt).tolist() == [*range(7), *range(20)]
+        cache.advance(prompt)
+        rows = Rows([7, 3, 1], [[-1, 0, 0, 1, 1, 3, 2], [-1, 0, -1], [-1]])
+        positions = cache.positions(rows)
+        assert positions.dtype == torch.int32
+        assert positions.tolist() == [7, 8, 8, 9, 9, 10, 9, 0, 1, 0, 20]
+        at, slots = cache.place(rows)  # where the rows lie until one path is kept
+        assert at.tolist() == [*range(7, 14), 0, 1, 2, 20]
+        table = cache.table.tolist()
+        owner = [0] * 7 + [1] * 3 + [2]
+        assert slots.tolist() == [table[b][p // 16] * 16 + p % 16 for b, p in zip(owner, at.tolist())]
+        draft = torch.arange(11, device="cuda")
+        target = torch.tensor([1, 3, 0, 5, 0, 99, 0, 99, 0, 0, 99], device="cuda")
+        path, count, _ = cache.commit(draft, target, rows)
+        assert count.tolist() == [4, 1, 1] and path[:4].tolist() == [0, 1, 3, 5]
+        assert positions[path[:4].long()].tolist() == [7, 8, 9, 10]  # lens + 0, 1, ...: where commit moved them
