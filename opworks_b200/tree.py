@@ -180,8 +180,9 @@ class PagedCache:
             self.table = torch.arange(blocks, dtype=torch.int32, device=device).view(self.stride, batch).t().contiguous()
         self.status = torch.zeros(1, dtype=torch.int32, device=device)  # of the last pages taken or given: 0
         self._placed = None        # the step that has been given its places: (rows, lens, its version, positions, slots)
+        self._step = None          # with shared pages the step that has taken its own: (rows, lens after all of them)
         with torch.inference_mode(False):  # (lens is a plain tensor in that mode too, so that its changes are counted)
-            self.lens = torch.zeros(batch, dtype=torch.int32, device=device)
+            self._set_lens(torch.zeros(batch, dtype=torch.int32, device=device))
         self.bounds = [0] * batch  # upper bounds of lens that the host knows
         self._before = None        # those before the last commit
 
@@ -194,6 +195,13 @@ class PagedCache:
         if self.lens.device.type != "cuda" or self.lens.device.index != torch.cuda.current_device():
             raise ValueError(f"the cache is on {self.lens.device}, which is not the current CUDA device")
         return torch.cuda.current_stream().cuda_stream
+
+    def _set_lens(self, lens):
+        self.lens = lens
+        self._own = (lens, lens._version)  # as this cache left it
+
+    def _unmoved(self):
+        return self.lens is self._own[0] and _version(self.lens) == self._own[1]
 
     def _pages(self, tokens):
         return sum(-(-n // self.PAGE) for n in tokens)
@@ -229,11 +237,21 @@ class PagedCache:
         shared pages those that the step needs are taken, once, whoever asks first: this, or the step's first write."""
         self._belongs(rows)
         self._room(rows)
-        if not self._has_places(rows):
-            if self._placed is not None and self.shared:
+        if self.shared:
+            self._own_lens()
+            if self._step is not None and self._step[0] is not rows:
                 raise ValueError("place: the step before has been given its places and is neither kept nor dropped (advance, commit, drop)")
-            self._placed = (rows, self.lens, _version(self.lens), *self._where(rows, self.shared))
+        if not self._has_places(rows):
+            self._placed = (rows, self.lens, _version(self.lens), *self._where(rows, self.shared and self._step is None))
+            if self.shared:
+                with torch.inference_mode(False):
+                    self._step = (rows, self.lens + rows.start.diff())
         return self._placed[3:]
+
+    def _own_lens(self):
+        if not self._unmoved():
+            raise ValueError("lens has been moved: with shared pages it goes with the pages that sequences have (advance, commit, release; drop "
+                             "sets it back to what it was before a step)")
 
     def positions(self, rows):
         """The positions that the rows are rotated by, int32: of a chain lens + 0, 1, ..., of a tree lens + the node's depth, so that
@@ -247,10 +265,15 @@ class PagedCache:
         return p is not None and p[0] is rows and p[1] is self.lens and p[2] is not None and p[2] == _version(self.lens)
 
     def drop(self):
-        """Forgets the rows of the step that was placed: their pages go back."""
-        if self._placed is not None and self.shared:
-            self._give(self.lens + self._placed[0].start.diff(), self.lens)
-        self._placed = None
+        """Forgets the rows of the step that was placed: their pages go back, and lens is what it was before it."""
+        if self._step is not None:
+            rows, after = self._step
+            with torch.inference_mode(False):
+                lens = after - rows.start.diff()
+            self._give(after, lens)
+            if not self._unmoved():
+                self._set_lens(lens)
+        self._placed = self._step = None
 
     def _give(self, old, new):
         self.ops.page_give(old, new, self.batch, self.table, self.stride, self.free, self.blocks, self.free_count, self.free_count,
@@ -263,14 +286,17 @@ class PagedCache:
             if not 0 <= int(b) < self.batch:
                 raise ValueError(f"release: sequences 0 to {self.batch - 1}, not {b}")
             gone[int(b)] = 1
-        if self._placed is not None and self.shared:
+        if self._step is not None:
             raise ValueError("release: between steps, not within one (advance, commit, drop)")
+        if self.shared:
+            self._own_lens()
         (mask,) = to_device(self.lens.device, gone)
         with torch.inference_mode(False):
             lens = torch.where(mask != 0, torch.zeros_like(self.lens), self.lens)
         if self.shared:
             self._give(self.lens, lens)
-        self.lens, self._placed = lens, None
+        self._set_lens(lens)
+        self._placed = None
         self.bounds, self._before = [0 if g else n for n, g in zip(self.bounds, gone)], None
 
     def write(self, layer, k, v, rows):
@@ -345,9 +371,9 @@ class PagedCache:
         self._belongs(rows)
         if self.shared:
             self.place(rows)
-        self._placed = None
         with torch.inference_mode(False):
-            self.lens = self.lens + rows.start.diff()
+            self._set_lens(self._step[1] if self.shared else self.lens + rows.start.diff())
+        self._placed = self._step = None
         self.bounds, self._before = [b + n for b, n in zip(self.bounds, rows.counts)], None
 
     def commit(self, draft, target, rows):
@@ -371,8 +397,9 @@ class PagedCache:
         else:
             self.ops.tree_commit(*head, self.k, self.v, self.k.stride(0), *tail)
         if self.shared:  # pages that the drafts had and the kept path does not need
-            self._give(self.lens + rows.start.diff(), lens)
-        self.lens, self._placed = lens, None
+            self._give(self._step[1], lens)
+        self._set_lens(lens)
+        self._placed = self._step = None
         self._before, self.bounds = self.bounds, [b + n for b, n in zip(self.bounds, rows.depths)]
         return path, count, nxt
 

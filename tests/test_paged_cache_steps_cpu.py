@@ -60,3 +60,40 @@ def test_depths_of_drafted_rows():
     assert [n + x for n, x in zip(node, rows.lift.tolist())] == [0, 1, 1, 2, 2, 3, 2, 0, 1, 0, 0]
     chain = [-1, 0, 1, 2]
     assert Rows([4], [chain], device="cpu").lift.tolist() == [0, 0, 0, 0] and Rows([4], device="cpu").lift is None
+
+
+@pytest.mark.parametrize("how", ["in place", "another"])
+def test_shared_pages_and_a_length_that_the_program_moves(how):
+    from opworks_b200.tree import Rows
+
+    def move(c):
+        if how == "in place":
+            c.lens += 30
+        else:
+            c.lens = c.lens + 30
+
+    c, rows = cache(blocks=12), Rows([20, 3], device="cpu")
+    c.place(rows)
+    move(c)
+    zeros = torch.zeros(23, dtype=torch.int32)
+    for call in (lambda: c.place(rows), lambda: c.advance(rows), lambda: c.commit(zeros, zeros, rows), lambda: c.write(0, zeros[:, None].expand(23, 64).float(), zeros[:, None].expand(23, 64).float(), rows)):
+        with pytest.raises(ValueError, match="lens"):
+            call()
+    assert c.ops.calls == ["page_take"]
+    c.drop()
+    assert c.ops.calls == ["page_take", "page_give"] and c.lens.tolist() == [0, 0]
+    c.advance(rows)
+    assert c.lens.tolist() == [20, 3] and c.bounds == [20, 3]
+    move(c)
+    for call in (lambda: c.place(rows), lambda: c.advance(rows), lambda: c.release([0])):
+        with pytest.raises(ValueError, match="lens"):
+            call()
+    with pytest.raises(ValueError, match="lens"):
+        c.positions(rows)
+    own = cache()  # without shared pages it may be moved
+    own.place(rows)
+    move(own)
+    own.place(rows)
+    own.advance(rows)
+    own.release([1])
+    assert own.lens.tolist() == [50, 0]

@@ -23,6 +23,13 @@ def held(cache, b, layer, first, n):
     return q4_plain.dequantise(kc[block, :, :, slot], ks[block, :, :, slot])
 
 
+def sound(cache, lens):
+    """Lengths are those expected, and every page has one owner."""
+    assert cache.lens.tolist() == lens and cache.status.item() == 0
+    owned = [int(x) for b, n in enumerate(lens) for x in cache.table[b, : -(-n // 16)].tolist()]
+    return sorted(owned + cache.free[: cache.free_count.item()].tolist()) == list(range(cache.blocks))
+
+
 @pytest.mark.parametrize("format,blocks", [("int4", None), ("int4", 12), ("int8", 12), ("int8", None), ("f32", 12)])
 @pytest.mark.parametrize("whole", [True, False])
 def test_steps_in_inference_mode(format, blocks, whole):
@@ -101,3 +108,52 @@ def test_drafted_rows_are_rotated_by_their_depth():
         path, count, _ = cache.commit(draft, target, rows)
         assert count.tolist() == [4, 1, 1] and path[:4].tolist() == [0, 1, 3, 5]
         assert positions[path[:4].long()].tolist() == [7, 8, 9, 10]  # lens + 0, 1, ...: where commit moved them
+
+
+@pytest.mark.parametrize("how", ["in place", "another"])
+def test_a_length_moved_within_a_shared_step_gives_no_page_two_owners(how):
+    from opworks_b200.tree import PagedCache, Rows
+
+    cache = PagedCache(1, 3, 96, 1, 64, "int4", blocks=12)
+    first = Rows([20, 40, 0])
+    cache.place(first)
+    cache.advance(first)
+    assert sound(cache, [20, 40, 0])
+    rows = Rows([30, 1, 9])
+    cache.place(rows)
+    if how == "in place":
+        cache.lens += 33
+    else:
+        cache.lens = cache.lens + 33
+    x = torch.randn(rows.total, 64, device="cuda")
+    for call in (lambda: cache.place(rows), lambda: cache.write(0, x, x, rows), lambda: cache.advance(rows),
+                 lambda: cache.commit(torch.zeros(40, dtype=torch.int32, device="cuda"), torch.zeros(40, dtype=torch.int32, device="cuda"), rows)):
+        with pytest.raises(ValueError):
+            call()
+    cache.drop()  # the step is as if it had not been: its pages and the lengths
+    assert sound(cache, [20, 40, 0])
+    cache.place(rows)
+    cache.advance(rows)
+    assert sound(cache, [50, 41, 9])
+
+
+@pytest.mark.parametrize("how", ["in place", "another"])
+def test_a_length_moved_between_shared_steps_is_refused(how):
+    """Its pages would not be those that the table has."""
+    from opworks_b200.tree import PagedCache, Rows
+
+    cache = PagedCache(1, 2, 96, 1, 64, "int8", blocks=12)
+    rows = Rows([20, 40])
+    cache.advance(rows)
+    kept = cache.lens
+    if how == "in place":
+        cache.lens -= 10
+    else:
+        cache.lens = cache.lens + 40
+    for call in (lambda: cache.place(rows), lambda: cache.advance(rows), lambda: cache.release([0])):
+        with pytest.raises(ValueError, match="lens"):
+            call()
+    if how == "another":
+        cache.lens = kept
+        cache.release([0, 1])
+        assert sound(cache, [0, 0]) and cache.free_count.item() == 12
