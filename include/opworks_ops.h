@@ -35,6 +35,9 @@ OPW_API const char *opw_ops_last_error(void);
 /* Waits for `stream`; returns 0, or -1 if the device error word is set (a
  * bounded device-side wait ran out), clearing it. */
 OPW_API int opw_ops_sync(void *stream);
+/* The number of the graph capture that `stream` takes part in, 0 where it takes
+ * part in none: what a caller keeps between calls belongs to one capture. */
+OPW_API int opw_ops_capture_id(void *stream, int64_t *id);
 
 /* ops::map with fixed functors (include/ops/elementwise.cuh:63-77;
  * tests/integration/vector_add.cu, relu.cu). */

@@ -121,6 +121,19 @@ int opw_ops_sync(void *stream) {
     return 0;
 }
 
+int opw_ops_capture_id(void *stream, int64_t *id) {
+    return guarded([&] {
+        cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+        unsigned long long number = 0;
+        const cudaError_t e = cudaStreamGetCaptureInfo(as_stream(stream), &status, &number);
+        if (e != cudaSuccess) {
+            cudaGetLastError(); // no more than an answer to the question
+            throw std::runtime_error(std::string("opw_ops_capture_id: ") + cudaGetErrorString(e));
+        }
+        *id = status == cudaStreamCaptureStatusNone ? 0 : static_cast<int64_t>(number);
+    });
+}
+
 int opw_map_add(const float *a, const float *b, float *out, int n, void *stream) {
     return guarded([&] { opworks::ops::map(a, b, out, n, AddF{}, as_stream(stream)); });
 }

@@ -17,6 +17,7 @@ F = ctypes.c_float
 
 SIGNATURES = {
     "opw_ops_sync": [P],
+    "opw_ops_capture_id": [P, P],
     "opw_map_add": [P, P, P, I, P],
     "opw_map_relu": [P, P, I, P],
     "opw_map_scale": [P, P, I, F, P],

@@ -31,6 +31,9 @@ Everything runs on torch's current stream; nothing here waits for the device.
 
 from __future__ import annotations
 
+import ctypes
+from typing import Any, NamedTuple
+
 import numpy as np
 import torch
 
@@ -155,6 +158,17 @@ def qk_norm_rope(q, k, positions, inv_freq=None, q_weight=None, k_weight=None, e
     return new
 
 
+class _Places(NamedTuple):
+    """Where the rows of a step go, and for which calls that holds."""
+
+    rows: Rows
+    lens: torch.Tensor
+    version: Any  # of lens
+    capture: int  # the graph capture that they are part of; 0: none
+    positions: torch.Tensor
+    slots: torch.Tensor
+
+
 class PagedCache:
     PAGE = 16
 
@@ -179,7 +193,7 @@ class PagedCache:
         else:
             self.table = torch.arange(blocks, dtype=torch.int32, device=device).view(self.stride, batch).t().contiguous()
         self.status = torch.zeros(1, dtype=torch.int32, device=device)  # of the last pages taken or given: 0
-        self._placed = None        # the step that has been given its places: (rows, lens, its version, positions, slots)
+        self._placed = None        # the places of the last step that asked for them
         self._step = None          # with shared pages the step that has taken its own: (rows, lens after all of them)
         with torch.inference_mode(False):  # (lens is a plain tensor in that mode too, so that its changes are counted)
             self._set_lens(torch.zeros(batch, dtype=torch.int32, device=device))
@@ -195,6 +209,18 @@ class PagedCache:
         if self.lens.device.type != "cuda" or self.lens.device.index != torch.cuda.current_device():
             raise ValueError(f"the cache is on {self.lens.device}, which is not the current CUDA device")
         return torch.cuda.current_stream().cuda_stream
+
+    def _capture(self):
+        """The number of the graph capture that torch's current stream takes part in; 0: none."""
+        if self.lens.device.type != "cuda" or not torch.cuda.is_current_stream_capturing():
+            return 0
+        number = ctypes.c_int64()
+        self.ops.ops_capture_id(torch.cuda.current_stream().cuda_stream, ctypes.byref(number))
+        return number.value
+
+    def _no_graph(self, what):
+        if self._capture():
+            raise ValueError(f"{what}: not while a graph is captured, where sequences share pages (each replay would take or give them again)")
 
     def _set_lens(self, lens):
         self.lens = lens
@@ -234,19 +260,25 @@ class PagedCache:
     def place(self, rows):
         """Where the rows of a step go: positions (int32, lens + 0, 1, ..., in a tree too: until commit every node has its own;
         ``positions`` is what rows are rotated by) and slots (int64, 16 * block + place in the page). With
-        shared pages those that the step needs are taken, once, whoever asks first: this, or the step's first write."""
+        shared pages those that the step needs are taken, once, whoever asks first: this, or the step's first write; not while a
+        graph is captured (write, read and attend may be captured once they are)."""
         self._belongs(rows)
         self._room(rows)
         if self.shared:
             self._own_lens()
             if self._step is not None and self._step[0] is not rows:
                 raise ValueError("place: the step before has been given its places and is neither kept nor dropped (advance, commit, drop)")
-        if not self._has_places(rows):
-            self._placed = (rows, self.lens, _version(self.lens), *self._where(rows, self.shared and self._step is None))
-            if self.shared:
+        at = self._places(rows)
+        if at is None:
+            take = self.shared and self._step is None
+            if take:
+                self._no_graph("place")
+            at = self._where(rows, take)
+            self._placed = _Places(rows, self.lens, _version(self.lens), self._capture(), *at)
+            if take:
                 with torch.inference_mode(False):
                     self._step = (rows, self.lens + rows.start.diff())
-        return self._placed[3:]
+        return at
 
     def _own_lens(self):
         if not self._unmoved():
@@ -260,13 +292,18 @@ class PagedCache:
         at, _ = self.place(rows)
         return at if rows.lift is None else at + rows.lift
 
-    def _has_places(self, rows):
-        p = self._placed  # (lens: a program that sets it itself has moved the rows)
-        return p is not None and p[0] is rows and p[1] is self.lens and p[2] is not None and p[2] == _version(self.lens)
+    def _places(self, rows):
+        """Positions and slots of the rows that the step has already, None: they are to be asked for. A program that moves lens has
+        moved the rows; what a graph computes is there when it is replayed, and only in it."""
+        p = self._placed
+        if p is None or p.rows is not rows or p.lens is not self.lens or p.version is None or p.version != _version(self.lens) or p.capture != self._capture():
+            return None
+        return p.positions, p.slots
 
     def drop(self):
         """Forgets the rows of the step that was placed: their pages go back, and lens is what it was before it."""
         if self._step is not None:
+            self._no_graph("drop")
             rows, after = self._step
             with torch.inference_mode(False):
                 lens = after - rows.start.diff()
@@ -289,6 +326,7 @@ class PagedCache:
         if self._step is not None:
             raise ValueError("release: between steps, not within one (advance, commit, drop)")
         if self.shared:
+            self._no_graph("release")
             self._own_lens()
         (mask,) = to_device(self.lens.device, gone)
         with torch.inference_mode(False):
@@ -337,7 +375,7 @@ class PagedCache:
         k = torch.empty(rows.total, self.kv_heads, self.head_dim, dtype=dtype, device=self.lens.device)
         v = torch.empty_like(k)
         if self.format == INT4:
-            _, slots = self._placed[3:] if self._has_places(rows) else self._where(rows, False)
+            _, slots = self._places(rows) or self._where(rows, False)
             width = self.kv_heads * self.head_dim
             self.ops.kv4_read(self.pool[layer], self.blocks, slots, rows.total, self.kv_heads, self.head_dim, k, width, v, width, TYPES[dtype],
                               self._stream())
@@ -370,6 +408,7 @@ class PagedCache:
         """Keeps all rows (a prompt, or a chain that needs no verification)."""
         self._belongs(rows)
         if self.shared:
+            self._no_graph("advance")
             self.place(rows)
         with torch.inference_mode(False):
             self._set_lens(self._step[1] if self.shared else self.lens + rows.start.diff())
@@ -390,6 +429,7 @@ class PagedCache:
         head = (draft, target, rows.parents, rows.start, self.lens, self.batch, rows.most)
         tail = (self.layers, self.table, self.stride, self.kv_heads, self.head_dim, path, count, nxt, lens, self._stream())
         if self.shared:
+            self._no_graph("commit")
             self.place(rows)
         if self.format:
             call = self.ops.tree_commit_q4 if self.format == INT4 else self.ops.tree_commit_q8

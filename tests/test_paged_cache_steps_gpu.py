@@ -157,3 +157,103 @@ def test_a_length_moved_between_shared_steps_is_refused(how):
         cache.lens = kept
         cache.release([0, 1])
         assert sound(cache, [0, 0]) and cache.free_count.item() == 12
+
+
+def test_a_captured_write_follows_the_lengths_after_an_eager_one():
+    from opworks_b200.tree import PagedCache, Rows
+
+    cache, rows = PagedCache(2, 1, 64, 1, 64, "int4"), Rows([2])
+    x = torch.randn(2, 64, device="cuda")
+    for layer in range(2):
+        cache.write(layer, x, x, rows)  # every kernel once, and the rows have places
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        for layer in range(2):
+            cache.write(layer, x, x, rows)
+    for at in (20, 33):
+        cache.lens.fill_(at)
+        x.normal_()
+        graph.replay()
+        for layer in range(2):
+            assert torch.equal(held(cache, 0, layer, at, 2), of(x))
+
+
+def test_an_eager_write_after_a_captured_one():
+    from opworks_b200.tree import PagedCache, Rows
+
+    cache, rows, other = PagedCache(1, 1, 640, 1, 64, "int4"), Rows([2]), Rows([2])
+    x, y = torch.randn(2, 2, 64, device="cuda")
+    cache.write(0, y, y, other)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):  # not replayed: its places are not there
+        cache.write(0, x, x, rows)
+    cache.write(0, x * 5, x, rows)
+    assert torch.equal(held(cache, 0, 0, 0, 2), of(x * 5))
+
+
+def test_two_graphs_have_places_of_their_own():
+    from opworks_b200.tree import PagedCache, Rows
+
+    cache, rows = PagedCache(1, 1, 640, 1, 64, "int4"), Rows([2])
+    x = torch.randn(2, 64, device="cuda")
+    cache.write(0, x, x, rows)
+    torch.cuda.synchronize()
+    graphs = [torch.cuda.CUDAGraph() for _ in range(2)]
+    for graph in graphs:
+        with torch.cuda.graph(graph):
+            cache.write(0, x, x, rows)
+    for at, graph in ((30, graphs[1]), (50, graphs[0]), (70, graphs[1])):
+        cache.lens.fill_(at)
+        x.normal_()
+        graph.replay()
+        assert torch.equal(held(cache, 0, 0, at, 2), of(x))
+
+
+def test_a_captured_write_takes_the_places_once():
+    """One launch for the places of all layers, as outside of a graph."""
+    from opworks_b200.tree import PagedCache, Rows
+
+    cache, rows = PagedCache(3, 1, 64, 1, 64, "int4"), Rows([2])
+    x = torch.randn(2, 64, device="cuda")
+    cache.write(0, x, x, rows)
+    torch.cuda.synchronize()
+    graph, calls, take = torch.cuda.CUDAGraph(), [], cache._where
+    cache._where = lambda *a: (calls.append(a), take(*a))[1]
+    with torch.cuda.graph(graph):
+        for layer in range(3):
+            cache.write(layer, x, x, rows)
+    assert len(calls) == 1
+
+
+def test_shared_pages_are_not_taken_by_a_graph():
+    """Each replay would take them again, and the host would not know. What was placed before may be written in one."""
+    from opworks_b200.tree import PagedCache, Rows
+
+    cache = PagedCache(1, 1, 64, 1, 64, "int4", blocks=4)
+    rows, x = Rows([3]), torch.randn(3, 64, device="cuda")
+    cache.write(0, x, x, rows)
+    cache.advance(rows)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = x + 1
+        for call in (lambda: cache.place(rows), lambda: cache.write(0, x, x, rows), lambda: cache.advance(rows), lambda: cache.release([0])):
+            with pytest.raises(ValueError, match="graph"):
+                call()
+    cache.place(rows)
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        cache.write(0, x, x, rows)
+        for call in (lambda: cache.advance(rows), cache.drop):
+            with pytest.raises(ValueError, match="graph"):
+                call()
+    x.normal_()
+    graph.replay()
+    assert torch.equal(held(cache, 0, 0, 3, 3), of(x))
+    cache.write(0, x * 2, x, rows)
+    assert torch.equal(held(cache, 0, 0, 3, 3), of(x * 2))
+    cache.advance(rows)
+    assert sound(cache, [6]) and y is not None
