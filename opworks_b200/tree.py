@@ -165,6 +165,7 @@ class _Places(NamedTuple):
     lens: torch.Tensor
     version: Any  # of lens
     capture: int  # the graph capture that they are part of; 0: none
+    stream: Any  # that computes them
     positions: torch.Tensor
     slots: torch.Tensor
 
@@ -210,16 +211,19 @@ class PagedCache:
             raise ValueError(f"the cache is on {self.lens.device}, which is not the current CUDA device")
         return torch.cuda.current_stream().cuda_stream
 
-    def _capture(self):
-        """The number of the graph capture that torch's current stream takes part in; 0: none."""
-        if self.lens.device.type != "cuda" or not torch.cuda.is_current_stream_capturing():
-            return 0
+    def _here(self):
+        """The number of the graph capture that torch's current stream takes part in (0: none), and the stream."""
+        if self.lens.device.type != "cuda":
+            return 0, None
+        stream = torch.cuda.current_stream(self.lens.device)
+        if not torch.cuda.is_current_stream_capturing():
+            return 0, stream
         number = ctypes.c_int64()
-        self.ops.ops_capture_id(torch.cuda.current_stream().cuda_stream, ctypes.byref(number))
-        return number.value
+        self.ops.ops_capture_id(stream.cuda_stream, ctypes.byref(number))
+        return number.value, stream
 
     def _no_graph(self, what):
-        if self._capture():
+        if self._here()[0]:
             raise ValueError(f"{what}: not while a graph is captured, where sequences share pages (each replay would take or give them again)")
 
     def _set_lens(self, lens):
@@ -274,7 +278,7 @@ class PagedCache:
             if take:
                 self._no_graph("place")
             at = self._where(rows, take)
-            self._placed = _Places(rows, self.lens, _version(self.lens), self._capture(), *at)
+            self._placed = _Places(rows, self.lens, _version(self.lens), *self._here(), *at)
             if take:
                 with torch.inference_mode(False):
                     self._step = (rows, self.lens + rows.start.diff())
@@ -294,17 +298,31 @@ class PagedCache:
 
     def _places(self, rows):
         """Positions and slots of the rows that the step has already, None: they are to be asked for. A program that moves lens has
-        moved the rows; what a graph computes is there when it is replayed, and only in it."""
+        moved the rows; what a graph computes is there when it is replayed, and only in it. Another stream than theirs waits for
+        them (and for the table, where pages were taken): the program does not know of them."""
         p = self._placed
-        if p is None or p.rows is not rows or p.lens is not self.lens or p.version is None or p.version != _version(self.lens) or p.capture != self._capture():
+        if p is None or p.rows is not rows or p.lens is not self.lens or p.version is None or p.version != _version(self.lens):
             return None
+        capture, stream = self._here()
+        if p.capture != capture:
+            return None
+        self._after(p.stream, stream, p.positions, p.slots, *([] if self._step is None else self._step[1:]))
         return p.positions, p.slots
+
+    @staticmethod
+    def _after(made, stream, *tensors):
+        """Lets a stream use what another one computes."""
+        if made != stream:
+            stream.wait_stream(made)
+            for t in tensors:
+                t.record_stream(stream)
 
     def drop(self):
         """Forgets the rows of the step that was placed: their pages go back, and lens is what it was before it."""
         if self._step is not None:
             self._no_graph("drop")
             rows, after = self._step
+            self._after(self._placed.stream, self._here()[1], after)
             with torch.inference_mode(False):
                 lens = after - rows.start.diff()
             self._give(after, lens)

@@ -227,6 +227,57 @@ def test_a_captured_write_takes_the_places_once():
     assert len(calls) == 1
 
 
+@pytest.mark.parametrize("format,blocks", [("int4", None), ("int4", 12), ("int8", 12)])
+def test_a_step_placed_on_one_stream_and_written_on_another(format, blocks):
+    """The program orders nothing but its own tensors: the places are the cache's."""
+    from opworks_b200.tree import PagedCache, Rows
+
+    cache = PagedCache(2, 2, 96, 1, 64, format, blocks=blocks)
+    warm = Rows([1, 1])
+    x = torch.randn(30, 64, device="cuda")
+    cache.write(0, x[:2], x[:2], warm)
+    cache.advance(warm)
+    rows = Rows([25, 5])
+    a, b = torch.cuda.Stream(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(a):
+        torch.cuda._sleep(100_000_000)  # about 50 ms: the places come late
+        cache.place(rows)
+    with torch.cuda.stream(b):
+        for layer in range(2):
+            cache.write(layer, x, x, rows)
+    torch.cuda.synchronize()
+    if format == "int4":
+        for layer in range(2):
+            assert torch.equal(held(cache, 0, layer, 1, 25), of(x[:25])) and torch.equal(held(cache, 1, layer, 1, 5), of(x[25:]))
+    else:
+        for layer in range(2):
+            k, v = cache.read(layer, rows)
+            assert torch.equal(k, v) and (k.flatten(1) - x).abs().max() <= x.abs().max() / 126
+
+
+@pytest.mark.parametrize("end", ["advance", "drop", "commit"])
+def test_a_shared_step_ended_on_another_stream(end):
+    from opworks_b200.tree import PagedCache, Rows
+
+    cache, rows = PagedCache(1, 2, 96, 1, 64, "int4", blocks=12), Rows([25, 5])
+    x, zeros = torch.randn(30, 64, device="cuda"), torch.zeros(30, dtype=torch.int32, device="cuda")
+    rows.parents  # made before: a commit reads them
+    a, b = torch.cuda.Stream(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(a):
+        torch.cuda._sleep(100_000_000)
+        cache.write(0, x, x, rows)
+    with torch.cuda.stream(b):
+        if end == "commit":
+            cache.commit(zeros, zeros + 1, rows)
+        else:
+            cache.advance(rows) if end == "advance" else cache.drop()
+    torch.cuda.synchronize()
+    assert sound(cache, {"advance": [25, 5], "drop": [0, 0], "commit": [1, 1]}[end])
+
+
+
 def test_shared_pages_are_not_taken_by_a_graph():
     """Each replay would take them again, and the host would not know. What was placed before may be written in one."""
     from opworks_b200.tree import PagedCache, Rows
