@@ -199,7 +199,7 @@ class PagedCache:
         with torch.inference_mode(False):  # (lens is a plain tensor in that mode too, so that its changes are counted)
             self._set_lens(torch.zeros(batch, dtype=torch.int32, device=device))
         self.bounds = [0] * batch  # upper bounds of lens that the host knows
-        self._before = None        # those before the last commit
+        self._before = None        # those before the last commit; None in it: a sequence that has ended since
 
     @property
     def max_len(self):
@@ -353,7 +353,9 @@ class PagedCache:
             self._give(self.lens, lens)
         self._set_lens(lens)
         self._placed = None
-        self.bounds, self._before = [0 if g else n for n, g in zip(self.bounds, gone)], None
+        self.bounds = [0 if g else n for n, g in zip(self.bounds, gone)]
+        if self._before is not None:
+            self._before = [None if g else n for n, g in zip(self._before, gone)]
 
     def write(self, layer, k, v, rows):
         """K and V rows [total, kv_heads * head_dim] (any row stride) at positions lens + 0, 1, ... of their sequences."""
@@ -463,11 +465,12 @@ class PagedCache:
 
     def kept(self, counts):
         """Tells the host what the last commit kept: its count, which the caller has read. Without it a sequence is taken
-        to have grown by its tree's deepest path, and the cache seems full before it is."""
+        to have grown by its tree's deepest path, and the cache seems full before it is. Sequences may have ended (release) in
+        between: theirs are passed over."""
         counts = [int(n) for n in counts]
         if self._before is None or len(counts) != self.batch:
             raise ValueError("kept: the counts of a commit, once after it")
-        bounds = [b + n for b, n in zip(self._before, counts)]
+        bounds = [most if b is None else b + n for b, n, most in zip(self._before, counts, self.bounds)]
         if any(n < 0 for n in counts) or any(b > most for b, most in zip(bounds, self.bounds)):
             raise ValueError("kept: no more than the deepest paths of the last commit's trees")
         self.bounds, self._before = bounds, None

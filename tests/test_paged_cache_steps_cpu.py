@@ -97,3 +97,21 @@ def test_shared_pages_and_a_length_that_the_program_moves(how):
     own.advance(rows)
     own.release([1])
     assert own.lens.tolist() == [50, 0]
+
+
+@pytest.mark.parametrize("blocks", [None, 12])
+def test_counts_told_after_a_release(blocks):
+    from opworks_b200.tree import Rows
+
+    c, rows = cache(blocks=blocks, batch=3), Rows([4, 3, 2], device="cpu")
+    tokens = torch.zeros(9, dtype=torch.int32)
+    c.write(0, torch.zeros(9, 64), torch.zeros(9, 64), rows)
+    c.commit(tokens, tokens, rows)
+    c.release([1])
+    for bad in ([1, 2], [5, 0, 1], [1, 0, -1], [1, -1, 1]):
+        with pytest.raises(ValueError, match="kept"):
+            c.kept(bad)
+    c.kept([2, 3, 1])
+    assert c.bounds == [2, 0, 1]
+    with pytest.raises(ValueError, match="kept"):
+        c.kept([2, 3, 1])

@@ -308,3 +308,19 @@ def test_shared_pages_are_not_taken_by_a_graph():
     assert torch.equal(held(cache, 0, 0, 3, 3), of(x * 2))
     cache.advance(rows)
     assert sound(cache, [6]) and y is not None
+
+
+def test_kept_after_some_of_the_sequences_have_ended():
+    from opworks_b200.tree import PagedCache, Rows
+
+    cache = PagedCache(1, 3, 64, 1, 64, "int4", blocks=12)
+    rows = Rows([4, 3, 2])
+    x = torch.randn(9, 64, device="cuda")
+    cache.write(0, x, x, rows)
+    _, count, _ = cache.commit(torch.zeros(9, dtype=torch.int32, device="cuda"), torch.ones(9, dtype=torch.int32, device="cuda"), rows)
+    cache.release([1])
+    assert cache.bounds == [4, 0, 2]
+    cache.kept(count.tolist())
+    assert cache.bounds == [1, 0, 1] and cache.lens.tolist() == [1, 0, 1]
+    with pytest.raises(ValueError, match="kept"):
+        cache.kept(count.tolist())
