@@ -97,7 +97,7 @@ class Rows:
         self.mask, self.words, self._parents = None, 0, None
         self.lift = None  # of a tree: a node's depth less its number
         if parents is None:
-            (self.start,) = to_device(device, start)
+            self.start, self.sizes = to_device(device, start, np.diff(start))
             return
         if [len(p) for p in parents] != self.counts:
             raise ValueError("parents: one list per sequence, as long as its rows")
@@ -105,7 +105,7 @@ class Rows:
         mask = np.concatenate([tree_mask(p, self.words) for p in parents])
         self.depths = [deepest(p) for p in parents]
         lift = np.concatenate([np.subtract(depths(p), range(len(p))) for p in parents]).astype(np.int32)
-        self.start, self.mask, self._parents, self.lift = to_device(device, start, mask, np.concatenate(parents).astype(np.int32), lift)
+        self.start, self.sizes, self.mask, self._parents, self.lift = to_device(device, start, np.diff(start), mask, np.concatenate(parents).astype(np.int32), lift)
 
     @property
     def parents(self):
@@ -127,6 +127,14 @@ def _current(device):
 def _version(t):
     """The number of changes in place of a tensor; None where nothing counts them (made in inference mode)."""
     return None if t.is_inference() else t._version
+
+
+def _plain(make):
+    """A tensor whose changes in place are counted, in inference mode too."""
+    if not torch.is_inference_mode_enabled():
+        return make()
+    with torch.inference_mode(False):
+        return make()
 
 
 def qk_norm_rope(q, k, positions, inv_freq=None, q_weight=None, k_weight=None, eps=1e-5, out=None):
@@ -170,6 +178,14 @@ class _Places(NamedTuple):
     slots: torch.Tensor
 
 
+class _Step(NamedTuple):
+    """A step that has taken its pages, where sequences share them."""
+
+    rows: Rows
+    after: torch.Tensor  # lens with all of its rows
+    stream: Any  # that takes them
+
+
 class PagedCache:
     PAGE = 16
 
@@ -195,9 +211,8 @@ class PagedCache:
             self.table = torch.arange(blocks, dtype=torch.int32, device=device).view(self.stride, batch).t().contiguous()
         self.status = torch.zeros(1, dtype=torch.int32, device=device)  # of the last pages taken or given: 0
         self._placed = None        # the places of the last step that asked for them
-        self._step = None          # with shared pages the step that has taken its own: (rows, lens after all of them)
-        with torch.inference_mode(False):  # (lens is a plain tensor in that mode too, so that its changes are counted)
-            self._set_lens(torch.zeros(batch, dtype=torch.int32, device=device))
+        self._step = None          # with shared pages the step that has taken its own and is not ended
+        self._set_lens(_plain(lambda: torch.zeros(batch, dtype=torch.int32, device=device)))
         self.bounds = [0] * batch  # upper bounds of lens that the host knows
         self._before = None        # those before the last commit; None in it: a sequence that has ended since
 
@@ -211,19 +226,19 @@ class PagedCache:
             raise ValueError(f"the cache is on {self.lens.device}, which is not the current CUDA device")
         return torch.cuda.current_stream().cuda_stream
 
-    def _here(self):
-        """The number of the graph capture that torch's current stream takes part in (0: none), and the stream."""
-        if self.lens.device.type != "cuda":
-            return 0, None
-        stream = torch.cuda.current_stream(self.lens.device)
-        if not torch.cuda.is_current_stream_capturing():
-            return 0, stream
+    def _capturing(self):
+        return self.lens.device.type == "cuda" and torch.cuda.is_current_stream_capturing()
+
+    def _capture(self, stream):
+        """The number of the graph capture that the current stream takes part in; 0: none."""
+        if not self._capturing():
+            return 0
         number = ctypes.c_int64()
-        self.ops.ops_capture_id(stream.cuda_stream, ctypes.byref(number))
-        return number.value, stream
+        self.ops.ops_capture_id(stream, ctypes.byref(number))
+        return number.value
 
     def _no_graph(self, what):
-        if self._here()[0]:
+        if self._capturing():
             raise ValueError(f"{what}: not while a graph is captured, where sequences share pages (each replay would take or give them again)")
 
     def _set_lens(self, lens):
@@ -252,13 +267,13 @@ class PagedCache:
         if self.shared and self._pages(b + n for b, n in zip(self.bounds, rows.counts)) > self.blocks:
             raise ValueError("the cache has no pages for these rows")
 
-    def _where(self, rows, take):
+    def _where(self, rows, take, stream):
         """Positions (int32) and slots (int64) of the rows; with ``take`` their pages come off the stack."""
         positions = torch.empty(rows.total, dtype=torch.int32, device=self.lens.device)
         slots = torch.empty(rows.total, dtype=torch.int64, device=self.lens.device)
         stack = (self.free, self.free_count) if take else (None, None)
         self.ops.page_take(self.lens, rows.start, self.batch, rows.total, self.table, self.stride, *stack, positions, slots, stack[1],
-                           self.status, self._stream())
+                           self.status, stream)
         return positions, slots
 
     def place(self, rows):
@@ -268,20 +283,26 @@ class PagedCache:
         graph is captured (write, read and attend may be captured once they are)."""
         self._belongs(rows)
         self._room(rows)
+        return self._at(rows, self._stream())
+
+    def _at(self, rows, stream):
         if self.shared:
             self._own_lens()
-            if self._step is not None and self._step[0] is not rows:
+            if self._step is not None and self._step.rows is not rows:
                 raise ValueError("place: the step before has been given its places and is neither kept nor dropped (advance, commit, drop)")
-        at = self._places(rows)
-        if at is None:
-            take = self.shared and self._step is None
-            if take:
-                self._no_graph("place")
-            at = self._where(rows, take)
-            self._placed = _Places(rows, self.lens, _version(self.lens), *self._here(), *at)
-            if take:
-                with torch.inference_mode(False):
-                    self._step = (rows, self.lens + rows.start.diff())
+        at = self._places(rows, stream)
+        if at is not None:
+            return at
+        capture, current = self._capture(stream), torch.cuda.current_stream() if self.lens.device.type == "cuda" else None
+        take = self.shared and self._step is None
+        if take:
+            self._no_graph("place")
+        elif self._step is not None and not capture:
+            self._after(self._step.stream, stream, self._step.after)
+        at = self._where(rows, take, stream)
+        self._placed = _Places(rows, self.lens, _version(self.lens), capture, current, *at)
+        if take:
+            self._step = _Step(rows, _plain(lambda: self.lens + rows.sizes), current)
         return at
 
     def _own_lens(self):
@@ -296,35 +317,34 @@ class PagedCache:
         at, _ = self.place(rows)
         return at if rows.lift is None else at + rows.lift
 
-    def _places(self, rows):
+    def _places(self, rows, stream):
         """Positions and slots of the rows that the step has already, None: they are to be asked for. A program that moves lens has
         moved the rows; what a graph computes is there when it is replayed, and only in it. Another stream than theirs waits for
         them (and for the table, where pages were taken): the program does not know of them."""
         p = self._placed
         if p is None or p.rows is not rows or p.lens is not self.lens or p.version is None or p.version != _version(self.lens):
             return None
-        capture, stream = self._here()
-        if p.capture != capture:
+        if p.capture != self._capture(stream):
             return None
-        self._after(p.stream, stream, p.positions, p.slots, *([] if self._step is None else self._step[1:]))
+        self._after(p.stream, stream, p.positions, p.slots, *([] if self._step is None else [self._step.after]))
         return p.positions, p.slots
 
     @staticmethod
     def _after(made, stream, *tensors):
-        """Lets a stream use what another one computes."""
-        if made != stream:
-            stream.wait_stream(made)
+        """Lets the current stream (its handle) use what another one computes."""
+        if made is not None and made.cuda_stream != stream:
+            current = torch.cuda.current_stream()
+            current.wait_stream(made)
             for t in tensors:
-                t.record_stream(stream)
+                t.record_stream(current)
 
     def drop(self):
         """Forgets the rows of the step that was placed: their pages go back, and lens is what it was before it."""
         if self._step is not None:
             self._no_graph("drop")
-            rows, after = self._step
-            self._after(self._placed.stream, self._here()[1], after)
-            with torch.inference_mode(False):
-                lens = after - rows.start.diff()
+            rows, after, made = self._step
+            self._after(made, self._stream(), after)
+            lens = _plain(lambda: after - rows.sizes)
             self._give(after, lens)
             if not self._unmoved():
                 self._set_lens(lens)
@@ -347,8 +367,7 @@ class PagedCache:
             self._no_graph("release")
             self._own_lens()
         (mask,) = to_device(self.lens.device, gone)
-        with torch.inference_mode(False):
-            lens = torch.where(mask != 0, torch.zeros_like(self.lens), self.lens)
+        lens = _plain(lambda: torch.where(mask != 0, torch.zeros_like(self.lens), self.lens))
         if self.shared:
             self._give(self.lens, lens)
         self._set_lens(lens)
@@ -364,21 +383,23 @@ class PagedCache:
         self._takes("k", k, shape, TYPES)
         self._takes("v", v, shape, (k.dtype,))
         self._room(rows)
+        if self.shared or self.format:
+            stream = self._stream()
         if self.shared or self.format == INT4:
-            _, slots = self.place(rows)
+            _, slots = self._at(rows, stream)
         if self.format == INT4:
             k, v = (x if x.stride(1) == 1 else x.contiguous() for x in (k, v))
             stride = lambda x: x.stride(0) if rows.total > 1 else shape[1]  # noqa: E731
             self.ops.kv4_write(k, stride(k), v, stride(v), TYPES[k.dtype], self.pool[layer], self.blocks, slots, rows.total, self.kv_heads,
-                               self.head_dim, self._stream())
+                               self.head_dim, stream)
             return
         if k.stride() != v.stride() or k.stride(1) != 1:  # the operator takes one row stride
             k, v = k.contiguous(), v.contiguous()
         if self.format:
             self.ops.kv_quant_write(k, v, TYPES[k.dtype], k.stride(0), self.pool[layer], self.format, self.table, self.stride,
-                                    self.lens, rows.start, self.batch, rows.total, self.kv_heads, self.head_dim, self._stream())
+                                    self.lens, rows.start, self.batch, rows.total, self.kv_heads, self.head_dim, stream)
             return
-        owner = torch.repeat_interleave(torch.arange(self.batch, device=k.device), rows.start.diff(), output_size=rows.total)
+        owner = torch.repeat_interleave(torch.arange(self.batch, device=k.device), rows.sizes, output_size=rows.total)
         pos = self.lens.long()[owner] + torch.arange(rows.total, device=k.device) - rows.start.long()[owner]
         block, slot = self.table.long()[owner, pos // self.PAGE], pos % self.PAGE
         shape = (rows.total, self.kv_heads, self.head_dim)
@@ -395,10 +416,10 @@ class PagedCache:
         k = torch.empty(rows.total, self.kv_heads, self.head_dim, dtype=dtype, device=self.lens.device)
         v = torch.empty_like(k)
         if self.format == INT4:
-            _, slots = self._places(rows) or self._where(rows, False)
+            stream = self._stream()
+            _, slots = self._places(rows, stream) or self._where(rows, False, stream)
             width = self.kv_heads * self.head_dim
-            self.ops.kv4_read(self.pool[layer], self.blocks, slots, rows.total, self.kv_heads, self.head_dim, k, width, v, width, TYPES[dtype],
-                              self._stream())
+            self.ops.kv4_read(self.pool[layer], self.blocks, slots, rows.total, self.kv_heads, self.head_dim, k, width, v, width, TYPES[dtype], stream)
             return k, v
         self.ops.kv_quant_read(self.pool[layer], self.format, self.table, self.stride, self.lens, rows.start, self.batch,
                                rows.total, self.kv_heads, self.head_dim, k, v, TYPES[dtype], self.kv_heads * self.head_dim,
@@ -430,8 +451,7 @@ class PagedCache:
         if self.shared:
             self._no_graph("advance")
             self.place(rows)
-        with torch.inference_mode(False):
-            self._set_lens(self._step[1] if self.shared else self.lens + rows.start.diff())
+        self._set_lens(self._step.after if self.shared else _plain(lambda: self.lens + rows.sizes))
         self._placed = self._step = None
         self.bounds, self._before = [b + n for b, n in zip(self.bounds, rows.counts)], None
 
@@ -444,8 +464,7 @@ class PagedCache:
         draft, target = draft.to(torch.int32).contiguous(), target.to(torch.int32).contiguous()
         new = lambda n: torch.empty(n, dtype=torch.int32, device=self.lens.device)  # noqa: E731
         path, count, nxt = new(rows.total), new(self.batch), new(self.batch)
-        with torch.inference_mode(False):
-            lens = new(self.batch)
+        lens = _plain(lambda: new(self.batch))
         head = (draft, target, rows.parents, rows.start, self.lens, self.batch, rows.most)
         tail = (self.layers, self.table, self.stride, self.kv_heads, self.head_dim, path, count, nxt, lens, self._stream())
         if self.shared:
@@ -457,7 +476,7 @@ class PagedCache:
         else:
             self.ops.tree_commit(*head, self.k, self.v, self.k.stride(0), *tail)
         if self.shared:  # pages that the drafts had and the kept path does not need
-            self._give(self._step[1], lens)
+            self._give(self._step.after, lens)
         self._set_lens(lens)
         self._placed = self._step = None
         self._before, self.bounds = self.bounds, [b + n for b, n in zip(self.bounds, rows.depths)]
