@@ -78,6 +78,9 @@ def to_device(device, *arrays):
     the copy is done)."""
     both = torch.from_numpy(np.concatenate([a.ravel() for a in arrays]))
     if torch.device(device).type == "cuda":
+        if torch.cuda.is_current_stream_capturing():
+            raise ValueError("rows and the numbers of sequences come from the host: not while a graph is captured (each replay would copy them again, "
+                             "from memory that holds others by then)")
         both = both.pin_memory().to(device, non_blocking=True)
     out, at = [], 0
     for a in arrays:
@@ -110,11 +113,14 @@ class Rows:
     @property
     def parents(self):
         """The node that each row follows, int32 on the device: in a chain the one before it."""
-        if self._parents is None:
-            owner = np.repeat(np.arange(len(self.counts)), self.counts)
-            node = np.arange(self.total) - np.concatenate([[0], np.cumsum(self.counts)])[owner]
-            (self._parents,) = to_device(self.start.device, (node - 1).astype(np.int32))
-        return self._parents
+        if self._parents is not None:
+            return self._parents
+        device = self.start.device
+        owner = torch.repeat_interleave(torch.arange(len(self.counts), device=device), self.sizes, output_size=self.total)
+        parents = torch.arange(self.total, dtype=torch.int32, device=device) - self.start[owner] - 1
+        if device.type != "cuda" or not torch.cuda.is_current_stream_capturing():  # (a graph's are there when it is replayed)
+            self._parents = parents
+        return parents
 
 
 def _current(device):
