@@ -143,6 +143,15 @@ def _plain(make):
         return make()
 
 
+def _lines(x, rows, width, elem):
+    """x, or a copy of it, as operators take rows of `width` elements of `elem` bytes (apart, and beginning where 16 bytes are
+    loaded at a time), and its row stride."""
+    stride = x.stride(0) if rows > 1 else width
+    if (x.data_ptr() | stride * elem) & 15 == 0 and stride >= width:
+        return x, stride
+    return x.clone(memory_format=torch.contiguous_format), width
+
+
 def qk_norm_rope(q, k, positions, inv_freq=None, q_weight=None, k_weight=None, eps=1e-5, out=None):
     """Queries [rows, q_heads, D] and keys [rows, kv_heads, D] (fp32 or bf16, any row stride), each head normalised (root mean
     square, fp32 weights [D]; None: that side is not) and its first 2 * len(inv_freq) dims rotated by its row's position (int32;
@@ -167,7 +176,8 @@ def qk_norm_rope(q, k, positions, inv_freq=None, q_weight=None, k_weight=None, e
     if rot and positions is None:
         raise ValueError("positions: a rotation needs them")
     stride = lambda t: t.stride(0) if rows > 1 else t.shape[1] * dim  # noqa: E731
-    ops_lib().qk_norm_rope(q, stride(q), k, stride(k), TYPES[q.dtype], q_weight, k_weight, eps, positions if rot else None, inv_freq if rot else None,
+    (q, qs), (k, ks) = ((x, stride(x)) if x is y else _lines(x, rows, x.shape[1] * dim, x.element_size()) for x, y in zip((q, k), new))
+    ops_lib().qk_norm_rope(q, qs, k, ks, TYPES[q.dtype], q_weight, k_weight, eps, positions if rot else None, inv_freq if rot else None,
                            rot, rows, q.shape[1], k.shape[1], dim, new[0], stride(new[0]), new[1], stride(new[1]), _current(q.device))
     return new
 
@@ -394,15 +404,21 @@ class PagedCache:
         if self.shared or self.format == INT4:
             _, slots = self._at(rows, stream)
         if self.format == INT4:
-            k, v = (x if x.stride(1) == 1 else x.contiguous() for x in (k, v))
-            stride = lambda x: x.stride(0) if rows.total > 1 else shape[1]  # noqa: E731
-            self.ops.kv4_write(k, stride(k), v, stride(v), TYPES[k.dtype], self.pool[layer], self.blocks, slots, rows.total, self.kv_heads,
+            elem = 4 if k.dtype is torch.float32 else 2
+            k, ks = _lines(k if k.stride(1) == 1 else k.contiguous(), rows.total, shape[1], elem)
+            v, vs = _lines(v if v.stride(1) == 1 else v.contiguous(), rows.total, shape[1], elem)
+            self.ops.kv4_write(k, ks, v, vs, TYPES[k.dtype], self.pool[layer], self.blocks, slots, rows.total, self.kv_heads,
                                self.head_dim, stream)
             return
         if k.stride() != v.stride() or k.stride(1) != 1:  # the operator takes one row stride
             k, v = k.contiguous(), v.contiguous()
         if self.format:
-            self.ops.kv_quant_write(k, v, TYPES[k.dtype], k.stride(0), self.pool[layer], self.format, self.table, self.stride,
+            elem = 4 if k.dtype is torch.float32 else 2
+            stride = k.stride(0) if rows.total > 1 else shape[1]
+            if (k.data_ptr() | v.data_ptr() | stride * elem) & 15 or stride < shape[1]:
+                k, v = (x.clone(memory_format=torch.contiguous_format) for x in (k, v))
+                stride = shape[1]
+            self.ops.kv_quant_write(k, v, TYPES[k.dtype], stride, self.pool[layer], self.format, self.table, self.stride,
                                     self.lens, rows.start, self.batch, rows.total, self.kv_heads, self.head_dim, stream)
             return
         owner = torch.repeat_interleave(torch.arange(self.batch, device=k.device), rows.sizes, output_size=rows.total)
