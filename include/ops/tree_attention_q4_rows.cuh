@@ -607,19 +607,6 @@ static __global__ void __launch_bounds__(Q4RowsGeo<T, D, kNT>::kThreads, kNT <= 
     cluster_sync_all(); // peers read this CTA's shared memory until here
 }
 
-// The tensor cores cut a sum off at every product of 16 keys, by less than a unit in its last
-// place. bf16 rows of more than 4 a head are summed there, and where V has one sign they come out
-// smaller by 2^-24.6 a product here, 2^-23.6 with tcgen05 (160 sequences of 1,000,000 tokens: by
-// 3.0e-4 over the 125,000 keys of a warp, by 2.5e-3 over the 500,000 of a stream of the tiles;
-// rounding to bf16 is 1.3e-3 in the mean). So the keys of a sum are held to kQ4SumKeys of a warp
-// here (2e-5) and kQ4SumTiles tiles of a CTA there (8e-5, or 1.6e-4 where its streams have rows of
-// their own), as far as clusters go: 8 of them reach 260,000 tokens, at 1,000,000 it is 3.1e-4
-// (6.4e-4). The other way, sums of one step added up outside as fp32 rows have them, costs 4 to 8 %
-// at every length (12 x 32,000 tokens, 8 rows a head, D 128: 91 us, 98 so), and tiles of 128 dims
-// have no room for it; clusters that would not be there else cost 2 % (a prompt's 2048 rows behind
-// 65,000 tokens: 2.40 ms, 2.45 so).
-constexpr int64_t kQ4SumKeys = 8192, kQ4SumTiles = 256;
-
 // CTAs of a kernel that run at once on the current device. Asked once.
 template <typename... P> inline int q4_slots(void (*kernel)(P...), int threads, int bytes) {
     struct Known {
@@ -656,10 +643,6 @@ template <typename T, int D, int kNT> inline void q4_rows_launch(const T *q, T *
     int64_t splits = 1;
     if (all < sms || steps >= 16 * G::kWarps)
         while (2 * splits <= cap && 2 * splits * all * 3 <= slots * 4)
-            splits *= 2;
-    // bf16 rows, more than 4: a warp's sum stays in the tensor cores over all of its keys, see kQ4SumKeys
-    if constexpr (!G::kWide && !G::kPair)
-        while (2 * splits <= most && keys > kQ4SumKeys * G::kWarps * splits)
             splits *= 2;
     require(groups * splits <= 0x7fffffff, "tree attention: too many rows for one call");
     // sequences in the order of their length, where SMs have more than one CTA (their list is short

@@ -821,11 +821,9 @@ template <typename T, int D, int kM> inline void q4_tiles_launch(const T *q, T *
     const int64_t rows = static_cast<int64_t>(a.t.max_rows) * (a.qh / a.kvh);
     const int64_t groups = (rows + G::kRows - 1) / G::kRows, all = groups * a.kvh * a.t.batch;
     const int64_t tiles = (static_cast<int64_t>(a.t.max_ctx) + a.t.max_rows + kTileKeys - 1) / kTileKeys;
-    // splits (powers of two) while all clusters still run at once and each CTA has four tiles, or as
-    // long as the sums of bf16 rows are longer than they should be
+    // splits (powers of two) while all clusters still run at once and each CTA has four tiles
     int splits = 1;
-    while (2 * splits <= 8 && 8 * splits <= tiles &&
-           ((!G::kWide && tiles > kQ4SumTiles * splits) || all <= q4_clusters(kernel, kTileThreads, G::kBytes, 2 * splits)))
+    while (2 * splits <= 8 && 8 * splits <= tiles && all <= q4_clusters(kernel, kTileThreads, G::kBytes, 2 * splits))
         splits *= 2;
     require(groups * splits <= 0x7fffffff, "tree attention: too many rows for one call");
     // more CTAs than places: sequences in the order of their length (the list of them lies over row_fac, stat and joined)
