@@ -41,6 +41,19 @@
 
 namespace opworks::detail {
 
+// The tensor cores cut a sum off at every product of 16 keys, by less than a unit in its last
+// place. bf16 rows of more than 4 a head are summed there, and over V of one sign they came out
+// smaller by 2^-23.6 a product (160 sequences of 1,000,000 tokens: by 3.0e-4 over the 62,500 keys
+// of a warp here, by 2.5e-3 over the 500,000 of a stream of the tiles; rounding to bf16 is 1.3e-3
+// in the mean). So the sum of kQ4SumKeys (4e-5), of kQ4SumTiles tiles (8e-5), is put by: added,
+// rounded, to one in local memory, which only a reference that is raised touches else. A kernel of
+// its own does that, where the context may be so long: the code alone costs 0 to 4 % (2048 rows
+// behind 40,000 tokens, D 128: 2.16 ms without, 2.20 with; 8 rows a head of 64 sequences of 2,000:
+// 46.4 us, 47.7). Sums of one step added up outside, as fp32 rows have them, cost 4 to 8 % at every
+// length, and tiles of 128 dims have no room for them; more splits by the bound of the context are
+// paid by every short sequence (a bound of 131,072: 2.5 to 4 times as long).
+constexpr int kQ4SumKeys = 8192, kQ4SumTiles = 128;
+
 // kNT: tiles of 8 columns; 0: one tile with two columns a row.
 template <typename T, int D, int kNT> struct Q4RowsGeo {
     static constexpr bool kWide = std::is_same_v<T, float>, kPair = kNT == 0;
@@ -59,6 +72,9 @@ template <typename T, int D, int kNT> struct Q4RowsGeo {
     static constexpr int kPairs = D == 64 && kNT <= 1 ? 2 : 1; // of pages
     static constexpr int kStepPages = 2 * kPairs, kStepKeys = kStepPages * kKvPage;
     static constexpr int kStages = kPairs == 2 ? 2 : 3;
+    static constexpr bool kInCore = !kWide && !kPair;           // O is summed by the tensor cores,
+    static constexpr int kPeriod = kQ4SumKeys / kStepKeys;      // and put by after so many steps of a warp
+    static constexpr int kFar = 8 * kGroups * kTiles;           // floats of O that a lane has
     static constexpr int kPageBytes = Kv4Record<D>::kBytes, kStage = kStepPages * kPageBytes;
     static constexpr int kQBytes = kSets * kTiles * kGroups * 2 * 32 * 8 + 128; // fragments; a factor a row
     static constexpr int kRing = kStages * kStage; // of a warp
@@ -178,7 +194,8 @@ __device__ __forceinline__ TreeSpan q4_span_by_work(const TreeBatch &t, int orde
     return s;
 }
 
-template <typename T, int D, int kNT>
+// kPutBy: a warp may have more than kPeriod steps, and sums are put by.
+template <typename T, int D, int kNT, bool kPutBy>
 static __global__ void __launch_bounds__(Q4RowsGeo<T, D, kNT>::kThreads, kNT <= 1 ? 2 : 1)
     q4_rows_kernel(const T *__restrict__ q, T *__restrict__ out, TreeArgs a, int rep, int splits, int descending) {
     using G = Q4RowsGeo<T, D, kNT>;
@@ -315,216 +332,240 @@ static __global__ void __launch_bounds__(Q4RowsGeo<T, D, kNT>::kThreads, kNT <= 
     for (int rr = 0; rr < G::kRPL; ++rr)
         m[rr] = kQ4None, l[rr] = 0.f;
 
+    [[maybe_unused]] float far_room[kPutBy ? G::kFar : 1]; // what has been put by, in the order of o
+    [[maybe_unused]] float *far = far_room;
+    if constexpr (kPutBy)
+        asm volatile("" : "+l"(far)); // (stays in local memory)
+
     const uint32_t ring_at = sm100::smem_u32(ring) + (lane / 16) * G::kPageBytes + lane % 16 * 16; // both pages' rows of a group
     int at = 0;
-    for (int i = 0; i < mine; ++i) {
-        q4_copy_wait<G::kStages - 2>();
-        __syncwarp(); // all lanes' copies are there; all have done with the stage that is filled next
-        fetch(i + G::kStages - 1, at == 0 ? G::kStages - 1 : at - 1);
-        const uint8_t *stage = ring + at * G::kStage;
-        const uint32_t stage_at = ring_at + at * G::kStage;
-        at = at + 1 == G::kStages ? 0 : at + 1;
-        const int key0 = (first + i * stride) * G::kStepKeys;
-        const bool edge = key0 + G::kStepKeys > span.ctx;
+    int i = 0;
+    for (int end = 0; i < mine;) {
+        end = kPutBy ? min(mine, end + G::kPeriod) : mine;
+        for (; i < end; ++i) {
+            q4_copy_wait<G::kStages - 2>();
+            __syncwarp(); // all lanes' copies are there; all have done with the stage that is filled next
+            fetch(i + G::kStages - 1, at == 0 ? G::kStages - 1 : at - 1);
+            const uint8_t *stage = ring + at * G::kStage;
+            const uint32_t stage_at = ring_at + at * G::kStage;
+            at = at + 1 == G::kStages ? 0 : at + 1;
+            const int key0 = (first + i * stride) * G::kStepKeys;
+            const bool edge = key0 + G::kStepKeys > span.ctx;
 
-        // ---- scores: of key 16 p + 8 e + g at place 2 p + e
-        float x[G::kRPL][2 * G::kStepPages] = {};
+            // ---- scores: of key 16 p + 8 e + g at place 2 p + e
+            float x[G::kRPL][2 * G::kStepPages] = {};
 #pragma unroll
-        for (int pp = 0; pp < G::kPairs; ++pp)
-#pragma unroll
-            for (int c = 0; c < G::kGroups; ++c) {
-                uint32_t w[4], k[4][4];
-                q4_ldmatrix<false>(stage_at + pp * 2 * G::kPageBytes + c * 256, w);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    __half2 codes[4];
-                    kv4_integers(w[j], codes);
-#pragma unroll
-                    for (int n = 0; n < 4; ++n)
-                        k[j][n] = kv4_bits(codes[n]);
-                }
-                float sum[2][G::kTiles][4];
-#pragma unroll
-                for (int p = 0; p < 2; ++p)
-#pragma unroll
-                    for (int nt = 0; nt < G::kTiles; ++nt)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            sum[p][nt][e] = 0.f;
-#pragma unroll
-                for (int set = G::kSets - 1; set >= 0; --set)
-#pragma unroll
-                    for (int u = 0; u < 2; ++u)
-#pragma unroll
-                        for (int nt = 0; nt < G::kTiles; ++nt) {
-                            uint32_t b0, b1;
-                            if constexpr (G::kQShared) {
-                                const uint2 f = q_shared[(((set * G::kTiles + nt) * G::kGroups + c) * 2 + u) * 32 + lane];
-                                b0 = f.x, b1 = f.y;
-                            } else {
-                                b0 = qf[set][nt][G::kQShared ? 0 : c][u][0], b1 = qf[set][nt][G::kQShared ? 0 : c][u][1];
-                            }
-#pragma unroll
-                            for (int p = 0; p < 2; ++p) {
-                                const uint32_t f[4] = {k[2 * p][2 * u], k[2 * p + 1][2 * u], k[2 * p][2 * u + 1], k[2 * p + 1][2 * u + 1]};
-                                mma_f16(sum[p][nt], f, b0, b1);
-                            }
-                        }
-#pragma unroll
-                for (int p = 0; p < 2; ++p)
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        const float s = __half2float(
-                            *reinterpret_cast<const __half *>(stage + (2 * pp + p) * G::kPageBytes + R::kKScale + (c * kKvPage + e * 8 + g) * 2));
-#pragma unroll
-                        for (int rr = 0; rr < G::kRPL; ++rr)
-                            x[rr][4 * pp + 2 * p + e] += s * (kPair ? sum[p][0][2 * e] + sum[p][0][2 * e + 1] : sum[p][rr / 2][2 * e + rr % 2]);
-                    }
-            }
-#pragma unroll
-        for (int rr = 0; rr < G::kRPL; ++rr)
-#pragma unroll
-            for (int n = 0; n < 2 * G::kStepPages; ++n)
-                x[rr][n] *= factor[rr];
-        if (edge) {
-            uint32_t bad = 0; // keys whose V is no number: a row that sees one gets NaN, the others nothing of it
-#pragma unroll
-            for (int n = 0; n < 2 * G::kStepPages; ++n)
+            for (int pp = 0; pp < G::kPairs; ++pp)
 #pragma unroll
                 for (int c = 0; c < G::kGroups; ++c) {
-                    const uint32_t v = *reinterpret_cast<const uint16_t *>(stage + n / 2 * G::kPageBytes + R::kVScale + (c * kKvPage + n % 2 * 8 + g) * 2);
-                    bad |= ((v & 0x7fffu) >= kQ4BadScale ? 1u : 0u) << n;
+                    uint32_t w[4], k[4][4];
+                    q4_ldmatrix<false>(stage_at + pp * 2 * G::kPageBytes + c * 256, w);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        __half2 codes[4];
+                        kv4_integers(w[j], codes);
+#pragma unroll
+                        for (int n = 0; n < 4; ++n)
+                            k[j][n] = kv4_bits(codes[n]);
+                    }
+                    float sum[2][G::kTiles][4];
+#pragma unroll
+                    for (int p = 0; p < 2; ++p)
+#pragma unroll
+                        for (int nt = 0; nt < G::kTiles; ++nt)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e)
+                                sum[p][nt][e] = 0.f;
+#pragma unroll
+                    for (int set = G::kSets - 1; set >= 0; --set)
+#pragma unroll
+                        for (int u = 0; u < 2; ++u)
+#pragma unroll
+                            for (int nt = 0; nt < G::kTiles; ++nt) {
+                                uint32_t b0, b1;
+                                if constexpr (G::kQShared) {
+                                    const uint2 f = q_shared[(((set * G::kTiles + nt) * G::kGroups + c) * 2 + u) * 32 + lane];
+                                    b0 = f.x, b1 = f.y;
+                                } else {
+                                    b0 = qf[set][nt][G::kQShared ? 0 : c][u][0], b1 = qf[set][nt][G::kQShared ? 0 : c][u][1];
+                                }
+#pragma unroll
+                                for (int p = 0; p < 2; ++p) {
+                                    const uint32_t f[4] = {k[2 * p][2 * u], k[2 * p + 1][2 * u], k[2 * p][2 * u + 1], k[2 * p + 1][2 * u + 1]};
+                                    mma_f16(sum[p][nt], f, b0, b1);
+                                }
+                            }
+#pragma unroll
+                    for (int p = 0; p < 2; ++p)
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            const float s = __half2float(
+                                *reinterpret_cast<const __half *>(stage + (2 * pp + p) * G::kPageBytes + R::kKScale + (c * kKvPage + e * 8 + g) * 2));
+#pragma unroll
+                            for (int rr = 0; rr < G::kRPL; ++rr)
+                                x[rr][4 * pp + 2 * p + e] += s * (kPair ? sum[p][0][2 * e] + sum[p][0][2 * e + 1] : sum[p][rr / 2][2 * e + rr % 2]);
+                        }
                 }
 #pragma unroll
+            for (int rr = 0; rr < G::kRPL; ++rr)
+#pragma unroll
+                for (int n = 0; n < 2 * G::kStepPages; ++n)
+                    x[rr][n] *= factor[rr];
+            if (edge) {
+                uint32_t bad = 0; // keys whose V is no number: a row that sees one gets NaN, the others nothing of it
+#pragma unroll
+                for (int n = 0; n < 2 * G::kStepPages; ++n)
+#pragma unroll
+                    for (int c = 0; c < G::kGroups; ++c) {
+                        const uint32_t v = *reinterpret_cast<const uint16_t *>(stage + n / 2 * G::kPageBytes + R::kVScale + (c * kKvPage + n % 2 * 8 + g) * 2);
+                        bad |= ((v & 0x7fffu) >= kQ4BadScale ? 1u : 0u) << n;
+                    }
+#pragma unroll
+                for (int rr = 0; rr < G::kRPL; ++rr) {
+                    const int r = row_base + (kPair ? t : rr / 2 * 8 + 2 * t + rr % 2);
+#pragma unroll
+                    for (int pp = 0; pp < G::kPairs; ++pp) {
+                        uint32_t seen = 0;
+                        if (r < rows)
+                            seen = tree_sees32(a.t, span.row0 + node_of(r), node_of(r), key0 + 32 * pp - span.ctx, keys - span.ctx);
+#pragma unroll
+                        for (int n = 0; n < 4; ++n) {
+                            if (bad >> (4 * pp + n) & 1u)
+                                x[rr][4 * pp + n] = __uint_as_float(0x7fc00000u);
+                            if (!(seen >> (n * 8 + g) & 1u))
+                                x[rr][4 * pp + n] = kNegInf;
+                        }
+                    }
+                }
+            }
+
+            // ---- weights
+            bool raise = false;
+            float top[G::kRPL];
+#pragma unroll
             for (int rr = 0; rr < G::kRPL; ++rr) {
-                const int r = row_base + (kPair ? t : rr / 2 * 8 + 2 * t + rr % 2);
+                top[rr] = x[rr][0];
+#pragma unroll
+                for (int n = 1; n < 2 * G::kStepPages; ++n)
+                    top[rr] = fmaxf(top[rr], x[rr][n]);
+                raise |= top[rr] - m[rr] > kQ4Top;
+            }
+            if (__any_sync(kFullWarpMask, raise)) {
+#pragma unroll
+                for (int rr = 0; rr < G::kRPL; ++rr) {
+#pragma unroll
+                    for (int off = 4; off < 32; off <<= 1)
+                        top[rr] = fmaxf(top[rr], __shfl_xor_sync(kFullWarpMask, top[rr], off));
+                    if (top[rr] - m[rr] > kQ4Top) {
+                        // below scores that are large a lift would be lost in the rounding, or grow by it
+                        const float up = fabsf(top[rr]) < 0x1p20f ? top[rr] - G::kLift : top[rr];
+                        const float fix = exp2_approx(m[rr] - up);
+                        m[rr] = up;
+                        l[rr] *= fix;
+                        if constexpr (kPutBy)
+                            if (end > G::kPeriod)
+#pragma unroll 1
+                                for (int n = rr / 2 * 4 + rr % 2; n < G::kFar; n += 4 * G::kTiles)
+                                    far[n] *= fix, far[n + 2] *= fix;
+#pragma unroll
+                        for (int c = 0; c < G::kGroups; ++c)
+#pragma unroll
+                            for (int n = 0; n < 2; ++n) {
+                                if constexpr (kPair) {
+                                    for (float &y : o[c][n][0])
+                                        y *= fix;
+                                } else {
+                                    o[c][n][rr / 2][rr % 2] *= fix, o[c][n][rr / 2][2 + rr % 2] *= fix;
+                                }
+                            }
+                    }
+                }
+            }
+            uint32_t pf[G::kSets][G::kTiles][G::kStepPages][2]; // of page p: keys 2t, 2t + 1, and 8 more, of column g
+#pragma unroll
+            for (int n = 0; n < 2 * G::kStepPages; ++n) {
+                if constexpr (kPair) {
+                    if (n % 2)
+                        continue;
+                    const float p0 = exp2_approx(x[0][n] - m[0]), p1 = exp2_approx(x[0][n + 1] - m[0]);
+                    l[0] += p0 + p1;
+                    uint32_t t0, t1;
+                    if constexpr (G::kWide)
+                        q4_terms(p0, p1, t0, t1);
+                    else
+                        t0 = half2_rn(p0, 0.f), t1 = half2_rn(p1, 0.f);
+                    pf[0][0][n / 2][0] = q4_transposed(t0), pf[0][0][n / 2][1] = q4_transposed(t1);
+                } else {
+#pragma unroll
+                    for (int nt = 0; nt < G::kTiles; ++nt) {
+                        float p0 = exp2_approx(x[2 * nt][n] - m[2 * nt]), p1 = exp2_approx(x[2 * nt + 1][n] - m[2 * nt + 1]);
+                        l[2 * nt] += p0, l[2 * nt + 1] += p1;
+                        if constexpr (G::kSets == 2) {
+                            pf[0][nt][n / 2][n % 2] = q4_transposed(q4_term(p0, p1));
+                            pf[1][nt][n / 2][n % 2] = q4_transposed(half2_rn(p0, p1));
+                        } else {
+                            pf[0][nt][n / 2][n % 2] = q4_transposed(half2_rn(p0, p1));
+                        }
+                    }
+                }
+            }
+
+            // ---- output
+#pragma unroll
+            for (int c = 0; c < G::kGroups; ++c) {
+                uint32_t v[2 * G::kStepPages][4];
 #pragma unroll
                 for (int pp = 0; pp < G::kPairs; ++pp) {
-                    uint32_t seen = 0;
-                    if (r < rows)
-                        seen = tree_sees32(a.t, span.row0 + node_of(r), node_of(r), key0 + 32 * pp - span.ctx, keys - span.ctx);
+                    uint32_t w[4];
+                    q4_ldmatrix<true>(stage_at + pp * 2 * G::kPageBytes + R::kCodes + c * 256, w);
 #pragma unroll
-                    for (int n = 0; n < 4; ++n) {
-                        if (bad >> (4 * pp + n) & 1u)
-                            x[rr][4 * pp + n] = __uint_as_float(0x7fc00000u);
-                        if (!(seen >> (n * 8 + g) & 1u))
-                            x[rr][4 * pp + n] = kNegInf;
+                    for (int j = 0; j < 4; ++j) {
+                        uint32_t s = *reinterpret_cast<const uint32_t *>(stage + (2 * pp + j / 2) * G::kPageBytes + R::kVScale +
+                                                                         (c * kKvPage + j % 2 * 8 + 2 * t) * 2);
+                        if (edge) // (times a weight of zero it would be NaN)
+                            s &= ((s & 0x7fffu) >= kQ4BadScale ? 0u : 0xffffu) | ((s >> 16 & 0x7fffu) >= kQ4BadScale ? 0u : 0xffff0000u);
+                        kv4_widen(w[j], kv4_half2(s), v[4 * pp + j]);
                     }
                 }
-            }
-        }
-
-        // ---- weights
-        bool raise = false;
-        float top[G::kRPL];
 #pragma unroll
-        for (int rr = 0; rr < G::kRPL; ++rr) {
-            top[rr] = x[rr][0];
+                for (int n = 0; n < 2; ++n) {
+                    float sum[G::kTiles][4] = {};
 #pragma unroll
-            for (int n = 1; n < 2 * G::kStepPages; ++n)
-                top[rr] = fmaxf(top[rr], x[rr][n]);
-            raise |= top[rr] - m[rr] > kQ4Top;
-        }
-        if (__any_sync(kFullWarpMask, raise)) {
+                    for (int set = G::kSets - 1; set >= 0; --set)
 #pragma unroll
-            for (int rr = 0; rr < G::kRPL; ++rr) {
+                        for (int p = 0; p < G::kStepPages; ++p) {
+                            const uint32_t f[4] = {v[2 * p][2 * n], v[2 * p][2 * n + 1], v[2 * p + 1][2 * n], v[2 * p + 1][2 * n + 1]};
 #pragma unroll
-                for (int off = 4; off < 32; off <<= 1)
-                    top[rr] = fmaxf(top[rr], __shfl_xor_sync(kFullWarpMask, top[rr], off));
-                if (top[rr] - m[rr] > kQ4Top) {
-                    // below scores that are large a lift would be lost in the rounding, or grow by it
-                    const float up = fabsf(top[rr]) < 0x1p20f ? top[rr] - G::kLift : top[rr];
-                    const float fix = exp2_approx(m[rr] - up);
-                    m[rr] = up;
-                    l[rr] *= fix;
-#pragma unroll
-                    for (int c = 0; c < G::kGroups; ++c)
-#pragma unroll
-                        for (int n = 0; n < 2; ++n) {
-                            if constexpr (kPair) {
-                                for (float &y : o[c][n][0])
-                                    y *= fix;
-                            } else {
-                                o[c][n][rr / 2][rr % 2] *= fix, o[c][n][rr / 2][2 + rr % 2] *= fix;
+                            for (int nt = 0; nt < G::kTiles; ++nt) {
+                                if constexpr (G::kWide || kPair)
+                                    mma_f16(sum[nt], f, pf[set][nt][p][0], pf[set][nt][p][1]);
+                                else
+                                    mma_f16(o[c][n][nt], f, pf[set][nt][p][0], pf[set][nt][p][1]);
                             }
                         }
-                }
-            }
-        }
-        uint32_t pf[G::kSets][G::kTiles][G::kStepPages][2]; // of page p: keys 2t, 2t + 1, and 8 more, of column g
+                    if constexpr (kPair) { // (the second column of bf16 rows is zero)
+                        o[c][n][0][0] += G::kWide ? sum[0][0] + sum[0][1] : sum[0][0];
+                        o[c][n][0][1] += G::kWide ? sum[0][2] + sum[0][3] : sum[0][2];
+                    } else if constexpr (G::kWide) {
 #pragma unroll
-        for (int n = 0; n < 2 * G::kStepPages; ++n) {
-            if constexpr (kPair) {
-                if (n % 2)
-                    continue;
-                const float p0 = exp2_approx(x[0][n] - m[0]), p1 = exp2_approx(x[0][n + 1] - m[0]);
-                l[0] += p0 + p1;
-                uint32_t t0, t1;
-                if constexpr (G::kWide)
-                    q4_terms(p0, p1, t0, t1);
-                else
-                    t0 = half2_rn(p0, 0.f), t1 = half2_rn(p1, 0.f);
-                pf[0][0][n / 2][0] = q4_transposed(t0), pf[0][0][n / 2][1] = q4_transposed(t1);
-            } else {
+                        for (int nt = 0; nt < G::kTiles; ++nt)
 #pragma unroll
-                for (int nt = 0; nt < G::kTiles; ++nt) {
-                    float p0 = exp2_approx(x[2 * nt][n] - m[2 * nt]), p1 = exp2_approx(x[2 * nt + 1][n] - m[2 * nt + 1]);
-                    l[2 * nt] += p0, l[2 * nt + 1] += p1;
-                    if constexpr (G::kSets == 2) {
-                        pf[0][nt][n / 2][n % 2] = q4_transposed(q4_term(p0, p1));
-                        pf[1][nt][n / 2][n % 2] = q4_transposed(half2_rn(p0, p1));
-                    } else {
-                        pf[0][nt][n / 2][n % 2] = q4_transposed(half2_rn(p0, p1));
+                            for (int e = 0; e < 4; ++e)
+                                o[c][n][nt][e] += sum[nt][e];
                     }
                 }
             }
         }
-
-        // ---- output
+        if constexpr (kPutBy)
+            if (mine > G::kPeriod)
 #pragma unroll
-        for (int c = 0; c < G::kGroups; ++c) {
-            uint32_t v[2 * G::kStepPages][4];
-#pragma unroll
-            for (int pp = 0; pp < G::kPairs; ++pp) {
-                uint32_t w[4];
-                q4_ldmatrix<true>(stage_at + pp * 2 * G::kPageBytes + R::kCodes + c * 256, w);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    uint32_t s = *reinterpret_cast<const uint32_t *>(stage + (2 * pp + j / 2) * G::kPageBytes + R::kVScale +
-                                                                     (c * kKvPage + j % 2 * 8 + 2 * t) * 2);
-                    if (edge) // (times a weight of zero it would be NaN)
-                        s &= ((s & 0x7fffu) >= kQ4BadScale ? 0u : 0xffffu) | ((s >> 16 & 0x7fffu) >= kQ4BadScale ? 0u : 0xffff0000u);
-                    kv4_widen(w[j], kv4_half2(s), v[4 * pp + j]);
+                for (int n = 0; n < G::kFar; ++n) {
+                    float &y = o[n / (8 * G::kTiles)][n / (4 * G::kTiles) % 2][n / 4 % G::kTiles][n % 4];
+                    if (end > G::kPeriod)
+                        y += far[n];
+                    if (end < mine)
+                        far[n] = y, y = 0.f;
                 }
-            }
-#pragma unroll
-            for (int n = 0; n < 2; ++n) {
-                float sum[G::kTiles][4] = {};
-#pragma unroll
-                for (int set = G::kSets - 1; set >= 0; --set)
-#pragma unroll
-                    for (int p = 0; p < G::kStepPages; ++p) {
-                        const uint32_t f[4] = {v[2 * p][2 * n], v[2 * p][2 * n + 1], v[2 * p + 1][2 * n], v[2 * p + 1][2 * n + 1]};
-#pragma unroll
-                        for (int nt = 0; nt < G::kTiles; ++nt) {
-                            if constexpr (G::kWide || kPair)
-                                mma_f16(sum[nt], f, pf[set][nt][p][0], pf[set][nt][p][1]);
-                            else
-                                mma_f16(o[c][n][nt], f, pf[set][nt][p][0], pf[set][nt][p][1]);
-                        }
-                    }
-                if constexpr (kPair) { // (the second column of bf16 rows is zero)
-                    o[c][n][0][0] += G::kWide ? sum[0][0] + sum[0][1] : sum[0][0];
-                    o[c][n][0][1] += G::kWide ? sum[0][2] + sum[0][3] : sum[0][2];
-                } else if constexpr (G::kWide) {
-#pragma unroll
-                    for (int nt = 0; nt < G::kTiles; ++nt)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            o[c][n][nt][e] += sum[nt][e];
-                }
-            }
-        }
     }
     q4_copy_wait<0>();
 
@@ -626,7 +667,7 @@ template <typename... P> inline int q4_slots(void (*kernel)(P...), int threads, 
 
 template <typename T, int D, int kNT> inline void q4_rows_launch(const T *q, T *out, const TreeArgs &a, cudaStream_t stream) {
     using G = Q4RowsGeo<T, D, kNT>;
-    const auto kernel = q4_rows_kernel<T, D, kNT>;
+    auto kernel = q4_rows_kernel<T, D, kNT, false>;
     const int most = allow_shared_bytes(kernel, G::kThreads, G::kBytes);
     const int64_t slots = q4_slots(kernel, G::kThreads, G::kBytes), sms = device_facts().sm_count;
     const int64_t rows = static_cast<int64_t>(a.t.max_rows) * (a.qh / a.kvh);
@@ -645,6 +686,11 @@ template <typename T, int D, int kNT> inline void q4_rows_launch(const T *q, T *
         while (2 * splits <= cap && 2 * splits * all * 3 <= slots * 4)
             splits *= 2;
     require(groups * splits <= 0x7fffffff, "tree attention: too many rows for one call");
+    if constexpr (G::kInCore)
+        if (steps > G::kPeriod * G::kWarps * splits) {
+            kernel = q4_rows_kernel<T, D, kNT, true>;
+            allow_shared_bytes(kernel, G::kThreads, G::kBytes);
+        }
     // sequences in the order of their length, where SMs have more than one CTA (their list is short
     // beside the rings)
     const int64_t per_sequence = groups * splits * a.kvh, total = per_sequence * a.t.batch;

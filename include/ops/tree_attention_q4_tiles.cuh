@@ -62,6 +62,7 @@ template <typename T, int D, int kM> struct Q4TilesGeo {
     static constexpr int kBytes = kBuf + 4 * 256 + 8 * 256 + 8 * 256 + 4 * 16 + 256;
     static constexpr int kPages = kTileKeys / kKvPage, kItems = 2 * kPages; // of a tile: K's pages, then V's
     static constexpr int kLoads = D / 64;                     // pieces of 16 bytes a lane and page
+    static constexpr int kPeriod = kQ4SumTiles;               // steps of a stream after which the sum of bf16 rows is put by
 };
 
 constexpr float kQ4Wary = 0x1p20f; // scores from here on are so coarse that they are rounded before the reference is taken off
@@ -113,7 +114,28 @@ template <int kTerms> __device__ __forceinline__ void q4_lower_weights(uint32_t 
 // inlined, 433 with a call.)
 __device__ __noinline__ void q4_lower_weights_apart(uint32_t at, float fix) { q4_lower_weights<1>(at, fix); }
 
-template <typename T, int D, int kM>
+// Adds a row's O (sets, the first time) to what has been put by of it, in local memory; and that,
+// times the factor of a reference that is raised. Calls, since they hardly ever run.
+template <int D> __device__ __noinline__ void q4_put_by(uint32_t ot, float *far, bool first) {
+#pragma unroll 1
+    for (int d = 0; d < D; d += 16) {
+        uint32_t o[16];
+        sm100::tmem_ld_32x16(ot + static_cast<uint32_t>(d), o);
+        sm100::tmem_wait_ld();
+        sm100::tmem_reg_fence(o);
+#pragma unroll
+        for (int k = 0; k < 16; ++k)
+            far[d + k] = first ? __uint_as_float(o[k]) : far[d + k] + __uint_as_float(o[k]);
+    }
+}
+template <int D> __device__ __noinline__ void q4_lower_far(float *far, float fix) {
+#pragma unroll 4
+    for (int d = 0; d < D; ++d)
+        far[d] *= fix;
+}
+
+// kPutBy: a stream may have more than kPeriod steps, and sums are put by.
+template <typename T, int D, int kM, bool kPutBy>
 static __global__ void __launch_bounds__(kTileThreads, 1)
     q4_tiles_kernel(const T *__restrict__ q, T *__restrict__ out, TreeArgs a, int rep, int splits, bool sorted, int *err) {
     using G = Q4TilesGeo<T, D, kM>;
@@ -346,7 +368,7 @@ static __global__ void __launch_bounds__(kTileThreads, 1)
                             break;
                         }
                         sm100::tc_fence_after();
-                        weigh(s, i, half, half == 1 || (!G::kWide && e > 0));
+                        weigh(s, i, half, half == 1 || (!G::kWide && (kPutBy ? e % G::kPeriod != 0 : e > 0)));
                         if (half == 0)
                             commit(&half_done[s]);
                     }
@@ -443,6 +465,7 @@ static __global__ void __launch_bounds__(kTileThreads, 1)
         const uint32_t ot = tmem + quarter + 256u + static_cast<uint32_t>(stream * D);
         constexpr uint32_t kLong = 128; // columns from O to the sum of fp32 rows
         float m = kQ4None, l = 0.f;
+        [[maybe_unused]] float far[kPutBy ? D : 1]; // what has been put by of O
         bool wary = false; // the same in a warp
         int e = 0; // steps done
         for (; ok; ++e) {
@@ -473,6 +496,9 @@ static __global__ void __launch_bounds__(kTileThreads, 1)
                 sm100::tmem_reg_fence(x[0]);
                 sm100::tmem_reg_fence(x[1]);
             };
+            if constexpr (kPutBy)
+                if (e > 0 && e % G::kPeriod == 0) // (this tile's S is there, so the products before it are done)
+                    q4_put_by<D>(ot, far, e == G::kPeriod);
             uint32_t xa[2][16], xb[2][16];
             ask(0, xa);
             ask(1, xb);
@@ -522,8 +548,11 @@ static __global__ void __launch_bounds__(kTileThreads, 1)
                         tile_tmem_st16(at + static_cast<uint32_t>(d), o);
                     }
                 };
-                if (second || (!G::kWide && e > 0))
+                if (second || (!G::kWide && (kPutBy ? e % G::kPeriod != 0 : e > 0)))
                     scale(ot);
+                if constexpr (kPutBy)
+                    if (e >= G::kPeriod)
+                        q4_lower_far<D>(far, fix);
                 if (G::kWide && e > 0)
                     scale(ot + kLong);
                 tile_tmem_wait_st(); // the chunks' weights are stored before they are read
@@ -655,6 +684,11 @@ static __global__ void __launch_bounds__(kTileThreads, 1)
                     for (int k = 0; k < 16; ++k)
                         o[k] = __float_as_uint(__uint_as_float(o[k]) + __uint_as_float(x[k]));
                 }
+                if constexpr (kPutBy)
+                    if (e > G::kPeriod)
+#pragma unroll
+                        for (int k = 0; k < 16; ++k)
+                            o[k] = __float_as_uint(__uint_as_float(o[k]) + far[c + k]);
             } else {
 #pragma unroll
                 for (int k = 0; k < 16; ++k)
@@ -816,7 +850,7 @@ template <typename... P> inline int q4_clusters(void (*kernel)(P...), int thread
 template <typename T, int D, int kM> inline void q4_tiles_launch(const T *q, T *out, const TreeArgs &a, cudaStream_t stream) {
     using G = Q4TilesGeo<T, D, kM>;
     static_assert(G::kBytes <= 232448, "shared memory");
-    const auto kernel = q4_tiles_kernel<T, D, kM>;
+    auto kernel = q4_tiles_kernel<T, D, kM, false>;
     allow_shared_bytes(kernel, kTileThreads, G::kBytes);
     const int64_t rows = static_cast<int64_t>(a.t.max_rows) * (a.qh / a.kvh);
     const int64_t groups = (rows + G::kRows - 1) / G::kRows, all = groups * a.kvh * a.t.batch;
@@ -826,6 +860,11 @@ template <typename T, int D, int kM> inline void q4_tiles_launch(const T *q, T *
     while (2 * splits <= 8 && 8 * splits <= tiles && all <= q4_clusters(kernel, kTileThreads, G::kBytes, 2 * splits))
         splits *= 2;
     require(groups * splits <= 0x7fffffff, "tree attention: too many rows for one call");
+    if constexpr (!G::kWide)
+        if (tiles > static_cast<int64_t>(G::kPeriod) * (kM == 1 ? 2 : 1) * splits) {
+            kernel = q4_tiles_kernel<T, D, kM, true>;
+            allow_shared_bytes(kernel, kTileThreads, G::kBytes);
+        }
     // more CTAs than places: sequences in the order of their length (the list of them lies over row_fac, stat and joined)
     const bool sorted = a.t.batch > 1 && a.t.batch <= kTileThreads && all * splits > device_facts().sm_count;
     launch_ex_cluster(kernel, dim3(static_cast<unsigned>(groups * splits), a.kvh, a.t.batch), dim3(splits), dim3(kTileThreads), G::kBytes,
