@@ -12,7 +12,7 @@
 // 7). c s has at most 8 significant bits, so what is held is an fp16 number and
 // a bf16 number: attention multiplies codes and scales out for the tensor cores
 // with nothing lost, and reading back as bf16 is exact. 5 bits and not all of
-// fp16's cost 1.6 % of a scale at most. s goes up to 7,936, so the largest value
+// fp16's make a scale 3.1 % wider or narrower at most. s goes up to 7,936, so the largest value
 // is 55,552; a group with a larger one (its s would round above), an infinity or
 // a NaN gets s = NaN and reads back as NaN in every place. s = 0: all zeros.
 //
@@ -107,7 +107,8 @@ __device__ __forceinline__ uint32_t kv4_bits(__half2 h) { return *reinterpret_ca
 
 // Four pairs of codes from the eight of a word, as fp16 numbers: (0, 4), (1, 5), (2,
 // 6), (3, 7). A code + 8 goes into the low bits of fp16 1024 .. 1039 (or, 16-fold, 1024
-// .. 1264), from which 1032 (72) is taken away.
+// .. 1264), from which 1032 (72) is taken away: the way of Kim et al., "Who Says Elephants
+// Can't Run", 2022, from integers to floating point, with this format's offsets.
 __device__ __forceinline__ void kv4_integers(uint32_t w, __half2 (&h)[4]) {
     const uint32_t hi = w >> 8;
     const auto low = [](uint32_t u) { return __hsub2(kv4_half2(kv4_pick<0x000f000fu, 0x64006400u>(u)), kv4_half2(0x64086408u)); };

@@ -17,8 +17,8 @@
 // the same the other way round: the pages ceil(new / 16) .. ceil(old / 16) - 1 of
 // each sequence go onto the stack, in order.
 //
-// Both are bound by latency: a launch, three dependent rounds of loads (counts,
-// ids, the table) and the barriers between them. One cluster does it all, since
+// Both are bound by latency: a launch, and in this design three dependent rounds of
+// loads (counts, ids, the table) with barriers between them. One cluster does it all, since
 // the sums over the sequences come before everything else: every CTA repeats them
 // (they are short) and takes its share of the pages and rows, and a cluster
 // barrier stands where a second launch would. So the count may be updated in

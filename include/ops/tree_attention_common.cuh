@@ -88,16 +88,12 @@ template <typename... P> inline int allow_shared_bytes(void (*kernel)(P...), int
 // Keys and rows of a sequence, held inside the table and the row count.
 struct TreeSpan {
     int b, row0, n, ctx, keys;
-    TreeSpan() = default;
     __device__ TreeSpan(const TreeBatch &t, int b) : b(b) {
         row0 = max(0, t.row_start[b]);
         n = max(0, min(min(t.row_start[b + 1], t.rows) - row0, t.max_rows));
         const int64_t places = static_cast<int64_t>(t.table_stride) * kKvPage;
         ctx = static_cast<int>(min(static_cast<int64_t>(max(0, t.ctx_lens[b])), places));
-        set_keys(t);
-    }
-    __device__ void set_keys(const TreeBatch &t) {
-        keys = static_cast<int>(min(static_cast<int64_t>(ctx) + n, static_cast<int64_t>(t.table_stride) * kKvPage));
+        keys = static_cast<int>(min(static_cast<int64_t>(ctx) + n, places));
     }
 };
 

@@ -10,6 +10,12 @@
 // K's codes, and multiplies the sum over a group's dims by the scale in fp32). A query row is scaled by a power of two, to a
 // largest magnitude of 2^14 to 2^15, and is one fp16 term where it comes in bf16
 // (exact down to 2^-29 of the largest), two where it comes in fp32 (22 bits).
+//
+// The softmax weights of fp32 rows have 22 bits, two terms. Those of bf16 rows are one fp16 number
+// of 11 bits, while their sum takes them as they are: rows come out 1e-4 to 3e-4 off before they
+// are rounded to bf16 (1.7e-3), in the 2-norm. A second term, up to 4 rows a head in the column
+// that is empty there, takes as long as fp32 rows do: 12 sequences of 32,000 tokens, 8 x 128, 102
+// us for 88, and the error goes from 1.67e-3 to 1.66e-3.
 
 #include "tree_attention.cuh"
 #include "kv4.cuh"
@@ -26,7 +32,7 @@ template <typename T, int D> inline void q4_call(const T *q, T *out, const TreeA
     //   fp32 rows, D 64     n = 32  25 / 40 (38 / 61)   48  40 / 41 (61 / 63)   64  40 / 41 (65 / 64)   80  58 / 42 (89 / 65)
     //   bf16 rows, D 64     n = 32  19 / 31 (28 / 48)   48  29 / 32 (45 / 49)   64  29 / 31 (47 / 50)   80  43 / 32 (65 / 51)
     //   bf16 rows, D 128    n = 32  29 / 41 (45 / 63)   48  47 / 42 (72 / 64)   64  47 / 43 (76 / 65)   80  68 / 44 (102 / 66)
-    // It is the mean that tells. (fp32 rows of 128 dims have no tiles.)
+    // It is the mean that tells, in batches of like rows. (fp32 rows of 128 dims have no tiles.)
     constexpr bool kHasTiles = D == 64 || std::is_same_v<T, __nv_bfloat16>;
     constexpr int kFrom = D == 128 ? 32 : 53; // rows of a kv head
     const bool many = static_cast<int64_t>(a.t.rows) * (a.qh / a.kvh) > static_cast<int64_t>(kFrom) * a.t.batch;

@@ -31,12 +31,13 @@
 // the one before: 5,300 cycles for 256 rows x 128 keys, of which the products are 2,048
 // and the exponentials as much, side by side (tensor pipe 37 % busy, exponentials 38 %).
 // Measured (kernel time, one B200): 3 prompts' pieces of up to 2048 rows x 32 heads behind
-// up to 2100 tokens, 8 x 128 bf16: 324 us, 0.70 PFLOP/s; 8 trees of up to 26 nodes x 32
+// up to 2100 tokens, 8 x 128 bf16: 326 us, 0.69 PFLOP/s; 8 trees of up to 26 nodes x 32
 // heads over up to 4099 tokens, 8 x 64 fp32: 41 us.
 //
 // fp32 rows have two fp16 terms of Q and P. The tensor cores cut an accumulator off
 // at every step, so for them O is the sum over one tile and is added, rounded, to a
-// sum of its own in tensor memory, which has room for that at D = 64 only.
+// sum of its own in tensor memory, where two streams leave room for that at D = 64 only (at
+// D = 128 one stream would, with half the overlap; fp32 rows go to the kernel for few rows there).
 
 #include "detail/sm100.cuh"
 #include "tree_attention_q4_rows.cuh"
@@ -46,7 +47,7 @@ namespace opworks::detail {
 
 template <typename T, int D, int kM> struct Q4TilesGeo {
     static constexpr bool kWide = std::is_same_v<T, float>;
-    static_assert(!kWide || D == 64, "tensor memory has no room for the sums of fp32 rows of 128 dims");
+    static_assert(!kWide || D == 64, "two streams leave no room in tensor memory for the sums of fp32 rows of 128 dims");
     static constexpr int kTerms = kWide ? 2 : 1;             // of Q and P
     static constexpr float kLift = kWide ? 6.f : 0.f;         // see kQ4Top
     static constexpr int kSlabs = D / 64, kSlab = kTileKeys * 128; // 64 dims of 128 rows: 128 bytes each

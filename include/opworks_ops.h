@@ -277,7 +277,10 @@ OPW_API int opw_kv4_write(const void *k, int64_t k_stride, const void *v, int64_
                           int blocks, const int64_t *slots, int rows, int num_kv_heads, int head_dim, void *stream);
 OPW_API int opw_kv4_read(const uint8_t *pool, int blocks, const int64_t *slots, int rows, int num_kv_heads,
                          int head_dim, void *k, int64_t k_stride, void *v, int64_t v_stride, int type, void *stream);
-/* opw_tree_attention and opw_tree_commit over the 4-bit pool (layer_stride in bytes). */
+/* opw_tree_attention and opw_tree_commit over the 4-bit pool (layer_stride in bytes).
+ * Softmax weights: 22 bits where q is fp32, 11 where it is bf16 (their sum takes them
+ * unrounded), which puts rows 1e-4 to 3e-4 off before they are rounded to bf16. A table
+ * row that ends before ctx_lens + its rows ends the sequence there. */
 OPW_API int opw_tree_attention_q4(const void *q, int type, int64_t q_stride, const uint8_t *pool,
                                   const int32_t *block_table, int table_stride, const int32_t *ctx_lens,
                                   const int32_t *row_start, const uint32_t *mask, int mask_words, int batch, int rows,
