@@ -123,6 +123,7 @@ int opw_ops_sync(void *stream) {
 
 int opw_ops_capture_id(void *stream, int64_t *id) {
     return guarded([&] {
+        opworks::detail::require(id != nullptr, "opw_ops_capture_id: null pointer");
         cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
         unsigned long long number = 0;
         const cudaError_t e = cudaStreamGetCaptureInfo(as_stream(stream), &status, &number);

@@ -51,6 +51,13 @@ def test_a_step_in_inference_mode(made, format, blocks):
             assert c.place(rows)[0] is not second[0]
 
 
+def test_the_number_of_a_capture_wants_a_place():
+    import opworks_b200
+
+    with pytest.raises(ValueError, match="null"):
+        opworks_b200.ops_lib().ops_capture_id(0, None)
+
+
 def test_depths_of_drafted_rows():
     from opworks_b200.tree import Rows
 
