@@ -187,7 +187,8 @@ class _Places(NamedTuple):
 
     rows: Rows
     lens: torch.Tensor
-    version: Any  # of lens
+    table: torch.Tensor
+    versions: Any  # of both
     capture: int  # the graph capture that they are part of; 0: none
     stream: Any  # that computes them
     positions: torch.Tensor
@@ -220,11 +221,11 @@ class PagedCache:
             self.v = torch.zeros_like(self.k)
         # each sequence's pages spread over the pool, as an allocator would leave them
         if self.shared:
-            self.table = torch.zeros(batch, self.stride, dtype=torch.int32, device=device)
+            self.table = _plain(lambda: torch.zeros(batch, self.stride, dtype=torch.int32, device=device))
             self.free = torch.arange(blocks - 1, -1, -1, dtype=torch.int32, device=device)
             self.free_count = torch.full((1,), blocks, dtype=torch.int32, device=device)
         else:
-            self.table = torch.arange(blocks, dtype=torch.int32, device=device).view(self.stride, batch).t().contiguous()
+            self.table = _plain(lambda: torch.arange(blocks, dtype=torch.int32, device=device).view(self.stride, batch).t().contiguous())
         self.status = torch.zeros(1, dtype=torch.int32, device=device)  # of the last pages taken or given: 0
         self._placed = None        # the places of the last step that asked for them
         self._step = None          # with shared pages the step that has taken its own and is not ended
@@ -316,7 +317,7 @@ class PagedCache:
         elif self._step is not None and not capture:
             self._after(self._step.stream, stream, self._step.after)
         at = self._where(rows, take, stream)
-        self._placed = _Places(rows, self.lens, _version(self.lens), capture, current, *at)
+        self._placed = _Places(rows, self.lens, self.table, (_version(self.lens), _version(self.table)), capture, current, *at)
         if take:
             self._step = _Step(rows, _plain(lambda: self.lens + rows.sizes), current)
         return at
@@ -334,13 +335,14 @@ class PagedCache:
         return at if rows.lift is None else at + rows.lift
 
     def _places(self, rows, stream):
-        """Positions and slots of the rows that the step has already, None: they are to be asked for. A program that moves lens has
-        moved the rows; what a graph computes is there when it is replayed, and only in it. Another stream than theirs waits for
-        them (and for the table, where pages were taken): the program does not know of them."""
+        """Positions and slots of the rows that the step has already, None: they are to be asked for. A program that moves lens or
+        changes the table has moved the rows; what a graph computes is there when it is replayed, and only in it. Another stream than
+        theirs waits for them (and for the table, where pages were taken): the program does not know of them."""
         p = self._placed
-        if p is None or p.rows is not rows or p.lens is not self.lens or p.version is None or p.version != _version(self.lens):
+        if p is None or p.rows is not rows or p.lens is not self.lens or p.table is not self.table:
             return None
-        if p.capture != self._capture(stream):
+        versions = (_version(self.lens), _version(self.table))
+        if None in versions or p.versions != versions or p.capture != self._capture(stream):
             return None
         self._after(p.stream, stream, p.positions, p.slots, *([] if self._step is None else [self._step.after]))
         return p.positions, p.slots

@@ -122,3 +122,18 @@ def test_counts_told_after_a_release(blocks):
     assert c.bounds == [2, 0, 1]
     with pytest.raises(ValueError, match="kept"):
         c.kept([2, 3, 1])
+
+
+@pytest.mark.parametrize("inference", [False, True])
+@pytest.mark.parametrize("blocks", [None, 12])
+def test_a_table_that_the_program_changes_moves_the_rows(inference, blocks):
+    from opworks_b200.tree import Rows
+
+    with torch.inference_mode(inference):
+        c, rows = cache(blocks=blocks), Rows([5, 2], device="cpu")
+        first = c.place(rows)
+        c.table[0, 0] = 7
+        second = c.place(rows)
+        c.table = c.table.clone()
+        third = c.place(rows)
+        assert first[1] is not second[1] and second[1] is not third[1] and c.ops.calls == ["page_take"] * 3
